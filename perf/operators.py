@@ -242,9 +242,10 @@ def _write8(s, kv):
     grown = s0 * torch.exp2(torch.ceil(torch.log2(ratio.clamp(min=1.0)))).float()
     s1 = torch.where(s0 > 0, grown, amax / qmax)
     inv = torch.where(s1 > 0, 1.0 / s1.clamp(min=1e-37), 0.0)[:, :, None, :, :, None]
+    shrink = torch.where(s1 > 0, s0 / s1.clamp(min=1e-37), 0.0)[:, :, None, :, :, None]  # a power of two, exact
     sel = table, torch.full_like(table, _BLOCK_INDEX), pos % stride
     held = slab.view(torch.int8)[sel[0], sel[1], :, :, sel[2]].view(slab.dtype).float()  # [bs, slots, block, heads, 2, hd]
-    q = torch.where(fresh[..., None, None, None], x * inv, held * (s0[:, :, None, :, :, None] * inv)).clamp(-qmax, qmax)
+    q = torch.where(fresh[..., None, None, None], x * inv, held * shrink).clamp(-qmax, qmax)
     codes = (q.round() if case["cache"] == "int8" else q).to(slab.dtype).view(torch.int8)
     live = (fresh | old) & fresh.any(-1, keepdim=True)
     slab.view(torch.int8)[sel[0][live], sel[1][live], :, :, sel[2][live]] = codes[live]
