@@ -404,6 +404,96 @@ int b200moe_attn_decode(const void* q, int q_dtype, const void* slab, int cache_
                         int32_t max_seq_len, float scale, float softcap, void* out, int out_dtype,
                         void* scratch, size_t scratch_bytes, void* stream);
 
+/* ---- The 8-bit KV cache ----------------------------------------------------
+ * The paged cache with K and V held as 8-bit codes and one fp32 scale for each
+ * `scale_block` consecutive positions, kv head and K | V: a code c stands for c * s.
+ * It takes the place of the per-tensor `kv_cache.quantizer` that sharktank's attention
+ * block accepts.  Two arrays, a row of each per page:
+ *   slab    8-bit codes  [pages][blocks][kv_heads][2: K, V][stride][head_dim]
+ *   scales  fp32         [pages][blocks][kv_heads][stride / scale_block][2: K, V]
+ * so that the rows of one page and head are one contiguous stretch. */
+enum { B200MOE_KV8_INT8 = 0, B200MOE_KV8_E4M3 = 1 };
+
+typedef struct {
+  int32_t blocks;      /* transformer blocks in a page */
+  int32_t stride;      /* positions per page */
+  int32_t kv_heads;
+  int32_t head_dim;    /* 64 or 128 */
+  int32_t page_count;  /* rows of slab and scales */
+  int32_t scale_block; /* positions that share a scale: 1, 2, 4, ... 64, a divisor of stride */
+  int32_t code;        /* B200MOE_KV8_* */
+} b200moe_kv8_cache_t;
+
+/* The way of new queries, keys and values into the cache, in one pass: the RMS norm of
+ * every query and key head (q_norm, k_norm: fp32 [head_dim], each NULL for none), the
+ * rotation by position * freqs[i] (order 0: pairs (2i, 2i+1); 1: pairs (i, i + hd/2), the
+ * HuggingFace order) and the write of K and V to their pages.
+ *   q, k, v        [bs * tokens_per_seq] rows of heads (kv_heads) * head_dim elements of
+ *                  io_dtype, q_stride, k_stride, v_stride elements apart (views of one
+ *                  fused projection need no copy); not changed
+ *   q_out, k_out   contiguous rows of io_dtype, apart from the inputs; k_out may be NULL
+ *   start_positions[seq]  position of the sequence's first new token; negative: the
+ *                  sequence is padding, nothing of it is written
+ *   new_lens[seq]  how many of its tokens_per_seq rows are tokens (NULL: all); the rows
+ *                  behind them are padding.  q_out and k_out have them rotated like the
+ *                  others; the cache keeps what it has there
+ *   page_ids       [bs][pages_per_seq]
+ * Quantisation.  A scale block whose first position this call writes is fresh: its scale
+ * is amax / qmax over the rows written (qmax 127 or 448).  A block that is continued has
+ * live rows before the call's first position: its scale stays while the new rows fit
+ * (amax at most 2^-10 above qmax steps, which rounds back to qmax); else it grows by the
+ * smallest power of two that makes them fit, and the codes of the live rows are rounded
+ * to the new scale (exact for e4m3 but for subnormal codes).  Rows of the block behind
+ * the written ones keep their codes and are dead: no position behind the last written one
+ * may be read before it is written.  A block whose new rows are all below qmax * 2^-100
+ * counts as zero (scale 0); one with an infinity or NaN gets the scale NaN and reads as
+ * NaN until it is fresh again.
+ * The written pages of different sequences of a call have to be different pages.  A
+ * position whose page is missing or out of range sets the bounds bit of the status word
+ * and is not written, nor are the other positions of its scale block. */
+int b200moe_attn_norm_rope_kv8_write(const void* q, const void* k, const void* v, int io_dtype, int64_t q_stride,
+                                     int64_t k_stride, int64_t v_stride, const float* q_norm, const float* k_norm,
+                                     float eps, void* q_out, void* k_out, void* slab, float* scales,
+                                     const b200moe_kv8_cache_t* cache, int32_t block_index,
+                                     const int32_t* start_positions, const int32_t* new_lens,
+                                     const int32_t* page_ids, const float* freqs, int order, int32_t bs,
+                                     int32_t tokens_per_seq, int32_t pages_per_seq, int32_t heads, void* stream);
+
+/* The same pass into the 32- or 16-bit cache of b200moe_attn_rope_kv_write: K is rounded
+ * to io_dtype, as k_out is, then to cache_dtype. */
+int b200moe_attn_norm_rope_kv_write(const void* q, const void* k, const void* v, int io_dtype, int64_t q_stride,
+                                    int64_t k_stride, int64_t v_stride, const float* q_norm, const float* k_norm,
+                                    float eps, void* q_out, void* k_out, void* slab, int cache_dtype,
+                                    const b200moe_kv_cache_t* cache, int32_t block_index,
+                                    const int32_t* start_positions, const int32_t* new_lens,
+                                    const int32_t* page_ids, const float* freqs, int order, int32_t bs,
+                                    int32_t tokens_per_seq, int32_t pages_per_seq, int32_t heads, void* stream);
+
+/* PagedKVCache.read (layers/kv_cache.py:351-426) of an 8-bit cache: the values of the
+ * listed pages' first seq_lens[seq] positions as contiguous k_out, v_out
+ * [bs][max_seq_len][kv_heads][head_dim] of out_dtype, each c * s rounded once.  Rows at
+ * and behind a sequence's length are zero.  A missing page sets the bounds bit and reads
+ * as zeros. */
+int b200moe_kv8_read(const void* slab, const float* scales, const b200moe_kv8_cache_t* cache, int32_t block_index,
+                     const int32_t* page_ids, const int32_t* seq_lens, int32_t bs, int32_t pages_per_seq,
+                     int32_t max_seq_len, void* k_out, void* v_out, int out_dtype, void* stream);
+
+/* Attention of each sequence's last new_tokens (1 ... 16) positions over the 8-bit cache:
+ * b200moe_attn_decode's operation, for one or a few tokens at once.  seq_lens[seq] counts
+ * the positions in the cache, the new ones included; new token i attends the positions up
+ * to and including seq_lens[seq] - new_tokens + i, and its output is zero where that
+ * leaves none.  q [bs * new_tokens] rows of heads * head_dim elements, q_stride apart;
+ * out [bs][new_tokens][heads][head_dim] contiguous.  Any heads / kv_heads; softcap <= 0
+ * means none.  A missing page sets the bounds bit; its positions are not attended.
+ * scratch: b200moe_kv8_attend_scratch_bytes(...) bytes, 16-byte aligned. */
+size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_t bs, int32_t new_tokens,
+                                        int32_t heads, int32_t max_seq_len);
+int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void* slab, const float* scales,
+                       const b200moe_kv8_cache_t* cache, int32_t block_index, const int32_t* page_ids,
+                       const int32_t* seq_lens, int32_t bs, int32_t new_tokens, int32_t pages_per_seq,
+                       int32_t heads, int32_t max_seq_len, float scale, float softcap, void* out, int out_dtype,
+                       void* scratch, size_t scratch_bytes, void* stream);
+
 /* A stream of batches from host memory (no reference counterpart: the
  * reference's eager layer takes whatever device its tensors are on).  The
  * pipeline keeps `depth` steps in flight: the host->device copy of a step's

@@ -18,6 +18,7 @@ HEADER_PATH = os.path.join(os.path.dirname(HERE), "include", "b200moe.h")
 LAYOUT_Q8_0, LAYOUT_Q4_K, LAYOUT_F16 = 0, 1, 2
 ACT_SILU, ACT_GELU = 0, 1
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+KV8_INT8, KV8_E4M3 = 0, 1
 REGIME_AUTO, REGIME_STREAM, REGIME_TENSOR, REGIME_TENSOR_PAIR = 0, 1, 2, 3
 
 
@@ -63,6 +64,18 @@ class KvCacheDesc(ctypes.Structure):
         ("kv_heads", c_int32),
         ("head_dim", c_int32),
         ("page_count", c_int32),
+    ]
+
+
+class Kv8CacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("blocks", c_int32),
+        ("stride", c_int32),
+        ("kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("page_count", c_int32),
+        ("scale_block", c_int32),
+        ("code", c_int32),
     ]
 
 
@@ -144,6 +157,17 @@ _PROTOS = {
     "b200moe_attn_decode_scratch_bytes": (c_size_t, [POINTER(KvCacheDesc), c_int32, c_int32, c_int32]),
     "b200moe_attn_decode": (c_int, [_P, c_int, _P, c_int, POINTER(KvCacheDesc), c_int32, _P, _P, c_int32, c_int32,
                                     c_int32, c_int32, c_float, c_float, _P, c_int, _P, c_size_t, _P]),
+    "b200moe_attn_norm_rope_kv8_write": (c_int, [_P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, c_float, _P, _P, _P,
+                                                 _P, POINTER(Kv8CacheDesc), c_int32, _P, _P, _P, _P, c_int, c_int32,
+                                                 c_int32, c_int32, c_int32, _P]),
+    "b200moe_attn_norm_rope_kv_write": (c_int, [_P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, c_float, _P, _P, _P,
+                                                c_int, POINTER(KvCacheDesc), c_int32, _P, _P, _P, _P, c_int, c_int32,
+                                                c_int32, c_int32, c_int32, _P]),
+    "b200moe_kv8_read": (c_int, [_P, _P, POINTER(Kv8CacheDesc), c_int32, _P, _P, c_int32, c_int32, c_int32, _P, _P, c_int,
+                                 _P]),
+    "b200moe_kv8_attend_scratch_bytes": (c_size_t, [POINTER(Kv8CacheDesc), c_int32, c_int32, c_int32, c_int32]),
+    "b200moe_kv8_attend": (c_int, [_P, c_int, c_int64, _P, _P, POINTER(Kv8CacheDesc), c_int32, _P, _P, c_int32, c_int32,
+                                   c_int32, c_int32, c_int32, c_float, c_float, _P, c_int, _P, c_size_t, _P]),
     "b200moe_pipeline_bytes": (c_size_t, [_L, c_int, c_int32, c_int32]),
     "b200moe_pipeline_create": (c_int, [_L, c_int, c_int32, c_int, c_int32, _P, c_size_t, POINTER(c_void_p)]),
     "b200moe_pipeline_submit": (c_int, [_P, _P, _P, c_int32, _P]),

@@ -7,6 +7,14 @@ works on the same objects: the model's theta (`attn_norm`, `attn_q`, `attn_k`,
 (layers/kv_cache.py:222-526; sharktank's own or the mirror below), the list
 `cache_state` holding the page slab, and a rotary embedding layer.
 
+With a cache of 8-bit codes (`PagedKVCache(dtype=torch.int8 | torch.float8_e4m3fn)`),
+per-head query / key norms (`attn_q_norm`, `attn_k_norm` in the theta), the HuggingFace
+rotation order or `new_lens`, the block takes the operators below instead of the rotary
+kernel; they are public on their own:
+  * `norm_rope_kv_write`: norms, rotation and the (quantising) cache write in one pass;
+  * `kv_attend`: attention of one or a few new tokens over an 8-bit cache;
+  * `kv_read`: the values of an 8-bit cache as plain K and V.
+
 What runs where:
   * RMS norm, rotary embedding fused with the KV page write, and the decode
     attention over the pages: this library's kernels (`b200moe_rms_norm`,
@@ -42,14 +50,25 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+_KV8_CODES = {torch.int8: C.KV8_INT8, torch.float8_e4m3fn: C.KV8_E4M3}
+MAX_NEW_TOKENS = 16  # of one kv_attend call
+
+
 class PagedKVCache:
     """Mirror of sharktank's PagedKVCache (layers/kv_cache.py:222-340) for use
     without sharktank: geometry plus `allocate`.  Reads and writes happen inside
-    the attention block's kernels."""
+    the attention block's kernels.
+
+    `dtype` int8 or float8_e4m3fn makes it a cache of 8-bit codes with one fp32
+    scale for each `scale_block` consecutive positions of a page, kv head and K | V
+    (a power of two up to 64 that divides `block_seq_stride`; by default the largest
+    one up to 16): 1 + 4 / scale_block / head_dim bytes per value.  Small blocks follow
+    single large rows more closely, large ones have fewer scales to read."""
 
     def __init__(self, *, transformer_block_count: int, attn_head_count: int, attn_head_dim: int,
                  cache_partition_count: int = 2, block_seq_stride: int = 16,
-                 dtype: torch.dtype = torch.float32, device=None, shard_count: int = 1):
+                 dtype: torch.dtype = torch.float32, device=None, shard_count: int = 1,
+                 scale_block: Optional[int] = None):
         if cache_partition_count != 2 or shard_count != 1:
             raise C.B200MoeError("the cache holds K and V on one device")
         self.transformer_block_count = transformer_block_count
@@ -59,11 +78,213 @@ class PagedKVCache:
         self.block_seq_stride = block_seq_stride
         self.shard_count = shard_count
         self.dtype, self.device = dtype, device
-        self.sub_page_dims = [transformer_block_count, 2, block_seq_stride, attn_head_count, attn_head_dim]
+        self.quantized = dtype in _KV8_CODES
+        if self.quantized:
+            # the largest power of two that divides the stride, up to 16
+            self.scale_block = min(block_seq_stride & -block_seq_stride, 16) if scale_block is None else scale_block
+            b = self.scale_block
+            if b < 1 or b > 64 or b & (b - 1) or block_seq_stride % b:
+                raise C.B200MoeError(f"scale_block {b}: a power of two up to 64 that divides the page stride "
+                                     f"({block_seq_stride})")
+            # a page's rows of one head are one contiguous stretch
+            self.sub_page_dims = [transformer_block_count, attn_head_count, 2, block_seq_stride, attn_head_dim]
+            self.scale_page_dims = [transformer_block_count, attn_head_count, block_seq_stride // b, 2]
+            self.scale_flat_dim = math.prod(self.scale_page_dims)
+        else:
+            if scale_block is not None:
+                raise C.B200MoeError(f"scale_block is for caches of 8-bit codes, not {dtype}")
+            self.scale_block = None
+            self.sub_page_dims = [transformer_block_count, 2, block_seq_stride, attn_head_count, attn_head_dim]
         self.page_slab_flat_dim = math.prod(self.sub_page_dims)
 
     def allocate(self, page_count: int) -> list[torch.Tensor]:
-        return [torch.zeros(page_count, self.page_slab_flat_dim, dtype=self.dtype, device=self.device)]
+        """[page slab], or [page slab, scales] for 8-bit codes: a row of each per page."""
+        state = [torch.zeros(page_count, self.page_slab_flat_dim, dtype=self.dtype, device=self.device)]
+        if self.quantized:
+            state.append(torch.zeros(page_count, self.scale_flat_dim, dtype=torch.float32, device=self.device))
+        return state
+
+
+# ------------------------------------------------------------- cache operators
+def _need(ok: bool, message: str) -> None:
+    if not ok:
+        raise C.B200MoeError(message)
+
+
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _check_cache(cache, state, block_index: int, seq_block_ids: torch.Tensor, bs: int, dev) -> None:
+    slab = state[0]
+    _need(0 <= block_index < cache.transformer_block_count, f"block_index {block_index} is not one of the cache's "
+          f"{cache.transformer_block_count} transformer blocks")
+    _need(slab.dim() == 2 and slab.shape[1] == math.prod(cache.sub_page_dims) and slab.is_contiguous(),
+          "the page slab must be contiguous, a row of the cache's page size per page")
+    if getattr(cache, "quantized", False):
+        _need(len(state) == 2, "a cache of 8-bit codes is [page slab, scales], as allocate() gives it")
+        _need(slab.dtype == cache.dtype, f"the page slab must be {cache.dtype}, got {slab.dtype}")
+        scales = state[1]
+        _need(scales.dtype == torch.float32 and scales.shape == (slab.shape[0], cache.scale_flat_dim) and
+              scales.is_contiguous() and scales.device == slab.device,
+              "scales must be fp32, contiguous, beside the slab, a row per page")
+    else:
+        _need(slab.dtype in _DT, "the page slab must be a contiguous fp32, fp16 or bf16 tensor")
+    _need(seq_block_ids.dim() == 2 and seq_block_ids.shape[0] == bs and seq_block_ids.shape[1] >= 1,
+          f"seq_block_ids must be [{bs}, pages of a sequence], got {list(seq_block_ids.shape)}")
+    _need(slab.device == dev and seq_block_ids.device == dev, "cache, page ids and activations must be on one device")
+
+
+def _kv8_desc(cache, pages: int):
+    return C.Kv8CacheDesc(cache.transformer_block_count, cache.block_seq_stride, cache.attn_head_count,
+                          cache.attn_head_dim, pages, cache.scale_block, _KV8_CODES[cache.dtype])
+
+
+def _rows(x: torch.Tensor):
+    """x [bs, sl, heads, hd] as rows of heads * hd elements one stride apart, 16-byte
+    aligned (a view of a fused projection is that already): (tensor, stride)."""
+    bs, sl, heads, hd = x.shape
+    s = x.stride()
+    per16 = 16 // x.element_size()
+    ok = (s[3] == 1 and (heads == 1 or s[2] == hd) and (bs == 1 or sl == 1 or s[0] == sl * s[1])
+          and x.data_ptr() % 16 == 0)
+    if ok:
+        stride = s[1] if sl > 1 else s[0] if bs > 1 else heads * hd
+        if stride >= heads * hd and stride % per16 == 0:
+            return x, stride
+    # rows must start on 16 bytes: a contiguous view that does not is copied too
+    return x.clone(memory_format=torch.contiguous_format), heads * hd
+
+
+def norm_rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, cache_state: list, *,
+                       block_index: int, seq_block_ids: torch.Tensor, start_positions: torch.Tensor,
+                       freqs: torch.Tensor, new_lens: Optional[torch.Tensor] = None,
+                       q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
+                       eps: float = 1e-5, use_hf: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Puts new tokens into the cache: RMS norm of every query and key head (`q_norm`,
+    `k_norm`: fp32 [head_dim], or None), rotation by position * `freqs` (fp32
+    [head_dim / 2]; pairs (2i, 2i + 1), with `use_hf` (i, i + head_dim / 2)), and K and V
+    written to their pages, quantised if the cache holds 8-bit codes: one pass.
+
+    q [bs, sl, heads, head_dim], k and v [bs, sl, kv_heads, head_dim] (views of one fused
+    projection are taken as they are) hold tokens start_positions[b] ... + sl - 1 of
+    sequence b; those at and behind new_lens[b] are padding: rotated, not written.  A
+    negative start position makes a whole sequence padding.  Sequences of one call must
+    not share the pages they write.  Returns the rotated q and k, contiguous.
+
+    8-bit codes: a scale block that the call begins has the scale amax / 127 (448 for
+    e4m3) of the rows written; one that it continues keeps its scale while the new rows
+    fit, else the scale grows by a power of two and the block's earlier codes are rounded
+    to it.  Positions behind the last written one of a block are dead until written.  An
+    infinity or NaN makes its block read as NaN."""
+    bs, sl, heads, hd = q.shape
+    kvh = cache.attn_head_count
+    _need(q.dtype in _DT and k.dtype == q.dtype and v.dtype == q.dtype,
+          f"q, k and v must be fp32, fp16 or bf16 alike, got {q.dtype}, {k.dtype}, {v.dtype}")
+    _need(hd == cache.attn_head_dim and k.shape == (bs, sl, kvh, hd) and v.shape == k.shape and heads % kvh == 0,
+          f"q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} do not fit a cache of {kvh} heads of "
+          f"{cache.attn_head_dim}")
+    _need(start_positions.shape == (bs,) and (new_lens is None or new_lens.shape == (bs,)),
+          f"start_positions and new_lens are [{bs}]")
+    _need(freqs.dtype == torch.float32 and freqs.shape == (hd // 2,) and freqs.is_contiguous(),
+          f"freqs must be fp32 [{hd // 2}]")
+    for w in (q_norm, k_norm):
+        _need(w is None or (w.dtype == torch.float32 and w.shape == (hd,) and w.is_contiguous()),
+              f"norm weights must be fp32 [{hd}]")
+    dev = q.device
+    _check_cache(cache, cache_state, block_index, seq_block_ids, bs, dev)
+    _moe._require_cuda(q, "q")
+    _need(all(t is None or t.device == dev for t in (k, v, start_positions, new_lens, freqs, q_norm, k_norm)),
+          "all arguments must be on one device")
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
+    q_out = torch.empty(bs, sl, heads, hd, dtype=q.dtype, device=dev)
+    k_out = torch.empty(bs, sl, kvh, hd, dtype=q.dtype, device=dev)
+    if bs * sl == 0:
+        return q_out, k_out
+    start, ids = _int32(start_positions), _int32(seq_block_ids)
+    lens = None if new_lens is None else _int32(new_lens)
+    slab = cache_state[0]
+    head = (_p(q), _p(k), _p(v), _DT[q.dtype], qs, ks, vs, _p(q_norm), _p(k_norm), float(eps), _p(q_out), _p(k_out),
+            _p(slab))
+    tail = (block_index, _p(start), _p(lens), _p(ids), _p(freqs), 1 if use_hf else 0, bs, sl, ids.shape[1], heads)
+    with torch.cuda.device(dev):
+        if cache.quantized:
+            C.check(C.lib.b200moe_attn_norm_rope_kv8_write(
+                *head, _p(cache_state[1]), ctypes.byref(_kv8_desc(cache, slab.shape[0])), *tail, _moe._stream()),
+                "attn_norm_rope_kv8_write")
+        else:
+            desc = C.KvCacheDesc(cache.transformer_block_count, cache.block_seq_stride, kvh, hd, slab.shape[0])
+            C.check(C.lib.b200moe_attn_norm_rope_kv_write(
+                *head, _DT[slab.dtype], ctypes.byref(desc), *tail, _moe._stream()), "attn_norm_rope_kv_write")
+    return q_out, k_out
+
+
+def kv_read(cache: PagedKVCache, cache_state: list, *, block_index: int, seq_block_ids: torch.Tensor,
+            seq_lens: torch.Tensor, max_seq_len: Optional[int] = None,
+            dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V of the listed pages of an 8-bit cache, [bs, max_seq_len, kv_heads, head_dim]
+    each (`max_seq_len`: all of the listed pages by default); every value code * scale,
+    rounded once to `dtype`.  Rows at and behind seq_lens[b] are zero."""
+    _need(cache.quantized, "kv_read reads caches of 8-bit codes")
+    _need(dtype in _DT, f"K and V are read as fp32, fp16 or bf16, not {dtype}")
+    bs = seq_block_ids.shape[0]
+    dev = cache_state[0].device
+    _need(seq_lens.shape == (bs,) and seq_lens.device == dev, f"seq_lens is [{bs}], on the cache's device")
+    _check_cache(cache, cache_state, block_index, seq_block_ids, bs, dev)
+    _moe._require_cuda(cache_state[0], "the page slab")
+    n = seq_block_ids.shape[1] * cache.block_seq_stride if max_seq_len is None else int(max_seq_len)
+    _need(0 <= n <= seq_block_ids.shape[1] * cache.block_seq_stride,
+          f"max_seq_len {n} is more than the listed pages hold")
+    k, v = torch.empty(2, bs, n, cache.attn_head_count, cache.attn_head_dim, dtype=dtype, device=dev)
+    if bs * n == 0:
+        return k, v
+    ids, lens = _int32(seq_block_ids), _int32(seq_lens)
+    with torch.cuda.device(dev):
+        C.check(C.lib.b200moe_kv8_read(
+            _p(cache_state[0]), _p(cache_state[1]), ctypes.byref(_kv8_desc(cache, cache_state[0].shape[0])), block_index,
+            _p(ids), _p(lens), bs, ids.shape[1], n, _p(k), _p(v), _DT[dtype], _moe._stream()), "kv8_read")
+    return k, v
+
+
+def kv_attend(q: torch.Tensor, cache: PagedKVCache, cache_state: list, *, block_index: int,
+              seq_block_ids: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
+              softcap: Optional[float] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Attention of the last sl (1 ... 16) positions of each sequence over an 8-bit cache.
+
+    q [bs, sl, heads, head_dim], rotated; seq_lens[b] counts the positions in the cache,
+    the sl new ones included (`norm_rope_kv_write` first).  Token i attends the positions
+    up to and including its own, seq_lens[b] - sl + i; where that leaves none its output is
+    zero.  scale: 1 / sqrt(head_dim) by default; softcap: c * tanh(score / c).  Returns
+    [bs, sl, heads, head_dim]."""
+    _need(cache.quantized, "kv_attend reads caches of 8-bit codes")
+    bs, sl, heads, hd = q.shape
+    out_dtype = q.dtype if out_dtype is None else out_dtype
+    _need(q.dtype in _DT and out_dtype in _DT, f"activations must be fp32, fp16 or bf16, got {q.dtype}, {out_dtype}")
+    _need(hd == cache.attn_head_dim and heads % cache.attn_head_count == 0,
+          f"q {list(q.shape)} does not fit a cache of {cache.attn_head_count} heads of {cache.attn_head_dim}")
+    _need(1 <= sl <= MAX_NEW_TOKENS, f"{sl} new tokens: 1 to {MAX_NEW_TOKENS}; longer stretches attend kv_read's K and V")
+    _need(softcap is None or softcap > 0, "softcap must be positive")
+    dev = q.device
+    _need(seq_lens.shape == (bs,) and seq_lens.device == dev, f"seq_lens is [{bs}], on q's device")
+    _check_cache(cache, cache_state, block_index, seq_block_ids, bs, dev)
+    _moe._require_cuda(q, "q")
+    q, qs = _rows(q)
+    out = torch.empty(bs, sl, heads, hd, dtype=out_dtype, device=dev)
+    if bs == 0:
+        return out
+    ids, lens = _int32(seq_block_ids), _int32(seq_lens)
+    max_len = ids.shape[1] * cache.block_seq_stride
+    desc = _kv8_desc(cache, cache_state[0].shape[0])
+    with torch.cuda.device(dev):
+        nbytes = C.lib.b200moe_kv8_attend_scratch_bytes(ctypes.byref(desc), bs, sl, heads, max_len)
+        # per call: other streams and captured graphs have their own
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        C.check(C.lib.b200moe_kv8_attend(
+            _p(q), _DT[q.dtype], qs, _p(cache_state[0]), _p(cache_state[1]), ctypes.byref(desc), block_index, _p(ids),
+            _p(lens), bs, sl, ids.shape[1], heads, max_len, float(1.0 / math.sqrt(hd) if scale is None else scale),
+            0.0 if softcap is None else float(softcap), _p(out), _DT[out_dtype], _p(scratch), nbytes, _moe._stream()),
+            "kv8_attend")
+    return out
 
 
 class RotaryEmbeddingLayer:
