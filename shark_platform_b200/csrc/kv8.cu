@@ -367,6 +367,8 @@ int check_kv8(const char* who, const b200moe_kv8_cache_t* c, int32_t block_index
                    c->stride % c->scale_block == 0,
                "%s: scale_block %d must be a power of two up to %d that divides the stride (%d)", who, c->scale_block,
                MAX_SCALE_BLOCK, c->stride);
+  B200_REQUIRE(static_cast<double>(c->page_count) * c->blocks * c->kv_heads * 2.0 * c->stride < 4294967295.0,
+               "%s: the cache has more than 2^32 rows", who);
   B200_REQUIRE(c->code == B200MOE_KV8_INT8 || c->code == B200MOE_KV8_E4M3, "%s: unknown code %d", who, c->code);
   return B200MOE_OK;
 }
@@ -416,83 +418,466 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
 }
 
 // -------------------------------------------------------------------- attention
+// o = sum_p softmax(S)_p c_v(p) s_v(p),  S = scale * s_k(p) * (q . c_k(p)).
+//
+// Both products run on tensor cores with the codes widened to fp16 in registers (int8 and
+// e4m3 are exact there), positions and head elements as the rows of A, the query rows that
+// share a kv head as the eight columns of B (mma.m16n8k16):
+//   S^T[pos][row] = K[pos][:] . q[row][:]      O^T[d][row] = sum_pos V^T[d][pos] P^T[pos][row]
+// so that eight rows cost one MMA per 16 positions and 16 elements, and nothing is padded
+// beyond eight rows (G = heads / kv_heads rows for one new token, G * new_tokens for
+// several; NT = 2 takes sixteen).
+//   * K is the A operand as it lies: ldmatrix of 16-byte chunks gives a lane four
+//     consecutive bytes of a row, and the order of the 16 elements of an MMA is free as
+//     long as q's fragments have the same one (a lane holds q[16c + 4 tig .. + 3]).
+//   * V^T comes from ldmatrix.trans on pairs of bytes: a lane gets two elements of two
+//     positions, and taking bytes 0, 2 and 1, 3 apart makes rows 2 gid and 2 gid + 1 of V^T.
+//   * P^T is S^T's accumulator, packed and transposed within the warp (movmatrix).
+// The scale of V joins the softmax: with t = S log2(e) + log2(s_v), P = 2^(t - max t) is at
+// most 1 whatever the scales are, the sum of P c_v is the numerator and that of P / s_v
+// the denominator.  P and q are fp16 with their largest value near 2^15, so that what is
+// rounded is 2^-11 of a value down to 2^-29 of the largest.  SPLIT (32-bit activations):
+// q and P are the sums of two fp16 parts, 2^-22, at twice the MMAs.
+//
+// A warp owns units of 32 positions with its own softmax state and its own ring of two
+// slots, filled by 16-byte cp.async; chunks are swizzled so that ldmatrix has no bank
+// conflicts.  Positions are split over CTAs; the merge kernel joins the splits.
 struct AttendArgs {
   const void* q;
   int64_t q_stride;
+  int q_dtype;
   const uint8_t* slab;
   const float* scales;
   const int32_t *page_ids, *seq_lens;
   void* out;
+  float* partial;  // [bs][kv_heads * row tiles][splits][rows of a tile][HD + 2]
   int out_dtype, bs, sl, pages_per_seq, page_count, heads, kv_heads, stride, blocks, block_index, scale_block;
+  int splits, row_tiles;
   float scale, softcap;
   int32_t* status;
 };
 
-// One CTA per (head, new token, sequence), a warp per position, HD / 32 elements per lane.
-template <typename T, int HD, int CODE>
-__global__ void __launch_bounds__(128) kv8_attend_kernel(const AttendArgs a) {
-  constexpr int N = HD / 32;
-  __shared__ float s_o[4][HD], s_m[4], s_l[4];
-  const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = h / (a.heads / a.kv_heads);
-  const int end = min(a.seq_lens[b] - a.sl + 1 + i, a.pages_per_seq * a.stride);
-  float q[N], o[N], m = -INFINITY, l = 0.f;
-  load_elems(static_cast<const T*>(a.q) + (static_cast<int64_t>(b) * a.sl + i) * a.q_stride + h * HD + lane * N, q);
-#pragma unroll
-  for (int j = 0; j < N; ++j) o[j] = 0.f;
-  for (int pos = warp; pos < end; pos += 4) {
-    const int slot = pos / a.stride, off = pos % a.stride;
-    const long long page = a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot];
-    if (page < 0 || page >= a.page_count) {
-      if (lane == 0) atomicOr(a.status, DEV_ERR_BOUNDS);
-      continue;
-    }
-    const size_t head = (static_cast<size_t>(page) * a.blocks + a.block_index) * a.kv_heads + kvh;
-    const uint8_t* k = a.slab + (head * 2 * a.stride + off) * HD + lane * N;
-    const uint8_t* v = k + static_cast<size_t>(a.stride) * HD;
-    const float* sc = a.scales + 2 * (head * (a.stride / a.scale_block) + off / a.scale_block);
-    float dot = 0.f;
-#pragma unroll
-    for (int j = 0; j < N; ++j) dot = fmaf(q[j], code_to_float<CODE>(k[j]), dot);
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-    dot *= sc[0] * a.scale;
-    if (a.softcap > 0.f) dot = a.softcap * tanhf(dot / a.softcap);
-    const float m_new = fmaxf(m, dot), alpha = expf(m - m_new), p = expf(dot - m_new);
-    m = m_new;
-    l = l * alpha + p;
-#pragma unroll
-    for (int j = 0; j < N; ++j) o[j] = o[j] * alpha + p * sc[1] * code_to_float<CODE>(v[j]);
+constexpr int AT_THREADS = 128, AT_WARPS = 4;
+constexpr int AT_UNIT = 32;   // positions of a warp's step
+constexpr int AT_SLOTS = 2;
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v & 0xffffu), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+// Four codes as two fp16 pairs: bytes (0, 1), (2, 3), or with PAIRS_APART (0, 2), (1, 3).
+template <int CODE, bool PAIRS_APART>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CODE == B200MOE_KV8_INT8) {
+    // 0x6400 | b is the fp16 number 1024 + b; the byte is biased to unsigned first
+    const uint32_t x = w ^ 0x80808080u;
+    const __half2 bias = u32_as_h2(0x64806480u);
+    lo = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, PAIRS_APART ? 0x4240 : 0x4140)), bias));
+    hi = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, PAIRS_APART ? 0x4341 : 0x4342)), bias));
+  } else {
+    if constexpr (PAIRS_APART) w = __byte_perm(w, 0, 0x3120);
+    lo = e4m3x2_to_h2(w);
+    hi = e4m3x2_to_h2(w >> 16);
   }
-#pragma unroll
-  for (int j = 0; j < N; ++j) s_o[warp][lane * N + j] = o[j];
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-  __syncthreads();
-  if (warp != 0) return;
-  const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  float den = 0.f;
-#pragma unroll
-  for (int j = 0; j < N; ++j) o[j] = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    if (s_l[w] == 0.f) continue;
-    const float f = expf(s_m[w] - top);
-    den += f * s_l[w];
-#pragma unroll
-    for (int j = 0; j < N; ++j) o[j] += f * s_o[w][lane * N + j];
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j) o[j] = den == 0.f ? 0.f : o[j] / den;
-  store_as(a.out, a.out_dtype, ((static_cast<size_t>(b) * a.sl + i) * a.heads + h) * HD + lane * N, o);
 }
 
-template <typename T, int HD>
-int launch_attend(const AttendArgs& a, int code, cudaStream_t st) {
-  const dim3 grid(a.heads, a.sl, a.bs);
-  if (code == B200MOE_KV8_INT8) kv8_attend_kernel<T, HD, B200MOE_KV8_INT8><<<grid, 128, 0, st>>>(a);
-  else kv8_attend_kernel<T, HD, B200MOE_KV8_E4M3><<<grid, 128, 0, st>>>(a);
-  B200_CHECK_CUDA(cudaGetLastError());
+__device__ __forceinline__ float load_one(const void* p, int dtype, int64_t i) {
+  if (dtype == B200MOE_DT_F32) return static_cast<const float*>(p)[i];
+  if (dtype == B200MOE_DT_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// Byte offset of 16-byte chunk c of row r in a tile of rows of HD bytes: the eight chunks
+// that one ldmatrix phase reads (eight rows, one c) lie in eight different bank groups.
+template <int HD>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  if constexpr (HD == 128) return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4));
+  else return static_cast<uint32_t>((r >> 1) * 128 + ((((r & 1) * 4 + c) ^ ((r >> 1) & 3)) << 4));
+}
+
+// The sums of several states (max, denominator, numerator) of one row: weights 2^(m - M).
+__device__ __forceinline__ float state_weight(float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); }
+
+template <int HD, int CODE, int NT, bool SPLIT>
+__global__ void __launch_bounds__(AT_THREADS) kv8_attend_kernel(const AttendArgs a) {
+  constexpr int CH = HD / 16;                       // chunks of a row: MMA steps of q.k, row tiles of V^T
+  constexpr int PARTS = SPLIT ? 2 : 1;
+  constexpr int ROWS = 8 * NT;
+  constexpr int TILE = AT_UNIT * HD;                // bytes of a unit's K (or V)
+  constexpr int OPITCH = HD + 8;                    // floats
+  extern __shared__ __align__(128) uint8_t smem[];  // [warp][slot][K | V], then in place [warp][row][OPITCH] fp32
+  __shared__ float4 s_pos[AT_WARPS][AT_UNIT];       // of each position: s_k, log2 s_v, 1 / s_v
+  __shared__ float2 s_ml[AT_WARPS][ROWS];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gid = lane >> 2, tig = lane & 3;
+  const int split = blockIdx.x, kvh = blockIdx.y / a.row_tiles, tile = blockIdx.y % a.row_tiles, b = blockIdx.z;
+  const int G = a.heads / a.kv_heads, rows = G * a.sl;
+  int len = a.seq_lens[b];
+  const long long room = static_cast<long long>(a.pages_per_seq) * a.stride;
+  if (len > room) {
+    if (t == 0) atomicOr(a.status, DEV_ERR_BOUNDS);
+    len = static_cast<int>(room);
+  }
+  // this split's positions, in whole steps of the CTA
+  constexpr int STEP = AT_WARPS * AT_UNIT;
+  const int steps = len > 0 ? (len + STEP - 1) / STEP : 0, per = (steps + a.splits - 1) / a.splits;
+  const int p_begin = split * per * STEP, p_end = min(len, (split + 1) * per * STEP);
+  const int units = p_end > p_begin + warp * AT_UNIT ? (p_end - p_begin - warp * AT_UNIT + STEP - 1) / STEP : 0;
+
+  // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two
+  uint32_t qb[PARTS][NT][CH][2];
+  float fold[NT][2];  // of this lane's accumulator columns 2 tig, 2 tig + 1: back to scores (in halvings, without softcap)
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = tile * ROWS + 8 * n + gid;
+    float x[CH][4], top = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[c][e] = r < rows ? load_one(a.q, a.q_dtype, (static_cast<int64_t>(b) * a.sl + r / G) * a.q_stride +
+                                                          static_cast<int64_t>(kvh * G + r % G) * HD + 16 * c + 4 * tig + e)
+                           : 0.f;
+        top = fmaxf(top, fabsf(x[c][e]));
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^e <= top < 2^(e + 1), so that the largest value lies in [2^14, 2^15)
+    int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+    e = e < -100 || e > 127 ? -100 : e;
+    if (__float_as_uint(top) == 0x7f800000u) e = 100;
+    const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
+    const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23) * a.scale * (a.softcap > 0.f ? 1.f : LOG2E);
+    fold[n][0] = __shfl_sync(0xffffffffu, down, (2 * tig) * 4);
+    fold[n][1] = __shfl_sync(0xffffffffu, down, (2 * tig + 1) * 4);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float u = x[c][2 * i] * up, v = x[c][2 * i + 1] * up;
+        const __half2 h = __floats2half2_rn(u, v);
+        qb[0][n][c][i] = h2_as_u32(h);
+        if constexpr (SPLIT) {
+          const float2 f = __half22float2(h);
+          qb[PARTS - 1][n][c][i] = h2_as_u32(__floats2half2_rn(u - f.x, v - f.y));
+        }
+      }
+  }
+  // the first position that a column does not see
+  int seen[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) seen[n][j] = len - a.sl + 1 + (tile * ROWS + 8 * n + 2 * tig + j) / G;
+  const int all_see = len - a.sl + 1;
+
+  const uint32_t ring = smem_u32(smem) + warp * (AT_SLOTS * 2 * TILE);
+  // the K row of this lane's position of unit u in the slab, in rows of HD bytes; ~0: none
+  auto row_of = [&](int u) -> uint32_t {
+    const int pos = p_begin + u * STEP + warp * AT_UNIT + lane;
+    if (pos >= p_end) return 0xffffffffu;
+    const int slot = pos / a.stride, off = pos - slot * a.stride;
+    const int page = a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot];
+    if (page < 0 || page >= a.page_count) {
+      atomicOr(a.status, DEV_ERR_BOUNDS);
+      return 0xffffffffu;
+    }
+    return ((static_cast<uint32_t>(page) * a.blocks + a.block_index) * a.kv_heads + kvh) * 2u * a.stride + off;
+  };
+  const size_t v_off = static_cast<size_t>(a.stride) * HD;
+  // starts the copies of unit u and the load of its scales; one group per call, also past the end
+  auto issue = [&](int u, uint32_t row, float2& sc) {
+    sc = make_float2(0.f, -1.f);
+    if (u < units) {
+      const uint32_t kt = ring + (u % AT_SLOTS) * 2 * TILE;
+      constexpr int RPI = 32 / CH;  // rows of one pass of the warp
+      const int r0 = lane / CH, c = lane % CH;
+#pragma unroll
+      for (int i = 0; i < AT_UNIT / RPI; ++i) {
+        const int r = i * RPI + r0;
+        const uint32_t at = __shfl_sync(0xffffffffu, row, r);
+        const bool ok = at != 0xffffffffu;
+        const uint8_t* src = a.slab + static_cast<size_t>(ok ? at : 0u) * HD + c * 16;
+        copy16(kt + tile_at<HD>(r, c), src, ok);
+        copy16(kt + TILE + tile_at<HD>(r, c), src + v_off, ok);
+      }
+      if (row != 0xffffffffu) {
+        const uint32_t head = row / (2u * a.stride), off = row % a.stride;
+        sc = reinterpret_cast<const float2*>(a.scales)[static_cast<size_t>(head) * (a.stride / a.scale_block) +
+                                                       off / a.scale_block];
+      }
+    }
+    copy_commit();
+  };
+
+  float m[NT][2], l[NT][2], o[NT][CH][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.f;
+  }
+
+  float2 sc_now, sc_next;
+  issue(0, row_of(0), sc_next);
+  uint32_t row_next = row_of(1);
+  for (int u = 0; u < units; ++u) {
+    sc_now = sc_next;
+    issue(u + 1, row_next, sc_next);
+    row_next = row_of(u + 2);
+    {
+      // dead positions (sc.y < 0: scales are never negative): weight 0 without touching the others
+      const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f);  // 2^-100 in the place of 0
+      const bool dead = sc_now.y < 0.f;
+      const bool bad = sc_now.y != sc_now.y;
+      s_pos[warp][lane] = make_float4(sc_now.x, dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : 1.f / vs, 0.f);
+    }
+    copy_wait<AT_SLOTS - 1>();
+    __syncwarp();
+    const uint32_t kt = ring + (u % AT_SLOTS) * 2 * TILE, vt = kt + TILE;
+    const int p0 = p_begin + u * STEP + warp * AT_UNIT;
+
+    float s[2][NT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; c += 2) {
+        uint32_t w[4];
+        ldsm_x4(kt + tile_at<HD>(16 * h + (lane & 15), c + (lane >> 4)), w);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t a0, a1, a2, a3;
+          widen4<CODE, false>(w[2 * i], a0, a2);
+          widen4<CODE, false>(w[2 * i + 1], a1, a3);
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816(s[h][n], a0, a1, a2, a3, qb[p][n][c + i][0], qb[p][n][c + i][1]);
+        }
+      }
+    }
+    // scores of positions 16 h + 8 j + gid, columns 2 tig + e
+    float top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+    float ivs[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 f = s_pos[warp][16 * h + 8 * j + gid];
+        ivs[h][j] = f.z;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = s[h][n][2 * j + e] * (f.x * fold[n][e]);
+            if (a.softcap > 0.f) x = a.softcap * LOG2E * tanhf(x / a.softcap);
+            x += f.y;
+            if (p0 + AT_UNIT > all_see && p0 + 16 * h + 8 * j + gid >= seen[n][e]) x = -INFINITY;
+            s[h][n][2 * j + e] = x;
+            top[n][e] = fmaxf(top[n][e], x);
+          }
+      }
+    uint32_t pb[PARTS][NT][2][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float base[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = top[n][e];
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+        const float m_new = fmaxf(m[n][e], v);
+        const float safe = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = ex2(m[n][e] - safe);
+        m[n][e] = m_new;
+        l[n][e] *= alpha;
+        base[e] = 15.f - safe;  // the largest P is 2^15
+#pragma unroll
+        for (int c = 0; c < CH; ++c) { o[n][c][e] *= alpha; o[n][c][2 + e] *= alpha; }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float p0v = ex2(s[h][n][2 * j] + base[0]), p1v = ex2(s[h][n][2 * j + 1] + base[1]);
+          l[n][0] = fmaf(p0v, ivs[h][j], l[n][0]);
+          l[n][1] = fmaf(p1v, ivs[h][j], l[n][1]);
+          const __half2 hp = __floats2half2_rn(p0v, p1v);
+          pb[0][n][h][j] = transpose8x8(h2_as_u32(hp));
+          if constexpr (SPLIT) {
+            const float2 f = __half22float2(hp);
+            pb[PARTS - 1][n][h][j] = transpose8x8(h2_as_u32(__floats2half2_rn(p0v - f.x, p1v - f.y)));
+          }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < CH; c += 2) {
+        uint32_t w[4];
+        ldsm_x4_trans(vt + tile_at<HD>(16 * h + (lane & 15), c + (lane >> 4)), w);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t a0, a1, a2, a3;
+          widen4<CODE, true>(w[2 * i], a0, a1);
+          widen4<CODE, true>(w[2 * i + 1], a2, a3);
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816(o[n][c + i], a0, a1, a2, a3, pb[p][n][h][0], pb[p][n][h][1]);
+        }
+      }
+    __syncwarp();  // the slot and s_pos are read: the next pass refills them
+  }
+  copy_wait<0>();
+  __syncthreads();  // the ring is free
+  // the four warps' states through shared memory
+  float* s_o = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * n + 2 * tig + e;
+      float v = l[n][e];
+      v += __shfl_xor_sync(0xffffffffu, v, 4);
+      v += __shfl_xor_sync(0xffffffffu, v, 8);
+      v += __shfl_xor_sync(0xffffffffu, v, 16);
+      if (gid == 0) s_ml[warp][r] = make_float2(m[n][e], v);
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        *reinterpret_cast<float2*>(&s_o[(warp * ROWS + r) * OPITCH + 16 * c + 2 * gid]) =
+            make_float2(o[n][c][e], o[n][c][2 + e]);
+    }
+  __syncthreads();
+  for (int i = t; i < ROWS * (HD / 4); i += AT_THREADS) {
+    const int r = i / (HD / 4), d = i % (HD / 4) * 4, row = tile * ROWS + r;
+    if (row >= rows) break;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < AT_WARPS; ++w) top = fmaxf(top, s_ml[w][r].x);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < AT_WARPS; ++w) {
+      const float2 ml = s_ml[w][r];
+      const float f = state_weight(ml.x, top);
+      den = fmaf(ml.y, f, den);
+      const float4 v = *reinterpret_cast<const float4*>(&s_o[(w * ROWS + r) * OPITCH + d]);
+      acc[0] = fmaf(v.x, f, acc[0]); acc[1] = fmaf(v.y, f, acc[1]);
+      acc[2] = fmaf(v.z, f, acc[2]); acc[3] = fmaf(v.w, f, acc[3]);
+    }
+    if (a.splits == 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = den == 0.f ? 0.f : acc[j] / den;
+      store_as(a.out, a.out_dtype,
+               ((static_cast<size_t>(b) * a.sl + row / G) * a.heads + kvh * G + row % G) * HD + d, acc);
+    } else {
+      float* out = a.partial + (((static_cast<size_t>(b) * gridDim.y + blockIdx.y) * a.splits + split) * ROWS + r) * (HD + 4);
+      *reinterpret_cast<float4*>(out + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (d == 0) *reinterpret_cast<float2*>(out + HD) = make_float2(top, den);
+    }
+  }
+}
+
+// Joins the position splits: a warp per row.
+template <int HD>
+__global__ void __launch_bounds__(128) kv8_attend_merge_kernel(const AttendArgs a, int tile_rows) {
+  constexpr int N = HD / 32;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int G = a.heads / a.kv_heads, rows = G * a.sl;
+  const int lane = threadIdx.x & 31;
+  const long long i = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (i >= static_cast<long long>(a.bs) * a.kv_heads * rows) return;
+  const int row = static_cast<int>(i % rows), kvh = static_cast<int>(i / rows % a.kv_heads);
+  const int b = static_cast<int>(i / rows / a.kv_heads);
+  const size_t group = (static_cast<size_t>(b) * a.kv_heads + kvh) * a.row_tiles + row / tile_rows;
+  const float* in = a.partial + (group * a.splits * tile_rows + row % tile_rows) * (HD + 4);
+  const size_t step = static_cast<size_t>(tile_rows) * (HD + 4);
+  float top = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, in[s * step + HD]);
+  float acc[N], den = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = state_weight(in[s * step + HD], top);
+    den = fmaf(in[s * step + HD + 1], f, den);
+    float v[N];
+    load_elems(in + s * step + lane * N, v);
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] = fmaf(v[j], f, acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = den == 0.f ? 0.f : acc[j] / den;
+  store_as(a.out, a.out_dtype, ((static_cast<size_t>(b) * a.sl + row / G) * a.heads + kvh * G + row % G) * HD + lane * N,
+           acc);
+}
+
+// Rows of a CTA's tile, and position splits: CTAs for three to four per SM, none shorter
+// than two steps.
+inline int attend_tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
+int attend_splits(int bs, int kv_heads, int rows, int max_seq_len) {
+  const int64_t base = static_cast<int64_t>(bs) * kv_heads * ((rows + attend_tile_rows(rows) - 1) / attend_tile_rows(rows));
+  const int sms = sm_count();
+  int64_t splits = (3 * sms + base - 1) / base;
+  const int64_t most = (static_cast<int64_t>(max_seq_len) + 255) / 256;
+  if (splits > most) splits = most;
+  if (splits > 64) splits = 64;
+  return splits < 1 ? 1 : static_cast<int>(splits);
+}
+
+template <int HD, int CODE, int NT, bool SPLIT>
+int launch_attend(const AttendArgs& a, cudaStream_t st) {
+  constexpr int RING = AT_WARPS * AT_SLOTS * 2 * AT_UNIT * HD, MERGE = AT_WARPS * 8 * NT * (HD + 8) * 4;
+  constexpr int SMEM = RING > MERGE ? RING : MERGE;
+  auto kern = kv8_attend_kernel<HD, CODE, NT, SPLIT>;
+  static bool configured[16] = {};
+  int dev = 0;
+  B200_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev >= 16 || !configured[dev]) {
+    B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    if (dev < 16) configured[dev] = true;
+  }
+  B200_CHECK_CUDA(launch_dependent(kern, dim3(a.splits, a.kv_heads * a.row_tiles, a.bs), dim3(AT_THREADS), SMEM, st, a));
   return B200MOE_OK;
+}
+template <int HD, int CODE>
+int launch_attend_rows(const AttendArgs& a, bool split, int tile_rows, cudaStream_t st) {
+  if (tile_rows == 8) return split ? launch_attend<HD, CODE, 1, true>(a, st) : launch_attend<HD, CODE, 1, false>(a, st);
+  return split ? launch_attend<HD, CODE, 2, true>(a, st) : launch_attend<HD, CODE, 2, false>(a, st);
 }
 
 }  // namespace
@@ -590,8 +975,13 @@ int b200moe_kv8_read(const void* slab, const float* scales, const b200moe_kv8_ca
 
 size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_t bs, int32_t new_tokens,
                                         int32_t heads, int32_t max_seq_len) {
-  if (cache == nullptr || bs <= 0 || new_tokens <= 0 || heads <= 0 || max_seq_len <= 0) return 0;
-  return 16;
+  if (cache == nullptr || bs <= 0 || new_tokens <= 0 || new_tokens > MAX_NEW_TOKENS || heads <= 0 || max_seq_len <= 0 ||
+      cache->kv_heads <= 0 || heads % cache->kv_heads != 0)
+    return 0;
+  const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows);
+  const size_t padded = static_cast<size_t>((rows + tile - 1) / tile) * tile;
+  const int splits = attend_splits(bs, cache->kv_heads, rows, max_seq_len);
+  return static_cast<size_t>(bs) * cache->kv_heads * padded * splits * (cache->head_dim + 4) * sizeof(float);
 }
 
 int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void* slab, const float* scales,
@@ -602,6 +992,7 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   const char* who = "kv8_attend";
   if (const int rc = check_kv8(who, cache, block_index)) return rc;
   B200_REQUIRE(bs >= 0 && bs <= 65535 && pages_per_seq >= 1 && heads >= 1 && max_seq_len >= 1, "%s: bad sizes", who);
+  B200_REQUIRE(static_cast<int64_t>(pages_per_seq) * cache->stride <= 1 << 30, "%s: more than 2^30 positions", who);
   B200_REQUIRE(new_tokens >= 1 && new_tokens <= MAX_NEW_TOKENS, "%s: new_tokens %d (1 to %d)", who, new_tokens,
                MAX_NEW_TOKENS);
   if (bs == 0) return B200MOE_OK;
@@ -619,21 +1010,34 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
     return B200MOE_ERR_WORKSPACE;
   }
   AttendArgs a;
-  a.q = q; a.q_stride = q_stride; a.slab = static_cast<const uint8_t*>(slab); a.scales = scales;
-  a.page_ids = page_ids; a.seq_lens = seq_lens; a.out = out; a.out_dtype = out_dtype; a.bs = bs; a.sl = new_tokens;
+  a.q = q; a.q_stride = q_stride; a.q_dtype = q_dtype; a.slab = static_cast<const uint8_t*>(slab); a.scales = scales;
+  a.page_ids = page_ids; a.seq_lens = seq_lens; a.out = out; a.partial = static_cast<float*>(scratch);
+  a.out_dtype = out_dtype; a.bs = bs; a.sl = new_tokens;
   a.pages_per_seq = pages_per_seq; a.page_count = cache->page_count; a.heads = heads; a.kv_heads = cache->kv_heads;
   a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index; a.scale_block = cache->scale_block;
+  const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows), hd = cache->head_dim;
+  a.row_tiles = (rows + tile - 1) / tile;
+  a.splits = attend_splits(bs, cache->kv_heads, rows, max_seq_len);
+  B200_REQUIRE(static_cast<int64_t>(a.kv_heads) * a.row_tiles <= 65535, "%s: %d heads are too many", who, heads);
   a.scale = scale; a.softcap = softcap;
   a.status = device_status_ptr();
   if (a.status == nullptr) return B200MOE_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool h64 = cache->head_dim == 64;
-  if (q_dtype == B200MOE_DT_F32)
-    return h64 ? launch_attend<float, 64>(a, cache->code, st) : launch_attend<float, 128>(a, cache->code, st);
-  if (q_dtype == B200MOE_DT_F16)
-    return h64 ? launch_attend<__half, 64>(a, cache->code, st) : launch_attend<__half, 128>(a, cache->code, st);
-  return h64 ? launch_attend<__nv_bfloat16, 64>(a, cache->code, st)
-             : launch_attend<__nv_bfloat16, 128>(a, cache->code, st);
+  const bool i8 = cache->code == B200MOE_KV8_INT8;
+  // 32-bit activations: 22 bits of q and of the probabilities
+  const bool split = q_dtype == B200MOE_DT_F32 || out_dtype == B200MOE_DT_F32;
+  int rc;
+  if (hd == 64)
+    rc = i8 ? launch_attend_rows<64, B200MOE_KV8_INT8>(a, split, tile, st)
+            : launch_attend_rows<64, B200MOE_KV8_E4M3>(a, split, tile, st);
+  else
+    rc = i8 ? launch_attend_rows<128, B200MOE_KV8_INT8>(a, split, tile, st)
+            : launch_attend_rows<128, B200MOE_KV8_E4M3>(a, split, tile, st);
+  if (rc || a.splits == 1) return rc;
+  const int64_t ctas = (static_cast<int64_t>(bs) * a.kv_heads * rows + 3) / 4;
+  auto merge = hd == 64 ? kv8_attend_merge_kernel<64> : kv8_attend_merge_kernel<128>;
+  B200_CHECK_CUDA(launch_dependent(merge, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, st, a, tile));
+  return B200MOE_OK;
 }
 
 }  // extern "C"
