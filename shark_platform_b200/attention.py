@@ -106,33 +106,45 @@ class PagedKVCache:
 
 
 # ------------------------------------------------------------- cache operators
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise C.B200MoeError(message)
-
-
+# Called once per layer and token: messages are built only when raised, the device is
+# switched only where it is not the current one.
 def _int32(t: torch.Tensor) -> torch.Tensor:
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _launch(what: str, dev: torch.device, fn, *args) -> None:
+    """fn(*args, stream) with `dev` current, on dev's current stream."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        C.check(rc, what)
 
 
 def _check_cache(cache, state, block_index: int, seq_block_ids: torch.Tensor, bs: int, dev) -> None:
     slab = state[0]
-    _need(0 <= block_index < cache.transformer_block_count, f"block_index {block_index} is not one of the cache's "
-          f"{cache.transformer_block_count} transformer blocks")
-    _need(slab.dim() == 2 and slab.shape[1] == math.prod(cache.sub_page_dims) and slab.is_contiguous(),
-          "the page slab must be contiguous, a row of the cache's page size per page")
+    if not 0 <= block_index < cache.transformer_block_count:
+        raise C.B200MoeError(f"block_index {block_index} is not one of the cache's {cache.transformer_block_count} "
+                             "transformer blocks")
+    if slab.dim() != 2 or slab.shape[1] != cache.page_slab_flat_dim or not slab.is_contiguous():
+        raise C.B200MoeError("the page slab must be contiguous, a row of the cache's page size per page")
     if getattr(cache, "quantized", False):
-        _need(len(state) == 2, "a cache of 8-bit codes is [page slab, scales], as allocate() gives it")
-        _need(slab.dtype == cache.dtype, f"the page slab must be {cache.dtype}, got {slab.dtype}")
+        if len(state) != 2:
+            raise C.B200MoeError("a cache of 8-bit codes is [page slab, scales], as allocate() gives it")
         scales = state[1]
-        _need(scales.dtype == torch.float32 and scales.shape == (slab.shape[0], cache.scale_flat_dim) and
-              scales.is_contiguous() and scales.device == slab.device,
-              "scales must be fp32, contiguous, beside the slab, a row per page")
-    else:
-        _need(slab.dtype in _DT, "the page slab must be a contiguous fp32, fp16 or bf16 tensor")
-    _need(seq_block_ids.dim() == 2 and seq_block_ids.shape[0] == bs and seq_block_ids.shape[1] >= 1,
-          f"seq_block_ids must be [{bs}, pages of a sequence], got {list(seq_block_ids.shape)}")
-    _need(slab.device == dev and seq_block_ids.device == dev, "cache, page ids and activations must be on one device")
+        if slab.dtype is not cache.dtype:
+            raise C.B200MoeError(f"the page slab must be {cache.dtype}, got {slab.dtype}")
+        if (scales.dtype is not torch.float32 or scales.shape != (slab.shape[0], cache.scale_flat_dim) or
+                not scales.is_contiguous() or scales.device != dev):
+            raise C.B200MoeError("scales must be fp32, contiguous, beside the slab, a row per page")
+    elif slab.dtype not in _DT:
+        raise C.B200MoeError("the page slab must be a contiguous fp32, fp16 or bf16 tensor")
+    if seq_block_ids.dim() != 2 or seq_block_ids.shape[0] != bs or seq_block_ids.shape[1] < 1:
+        raise C.B200MoeError(f"seq_block_ids must be [{bs}, pages of a sequence], got {list(seq_block_ids.shape)}")
+    if slab.device != dev or seq_block_ids.device != dev:
+        raise C.B200MoeError("cache, page ids and activations must be on one device")
 
 
 def _kv8_desc(cache, pages: int):
@@ -145,14 +157,11 @@ def _rows(x: torch.Tensor):
     aligned (a view of a fused projection is that already): (tensor, stride)."""
     bs, sl, heads, hd = x.shape
     s = x.stride()
-    per16 = 16 // x.element_size()
-    ok = (s[3] == 1 and (heads == 1 or s[2] == hd) and (bs == 1 or sl == 1 or s[0] == sl * s[1])
-          and x.data_ptr() % 16 == 0)
-    if ok:
+    if s[3] == 1 and (heads == 1 or s[2] == hd) and (bs == 1 or sl == 1 or s[0] == sl * s[1]):
         stride = s[1] if sl > 1 else s[0] if bs > 1 else heads * hd
-        if stride >= heads * hd and stride % per16 == 0:
+        if stride >= heads * hd and stride * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0:
             return x, stride
-    # rows must start on 16 bytes: a contiguous view that does not is copied too
+    # a contiguous view that does not start on 16 bytes is copied too
     return x.clone(memory_format=torch.contiguous_format), heads * hd
 
 
@@ -179,43 +188,44 @@ def norm_rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache:
     infinity or NaN makes its block read as NaN."""
     bs, sl, heads, hd = q.shape
     kvh = cache.attn_head_count
-    _need(q.dtype in _DT and k.dtype == q.dtype and v.dtype == q.dtype,
-          f"q, k and v must be fp32, fp16 or bf16 alike, got {q.dtype}, {k.dtype}, {v.dtype}")
-    _need(hd == cache.attn_head_dim and k.shape == (bs, sl, kvh, hd) and v.shape == k.shape and heads % kvh == 0,
-          f"q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} do not fit a cache of {kvh} heads of "
-          f"{cache.attn_head_dim}")
-    _need(start_positions.shape == (bs,) and (new_lens is None or new_lens.shape == (bs,)),
-          f"start_positions and new_lens are [{bs}]")
-    _need(freqs.dtype == torch.float32 and freqs.shape == (hd // 2,) and freqs.is_contiguous(),
-          f"freqs must be fp32 [{hd // 2}]")
-    for w in (q_norm, k_norm):
-        _need(w is None or (w.dtype == torch.float32 and w.shape == (hd,) and w.is_contiguous()),
-              f"norm weights must be fp32 [{hd}]")
+    dt = q.dtype
+    if dt not in _DT or k.dtype is not dt or v.dtype is not dt:
+        raise C.B200MoeError(f"q, k and v must be fp32, fp16 or bf16 alike, got {dt}, {k.dtype}, {v.dtype}")
+    if hd != cache.attn_head_dim or k.shape != (bs, sl, kvh, hd) or v.shape != k.shape or heads % kvh:
+        raise C.B200MoeError(f"q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} do not fit a cache of {kvh} "
+                             f"heads of {cache.attn_head_dim}")
+    if start_positions.shape != (bs,) or (new_lens is not None and new_lens.shape != (bs,)):
+        raise C.B200MoeError(f"start_positions and new_lens are [{bs}]")
+    if freqs.dtype is not torch.float32 or freqs.shape != (hd // 2,) or not freqs.is_contiguous():
+        raise C.B200MoeError(f"freqs must be fp32 [{hd // 2}]")
     dev = q.device
+    for w in (q_norm, k_norm):
+        if w is not None and (w.dtype is not torch.float32 or w.shape != (hd,) or not w.is_contiguous() or
+                              w.device != dev):
+            raise C.B200MoeError(f"norm weights must be fp32 [{hd}], on q's device")
     _check_cache(cache, cache_state, block_index, seq_block_ids, bs, dev)
+    if (k.device != dev or v.device != dev or start_positions.device != dev or freqs.device != dev or
+            (new_lens is not None and new_lens.device != dev)):
+        raise C.B200MoeError("all arguments must be on one device")
     _moe._require_cuda(q, "q")
-    _need(all(t is None or t.device == dev for t in (k, v, start_positions, new_lens, freqs, q_norm, k_norm)),
-          "all arguments must be on one device")
     (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
-    q_out = torch.empty(bs, sl, heads, hd, dtype=q.dtype, device=dev)
-    k_out = torch.empty(bs, sl, kvh, hd, dtype=q.dtype, device=dev)
+    q_out = torch.empty((bs, sl, heads, hd), dtype=dt, device=dev)
+    k_out = torch.empty((bs, sl, kvh, hd), dtype=dt, device=dev)
     if bs * sl == 0:
         return q_out, k_out
     start, ids = _int32(start_positions), _int32(seq_block_ids)
     lens = None if new_lens is None else _int32(new_lens)
     slab = cache_state[0]
-    head = (_p(q), _p(k), _p(v), _DT[q.dtype], qs, ks, vs, _p(q_norm), _p(k_norm), float(eps), _p(q_out), _p(k_out),
-            _p(slab))
-    tail = (block_index, _p(start), _p(lens), _p(ids), _p(freqs), 1 if use_hf else 0, bs, sl, ids.shape[1], heads)
-    with torch.cuda.device(dev):
-        if cache.quantized:
-            C.check(C.lib.b200moe_attn_norm_rope_kv8_write(
-                *head, _p(cache_state[1]), ctypes.byref(_kv8_desc(cache, slab.shape[0])), *tail, _moe._stream()),
-                "attn_norm_rope_kv8_write")
-        else:
-            desc = C.KvCacheDesc(cache.transformer_block_count, cache.block_seq_stride, kvh, hd, slab.shape[0])
-            C.check(C.lib.b200moe_attn_norm_rope_kv_write(
-                *head, _DT[slab.dtype], ctypes.byref(desc), *tail, _moe._stream()), "attn_norm_rope_kv_write")
+    head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[dt], qs, ks, vs, None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), eps, q_out.data_ptr(), k_out.data_ptr(), slab.data_ptr())
+    tail = (block_index, start.data_ptr(), None if lens is None else lens.data_ptr(), ids.data_ptr(), freqs.data_ptr(),
+            1 if use_hf else 0, bs, sl, ids.shape[1], heads)
+    if getattr(cache, "quantized", False):
+        _launch("attn_norm_rope_kv8_write", dev, C.lib.b200moe_attn_norm_rope_kv8_write, *head, cache_state[1].data_ptr(),
+                _kv8_desc(cache, slab.shape[0]), *tail)
+    else:
+        desc = C.KvCacheDesc(cache.transformer_block_count, cache.block_seq_stride, kvh, hd, slab.shape[0])
+        _launch("attn_norm_rope_kv_write", dev, C.lib.b200moe_attn_norm_rope_kv_write, *head, _DT[slab.dtype], desc, *tail)
     return q_out, k_out
 
 
@@ -225,24 +235,28 @@ def kv_read(cache: PagedKVCache, cache_state: list, *, block_index: int, seq_blo
     """K and V of the listed pages of an 8-bit cache, [bs, max_seq_len, kv_heads, head_dim]
     each (`max_seq_len`: all of the listed pages by default); every value code * scale,
     rounded once to `dtype`.  Rows at and behind seq_lens[b] are zero."""
-    _need(cache.quantized, "kv_read reads caches of 8-bit codes")
-    _need(dtype in _DT, f"K and V are read as fp32, fp16 or bf16, not {dtype}")
-    bs = seq_block_ids.shape[0]
-    dev = cache_state[0].device
-    _need(seq_lens.shape == (bs,) and seq_lens.device == dev, f"seq_lens is [{bs}], on the cache's device")
+    if not getattr(cache, "quantized", False):
+        raise C.B200MoeError("kv_read reads caches of 8-bit codes")
+    if dtype not in _DT:
+        raise C.B200MoeError(f"K and V are read as fp32, fp16 or bf16, not {dtype}")
+    slab = cache_state[0]
+    bs, dev = seq_block_ids.shape[0], slab.device
+    if seq_lens.shape != (bs,) or seq_lens.device != dev:
+        raise C.B200MoeError(f"seq_lens is [{bs}], on the cache's device")
     _check_cache(cache, cache_state, block_index, seq_block_ids, bs, dev)
-    _moe._require_cuda(cache_state[0], "the page slab")
-    n = seq_block_ids.shape[1] * cache.block_seq_stride if max_seq_len is None else int(max_seq_len)
-    _need(0 <= n <= seq_block_ids.shape[1] * cache.block_seq_stride,
-          f"max_seq_len {n} is more than the listed pages hold")
-    k, v = torch.empty(2, bs, n, cache.attn_head_count, cache.attn_head_dim, dtype=dtype, device=dev)
+    _moe._require_cuda(slab, "the page slab")
+    held = seq_block_ids.shape[1] * cache.block_seq_stride
+    n = held if max_seq_len is None else int(max_seq_len)
+    if not 0 <= n <= held:
+        raise C.B200MoeError(f"max_seq_len {n}: the listed pages hold {held} positions")
+    shape = (bs, n, cache.attn_head_count, cache.attn_head_dim)
+    k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
     if bs * n == 0:
         return k, v
     ids, lens = _int32(seq_block_ids), _int32(seq_lens)
-    with torch.cuda.device(dev):
-        C.check(C.lib.b200moe_kv8_read(
-            _p(cache_state[0]), _p(cache_state[1]), ctypes.byref(_kv8_desc(cache, cache_state[0].shape[0])), block_index,
-            _p(ids), _p(lens), bs, ids.shape[1], n, _p(k), _p(v), _DT[dtype], _moe._stream()), "kv8_read")
+    _launch("kv8_read", dev, C.lib.b200moe_kv8_read, slab.data_ptr(), cache_state[1].data_ptr(),
+            _kv8_desc(cache, slab.shape[0]), block_index, ids.data_ptr(), lens.data_ptr(), bs, ids.shape[1], n,
+            k.data_ptr(), v.data_ptr(), _DT[dtype])
     return k, v
 
 
@@ -256,34 +270,40 @@ def kv_attend(q: torch.Tensor, cache: PagedKVCache, cache_state: list, *, block_
     up to and including its own, seq_lens[b] - sl + i; where that leaves none its output is
     zero.  scale: 1 / sqrt(head_dim) by default; softcap: c * tanh(score / c).  Returns
     [bs, sl, heads, head_dim]."""
-    _need(cache.quantized, "kv_attend reads caches of 8-bit codes")
+    if not getattr(cache, "quantized", False):
+        raise C.B200MoeError("kv_attend reads caches of 8-bit codes")
     bs, sl, heads, hd = q.shape
-    out_dtype = q.dtype if out_dtype is None else out_dtype
-    _need(q.dtype in _DT and out_dtype in _DT, f"activations must be fp32, fp16 or bf16, got {q.dtype}, {out_dtype}")
-    _need(hd == cache.attn_head_dim and heads % cache.attn_head_count == 0,
-          f"q {list(q.shape)} does not fit a cache of {cache.attn_head_count} heads of {cache.attn_head_dim}")
-    _need(1 <= sl <= MAX_NEW_TOKENS, f"{sl} new tokens: 1 to {MAX_NEW_TOKENS}; longer stretches attend kv_read's K and V")
-    _need(softcap is None or softcap > 0, "softcap must be positive")
-    dev = q.device
-    _need(seq_lens.shape == (bs,) and seq_lens.device == dev, f"seq_lens is [{bs}], on q's device")
+    dt, dev, slab = q.dtype, q.device, cache_state[0]
+    if out_dtype is None:
+        out_dtype = dt
+    if dt not in _DT or out_dtype not in _DT:
+        raise C.B200MoeError(f"activations must be fp32, fp16 or bf16, got {dt}, {out_dtype}")
+    if hd != cache.attn_head_dim or heads % cache.attn_head_count:
+        raise C.B200MoeError(f"q {list(q.shape)} does not fit a cache of {cache.attn_head_count} heads of "
+                             f"{cache.attn_head_dim}")
+    if not 1 <= sl <= MAX_NEW_TOKENS:
+        raise C.B200MoeError(f"{sl} new tokens: 1 to {MAX_NEW_TOKENS}; longer stretches attend kv_read's K and V")
+    if softcap is not None and not softcap > 0:
+        raise C.B200MoeError("softcap must be positive")
+    if seq_lens.shape != (bs,) or seq_lens.device != dev:
+        raise C.B200MoeError(f"seq_lens is [{bs}], on q's device")
     _check_cache(cache, cache_state, block_index, seq_block_ids, bs, dev)
     _moe._require_cuda(q, "q")
     q, qs = _rows(q)
-    out = torch.empty(bs, sl, heads, hd, dtype=out_dtype, device=dev)
+    out = torch.empty((bs, sl, heads, hd), dtype=out_dtype, device=dev)
     if bs == 0:
         return out
     ids, lens = _int32(seq_block_ids), _int32(seq_lens)
-    max_len = ids.shape[1] * cache.block_seq_stride
-    desc = _kv8_desc(cache, cache_state[0].shape[0])
-    with torch.cuda.device(dev):
-        nbytes = C.lib.b200moe_kv8_attend_scratch_bytes(ctypes.byref(desc), bs, sl, heads, max_len)
-        # per call: other streams and captured graphs have their own
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        C.check(C.lib.b200moe_kv8_attend(
-            _p(q), _DT[q.dtype], qs, _p(cache_state[0]), _p(cache_state[1]), ctypes.byref(desc), block_index, _p(ids),
-            _p(lens), bs, sl, ids.shape[1], heads, max_len, float(1.0 / math.sqrt(hd) if scale is None else scale),
-            0.0 if softcap is None else float(softcap), _p(out), _DT[out_dtype], _p(scratch), nbytes, _moe._stream()),
-            "kv8_attend")
+    per_seq = ids.shape[1]
+    max_len = per_seq * cache.block_seq_stride
+    desc = _kv8_desc(cache, slab.shape[0])
+    nbytes = C.lib.b200moe_kv8_attend_scratch_bytes(desc, bs, sl, heads, max_len)
+    # per call: other streams and captured graphs have their own
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch("kv8_attend", dev, C.lib.b200moe_kv8_attend, q.data_ptr(), _DT[dt], qs, slab.data_ptr(),
+            cache_state[1].data_ptr(), desc, block_index, ids.data_ptr(), lens.data_ptr(), bs, sl, per_seq, heads, max_len,
+            1.0 / math.sqrt(hd) if scale is None else scale, 0.0 if softcap is None else softcap, out.data_ptr(),
+            _DT[out_dtype], scratch.data_ptr(), nbytes)
     return out
 
 
