@@ -441,7 +441,11 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
 //
 // A warp owns units of 32 positions with its own softmax state and its own ring of two
 // slots, filled by 16-byte cp.async; chunks are swizzled so that ldmatrix has no bank
-// conflicts.  Positions are split over CTAs; the merge kernel joins the splits.
+// conflicts.  A step of the CTA is 128 positions.  The steps of all (sequence, kv head, row
+// tile) segments form one list, cut into equal stretches, one for each resident CTA: ragged
+// lengths leave no SM idle, and the cut does not depend on how wide the page table is.  A
+// segment that lies within one stretch is finished there; of the others every CTA leaves a
+// state (at most two: its first and its last segment), which the merge kernel joins.
 struct AttendArgs {
   const void* q;
   int64_t q_stride;
@@ -450,9 +454,10 @@ struct AttendArgs {
   const float* scales;
   const int32_t *page_ids, *seq_lens;
   void* out;
-  float* partial;  // [bs][kv_heads * row tiles][splits][rows of a tile][HD + 2]
+  float* partial;  // [CTA][2: its first, its last segment][rows of a tile][HD + 4]: numerator, max, denominator
   int out_dtype, bs, sl, pages_per_seq, page_count, heads, kv_heads, stride, blocks, block_index, scale_block;
-  int splits, row_tiles;
+  int stride_shift, block_shift;  // log2; -1 where the stride is no power of two
+  int row_tiles, ctas;
   float scale, softcap;
   int32_t* status;
 };
@@ -460,6 +465,7 @@ struct AttendArgs {
 constexpr int AT_THREADS = 128, AT_WARPS = 4;
 constexpr int AT_UNIT = 32;   // positions of a warp's step
 constexpr int AT_SLOTS = 2;
+constexpr int AT_STEP = AT_WARPS * AT_UNIT;
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -508,10 +514,11 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   }
 }
 
-__device__ __forceinline__ float load_one(const void* p, int dtype, int64_t i) {
-  if (dtype == B200MOE_DT_F32) return static_cast<const float*>(p)[i];
-  if (dtype == B200MOE_DT_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+template <int N>
+__device__ __forceinline__ void load_as(const void* p, int dtype, int64_t i, float (&v)[N]) {
+  if (dtype == B200MOE_DT_F32) load_elems(static_cast<const float*>(p) + i, v);
+  else if (dtype == B200MOE_DT_F16) load_elems(static_cast<const __half*>(p) + i, v);
+  else load_elems(static_cast<const __nv_bfloat16*>(p) + i, v);
 }
 
 // Byte offset of 16-byte chunk c of row r in a tile of rows of HD bytes: the eight chunks
@@ -525,294 +532,381 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
 // The sums of several states (max, denominator, numerator) of one row: weights 2^(m - M).
 __device__ __forceinline__ float state_weight(float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); }
 
+// Positions that a sequence's length names, and steps of its segments.
+__device__ __forceinline__ int live_positions(const AttendArgs& a, int b) {
+  const int len = a.seq_lens[b], room = a.pages_per_seq * a.stride;
+  return len < 0 ? 0 : len < room ? len : room;
+}
+__device__ __forceinline__ int steps_of(int len) { return len > AT_STEP ? (len + AT_STEP - 1) / AT_STEP : 1; }
+
+// The list of steps, looked at by a whole warp: all of them, and those of the sequences
+// before `until` or, with until < 0, up to the sequence that holds step `want`.
+struct ListSum { int before, seq; };
+__device__ __forceinline__ ListSum walk_list(const AttendArgs& a, int lane, int until, int want) {
+  const int per_step = a.kv_heads * a.row_tiles, stop = until < 0 ? a.bs : until;
+  int before = 0;
+  for (int b0 = 0; b0 < stop; b0 += 32) {
+    const int b = b0 + lane;
+    const int own = b < stop ? steps_of(live_positions(a, b)) * per_step : 0;
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (until < 0) {
+      const unsigned past = __ballot_sync(0xffffffffu, before + sum > want && own > 0);
+      if (past != 0) {
+        const int at = __ffs(past) - 1;
+        return {before + __shfl_sync(0xffffffffu, sum - own, at), b0 + at};
+      }
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return {before, stop};
+}
+// First step of CTA i's stretch, and the CTA that holds step g.
+__device__ __forceinline__ int stretch_begin(int i, int total, int ctas) {
+  return static_cast<int>(static_cast<long long>(i) * total / ctas);
+}
+__device__ __forceinline__ int cta_of(int g, int total, int ctas) {
+  return static_cast<int>(((static_cast<long long>(g) + 1) * ctas - 1) / total);
+}
+
+// CTAs per SM: shared memory of the ring, registers
+template <int HD, int NT, bool SPLIT>
+constexpr int attend_resident() { return HD == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3); }
+
 template <int HD, int CODE, int NT, bool SPLIT>
-__global__ void __launch_bounds__(AT_THREADS) kv8_attend_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())) kv8_attend_kernel(const AttendArgs a) {
   constexpr int CH = HD / 16;                       // chunks of a row: MMA steps of q.k, row tiles of V^T
   constexpr int PARTS = SPLIT ? 2 : 1;
   constexpr int ROWS = 8 * NT;
   constexpr int TILE = AT_UNIT * HD;                // bytes of a unit's K (or V)
   constexpr int OPITCH = HD + 8;                    // floats
+  constexpr float P_TOP = 7.f, P_SLACK = 8.f;       // P is at most 2^7 when the maximum is taken, 2^15 before it is again
   extern __shared__ __align__(128) uint8_t smem[];  // [warp][slot][K | V], then in place [warp][row][OPITCH] fp32
   __shared__ float4 s_pos[AT_WARPS][AT_UNIT];       // of each position: s_k, log2 s_v, 1 / s_v
   __shared__ float2 s_ml[AT_WARPS][ROWS];
   grid_dep_wait();
   grid_dep_launch();
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gid = lane >> 2, tig = lane & 3;
-  const int split = blockIdx.x, kvh = blockIdx.y / a.row_tiles, tile = blockIdx.y % a.row_tiles, b = blockIdx.z;
   const int G = a.heads / a.kv_heads, rows = G * a.sl;
-  int len = a.seq_lens[b];
-  const long long room = static_cast<long long>(a.pages_per_seq) * a.stride;
-  if (len > room) {
-    if (t == 0) atomicOr(a.status, DEV_ERR_BOUNDS);
-    len = static_cast<int>(room);
-  }
-  // this split's positions, in whole steps of the CTA
-  constexpr int STEP = AT_WARPS * AT_UNIT;
-  const int steps = len > 0 ? (len + STEP - 1) / STEP : 0, per = (steps + a.splits - 1) / a.splits;
-  const int p_begin = split * per * STEP, p_end = min(len, (split + 1) * per * STEP);
-  const int units = p_end > p_begin + warp * AT_UNIT ? (p_end - p_begin - warp * AT_UNIT + STEP - 1) / STEP : 0;
-
-  // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two
-  uint32_t qb[PARTS][NT][CH][2];
-  float fold[NT][2];  // of this lane's accumulator columns 2 tig, 2 tig + 1: back to scores (in halvings, without softcap)
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = tile * ROWS + 8 * n + gid;
-    float x[CH][4], top = 0.f;
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[c][e] = r < rows ? load_one(a.q, a.q_dtype, (static_cast<int64_t>(b) * a.sl + r / G) * a.q_stride +
-                                                          static_cast<int64_t>(kvh * G + r % G) * HD + 16 * c + 4 * tig + e)
-                           : 0.f;
-        top = fmaxf(top, fabsf(x[c][e]));
-      }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^e <= top < 2^(e + 1), so that the largest value lies in [2^14, 2^15)
-    int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-    e = e < -100 || e > 127 ? -100 : e;
-    if (__float_as_uint(top) == 0x7f800000u) e = 100;
-    const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
-    const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23) * a.scale * (a.softcap > 0.f ? 1.f : LOG2E);
-    fold[n][0] = __shfl_sync(0xffffffffu, down, (2 * tig) * 4);
-    fold[n][1] = __shfl_sync(0xffffffffu, down, (2 * tig + 1) * 4);
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float u = x[c][2 * i] * up, v = x[c][2 * i + 1] * up;
-        const __half2 h = __floats2half2_rn(u, v);
-        qb[0][n][c][i] = h2_as_u32(h);
-        if constexpr (SPLIT) {
-          const float2 f = __half22float2(h);
-          qb[PARTS - 1][n][c][i] = h2_as_u32(__floats2half2_rn(u - f.x, v - f.y));
-        }
-      }
-  }
-  // the first position that a column does not see
-  int seen[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) seen[n][j] = len - a.sl + 1 + (tile * ROWS + 8 * n + 2 * tig + j) / G;
-  const int all_see = len - a.sl + 1;
+  const int total = walk_list(a, lane, a.bs, 0).before, ctas = min(a.ctas, total);
+  if (blockIdx.x >= ctas) return;
+  const int g_begin = stretch_begin(blockIdx.x, total, ctas), g_end = stretch_begin(blockIdx.x + 1, total, ctas);
+  ListSum at = walk_list(a, lane, -1, g_begin);
 
   const uint32_t ring = smem_u32(smem) + warp * (AT_SLOTS * 2 * TILE);
-  // the K row of this lane's position of unit u in the slab, in rows of HD bytes; ~0: none
-  auto row_of = [&](int u) -> uint32_t {
-    const int pos = p_begin + u * STEP + warp * AT_UNIT + lane;
-    if (pos >= p_end) return 0xffffffffu;
-    const int slot = pos / a.stride, off = pos - slot * a.stride;
-    const int page = a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot];
-    if (page < 0 || page >= a.page_count) {
-      atomicOr(a.status, DEV_ERR_BOUNDS);
-      return 0xffffffffu;
-    }
-    return ((static_cast<uint32_t>(page) * a.blocks + a.block_index) * a.kv_heads + kvh) * 2u * a.stride + off;
-  };
   const size_t v_off = static_cast<size_t>(a.stride) * HD;
-  // starts the copies of unit u and the load of its scales; one group per call, also past the end
-  auto issue = [&](int u, uint32_t row, float2& sc) {
-    sc = make_float2(0.f, -1.f);
-    if (u < units) {
-      const uint32_t kt = ring + (u % AT_SLOTS) * 2 * TILE;
-      constexpr int RPI = 32 / CH;  // rows of one pass of the warp
-      const int r0 = lane / CH, c = lane % CH;
+  // byte offsets in a tile that this lane addresses with ldmatrix: rows 16 h + (lane & 15), chunks 2 i + (lane >> 4)
+  uint32_t ld_at[CH / 2];
 #pragma unroll
-      for (int i = 0; i < AT_UNIT / RPI; ++i) {
-        const int r = i * RPI + r0;
-        const uint32_t at = __shfl_sync(0xffffffffu, row, r);
-        const bool ok = at != 0xffffffffu;
-        const uint8_t* src = a.slab + static_cast<size_t>(ok ? at : 0u) * HD + c * 16;
-        copy16(kt + tile_at<HD>(r, c), src, ok);
-        copy16(kt + TILE + tile_at<HD>(r, c), src + v_off, ok);
+  for (int i = 0; i < CH / 2; ++i) ld_at[i] = tile_at<HD>(lane & 15, 2 * i + (lane >> 4));
+
+  int seg_first = at.before;  // step of the current sequence's first segment
+  for (int g = g_begin; g < g_end;) {
+    const int b = at.seq, len = live_positions(a, b), steps = steps_of(len);
+    const int seg = (g - seg_first) / steps, kvh = seg / a.row_tiles, tile = seg % a.row_tiles;
+    const int seg_begin = seg_first + seg * steps, seg_end = seg_begin + steps;
+    const int x0 = g - seg_begin, x1 = min(g_end, seg_end) - seg_begin;
+    if (x0 == 0 && t == 0 && a.seq_lens[b] > a.pages_per_seq * a.stride) atomicOr(a.status, DEV_ERR_BOUNDS);
+    const int p_begin = x0 * AT_STEP, p_end = min(len, x1 * AT_STEP);
+    const int units = p_end > p_begin + warp * AT_UNIT ? (p_end - p_begin - warp * AT_UNIT + AT_STEP - 1) / AT_STEP : 0;
+
+    // the K row of this lane's position of unit u in the slab, in rows of HD bytes, ~0: none; and its scale pair
+    auto row_of = [&](int u, uint32_t& pair) -> uint32_t {
+      const int pos = p_begin + u * AT_STEP + warp * AT_UNIT + lane;
+      if (pos >= p_end) return 0xffffffffu;
+      const int slot = a.stride_shift >= 0 ? pos >> a.stride_shift : pos / a.stride, off = pos - slot * a.stride;
+      const int page = a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot];
+      if (page < 0 || page >= a.page_count) {
+        atomicOr(a.status, DEV_ERR_BOUNDS);
+        return 0xffffffffu;
       }
-      if (row != 0xffffffffu) {
-        const uint32_t head = row / (2u * a.stride), off = row % a.stride;
-        sc = reinterpret_cast<const float2*>(a.scales)[static_cast<size_t>(head) * (a.stride / a.scale_block) +
-                                                       off / a.scale_block];
+      const uint32_t head = (static_cast<uint32_t>(page) * a.blocks + a.block_index) * a.kv_heads + kvh;
+      pair = head * static_cast<uint32_t>(a.stride >> a.block_shift) + (off >> a.block_shift);
+      return head * 2u * a.stride + off;
+    };
+    // starts the copies of unit u and the load of its scales; one group per call, also past the end
+    auto issue = [&](int u, uint32_t row, uint32_t pair, float2& sc) {
+      sc = make_float2(0.f, -1.f);
+      if (u < units) {
+        const uint32_t kt = ring + (u % AT_SLOTS) * 2 * TILE;
+        constexpr int RPI = 32 / CH;  // rows of one pass of the warp
+        const int r0 = lane / CH, c = lane % CH;
+#pragma unroll
+        for (int i = 0; i < AT_UNIT / RPI; ++i) {
+          const int r = i * RPI + r0;
+          const uint32_t from = __shfl_sync(0xffffffffu, row, r);
+          const bool ok = from != 0xffffffffu;
+          const uint8_t* src = a.slab + static_cast<size_t>(ok ? from : 0u) * HD + c * 16;
+          copy16(kt + tile_at<HD>(r, c), src, ok);
+          copy16(kt + TILE + tile_at<HD>(r, c), src + v_off, ok);
+        }
+        if (row != 0xffffffffu) sc = reinterpret_cast<const float2*>(a.scales)[pair];
       }
-    }
-    copy_commit();
-  };
+      copy_commit();
+    };
 
-  float m[NT][2], l[NT][2], o[NT][CH][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.f;
-  }
+    // the first copies are on their way while q is fetched
+    float2 sc_now, sc_next;
+    uint32_t pair_next = 0, row_next = row_of(0, pair_next);
+    issue(0, row_next, pair_next, sc_next);
+    row_next = row_of(1, pair_next);
 
-  float2 sc_now, sc_next;
-  issue(0, row_of(0), sc_next);
-  uint32_t row_next = row_of(1);
-  for (int u = 0; u < units; ++u) {
-    sc_now = sc_next;
-    issue(u + 1, row_next, sc_next);
-    row_next = row_of(u + 2);
-    {
-      // dead positions (sc.y < 0: scales are never negative): weight 0 without touching the others
-      const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f);  // 2^-100 in the place of 0
-      const bool dead = sc_now.y < 0.f;
-      const bool bad = sc_now.y != sc_now.y;
-      s_pos[warp][lane] = make_float4(sc_now.x, dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : 1.f / vs, 0.f);
-    }
-    copy_wait<AT_SLOTS - 1>();
-    __syncwarp();
-    const uint32_t kt = ring + (u % AT_SLOTS) * 2 * TILE, vt = kt + TILE;
-    const int p0 = p_begin + u * STEP + warp * AT_UNIT;
-
-    float s[2][NT][4];
+    // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two
+    uint32_t qb[PARTS][NT][CH][2];
+    float fold[NT][2];  // of this lane's accumulator columns 2 tig, 2 tig + 1: back to scores (times log2 e without softcap)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int n = 0; n < NT; ++n) {
+      const int r = tile * ROWS + 8 * n + gid;
+      float x[CH][4], top = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
+      for (int c = 0; c < CH; ++c) {
+        x[c][0] = x[c][1] = x[c][2] = x[c][3] = 0.f;
+        if (r < rows)
+          load_as(a.q, a.q_dtype, (static_cast<int64_t>(b) * a.sl + r / G) * a.q_stride +
+                                      static_cast<int64_t>(kvh * G + r % G) * HD + 16 * c + 4 * tig, x[c]);
+      }
 #pragma unroll
-      for (int c = 0; c < CH; c += 2) {
-        uint32_t w[4];
-        ldsm_x4(kt + tile_at<HD>(16 * h + (lane & 15), c + (lane >> 4)), w);
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[c][e]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^e <= top < 2^(e + 1), so that the largest value lies in [2^14, 2^15)
+      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+      e = e < -100 || e > 127 ? -100 : e;
+      if (__float_as_uint(top) == 0x7f800000u) e = 100;
+      const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
+      const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23) * a.scale * (a.softcap > 0.f ? 1.f : LOG2E);
+      fold[n][0] = __shfl_sync(0xffffffffu, down, (2 * tig) * 4);
+      fold[n][1] = __shfl_sync(0xffffffffu, down, (2 * tig + 1) * 4);
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t a0, a1, a2, a3;
-          widen4<CODE, false>(w[2 * i], a0, a2);
-          widen4<CODE, false>(w[2 * i + 1], a1, a3);
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816(s[h][n], a0, a1, a2, a3, qb[p][n][c + i][0], qb[p][n][c + i][1]);
+          const float u = x[c][2 * i] * up, v = x[c][2 * i + 1] * up;
+          const __half2 h = __floats2half2_rn(u, v);
+          qb[0][n][c][i] = h2_as_u32(h);
+          if constexpr (SPLIT) {
+            const float2 f = __half22float2(h);
+            qb[PARTS - 1][n][c][i] = h2_as_u32(__floats2half2_rn(u - f.x, v - f.y));
+          }
         }
-      }
     }
-    // scores of positions 16 h + 8 j + gid, columns 2 tig + e
-    float top[NT][2];
+    // the first position that a column does not see
+    int seen[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
-    float ivs[2][2];
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int j = 0; j < 2; ++j) seen[n][j] = len - a.sl + 1 + (tile * ROWS + 8 * n + 2 * tig + j) / G;
+    const int all_see = len - a.sl + 1;
+
+    float m[NT][2], l[NT][2], o[NT][CH][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 f = s_pos[warp][16 * h + 8 * j + gid];
-        ivs[h][j] = f.z;
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.f;
+    }
+
+    for (int u = 0; u < units; ++u) {
+      sc_now = sc_next;
+      issue(u + 1, row_next, pair_next, sc_next);
+      row_next = row_of(u + 2, pair_next);
+      {
+        // dead positions (sc.y < 0: scales are never negative): weight 0 without touching the others
+        const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f);  // 2^-100 in the place of 0
+        const bool dead = sc_now.y < 0.f, bad = sc_now.y != sc_now.y;
+        s_pos[warp][lane] =
+            make_float4(sc_now.x, dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : __frcp_rn(vs), 0.f);
+      }
+      copy_wait<AT_SLOTS - 1>();
+      __syncwarp();
+      const uint32_t kt = ring + (u % AT_SLOTS) * 2 * TILE, vt = kt + TILE;
+      const int p0 = p_begin + u * AT_STEP + warp * AT_UNIT;
+
+      // two accumulators for each 16 positions where there are no others to alternate with
+      constexpr int ACC = NT == 1 ? 2 : 1;
+      float s[2][NT][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float acc[ACC][NT][4];
+#pragma unroll
+        for (int k = 0; k < ACC; ++k)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) acc[k][n][0] = acc[k][n][1] = acc[k][n][2] = acc[k][n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; c += 2) {
+          uint32_t w[4];
+          ldsm_x4(kt + ld_at[c / 2] + 16 * h * HD, w);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a0, a1, a2, a3;
+            widen4<CODE, false>(w[2 * i], a0, a2);
+            widen4<CODE, false>(w[2 * i + 1], a1, a3);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                mma_16816(acc[i % ACC][n], a0, a1, a2, a3, qb[p][n][c + i][0], qb[p][n][c + i][1]);
+          }
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = s[h][n][2 * j + e] * (f.x * fold[n][e]);
-            if (a.softcap > 0.f) x = a.softcap * LOG2E * tanhf(x / a.softcap);
-            x += f.y;
-            if (p0 + AT_UNIT > all_see && p0 + 16 * h + 8 * j + gid >= seen[n][e]) x = -INFINITY;
-            s[h][n][2 * j + e] = x;
-            top[n][e] = fmaxf(top[n][e], x);
-          }
+          for (int k = 0; k < 4; ++k) s[h][n][k] = ACC == 2 ? acc[0][n][k] + acc[ACC - 1][n][k] : acc[0][n][k];
       }
-    uint32_t pb[PARTS][NT][2][2];
+      // scores of positions 16 h + 8 j + gid, columns 2 tig + e
+      float top[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float base[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float v = top[n][e];
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-        const float m_new = fmaxf(m[n][e], v);
-        const float safe = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = ex2(m[n][e] - safe);
-        m[n][e] = m_new;
-        l[n][e] *= alpha;
-        base[e] = 15.f - safe;  // the largest P is 2^15
-#pragma unroll
-        for (int c = 0; c < CH; ++c) { o[n][c][e] *= alpha; o[n][c][2 + e] *= alpha; }
-      }
+      for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+      float ivs[2][2];
+      const bool edge = p0 + AT_UNIT > all_see;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float p0v = ex2(s[h][n][2 * j] + base[0]), p1v = ex2(s[h][n][2 * j + 1] + base[1]);
-          l[n][0] = fmaf(p0v, ivs[h][j], l[n][0]);
-          l[n][1] = fmaf(p1v, ivs[h][j], l[n][1]);
-          const __half2 hp = __floats2half2_rn(p0v, p1v);
-          pb[0][n][h][j] = transpose8x8(h2_as_u32(hp));
-          if constexpr (SPLIT) {
-            const float2 f = __half22float2(hp);
-            pb[PARTS - 1][n][h][j] = transpose8x8(h2_as_u32(__floats2half2_rn(p0v - f.x, p1v - f.y)));
+          const float4 f = s_pos[warp][16 * h + 8 * j + gid];
+          ivs[h][j] = f.z;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = s[h][n][2 * j + e] * (f.x * fold[n][e]);
+              if (a.softcap > 0.f) x = a.softcap * LOG2E * tanhf(x / a.softcap);
+              x += f.y;
+              if (edge && p0 + 16 * h + 8 * j + gid >= seen[n][e]) x = -INFINITY;
+              s[h][n][2 * j + e] = x;
+              top[n][e] = fmaxf(top[n][e], x);
+            }
+        }
+      // a column's maximum moves only when P could leave fp16's range
+      bool moves = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float v = top[n][e];
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          top[n][e] = v;
+          moves |= v > m[n][e] + P_SLACK;
+        }
+      if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float m_new = fmaxf(m[n][e], top[n][e]);
+            const float alpha = m_new == -INFINITY ? 1.f : ex2(m[n][e] - m_new);
+            m[n][e] = m_new;
+            l[n][e] *= alpha;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) { o[n][c][e] *= alpha; o[n][c][2 + e] *= alpha; }
+          }
+      }
+      uint32_t pb[PARTS][NT][2][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float base0 = P_TOP - (m[n][0] == -INFINITY ? 0.f : m[n][0]);
+        const float base1 = P_TOP - (m[n][1] == -INFINITY ? 0.f : m[n][1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float u0 = ex2(s[h][n][2 * j] + base0), u1 = ex2(s[h][n][2 * j + 1] + base1);
+            l[n][0] = fmaf(u0, ivs[h][j], l[n][0]);
+            l[n][1] = fmaf(u1, ivs[h][j], l[n][1]);
+            const __half2 hp = __floats2half2_rn(u0, u1);
+            pb[0][n][h][j] = transpose8x8(h2_as_u32(hp));
+            if constexpr (SPLIT) {
+              const float2 f = __half22float2(hp);
+              pb[PARTS - 1][n][h][j] = transpose8x8(h2_as_u32(__floats2half2_rn(u0 - f.x, u1 - f.y)));
+            }
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < CH; c += 2) {
+          uint32_t w[4];
+          ldsm_x4_trans(vt + ld_at[c / 2] + 16 * h * HD, w);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a0, a1, a2, a3;
+            widen4<CODE, true>(w[2 * i], a0, a1);
+            widen4<CODE, true>(w[2 * i + 1], a2, a3);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_16816(o[n][c + i], a0, a1, a2, a3, pb[p][n][h][0], pb[p][n][h][1]);
           }
         }
+      __syncwarp();  // the slot and s_pos are read: the next pass refills them
     }
+    copy_wait<0>();
+    __syncthreads();  // the ring is free
+    // the four warps' states through shared memory
+    float* s_o = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < CH; c += 2) {
-        uint32_t w[4];
-        ldsm_x4_trans(vt + tile_at<HD>(16 * h + (lane & 15), c + (lane >> 4)), w);
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * n + 2 * tig + e;
+        float v = l[n][e];
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        v += __shfl_xor_sync(0xffffffffu, v, 16);
+        if (gid == 0) s_ml[warp][r] = make_float2(m[n][e], v);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t a0, a1, a2, a3;
-          widen4<CODE, true>(w[2 * i], a0, a1);
-          widen4<CODE, true>(w[2 * i + 1], a2, a3);
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816(o[n][c + i], a0, a1, a2, a3, pb[p][n][h][0], pb[p][n][h][1]);
-        }
+        for (int c = 0; c < CH; ++c)
+          *reinterpret_cast<float2*>(&s_o[(warp * ROWS + r) * OPITCH + 16 * c + 2 * gid]) =
+              make_float2(o[n][c][e], o[n][c][2 + e]);
       }
-    __syncwarp();  // the slot and s_pos are read: the next pass refills them
-  }
-  copy_wait<0>();
-  __syncthreads();  // the ring is free
-  // the four warps' states through shared memory
-  float* s_o = reinterpret_cast<float*>(smem);
+    __syncthreads();
+    const bool whole = x0 == 0 && x1 == steps;
+    float* part = a.partial + static_cast<size_t>(blockIdx.x * 2 + (g == g_begin ? 0 : 1)) * ROWS * (HD + 4);
+    for (int i = t; i < ROWS * (HD / 4); i += AT_THREADS) {
+      const int r = i / (HD / 4), d = i % (HD / 4) * 4, row = tile * ROWS + r;
+      if (row >= rows) break;
+      float top = -INFINITY;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+      for (int w = 0; w < AT_WARPS; ++w) top = fmaxf(top, s_ml[w][r].x);
+      float acc[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = 8 * n + 2 * tig + e;
-      float v = l[n][e];
-      v += __shfl_xor_sync(0xffffffffu, v, 4);
-      v += __shfl_xor_sync(0xffffffffu, v, 8);
-      v += __shfl_xor_sync(0xffffffffu, v, 16);
-      if (gid == 0) s_ml[warp][r] = make_float2(m[n][e], v);
+      for (int w = 0; w < AT_WARPS; ++w) {
+        const float2 ml = s_ml[w][r];
+        const float f = state_weight(ml.x, top);
+        den = fmaf(ml.y, f, den);
+        const float4 v = *reinterpret_cast<const float4*>(&s_o[(w * ROWS + r) * OPITCH + d]);
+        acc[0] = fmaf(v.x, f, acc[0]); acc[1] = fmaf(v.y, f, acc[1]);
+        acc[2] = fmaf(v.z, f, acc[2]); acc[3] = fmaf(v.w, f, acc[3]);
+      }
+      if (whole) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-        *reinterpret_cast<float2*>(&s_o[(warp * ROWS + r) * OPITCH + 16 * c + 2 * gid]) =
-            make_float2(o[n][c][e], o[n][c][2 + e]);
+        for (int j = 0; j < 4; ++j) acc[j] = den == 0.f ? 0.f : acc[j] / den;
+        store_as(a.out, a.out_dtype,
+                 ((static_cast<size_t>(b) * a.sl + row / G) * a.heads + kvh * G + row % G) * HD + d, acc);
+      } else {
+        *reinterpret_cast<float4*>(part + r * (HD + 4) + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (d == 0) *reinterpret_cast<float2*>(part + r * (HD + 4) + HD) = make_float2(top, den);
+      }
     }
-  __syncthreads();
-  for (int i = t; i < ROWS * (HD / 4); i += AT_THREADS) {
-    const int r = i / (HD / 4), d = i % (HD / 4) * 4, row = tile * ROWS + r;
-    if (row >= rows) break;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < AT_WARPS; ++w) top = fmaxf(top, s_ml[w][r].x);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
-#pragma unroll
-    for (int w = 0; w < AT_WARPS; ++w) {
-      const float2 ml = s_ml[w][r];
-      const float f = state_weight(ml.x, top);
-      den = fmaf(ml.y, f, den);
-      const float4 v = *reinterpret_cast<const float4*>(&s_o[(w * ROWS + r) * OPITCH + d]);
-      acc[0] = fmaf(v.x, f, acc[0]); acc[1] = fmaf(v.y, f, acc[1]);
-      acc[2] = fmaf(v.z, f, acc[2]); acc[3] = fmaf(v.w, f, acc[3]);
+    g = seg_begin + x1;
+    if (g == seg_first + steps * a.kv_heads * a.row_tiles) {
+      seg_first = g;
+      ++at.seq;
     }
-    if (a.splits == 1) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = den == 0.f ? 0.f : acc[j] / den;
-      store_as(a.out, a.out_dtype,
-               ((static_cast<size_t>(b) * a.sl + row / G) * a.heads + kvh * G + row % G) * HD + d, acc);
-    } else {
-      float* out = a.partial + (((static_cast<size_t>(b) * gridDim.y + blockIdx.y) * a.splits + split) * ROWS + r) * (HD + 4);
-      *reinterpret_cast<float4*>(out + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      if (d == 0) *reinterpret_cast<float2*>(out + HD) = make_float2(top, den);
-    }
+    __syncthreads();  // s_o is read: the next segment's copies may land there
   }
 }
 
-// Joins the position splits: a warp per row.
+// Joins the states of the segments that lie in several CTAs' stretches: a warp per row.
 template <int HD>
 __global__ void __launch_bounds__(128) kv8_attend_merge_kernel(const AttendArgs a, int tile_rows) {
   constexpr int N = HD / 32;
@@ -824,19 +918,32 @@ __global__ void __launch_bounds__(128) kv8_attend_merge_kernel(const AttendArgs 
   if (i >= static_cast<long long>(a.bs) * a.kv_heads * rows) return;
   const int row = static_cast<int>(i % rows), kvh = static_cast<int>(i / rows % a.kv_heads);
   const int b = static_cast<int>(i / rows / a.kv_heads);
-  const size_t group = (static_cast<size_t>(b) * a.kv_heads + kvh) * a.row_tiles + row / tile_rows;
-  const float* in = a.partial + (group * a.splits * tile_rows + row % tile_rows) * (HD + 4);
-  const size_t step = static_cast<size_t>(tile_rows) * (HD + 4);
+  const int total = walk_list(a, lane, a.bs, 0).before, ctas = min(a.ctas, total);
+  const int steps = steps_of(live_positions(a, b));
+  const int g0 = walk_list(a, lane, b, 0).before + (kvh * a.row_tiles + row / tile_rows) * steps;
+  const int first = cta_of(g0, total, ctas), last = cta_of(g0 + steps - 1, total, ctas);
+  if (first == last) return;  // finished by that CTA
+  const size_t pitch = static_cast<size_t>(tile_rows) * (HD + 4);
+  // the first CTA may have begun before this segment: its state is then its second; the others begin inside it
+  const float* in0 = a.partial + (2 * static_cast<size_t>(first) + (stretch_begin(first, total, ctas) < g0 ? 1 : 0)) * pitch +
+                     row % tile_rows * (HD + 4);
+  const float* in1 = a.partial + 2 * static_cast<size_t>(first) * pitch + row % tile_rows * (HD + 4);
+  auto state = [&](int s) { return s == 0 ? in0 : in1 + 2 * s * pitch; };
+  const int n = last - first + 1;
   float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, in[s * step + HD]);
+  for (int s = lane; s < n; s += 32) top = fmaxf(top, state(s)[HD]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   float acc[N], den = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = state_weight(in[s * step + HD], top);
-    den = fmaf(in[s * step + HD + 1], f, den);
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float* in = state(s);
+    const float f = state_weight(in[HD], top);
+    den = fmaf(in[HD + 1], f, den);
     float v[N];
-    load_elems(in + s * step + lane * N, v);
+    load_elems(in + lane * N, v);
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = fmaf(v[j], f, acc[j]);
   }
@@ -846,17 +953,15 @@ __global__ void __launch_bounds__(128) kv8_attend_merge_kernel(const AttendArgs 
            acc);
 }
 
-// Rows of a CTA's tile, and position splits: CTAs for three to four per SM, none shorter
-// than two steps.
+// Rows of a CTA's tile; CTAs of a call: as many as are resident at once, or one for each
+// step of a full page table where those are fewer.
 inline int attend_tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
-int attend_splits(int bs, int kv_heads, int rows, int max_seq_len) {
-  const int64_t base = static_cast<int64_t>(bs) * kv_heads * ((rows + attend_tile_rows(rows) - 1) / attend_tile_rows(rows));
-  const int sms = sm_count();
-  int64_t splits = (3 * sms + base - 1) / base;
-  const int64_t most = (static_cast<int64_t>(max_seq_len) + 255) / 256;
-  if (splits > most) splits = most;
-  if (splits > 64) splits = 64;
-  return splits < 1 ? 1 : static_cast<int>(splits);
+int attend_ctas(int bs, int kv_heads, int hd, int rows, int max_seq_len) {
+  const int tile = attend_tile_rows(rows);
+  const int64_t steps = (static_cast<int64_t>(max_seq_len) + AT_STEP - 1) / AT_STEP * bs * kv_heads * ((rows + tile - 1) / tile);
+  const int64_t resident = static_cast<int64_t>(sm_count()) * (hd == 128 ? (tile == 8 ? attend_resident<128, 1, false>() : attend_resident<128, 2, false>())
+                                                                         : (tile == 8 ? attend_resident<64, 1, false>() : attend_resident<64, 2, false>()));
+  return static_cast<int>(steps < resident ? steps : resident);
 }
 
 template <int HD, int CODE, int NT, bool SPLIT>
@@ -871,7 +976,7 @@ int launch_attend(const AttendArgs& a, cudaStream_t st) {
     B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     if (dev < 16) configured[dev] = true;
   }
-  B200_CHECK_CUDA(launch_dependent(kern, dim3(a.splits, a.kv_heads * a.row_tiles, a.bs), dim3(AT_THREADS), SMEM, st, a));
+  B200_CHECK_CUDA(launch_dependent(kern, dim3(a.ctas), dim3(AT_THREADS), SMEM, st, a));
   return B200MOE_OK;
 }
 template <int HD, int CODE>
@@ -979,9 +1084,8 @@ size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_
       cache->kv_heads <= 0 || heads % cache->kv_heads != 0)
     return 0;
   const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows);
-  const size_t padded = static_cast<size_t>((rows + tile - 1) / tile) * tile;
-  const int splits = attend_splits(bs, cache->kv_heads, rows, max_seq_len);
-  return static_cast<size_t>(bs) * cache->kv_heads * padded * splits * (cache->head_dim + 4) * sizeof(float);
+  const int ctas = attend_ctas(bs, cache->kv_heads, cache->head_dim, rows, max_seq_len);
+  return static_cast<size_t>(ctas) * 2 * tile * (cache->head_dim + 4) * sizeof(float);
 }
 
 int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void* slab, const float* scales,
@@ -1017,8 +1121,14 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index; a.scale_block = cache->scale_block;
   const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows), hd = cache->head_dim;
   a.row_tiles = (rows + tile - 1) / tile;
-  a.splits = attend_splits(bs, cache->kv_heads, rows, max_seq_len);
-  B200_REQUIRE(static_cast<int64_t>(a.kv_heads) * a.row_tiles <= 65535, "%s: %d heads are too many", who, heads);
+  a.ctas = attend_ctas(bs, cache->kv_heads, hd, rows, max_seq_len);
+  a.stride_shift = a.block_shift = -1;
+  for (int i = 0; i < 31; ++i) {
+    if (a.stride == 1 << i) a.stride_shift = i;
+    if (a.scale_block == 1 << i) a.block_shift = i;
+  }
+  B200_REQUIRE(static_cast<double>(bs) * a.kv_heads * a.row_tiles * (1.0 + pages_per_seq * static_cast<double>(a.stride) / AT_STEP) < 2147483647.0,
+               "%s: too many positions for one call", who);
   a.scale = scale; a.softcap = softcap;
   a.status = device_status_ptr();
   if (a.status == nullptr) return B200MOE_ERR_CUDA;
@@ -1033,7 +1143,8 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   else
     rc = i8 ? launch_attend_rows<128, B200MOE_KV8_INT8>(a, split, tile, st)
             : launch_attend_rows<128, B200MOE_KV8_E4M3>(a, split, tile, st);
-  if (rc || a.splits == 1) return rc;
+  if (rc) return rc;
+  if (static_cast<int64_t>(pages_per_seq) * a.stride <= AT_STEP) return B200MOE_OK;  // no segment is longer than a step
   const int64_t ctas = (static_cast<int64_t>(bs) * a.kv_heads * rows + 3) / 4;
   auto merge = hd == 64 ? kv8_attend_merge_kernel<64> : kv8_attend_merge_kernel<128>;
   B200_CHECK_CUDA(launch_dependent(merge, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, st, a, tile));
