@@ -473,6 +473,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -480,6 +485,13 @@ __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// mma_16816 that the compiler may move between the loads of other tiles
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -597,6 +609,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
   const int g_begin = stretch_begin(blockIdx.x, total, ctas), g_end = stretch_begin(blockIdx.x + 1, total, ctas);
   ListSum at = walk_list(a, lane, -1, g_begin);
 
+  // scores in halvings; with a softcap c, c tanh(x / c) = c - 2 c / (2^(2 log2(e) x / c) + 1)
+  const float to_score = a.scale * LOG2E * (a.softcap > 0.f ? 2.f / a.softcap : 1.f), cap2 = a.softcap * LOG2E;
   const uint32_t ring = smem_u32(smem) + warp * (AT_SLOTS * 2 * TILE);
   const size_t v_off = static_cast<size_t>(a.stride) * HD;
   // byte offsets in a tile that this lane addresses with ldmatrix: rows 16 h + (lane & 15), chunks 2 i + (lane >> 4)
@@ -614,50 +628,65 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
     const int p_begin = x0 * AT_STEP, p_end = min(len, x1 * AT_STEP);
     const int units = p_end > p_begin + warp * AT_UNIT ? (p_end - p_begin - warp * AT_UNIT + AT_STEP - 1) / AT_STEP : 0;
 
-    // the K row of this lane's position of unit u in the slab, in rows of HD bytes, ~0: none; and its scale pair
-    auto row_of = [&](int u, uint32_t& pair) -> uint32_t {
+    // the page of this lane's position of unit u, looked at one unit later; -1 behind the stretch
+    auto page_of = [&](int u) -> int {
       const int pos = p_begin + u * AT_STEP + warp * AT_UNIT + lane;
-      if (pos >= p_end) return 0xffffffffu;
-      const int slot = a.stride_shift >= 0 ? pos >> a.stride_shift : pos / a.stride, off = pos - slot * a.stride;
-      const int page = a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot];
-      if (page < 0 || page >= a.page_count) {
-        atomicOr(a.status, DEV_ERR_BOUNDS);
-        return 0xffffffffu;
-      }
-      const uint32_t head = (static_cast<uint32_t>(page) * a.blocks + a.block_index) * a.kv_heads + kvh;
-      pair = head * static_cast<uint32_t>(a.stride >> a.block_shift) + (off >> a.block_shift);
-      return head * 2u * a.stride + off;
+      if (pos >= p_end) return -1;
+      const int slot = a.stride_shift >= 0 ? pos >> a.stride_shift : pos / a.stride;
+      return a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot];
     };
     // starts the copies of unit u and the load of its scales; one group per call, also past the end
-    auto issue = [&](int u, uint32_t row, uint32_t pair, float2& sc) {
+    auto issue = [&](int u, int page, float2& sc) {
       sc = make_float2(0.f, -1.f);
       if (u < units) {
+        const int pos = p_begin + u * AT_STEP + warp * AT_UNIT + lane;
+        const int off = a.stride_shift >= 0 ? pos & (a.stride - 1) : pos % a.stride;
+        // the K row of this lane's position in the slab, in rows of HD bytes; ~0: none
+        uint32_t row = 0xffffffffu;
+        if (pos < p_end) {
+          if (page >= 0 && page < a.page_count) {
+            const uint32_t head = (static_cast<uint32_t>(page) * a.blocks + a.block_index) * a.kv_heads + kvh;
+            row = head * 2u * a.stride + off;
+            sc = reinterpret_cast<const float2*>(a.scales)[static_cast<size_t>(head) * (a.stride >> a.block_shift) +
+                                                           (off >> a.block_shift)];
+          } else {
+            atomicOr(a.status, DEV_ERR_BOUNDS);
+          }
+        }
         const uint32_t kt = ring + (u % AT_SLOTS) * 2 * TILE;
         constexpr int RPI = 32 / CH;  // rows of one pass of the warp
         const int r0 = lane / CH, c = lane % CH;
+        const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0);
+        if (__all_sync(0xffffffffu, row == row0 + lane && row != 0xffffffffu)) {  // within one page
+          const uint8_t* src = a.slab + static_cast<size_t>(row0 + r0) * HD + c * 16;
 #pragma unroll
-        for (int i = 0; i < AT_UNIT / RPI; ++i) {
-          const int r = i * RPI + r0;
-          const uint32_t from = __shfl_sync(0xffffffffu, row, r);
-          const bool ok = from != 0xffffffffu;
-          const uint8_t* src = a.slab + static_cast<size_t>(ok ? from : 0u) * HD + c * 16;
-          copy16(kt + tile_at<HD>(r, c), src, ok);
-          copy16(kt + TILE + tile_at<HD>(r, c), src + v_off, ok);
+          for (int i = 0; i < AT_UNIT / RPI; ++i) {
+            copy16(kt + tile_at<HD>(i * RPI + r0, c), src + i * RPI * HD, true);
+            copy16(kt + TILE + tile_at<HD>(i * RPI + r0, c), src + v_off + i * RPI * HD, true);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < AT_UNIT / RPI; ++i) {
+            const int r = i * RPI + r0;
+            const uint32_t from = __shfl_sync(0xffffffffu, row, r);
+            const bool ok = from != 0xffffffffu;
+            const uint8_t* src = a.slab + static_cast<size_t>(ok ? from : 0u) * HD + c * 16;
+            copy16(kt + tile_at<HD>(r, c), src, ok);
+            copy16(kt + TILE + tile_at<HD>(r, c), src + v_off, ok);
+          }
         }
-        if (row != 0xffffffffu) sc = reinterpret_cast<const float2*>(a.scales)[pair];
       }
       copy_commit();
     };
 
     // the first copies are on their way while q is fetched
     float2 sc_now, sc_next;
-    uint32_t pair_next = 0, row_next = row_of(0, pair_next);
-    issue(0, row_next, pair_next, sc_next);
-    row_next = row_of(1, pair_next);
+    issue(0, page_of(0), sc_next);
+    int page_next = page_of(1);
 
     // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two
     uint32_t qb[PARTS][NT][CH][2];
-    float fold[NT][2];  // of this lane's accumulator columns 2 tig, 2 tig + 1: back to scores (times log2 e without softcap)
+    float fold[NT][2];  // of this lane's accumulator columns 2 tig, 2 tig + 1: back to to_score units
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = tile * ROWS + 8 * n + gid;
@@ -680,7 +709,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
       e = e < -100 || e > 127 ? -100 : e;
       if (__float_as_uint(top) == 0x7f800000u) e = 100;
       const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
-      const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23) * a.scale * (a.softcap > 0.f ? 1.f : LOG2E);
+      const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23) * to_score;
       fold[n][0] = __shfl_sync(0xffffffffu, down, (2 * tig) * 4);
       fold[n][1] = __shfl_sync(0xffffffffu, down, (2 * tig + 1) * 4);
 #pragma unroll
@@ -697,12 +726,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
         }
     }
     // the first position that a column does not see
-    int seen[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) seen[n][j] = len - a.sl + 1 + (tile * ROWS + 8 * n + 2 * tig + j) / G;
     const int all_see = len - a.sl + 1;
+    auto seen = [&](int n, int j) { return all_see + (tile * ROWS + 8 * n + 2 * tig + j) / G; };
 
     float m[NT][2], l[NT][2], o[NT][CH][4];
 #pragma unroll
@@ -715,14 +740,14 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
 
     for (int u = 0; u < units; ++u) {
       sc_now = sc_next;
-      issue(u + 1, row_next, pair_next, sc_next);
-      row_next = row_of(u + 2, pair_next);
+      issue(u + 1, page_next, sc_next);
+      page_next = page_of(u + 2);
       {
         // dead positions (sc.y < 0: scales are never negative): weight 0 without touching the others
         const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f);  // 2^-100 in the place of 0
         const bool dead = sc_now.y < 0.f, bad = sc_now.y != sc_now.y;
         s_pos[warp][lane] =
-            make_float4(sc_now.x, dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : __frcp_rn(vs), 0.f);
+            make_float4(sc_now.x, dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : rcp(vs), 0.f);
       }
       copy_wait<AT_SLOTS - 1>();
       __syncwarp();
@@ -752,7 +777,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
               for (int n = 0; n < NT; ++n)
-                mma_16816(acc[i % ACC][n], a0, a1, a2, a3, qb[p][n][c + i][0], qb[p][n][c + i][1]);
+                mma(acc[i % ACC][n], a0, a1, a2, a3, qb[p][n][c + i][0], qb[p][n][c + i][1]);
           }
         }
 #pragma unroll
@@ -765,7 +790,6 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
 #pragma unroll
       for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
       float ivs[2][2];
-      const bool edge = p0 + AT_UNIT > all_see;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -776,14 +800,28 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x = s[h][n][2 * j + e] * (f.x * fold[n][e]);
-              if (a.softcap > 0.f) x = a.softcap * LOG2E * tanhf(x / a.softcap);
-              x += f.y;
-              if (edge && p0 + 16 * h + 8 * j + gid >= seen[n][e]) x = -INFINITY;
+              const float y = f.x * fold[n][e];
+              float x;
+              if (a.softcap > 0.f) x = fmaf(-2.f * cap2, rcp(ex2(s[h][n][2 * j + e] * y) + 1.f), cap2 + f.y);
+              else x = fmaf(s[h][n][2 * j + e], y, f.y);
               s[h][n][2 * j + e] = x;
-              top[n][e] = fmaxf(top[n][e], x);
             }
         }
+      if (p0 + AT_UNIT > all_see) {  // the last positions: not all of them are seen by all columns
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (p0 + 16 * h + 8 * (k >> 1) + gid >= seen(n, k & 1)) s[h][n][k] = -INFINITY;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top[n][k & 1] = fmaxf(top[n][k & 1], s[h][n][k]);
       // a column's maximum moves only when P could leave fp16's range
       bool moves = false;
 #pragma unroll
@@ -844,7 +882,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_16816(o[n][c + i], a0, a1, a2, a3, pb[p][n][h][0], pb[p][n][h][1]);
+              for (int n = 0; n < NT; ++n) mma(o[n][c + i], a0, a1, a2, a3, pb[p][n][h][0], pb[p][n][h][1]);
           }
         }
       __syncwarp();  // the slot and s_pos are read: the next pass refills them
@@ -906,21 +944,23 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
   }
 }
 
-// Joins the states of the segments that lie in several CTAs' stretches: a warp per row.
+// Joins the states of the segments that lie in several CTAs' stretches: a CTA per row, the
+// states shared out among its warps (up to some fifty for one long sequence: with one warp
+// per row their loads queued up, 22 us instead of 4).
+constexpr int MG_WARPS = 8;
 template <int HD>
-__global__ void __launch_bounds__(128) kv8_attend_merge_kernel(const AttendArgs a, int tile_rows) {
+__global__ void __launch_bounds__(32 * MG_WARPS) kv8_attend_merge_kernel(const AttendArgs a, int tile_rows) {
   constexpr int N = HD / 32;
+  __shared__ float s_o[MG_WARPS][HD];
+  __shared__ float2 s_ml[MG_WARPS];
   grid_dep_wait();
   grid_dep_launch();
   const int G = a.heads / a.kv_heads, rows = G * a.sl;
-  const int lane = threadIdx.x & 31;
-  const long long i = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (i >= static_cast<long long>(a.bs) * a.kv_heads * rows) return;
-  const int row = static_cast<int>(i % rows), kvh = static_cast<int>(i / rows % a.kv_heads);
-  const int b = static_cast<int>(i / rows / a.kv_heads);
-  const int total = walk_list(a, lane, a.bs, 0).before, ctas = min(a.ctas, total);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.x % rows, kvh = blockIdx.x / rows % a.kv_heads, b = blockIdx.x / rows / a.kv_heads;
   const int steps = steps_of(live_positions(a, b));
   const int g0 = walk_list(a, lane, b, 0).before + (kvh * a.row_tiles + row / tile_rows) * steps;
+  const int total = walk_list(a, lane, a.bs, 0).before, ctas = min(a.ctas, total);
   const int first = cta_of(g0, total, ctas), last = cta_of(g0 + steps - 1, total, ctas);
   if (first == last) return;  // finished by that CTA
   const size_t pitch = static_cast<size_t>(tile_rows) * (HD + 4);
@@ -928,29 +968,60 @@ __global__ void __launch_bounds__(128) kv8_attend_merge_kernel(const AttendArgs 
   const float* in0 = a.partial + (2 * static_cast<size_t>(first) + (stretch_begin(first, total, ctas) < g0 ? 1 : 0)) * pitch +
                      row % tile_rows * (HD + 4);
   const float* in1 = a.partial + 2 * static_cast<size_t>(first) * pitch + row % tile_rows * (HD + 4);
-  auto state = [&](int s) { return s == 0 ? in0 : in1 + 2 * s * pitch; };
   const int n = last - first + 1;
-  float top = -INFINITY;
-  for (int s = lane; s < n; s += 32) top = fmaxf(top, state(s)[HD]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float acc[N], den = 0.f;
+  float acc[N], top = -INFINITY, den = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float* in = state(s);
-    const float f = state_weight(in[HD], top);
-    den = fmaf(in[HD + 1], f, den);
-    float v[N];
-    load_elems(in + lane * N, v);
+  for (int s0 = warp; s0 < n; s0 += 4 * MG_WARPS) {
+    float v[4][N];
+    float2 ml[4];
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = fmaf(v[j], f, acc[j]);
+    for (int k = 0; k < 4; ++k) {
+      const int s = s0 + k * MG_WARPS;
+      ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[k][j] = 0.f;
+      if (s < n) {
+        const float* in = s == 0 ? in0 : in1 + 2 * s * pitch;
+        ml[k] = *reinterpret_cast<const float2*>(in + HD);
+        load_elems(in + lane * N, v[k]);
+      }
+    }
+    const float up = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top);
+    const float f0 = state_weight(top, up);
+    den *= f0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] *= f0;
+    top = up;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = state_weight(ml[k].x, top);
+      den = fmaf(ml[k].y, f, den);
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] = fmaf(v[k][j], f, acc[j]);
+    }
   }
 #pragma unroll
-  for (int j = 0; j < N; ++j) acc[j] = den == 0.f ? 0.f : acc[j] / den;
-  store_as(a.out, a.out_dtype, ((static_cast<size_t>(b) * a.sl + row / G) * a.heads + kvh * G + row % G) * HD + lane * N,
-           acc);
+  for (int j = 0; j < N; ++j) s_o[warp][lane * N + j] = acc[j];
+  if (lane == 0) s_ml[warp] = make_float2(top, den);
+  __syncthreads();
+  const int d = threadIdx.x * 2;
+  if (d >= HD) return;
+  top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < MG_WARPS; ++w) top = fmaxf(top, s_ml[w].x);
+  float o[2] = {0.f, 0.f};
+  den = 0.f;
+#pragma unroll
+  for (int w = 0; w < MG_WARPS; ++w) {
+    const float f = state_weight(s_ml[w].x, top);
+    den = fmaf(s_ml[w].y, f, den);
+    o[0] = fmaf(s_o[w][d], f, o[0]);
+    o[1] = fmaf(s_o[w][d + 1], f, o[1]);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) o[j] = den == 0.f ? 0.f : o[j] / den;
+  store_as(a.out, a.out_dtype, ((static_cast<size_t>(b) * a.sl + row / G) * a.heads + kvh * G + row % G) * HD + d, o);
 }
 
 // Rows of a CTA's tile; CTAs of a call: as many as are resident at once, or one for each
@@ -1145,9 +1216,9 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
             : launch_attend_rows<128, B200MOE_KV8_E4M3>(a, split, tile, st);
   if (rc) return rc;
   if (static_cast<int64_t>(pages_per_seq) * a.stride <= AT_STEP) return B200MOE_OK;  // no segment is longer than a step
-  const int64_t ctas = (static_cast<int64_t>(bs) * a.kv_heads * rows + 3) / 4;
+  const int64_t ctas = static_cast<int64_t>(bs) * a.kv_heads * rows;
   auto merge = hd == 64 ? kv8_attend_merge_kernel<64> : kv8_attend_merge_kernel<128>;
-  B200_CHECK_CUDA(launch_dependent(merge, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, st, a, tile));
+  B200_CHECK_CUDA(launch_dependent(merge, dim3(static_cast<unsigned>(ctas)), dim3(32 * MG_WARPS), 0, st, a, tile));
   return B200MOE_OK;
 }
 
