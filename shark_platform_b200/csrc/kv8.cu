@@ -16,10 +16,58 @@ constexpr int MAX_NEW_TOKENS = 16;
 
 inline bool dtype_ok(int dt) { return dt == B200MOE_DT_F32 || dt == B200MOE_DT_F16 || dt == B200MOE_DT_BF16; }
 inline size_t dt_bytes(int dt) { return dt == B200MOE_DT_F32 ? 4 : 2; }
+// log2 of a power of two, -1 of another number
+inline int log2_of(int n) {
+  for (int i = 0; i < 31; ++i)
+    if (n == 1 << i) return i;
+  return -1;
+}
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // ------------------------------------------------------------- rows of 16 or 32 bits
-// N consecutive elements as one load or store.
+// Eight consecutive elements as they lie in memory: one or two 16-byte words.
+template <typename T>
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 4) v[i] = e[i];
+      else if constexpr (std::is_same<T, __half>::value) v[i] = __half2float(e[i]);
+      else v[i] = __bfloat162float(e[i]);
+    }
+  }
+};
+__device__ __forceinline__ uint32_t pack2(const __half*, float a, float b) { return h2_as_u32(__floats2half2_rn(a, b)); }
+__device__ __forceinline__ uint32_t pack2(const __nv_bfloat16*, float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(p, v[0], v[1]), pack2(p, v[2], v[3]), pack2(p, v[4], v[5]), pack2(p, v[6], v[7]));
+  }
+}
+template <typename T>
+__device__ __forceinline__ float round_to(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(__float2half_rn(v));
+  else return __bfloat162float(__float2bfloat16_rn(v));
+}
+// 2 or 4 consecutive elements of a type known at run time
 template <int N>
 __device__ __forceinline__ void load_elems(const float* p, float (&v)[N]) {
   if constexpr (N == 4) {
@@ -46,42 +94,66 @@ __device__ __forceinline__ void load_elems(const __nv_bfloat16* p, float (&v)[N]
     v[i] = f.x; v[i + 1] = f.y;
   }
 }
-__device__ __forceinline__ void store_pair(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
-__device__ __forceinline__ void store_pair(__half* p, float a, float b) {
-  *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b);
-}
-__device__ __forceinline__ void store_pair(__nv_bfloat16* p, float a, float b) {
-  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
-}
-template <int N, typename T>
-__device__ __forceinline__ void store_elems(T* p, const float (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; i += 2) store_pair(p + i, v[i], v[i + 1]);
-}
-template <typename T>
-__device__ __forceinline__ float round_to(float v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(__float2half_rn(v));
-  else return __bfloat162float(__float2bfloat16_rn(v));
-}
 template <int N>
 __device__ __forceinline__ void store_as(void* p, int dtype, size_t i, const float (&v)[N]) {
-  if (dtype == B200MOE_DT_F32) store_elems(static_cast<float*>(p) + i, v);
-  else if (dtype == B200MOE_DT_F16) store_elems(static_cast<__half*>(p) + i, v);
-  else store_elems(static_cast<__nv_bfloat16*>(p) + i, v);
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    if (dtype == B200MOE_DT_F32) *reinterpret_cast<float2*>(static_cast<float*>(p) + i + j) = make_float2(v[j], v[j + 1]);
+    else if (dtype == B200MOE_DT_F16)
+      *reinterpret_cast<__half2*>(static_cast<__half*>(p) + i + j) = __floats2half2_rn(v[j], v[j + 1]);
+    else
+      *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p) + i + j) = __floats2bfloat162_rn(v[j], v[j + 1]);
+  }
 }
 
 // ------------------------------------------------------------------------- codes
-template <int CODE>
-__device__ __forceinline__ float code_to_float(uint8_t c) {
-  if constexpr (CODE == B200MOE_KV8_INT8) return static_cast<float>(static_cast<int8_t>(c));
-  else return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v & 0xffffu), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
 }
-// y = value / scale, at most 2^-10 above qmax: rounds to a code without clamping
+// Four codes as two fp16 pairs, exact: bytes (0, 1), (2, 3), or with PAIRS_APART (0, 2), (1, 3).
+template <int CODE, bool PAIRS_APART>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CODE == B200MOE_KV8_INT8) {
+    // 0x6400 | b is the fp16 number 1024 + b; the byte is biased to unsigned first
+    const uint32_t x = w ^ 0x80808080u;
+    const __half2 bias = u32_as_h2(0x64806480u);
+    lo = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, PAIRS_APART ? 0x4240 : 0x4140)), bias));
+    hi = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, PAIRS_APART ? 0x4341 : 0x4342)), bias));
+  } else {
+    if constexpr (PAIRS_APART) w = __byte_perm(w, 0, 0x3120);
+    lo = e4m3x2_to_h2(w);
+    hi = e4m3x2_to_h2(w >> 16);
+  }
+}
 template <int CODE>
-__device__ __forceinline__ uint8_t float_to_code(float y) {
-  if constexpr (CODE == B200MOE_KV8_INT8) return static_cast<uint8_t>(__float2int_rn(y));
-  else return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ void codes_to_floats(uint2 c, float (&v)[8]) {
+  uint32_t h[4];
+  widen4<CODE, false>(c.x, h[0], h[1]);
+  widen4<CODE, false>(c.y, h[2], h[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(u32_as_h2(h[i]));
+    v[2 * i] = f.x; v[2 * i + 1] = f.y;
+  }
+}
+// v[i] * by, values / scale at most 2^-10 above qmax, to the nearest codes: without clamping
+template <int CODE>
+__device__ __forceinline__ uint2 floats_to_codes(const float (&v)[8], float by) {
+  uint32_t c[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float* x = v + 4 * i;
+    if constexpr (CODE == B200MOE_KV8_INT8) {
+      const int a = __float2int_rn(x[0] * by), b = __float2int_rn(x[1] * by), e = __float2int_rn(x[2] * by),
+                f = __float2int_rn(x[3] * by);
+      c[i] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(e, f, 0x0040), 0x5410);
+    } else {
+      c[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * by, x[1] * by), __NV_SATFINITE, __NV_E4M3) |
+             static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x[2] * by, x[3] * by), __NV_SATFINITE, __NV_E4M3)) << 16;
+    }
+  }
+  return make_uint2(c[0], c[1]);
 }
 
 // ------------------------------------------------------------------------- write
@@ -97,7 +169,7 @@ struct WriteArgs {
   const int32_t *start_positions, *new_lens, *page_ids;
   const float* freqs;
   int order, bs, sl, pages_per_seq, page_count, heads, kv_heads, stride, blocks, block_index, scale_block;
-  int tile, tiles;                    // positions per tile; tiles per sequence
+  int tiles;                          // of a sequence
   int32_t* status;
 };
 
@@ -105,81 +177,96 @@ enum { CACHE_INT8 = B200MOE_KV8_INT8, CACHE_E4M3 = B200MOE_KV8_E4M3, CACHE_PLAIN
 
 constexpr int WR_THREADS = 256;
 constexpr int WR_WARPS = WR_THREADS / 32;
-constexpr int WR_TILE = 64;           // most positions of a tile
 constexpr float QMAX[2] = {127.f, 448.f};
 
-// A lane's N elements of a row, normed and rotated.  cs: the row's cosines and sines.
-template <int HD>
-__device__ __forceinline__ void norm_rotate(float (&x)[HD / 32], const float (&w)[HD / 32], bool norm, float eps,
-                                            const float2* cs, int order, int lane) {
-  constexpr int N = HD / 32;
+// A lane's eight elements of a row, normed and rotated; LPR lanes have a row.  cs: the
+// row's cosines and sines.
+template <int LPR>
+__device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], bool norm, float eps, const float2* cs,
+                                            int order, int c) {
   if (norm) {
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) ss = fmaf(x[i], x[i], ss);
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = 1.0f / sqrtf(ss / HD + eps);
+    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float r = 1.0f / sqrtf(ss / (8 * LPR) + eps);
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = w[i] * (x[i] * r);
+    for (int i = 0; i < 8; ++i) x[i] = w[i] * (x[i] * r);
   }
   if (order == 0) {
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 c = cs[(lane * N + i) / 2];
-      const float re = x[i], im = x[i + 1];
-      x[i] = re * c.x - im * c.y;
-      x[i + 1] = im * c.x + re * c.y;
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = cs[c * 4 + i];
+      const float re = x[2 * i], im = x[2 * i + 1];
+      x[2 * i] = re * t.x - im * t.y;
+      x[2 * i + 1] = im * t.x + re * t.y;
     }
-  } else {  // the other half of the pair is 16 lanes away
-    const float sign = lane < 16 ? -1.f : 1.f;
+  } else {  // the other half of the pair is LPR / 2 lanes away
+    const float sign = c < LPR / 2 ? -1.f : 1.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float2 c = cs[(lane & 15) * N + i];
-      const float other = __shfl_xor_sync(0xffffffffu, x[i], 16);
-      x[i] = x[i] * c.x + sign * other * c.y;
+    for (int i = 0; i < 8; ++i) {
+      const float2 t = cs[(c % (LPR / 2)) * 8 + i];
+      const float other = __shfl_xor_sync(0xffffffffu, x[i], LPR / 2);
+      x[i] = x[i] * t.x + sign * other * t.y;
     }
   }
 }
 
-// One CTA per (sequence, tile of positions, kv head): K and V of the tile and the queries
-// of the heads that share the kv head.  Tiles are aligned in absolute positions, so that a
-// tile holds whole scale blocks.  A warp takes one row at a time, a lane HD / 32
-// consecutive elements of it.
-template <typename T, int HD, int KIND>
+// One CTA per (sequence, tile of TILE positions, kv head): K and V of the tile and the
+// queries of the heads that share the kv head.  Tiles are aligned in absolute positions, so
+// that a tile holds whole scale blocks.  HD / 8 lanes have a row (16-byte loads and stores
+// of 16-bit rows), a warp two or four rows at a time.  K and V stay in registers from their
+// load to their codes: one read of everything.
+template <typename T, int HD, int KIND, int TILE>
 __global__ void __launch_bounds__(WR_THREADS) norm_rope_write_kernel(const WriteArgs a) {
-  constexpr int N = HD / 32;
-  __shared__ float2 s_cs[WR_TILE][HD / 2];
-  __shared__ long long s_row[WR_TILE];     // K row of each position in the slab, in rows of HD elements; -1: not written
-  __shared__ unsigned s_amax[2][WR_TILE];  // of each scale block, as bits
-  __shared__ float s_inv[2][WR_TILE], s_shrink[2];
-  const int b = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles, kvh = blockIdx.y;
+  constexpr int LPR = HD / 8, RPW = 32 / LPR;                 // lanes per row, rows of a warp
+  constexpr int RPP = WR_WARPS * RPW;                         // rows of a pass
+  constexpr int PASSES = (TILE + RPP - 1) / RPP;
+  __shared__ float2 s_cs[TILE][HD / 2];
+  __shared__ long long s_row[TILE];     // K row of each position in the slab, in rows of HD elements; -1: not written
+  __shared__ unsigned s_amax[2][TILE];  // of each scale block, as bits
+  __shared__ float s_inv[2][TILE], s_shrink[2];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads % a.tiles, b = blockIdx.x / a.kv_heads / a.tiles;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int G = a.heads / a.kv_heads, B = a.scale_block, TP = a.tile;
+  const int sub = warp * RPW + lane / LPR, c = lane % LPR;    // row of a pass, chunk of eight elements
+  const int G = a.heads / a.kv_heads, B = a.scale_block;
   const int start_in = a.start_positions[b];
   const long long start = start_in < 0 ? 0 : start_in;
   int count = start_in < 0 ? 0 : a.new_lens != nullptr ? a.new_lens[b] : a.sl;
   count = count < 0 ? 0 : count > a.sl ? a.sl : count;
-  const long long p0 = (start / TP + tile) * TP;  // first position of the tile
+  const long long p0 = (start / TILE + tile) * TILE;  // first position of the tile
   const int lo = static_cast<int>(start > p0 ? start - p0 : 0);
   const long long end = start + a.sl - p0, wend = start + count - p0;
-  const int hi = static_cast<int>(end < TP ? end : TP);     // rows lo .. hi are rotated,
-  const int whi = static_cast<int>(wend < TP ? wend : TP);  // rows lo .. whi written
+  const int hi = static_cast<int>(end < TILE ? end : TILE);     // rows lo .. hi are rotated,
+  const int whi = static_cast<int>(wend < TILE ? wend : TILE);  // rows lo .. whi written
   if (lo >= hi) return;
 
-  for (int i = t; i < (hi - lo) * (HD / 2); i += WR_THREADS) {
-    const int r = lo + i / (HD / 2), j = i % (HD / 2);
-    // the angle in half turns, reduced in 64 bits: exact to 2^-24 at any position
-    const double turns = static_cast<double>(p0 + r) * (static_cast<double>(a.freqs[j]) * 0.31830988618379067154);
-    float sn, cs;
-    sincospif(static_cast<float>(turns - 2.0 * rint(0.5 * turns)), &sn, &cs);
-    s_cs[r][j] = make_float2(cs, sn);
+  // K and V are on their way while the angles are computed
+  const long long tok0 = static_cast<long long>(b) * a.sl + (p0 - start);  // token of row 0
+  const T *q = static_cast<const T*>(a.q), *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v);
+  Raw8<T> kr[PASSES], vr[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = lo + i * RPP + sub;
+    kr[i].zero();
+    vr[i].zero();
+    if (r < hi) kr[i].load(k + (tok0 + r) * a.k_stride + kvh * HD + c * 8);
+    if (r < whi) vr[i].load(v + (tok0 + r) * a.v_stride + kvh * HD + c * 8);
+  }
+  float qw[8], kw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    qw[i] = a.q_norm != nullptr ? a.q_norm[c * 8 + i] : 1.f;
+    kw[i] = a.k_norm != nullptr ? a.k_norm[c * 8 + i] : 1.f;
   }
   const int first = lo - lo % (KIND == CACHE_PLAIN ? 1 : B);  // earlier rows of a continued block included
   for (int r = first + t; r < whi; r += WR_THREADS) {
     const long long pos = p0 + r, slot = pos / a.stride;
     long long row = -1;
-    const int off = static_cast<int>(pos % a.stride);
+    const int off = static_cast<int>(pos - slot * a.stride);
     const long long page = slot < a.pages_per_seq ? a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot] : -1;
     if (page < 0 || page >= a.page_count) {
       atomicOr(a.status, DEV_ERR_BOUNDS);
@@ -190,68 +277,72 @@ __global__ void __launch_bounds__(WR_THREADS) norm_rope_write_kernel(const Write
     }
     s_row[r] = row;
   }
-  for (int i = t; i < 2 * WR_TILE; i += WR_THREADS) (&s_amax[0][0])[i] = 0u;
+  for (int i = t; i < 2 * TILE; i += WR_THREADS) (&s_amax[0][0])[i] = 0u;
+  for (int i = t; i < (hi - lo) * (HD / 2); i += WR_THREADS) {
+    const int r = lo + i / (HD / 2), j = i % (HD / 2);
+    // the angle in half turns, reduced in 64 bits: good to 2^-24 at any position
+    const double turns = static_cast<double>(p0 + r) * (static_cast<double>(a.freqs[j]) * 0.31830988618379067154);
+    float sn, cs;
+    sincospif(static_cast<float>(turns - 2.0 * rint(0.5 * turns)), &sn, &cs);
+    s_cs[r][j] = make_float2(cs, sn);
+  }
   __syncthreads();
 
-  float qw[N], kw[N];
+  float kx[PASSES][8];
+  // all lanes take part in the shuffles of the norm and the rotation; rows outside lo .. hi are zeros, unused
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    qw[i] = a.q_norm != nullptr ? a.q_norm[lane * N + i] : 1.f;
-    kw[i] = a.k_norm != nullptr ? a.k_norm[lane * N + i] : 1.f;
-  }
-  const T *q = static_cast<const T*>(a.q), *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v);
-  const long long tok0 = static_cast<long long>(b) * a.sl + (p0 - start);  // token of row 0
-  auto k_row = [&](int r, float (&x)[N]) {
-    load_elems(k + (tok0 + r) * a.k_stride + kvh * HD + lane * N, x);
-    norm_rotate<HD>(x, kw, a.k_norm != nullptr, a.eps, s_cs[r], a.order, lane);
-  };
-  auto v_row = [&](int r, float (&x)[N]) { load_elems(v + (tok0 + r) * a.v_stride + kvh * HD + lane * N, x); };
-
-  // K: rotated rows; K and V: the largest magnitude of each scale block
-  for (int r = lo + warp; r < hi; r += WR_WARPS) {
-    float x[N];
-    k_row(r, x);
-    if (a.k_out != nullptr)
-      store_elems(static_cast<T*>(a.k_out) + ((tok0 + r) * a.kv_heads + kvh) * HD + lane * N, x);
-    if (r >= whi) continue;
-    float y[N];
-    v_row(r, y);
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = lo + i * RPP + sub;
+    if (lo + i * RPP >= hi) break;
+    kr[i].get(kx[i]);
+    norm_rotate<LPR>(kx[i], kw, a.k_norm != nullptr, a.eps, s_cs[min(r, hi - 1)], a.order, c);
+    if (r < hi && a.k_out != nullptr)
+      store8(static_cast<T*>(a.k_out) + ((tok0 + r) * a.kv_heads + kvh) * HD + c * 8, kx[i]);
     if constexpr (KIND == CACHE_PLAIN) {
-      if (s_row[r] < 0) continue;
+      if (r < whi && s_row[r] >= 0) {
+        float y[8];
+        vr[i].get(y);
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = round_to<T>(x[i]);
-      const size_t at = static_cast<size_t>(s_row[r]) * HD + lane * N;
-      store_as(a.slab, a.cache_dtype, at, x);
-      store_as(a.slab, a.cache_dtype, at + static_cast<size_t>(a.stride) * a.kv_heads * HD, y);
+        for (int j = 0; j < 8; ++j) kx[i][j] = round_to<T>(kx[i][j]);
+        const size_t at = static_cast<size_t>(s_row[r]) * HD + c * 8, v_at = at + static_cast<size_t>(a.stride) * a.kv_heads * HD;
+        if (a.cache_dtype == B200MOE_DT_F32) {
+          store8(static_cast<float*>(a.slab) + at, kx[i]);
+          store8(static_cast<float*>(a.slab) + v_at, y);
+        } else if (a.cache_dtype == B200MOE_DT_F16) {
+          store8(static_cast<__half*>(a.slab) + at, kx[i]);
+          store8(static_cast<__half*>(a.slab) + v_at, y);
+        } else {
+          store8(static_cast<__nv_bfloat16*>(a.slab) + at, kx[i]);
+          store8(static_cast<__nv_bfloat16*>(a.slab) + v_at, y);
+        }
+      }
     } else {
+      // the largest magnitude of the row, then of its scale block; as bits, so that NaN is the largest
+      float y[8];
+      vr[i].get(y);
       unsigned mk = 0, mv = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        mk = max(mk, __float_as_uint(x[i]) & 0x7fffffffu);
-        mv = max(mv, __float_as_uint(y[i]) & 0x7fffffffu);
+      for (int j = 0; j < 8; ++j) {
+        mk = max(mk, __float_as_uint(kx[i][j]) & 0x7fffffffu);
+        mv = max(mv, __float_as_uint(y[j]) & 0x7fffffffu);
       }
-      mk = __reduce_max_sync(0xffffffffu, mk);
-      mv = __reduce_max_sync(0xffffffffu, mv);
-      if (lane == 0) {
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) {
+        mk = max(mk, __shfl_xor_sync(0xffffffffu, mk, o));
+        mv = max(mv, __shfl_xor_sync(0xffffffffu, mv, o));
+      }
+      if (c == 0 && r < whi) {
         atomicMax(&s_amax[0][r / B], mk);
         atomicMax(&s_amax[1][r / B], mv);
       }
     }
-  }
-  // queries
-  for (int i = warp; i < (hi - lo) * G; i += WR_WARPS) {
-    const int r = lo + i / G, h = kvh * G + i % G;
-    float x[N];
-    load_elems(q + (tok0 + r) * a.q_stride + static_cast<long long>(h) * HD + lane * N, x);
-    norm_rotate<HD>(x, qw, a.q_norm != nullptr, a.eps, s_cs[r], a.order, lane);
-    store_elems(static_cast<T*>(a.q_out) + ((tok0 + r) * a.heads + h) * HD + lane * N, x);
   }
   if constexpr (KIND != CACHE_PLAIN) {
     __syncthreads();
     // the scale of each block: a thread for each block and K | V
     constexpr float qmax = QMAX[KIND];
     constexpr float tiny = 7.888609052210118e-31f;  // 2^-100
-    for (int i = t; i < 2 * (TP / B); i += WR_THREADS) {
+    for (int i = t; i < 2 * (TILE / B); i += WR_THREADS) {
       const int blk = i >> 1, kv = i & 1;
       const int r0 = max(blk * B, lo), r1 = min(blk * B + B, whi);
       if (r0 >= r1 || s_row[r0] < 0) continue;
@@ -283,46 +374,60 @@ __global__ void __launch_bounds__(WR_THREADS) norm_rope_write_kernel(const Write
     }
     __syncthreads();
     uint8_t* slab = static_cast<uint8_t*>(a.slab);
-    for (int r = lo + warp; r < whi; r += WR_WARPS) {
-      if (s_row[r] < 0) continue;
-      float x[N];
-      uint8_t* at = slab + static_cast<size_t>(s_row[r]) * HD + lane * N;
-      k_row(r, x);
+    const size_t v_off = static_cast<size_t>(a.stride) * HD;
 #pragma unroll
-      for (int i = 0; i < N; ++i) at[i] = float_to_code<KIND>(x[i] * s_inv[0][r / B]);
-      v_row(r, x);
-      at += static_cast<size_t>(a.stride) * HD;
-#pragma unroll
-      for (int i = 0; i < N; ++i) at[i] = float_to_code<KIND>(x[i] * s_inv[1][r / B]);
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = lo + i * RPP + sub;
+      if (r < whi && s_row[r] >= 0) {
+        uint8_t* at = slab + static_cast<size_t>(s_row[r]) * HD + c * 8;
+        *reinterpret_cast<uint2*>(at) = floats_to_codes<KIND>(kx[i], s_inv[0][r / B]);
+        float y[8];
+        vr[i].get(y);
+        *reinterpret_cast<uint2*>(at + v_off) = floats_to_codes<KIND>(y, s_inv[1][r / B]);
+      }
     }
     // the live rows of a continued block whose scale has grown
     if (first < lo && lo < whi && s_row[lo] >= 0) {
-      for (int i = warp; i < 2 * (lo - first); i += WR_WARPS) {
+      for (int i = sub; i < 2 * (lo - first); i += RPP) {
         const int kv = i & 1, r = first + (i >> 1);
         if (s_shrink[kv] == 1.f) continue;
-        uint8_t* at = slab + static_cast<size_t>(s_row[r] + (kv ? a.stride : 0)) * HD + lane * N;
-#pragma unroll
-        for (int j = 0; j < N; ++j) at[j] = float_to_code<KIND>(code_to_float<KIND>(at[j]) * s_shrink[kv]);
+        uint2* at = reinterpret_cast<uint2*>(slab + static_cast<size_t>(s_row[r]) * HD + (kv ? v_off : 0) + c * 8);
+        float y[8];
+        codes_to_floats<KIND>(*at, y);
+        *at = floats_to_codes<KIND>(y, s_shrink[kv]);
       }
     }
   }
+  // queries: rows (position, head) of the tile
+  const int q_rows = (hi - lo) * G;
+#pragma unroll 2
+  for (int i0 = 0; i0 < q_rows; i0 += RPP) {
+    const int i = min(i0 + sub, q_rows - 1);
+    const int r = lo + i / G, h = kvh * G + i % G;
+    Raw8<T> raw;
+    raw.load(q + (tok0 + r) * a.q_stride + static_cast<long long>(h) * HD + c * 8);
+    float x[8];
+    raw.get(x);
+    norm_rotate<LPR>(x, qw, a.q_norm != nullptr, a.eps, s_cs[r], a.order, c);
+    if (i0 + sub < q_rows) store8(static_cast<T*>(a.q_out) + ((tok0 + r) * a.heads + h) * HD + c * 8, x);
+  }
 }
 
-template <typename T, int HD, int KIND>
-int launch_write(const WriteArgs& a, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(a.bs) * a.tiles, a.kv_heads);
-  norm_rope_write_kernel<T, HD, KIND><<<grid, WR_THREADS, 0, st>>>(a);
-  B200_CHECK_CUDA(cudaGetLastError());
+template <typename T, int HD, int KIND, int TILE>
+int launch_write(WriteArgs& a, cudaStream_t st) {
+  a.tiles = a.sl == 1 ? 1 : (a.sl - 1) / TILE + 2;
+  B200_CHECK_CUDA(launch_dependent(norm_rope_write_kernel<T, HD, KIND, TILE>,
+                                   dim3(static_cast<unsigned>(a.bs) * a.tiles * a.kv_heads), dim3(WR_THREADS), 0, st, a));
   return B200MOE_OK;
 }
 template <typename T, int KIND>
-int launch_write_hd(const WriteArgs& a, int hd, cudaStream_t st) {
-  return hd == 64 ? launch_write<T, 64, KIND>(a, st) : launch_write<T, 128, KIND>(a, st);
+int launch_write_hd(WriteArgs& a, int hd, cudaStream_t st) {
+  if constexpr (KIND != CACHE_PLAIN)
+    if (a.scale_block > 32) return hd == 64 ? launch_write<T, 64, KIND, 64>(a, st) : launch_write<T, 128, KIND, 64>(a, st);
+  return hd == 64 ? launch_write<T, 64, KIND, 32>(a, st) : launch_write<T, 128, KIND, 32>(a, st);
 }
 template <int KIND>
 int launch_write_io(WriteArgs& a, int io_dtype, int hd, cudaStream_t st) {
-  a.tile = KIND == CACHE_PLAIN ? 16 : a.scale_block > 16 ? a.scale_block : 16;
-  a.tiles = a.sl == 1 ? 1 : (a.sl - 1) / a.tile + 2;
   if (io_dtype == B200MOE_DT_F32) return launch_write_hd<float, KIND>(a, hd, st);
   if (io_dtype == B200MOE_DT_F16) return launch_write_hd<__half, KIND>(a, hd, st);
   return launch_write_hd<__nv_bfloat16, KIND>(a, hd, st);
@@ -352,7 +457,7 @@ int check_write(const char* who, const WriteArgs& a, int io_dtype, int hd) {
   B200_REQUIRE(a.k_out != a.k && a.k_out != a.v && a.q_out != a.k && a.q_out != a.v && a.k_out != a.q && a.q_out != a.q &&
                    a.q_out != a.k_out,
                "%s: q_out and k_out must not be inputs", who);
-  const int64_t grid = static_cast<int64_t>(a.bs) * ((a.sl - 1) / 16 + 2);
+  const int64_t grid = static_cast<int64_t>(a.bs) * ((a.sl - 1) / 32 + 2) * a.kv_heads;
   B200_REQUIRE(grid <= 0x7fffffff, "%s: %d sequences of %d tokens are too many for one call", who, a.bs, a.sl);
   return B200MOE_OK;
 }
@@ -379,42 +484,68 @@ struct ReadArgs {
   const float* scales;
   const int32_t *page_ids, *seq_lens;
   void *k_out, *v_out;
-  int out_dtype, bs, pages_per_seq, page_count, max_len, kv_heads, stride, blocks, block_index, scale_block;
+  int bs, pages_per_seq, page_count, max_len, kv_heads, stride, blocks, block_index, block_shift;
   int32_t* status;
 };
 
-// A thread per 16 codes: one 16-byte load, 16 values stored.
-template <int HD, int CODE>
-__global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
-  constexpr int VEC = HD / 16;
-  const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
-  const size_t total = static_cast<size_t>(a.bs) * a.max_len * a.kv_heads * 2 * VEC;
-  if (i >= total) return;
-  // consecutive threads: chunk of the row, position, K | V, head, sequence
-  const int c = static_cast<int>(i % VEC);
-  const int pos = static_cast<int>(i / VEC % a.max_len);
-  const int kv = static_cast<int>(i / VEC / a.max_len % 2);
-  const int h = static_cast<int>(i / VEC / a.max_len / 2 % a.kv_heads);
-  const int b = static_cast<int>(i / VEC / a.max_len / 2 / a.kv_heads);
-  float y[16];
+// One CTA per (sequence, kv head, 64 positions); a thread takes eight codes of a row (eight
+// bytes loaded, 16 stored in 16 bits: both whole sectors), K and V of several rows at once.
+constexpr int RD_THREADS = 256, RD_TILE = 64;
+template <typename T, int HD, int CODE>
+__global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(const ReadArgs a) {
+  constexpr int LPR = HD / 8, RPP = RD_THREADS / LPR, PASSES = RD_TILE / RPP;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int tiles = (a.max_len + RD_TILE - 1) / RD_TILE;
+  const int tile = blockIdx.x % tiles, h = blockIdx.x / tiles % a.kv_heads, b = blockIdx.x / tiles / a.kv_heads;
+  const int sub = threadIdx.x / LPR, c = threadIdx.x % LPR;
+  const int len = a.seq_lens[b];
+  const size_t v_off = static_cast<size_t>(a.stride) * HD;
+  uint2 kc[PASSES], vc[PASSES];
+  float2 sc[PASSES];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) y[j] = 0.f;
-  if (pos < a.seq_lens[b]) {
-    const int slot = pos / a.stride, off = pos % a.stride;
-    const long long page = slot < a.pages_per_seq ? a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot] : -1;
-    if (page < 0 || page >= a.page_count) {
-      atomicOr(a.status, DEV_ERR_BOUNDS);
-    } else {
-      const size_t head = (static_cast<size_t>(page) * a.blocks + a.block_index) * a.kv_heads + h;
-      const uint4 raw = *reinterpret_cast<const uint4*>(a.slab + ((head * 2 + kv) * a.stride + off) * HD + 16 * c);
-      const float s = a.scales[2 * (head * (a.stride / a.scale_block) + off / a.scale_block) + kv];
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-      for (int j = 0; j < 16; ++j) y[j] = code_to_float<CODE>(static_cast<uint8_t>(w[j / 4] >> (8 * (j % 4)))) * s;
+  for (int i = 0; i < PASSES; ++i) {
+    const int pos = tile * RD_TILE + i * RPP + sub;
+    kc[i] = vc[i] = make_uint2(0, 0);
+    sc[i] = make_float2(0.f, 0.f);
+    if (pos < len && pos < a.max_len) {
+      const int slot = pos / a.stride, off = pos - slot * a.stride;
+      const int page = slot < a.pages_per_seq ? a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot] : -1;
+      if (page < 0 || page >= a.page_count) {
+        atomicOr(a.status, DEV_ERR_BOUNDS);
+      } else {
+        const size_t head = (static_cast<size_t>(page) * a.blocks + a.block_index) * a.kv_heads + h;
+        const uint8_t* at = a.slab + (head * 2 * a.stride + off) * HD + c * 8;
+        kc[i] = *reinterpret_cast<const uint2*>(at);
+        vc[i] = *reinterpret_cast<const uint2*>(at + v_off);
+        sc[i] = reinterpret_cast<const float2*>(a.scales)[head * (a.stride >> a.block_shift) + (off >> a.block_shift)];
+      }
     }
   }
-  const size_t at = ((static_cast<size_t>(b) * a.max_len + pos) * a.kv_heads + h) * HD + 16 * c;
-  store_as(kv ? a.v_out : a.k_out, a.out_dtype, at, y);
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int pos = tile * RD_TILE + i * RPP + sub;
+    if (pos >= a.max_len) return;
+    const size_t to = ((static_cast<size_t>(b) * a.max_len + pos) * a.kv_heads + h) * HD + c * 8;
+    const bool live = pos < len;  // a NaN scale shows in live rows only
+    float y[8];
+    codes_to_floats<CODE>(kc[i], y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = live ? y[j] * sc[i].x : 0.f;
+    store8(static_cast<T*>(a.k_out) + to, y);
+    codes_to_floats<CODE>(vc[i], y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = live ? y[j] * sc[i].y : 0.f;
+    store8(static_cast<T*>(a.v_out) + to, y);
+  }
+}
+
+template <typename T, int HD>
+int launch_read(const ReadArgs& a, int code, unsigned grid, cudaStream_t st) {
+  B200_CHECK_CUDA(launch_dependent(code == B200MOE_KV8_INT8 ? kv8_read_kernel<T, HD, B200MOE_KV8_INT8>
+                                                           : kv8_read_kernel<T, HD, B200MOE_KV8_E4M3>,
+                                   dim3(grid), dim3(RD_THREADS), 0, st, a));
+  return B200MOE_OK;
 }
 
 // -------------------------------------------------------------------- attention
@@ -439,8 +570,9 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const ReadArgs a) {
 // rounded is 2^-11 of a value down to 2^-29 of the largest.  SPLIT (32-bit activations):
 // q and P are the sums of two fp16 parts, 2^-22, at twice the MMAs.
 //
-// A warp owns units of 32 positions with its own softmax state and its own ring of two
-// slots, filled by 16-byte cp.async; chunks are swizzled so that ldmatrix has no bank
+// A warp owns units of 32 positions with its own softmax state and places for one unit's K
+// and V, filled by 16-byte cp.async, each again as soon as it is read: no barrier between
+// warps, and four CTAs an SM (with two units' places and three CTAs 51 instead of ... us); chunks are swizzled so that ldmatrix has no bank
 // conflicts.  A step of the CTA is 128 positions.  The steps of all (sequence, kv head, row
 // tile) segments form one list, cut into equal stretches, one for each resident CTA: ragged
 // lengths leave no SM idle, and the cut does not depend on how wide the page table is.  A
@@ -455,7 +587,7 @@ struct AttendArgs {
   const int32_t *page_ids, *seq_lens;
   void* out;
   float* partial;  // [CTA][2: its first, its last segment][rows of a tile][HD + 4]: numerator, max, denominator
-  int out_dtype, bs, sl, pages_per_seq, page_count, heads, kv_heads, stride, blocks, block_index, scale_block;
+  int out_dtype, bs, sl, pages_per_seq, page_count, heads, kv_heads, stride, blocks, block_index;
   int stride_shift, block_shift;  // log2; -1 where the stride is no power of two
   int row_tiles, ctas;
   float scale, softcap;
@@ -464,7 +596,6 @@ struct AttendArgs {
 
 constexpr int AT_THREADS = 128, AT_WARPS = 4;
 constexpr int AT_UNIT = 32;   // positions of a warp's step
-constexpr int AT_SLOTS = 2;
 constexpr int AT_STEP = AT_WARPS * AT_UNIT;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -506,26 +637,6 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v & 0xffffu), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
-}
-// Four codes as two fp16 pairs: bytes (0, 1), (2, 3), or with PAIRS_APART (0, 2), (1, 3).
-template <int CODE, bool PAIRS_APART>
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (CODE == B200MOE_KV8_INT8) {
-    // 0x6400 | b is the fp16 number 1024 + b; the byte is biased to unsigned first
-    const uint32_t x = w ^ 0x80808080u;
-    const __half2 bias = u32_as_h2(0x64806480u);
-    lo = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, PAIRS_APART ? 0x4240 : 0x4140)), bias));
-    hi = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, PAIRS_APART ? 0x4341 : 0x4342)), bias));
-  } else {
-    if constexpr (PAIRS_APART) w = __byte_perm(w, 0, 0x3120);
-    lo = e4m3x2_to_h2(w);
-    hi = e4m3x2_to_h2(w >> 16);
-  }
-}
-
 template <int N>
 __device__ __forceinline__ void load_as(const void* p, int dtype, int64_t i, float (&v)[N]) {
   if (dtype == B200MOE_DT_F32) load_elems(static_cast<const float*>(p) + i, v);
@@ -551,15 +662,21 @@ __device__ __forceinline__ int live_positions(const AttendArgs& a, int b) {
 }
 __device__ __forceinline__ int steps_of(int len) { return len > AT_STEP ? (len + AT_STEP - 1) / AT_STEP : 1; }
 
-// The list of steps, looked at by a whole warp: all of them, and those of the sequences
-// before `until` or, with until < 0, up to the sequence that holds step `want`.
+// Joining a segment in the middle of a stretch (the barrier and the output of the last one,
+// q) takes a CTA as long as three steps (7 us): in long stretches a segment counts
+// START_STEPS more than it has, so that the CTAs that join one get fewer.
+constexpr int START_STEPS = 3;
+__device__ __forceinline__ int start_steps(int steps, int ctas) { return steps >= 4 * ctas ? START_STEPS : 0; }
+
+// The list of steps, looked at by a whole warp: those of the sequences before `until` or,
+// with until < 0, before the sequence that holds step `want`; each segment with `start` more.
 struct ListSum { int before, seq; };
-__device__ __forceinline__ ListSum walk_list(const AttendArgs& a, int lane, int until, int want) {
+__device__ __forceinline__ ListSum walk_list(const AttendArgs& a, int lane, int until, int want, int start) {
   const int per_step = a.kv_heads * a.row_tiles, stop = until < 0 ? a.bs : until;
   int before = 0;
   for (int b0 = 0; b0 < stop; b0 += 32) {
     const int b = b0 + lane;
-    const int own = b < stop ? steps_of(live_positions(a, b)) * per_step : 0;
+    const int own = b < stop ? (start + steps_of(live_positions(a, b))) * per_step : 0;
     int sum = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -577,17 +694,21 @@ __device__ __forceinline__ ListSum walk_list(const AttendArgs& a, int lane, int 
   }
   return {before, stop};
 }
-// First step of CTA i's stretch, and the CTA that holds step g.
-__device__ __forceinline__ int stretch_begin(int i, int total, int ctas) {
-  return static_cast<int>(static_cast<long long>(i) * total / ctas);
-}
-__device__ __forceinline__ int cta_of(int g, int total, int ctas) {
-  return static_cast<int>(((static_cast<long long>(g) + 1) * ctas - 1) / total);
-}
+// First step of CTA i's stretch, and the CTA that holds step g: the first total % ctas
+// stretches are one step longer than the others.
+struct Stretches {
+  int each, longer;
+  __device__ Stretches(int total, int ctas) : each(total / ctas), longer(total - each * ctas) {}
+  __device__ int begin(int i) const { return i * each + min(i, longer); }
+  __device__ int cta_of(int g) const {
+    const int cut = longer * (each + 1);
+    return g < cut ? g / (each + 1) : longer + (g - cut) / each;
+  }
+};
 
 // CTAs per SM: shared memory of the ring, registers
 template <int HD, int NT, bool SPLIT>
-constexpr int attend_resident() { return HD == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3); }
+constexpr int attend_resident() { return HD == 128 ? (NT == 1 ? (SPLIT ? 3 : 4) : (SPLIT ? 2 : 3)) : (NT == 1 ? 5 : 4); }
 
 template <int HD, int CODE, int NT, bool SPLIT>
 __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())) kv8_attend_kernel(const AttendArgs a) {
@@ -597,92 +718,122 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
   constexpr int TILE = AT_UNIT * HD;                // bytes of a unit's K (or V)
   constexpr int OPITCH = HD + 8;                    // floats
   constexpr float P_TOP = 7.f, P_SLACK = 8.f;       // P is at most 2^7 when the maximum is taken, 2^15 before it is again
-  extern __shared__ __align__(128) uint8_t smem[];  // [warp][slot][K | V], then in place [warp][row][OPITCH] fp32
+  extern __shared__ __align__(128) uint8_t smem[];  // [warp][K | V], then [warp][row][OPITCH] fp32
+  float* s_o = reinterpret_cast<float*>(smem + AT_WARPS * 2 * TILE);
   __shared__ float4 s_pos[AT_WARPS][AT_UNIT];       // of each position: s_k, log2 s_v, 1 / s_v
   __shared__ float2 s_ml[AT_WARPS][ROWS];
   grid_dep_wait();
   grid_dep_launch();
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gid = lane >> 2, tig = lane & 3;
   const int G = a.heads / a.kv_heads, rows = G * a.sl;
-  const int total = walk_list(a, lane, a.bs, 0).before, ctas = min(a.ctas, total);
+  const int real = walk_list(a, lane, a.bs, 0, 0).before, start = start_steps(real, a.ctas);
+  const int total = real + start * a.bs * a.kv_heads * a.row_tiles, ctas = min(a.ctas, total);
   if (blockIdx.x >= ctas) return;
-  const int g_begin = stretch_begin(blockIdx.x, total, ctas), g_end = stretch_begin(blockIdx.x + 1, total, ctas);
-  ListSum at = walk_list(a, lane, -1, g_begin);
+  const Stretches cut(total, ctas);
+  const int g_begin = cut.begin(blockIdx.x), g_end = cut.begin(blockIdx.x + 1);
+  const ListSum at = walk_list(a, lane, -1, g_begin, start);
 
   // scores in halvings; with a softcap c, c tanh(x / c) = c - 2 c / (2^(2 log2(e) x / c) + 1)
   const float to_score = a.scale * LOG2E * (a.softcap > 0.f ? 2.f / a.softcap : 1.f), cap2 = a.softcap * LOG2E;
-  const uint32_t ring = smem_u32(smem) + warp * (AT_SLOTS * 2 * TILE);
+  const uint32_t ring = smem_u32(smem) + warp * (2 * TILE);
   const size_t v_off = static_cast<size_t>(a.stride) * HD;
   // byte offsets in a tile that this lane addresses with ldmatrix: rows 16 h + (lane & 15), chunks 2 i + (lane >> 4)
   uint32_t ld_at[CH / 2];
 #pragma unroll
   for (int i = 0; i < CH / 2; ++i) ld_at[i] = tile_at<HD>(lane & 15, 2 * i + (lane >> 4));
 
-  int seg_first = at.before;  // step of the current sequence's first segment
-  for (int g = g_begin; g < g_end;) {
-    const int b = at.seq, len = live_positions(a, b), steps = steps_of(len);
-    const int seg = (g - seg_first) / steps, kvh = seg / a.row_tiles, tile = seg % a.row_tiles;
-    const int seg_begin = seg_first + seg * steps, seg_end = seg_begin + steps;
-    const int x0 = g - seg_begin, x1 = min(g_end, seg_end) - seg_begin;
-    if (x0 == 0 && t == 0 && a.seq_lens[b] > a.pages_per_seq * a.stride) atomicOr(a.status, DEV_ERR_BOUNDS);
-    const int p_begin = x0 * AT_STEP, p_end = min(len, x1 * AT_STEP);
-    const int units = p_end > p_begin + warp * AT_UNIT ? (p_end - p_begin - warp * AT_UNIT + AT_STEP - 1) / AT_STEP : 0;
-
-    // the page of this lane's position of unit u, looked at one unit later; -1 behind the stretch
-    auto page_of = [&](int u) -> int {
-      const int pos = p_begin + u * AT_STEP + warp * AT_UNIT + lane;
-      if (pos >= p_end) return -1;
-      const int slot = a.stride_shift >= 0 ? pos >> a.stride_shift : pos / a.stride;
-      return a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot];
-    };
-    // starts the copies of unit u and the load of its scales; one group per call, also past the end
-    auto issue = [&](int u, int page, float2& sc) {
-      sc = make_float2(0.f, -1.f);
-      if (u < units) {
-        const int pos = p_begin + u * AT_STEP + warp * AT_UNIT + lane;
-        const int off = a.stride_shift >= 0 ? pos & (a.stride - 1) : pos % a.stride;
-        // the K row of this lane's position in the slab, in rows of HD bytes; ~0: none
-        uint32_t row = 0xffffffffu;
-        if (pos < p_end) {
-          if (page >= 0 && page < a.page_count) {
-            const uint32_t head = (static_cast<uint32_t>(page) * a.blocks + a.block_index) * a.kv_heads + kvh;
-            row = head * 2u * a.stride + off;
-            sc = reinterpret_cast<const float2*>(a.scales)[static_cast<size_t>(head) * (a.stride >> a.block_shift) +
-                                                           (off >> a.block_shift)];
-          } else {
-            atomicOr(a.status, DEV_ERR_BOUNDS);
-          }
-        }
-        const uint32_t kt = ring + (u % AT_SLOTS) * 2 * TILE;
-        constexpr int RPI = 32 / CH;  // rows of one pass of the warp
-        const int r0 = lane / CH, c = lane % CH;
-        const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0);
-        if (__all_sync(0xffffffffu, row == row0 + lane && row != 0xffffffffu)) {  // within one page
-          const uint8_t* src = a.slab + static_cast<size_t>(row0 + r0) * HD + c * 16;
+  // what of a segment lies in this stretch, and the warp's units of it
+  struct Piece { int b, kvh, tile, len, x0, x1, steps, end, p_begin, p_end, units; };
+  int seq_first = at.before, seq = at.seq;  // the current sequence and the first of its steps
+  auto piece_at = [&](int g) {
+    Piece p;
+    p.len = live_positions(a, seq);
+    p.steps = steps_of(p.len);
+    while (g - seq_first >= (start + p.steps) * a.kv_heads * a.row_tiles) {  // at most once: g is a step of this or the next
+      seq_first += (start + p.steps) * a.kv_heads * a.row_tiles;
+      p.len = live_positions(a, ++seq);
+      p.steps = steps_of(p.len);
+    }
+    const int seg = (g - seq_first) / (start + p.steps), x = g - seq_first - seg * (start + p.steps);
+    p.b = seq;
+    p.kvh = seg / a.row_tiles;
+    p.tile = seg - p.kvh * a.row_tiles;
+    p.end = min(g + start + p.steps - x, g_end);
+    p.x0 = max(0, x - start);
+    p.x1 = max(0, x + p.end - g - start);  // 0: no step of it
+    p.p_begin = p.x0 * AT_STEP + warp * AT_UNIT;
+    p.p_end = min(p.len, p.x1 * AT_STEP);
+    p.units = p.p_end > p.p_begin ? (p.p_end - p.p_begin + AT_STEP - 1) / AT_STEP : 0;
+    return p;
+  };
+  // the page of this lane's position of unit u, looked at one unit later; -1 behind the stretch
+  auto page_of = [&](const Piece& p, int u) -> int {
+    const int pos = p.p_begin + u * AT_STEP + lane;
+    if (pos >= p.p_end) return -1;
+    const int slot = a.stride_shift >= 0 ? pos >> a.stride_shift : pos / a.stride;
+    return a.page_ids[static_cast<size_t>(p.b) * a.pages_per_seq + slot];
+  };
+  // of unit u: this lane's K row in the slab, in rows of HD bytes (~0: none), and its scales
+  auto locate = [&](const Piece& p, int u, int page, float2& sc) -> uint32_t {
+    sc = make_float2(0.f, -1.f);
+    const int pos = p.p_begin + u * AT_STEP + lane;
+    if (pos >= p.p_end) return 0xffffffffu;
+    if (page < 0 || page >= a.page_count) {
+      atomicOr(a.status, DEV_ERR_BOUNDS);
+      return 0xffffffffu;
+    }
+    const int off = a.stride_shift >= 0 ? pos & (a.stride - 1) : pos % a.stride;
+    const uint32_t head = (static_cast<uint32_t>(page) * a.blocks + a.block_index) * a.kv_heads + p.kvh;
+    sc = reinterpret_cast<const float2*>(a.scales)[static_cast<size_t>(head) * (a.stride >> a.block_shift) +
+                                                   (off >> a.block_shift)];
+    return head * 2u * a.stride + off;
+  };
+  // starts the copies of a unit's K or V rows (zeros in the place of missing ones); one group per call, also without a unit
+  auto issue = [&](bool unit, uint32_t row, int kv) {
+    if (unit) {
+      const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0);
+      const uint32_t to = ring + kv * TILE;
+      constexpr int RPI = 32 / CH;  // rows of one pass of the warp
+      const int r0 = lane / CH, c = lane % CH;
+      const uint8_t* from = a.slab + (kv ? v_off : 0) + c * 16;
+      if (__all_sync(0xffffffffu, row == row0 + lane && row != 0xffffffffu)) {  // within one page
+        from += static_cast<size_t>(row0 + r0) * HD;
 #pragma unroll
-          for (int i = 0; i < AT_UNIT / RPI; ++i) {
-            copy16(kt + tile_at<HD>(i * RPI + r0, c), src + i * RPI * HD, true);
-            copy16(kt + TILE + tile_at<HD>(i * RPI + r0, c), src + v_off + i * RPI * HD, true);
-          }
-        } else {
+        for (int i = 0; i < AT_UNIT / RPI; ++i) copy16(to + tile_at<HD>(i * RPI + r0, c), from + i * RPI * HD, true);
+      } else {
 #pragma unroll
-          for (int i = 0; i < AT_UNIT / RPI; ++i) {
-            const int r = i * RPI + r0;
-            const uint32_t from = __shfl_sync(0xffffffffu, row, r);
-            const bool ok = from != 0xffffffffu;
-            const uint8_t* src = a.slab + static_cast<size_t>(ok ? from : 0u) * HD + c * 16;
-            copy16(kt + tile_at<HD>(r, c), src, ok);
-            copy16(kt + TILE + tile_at<HD>(r, c), src + v_off, ok);
-          }
+        for (int i = 0; i < AT_UNIT / RPI; ++i) {
+          const int r = i * RPI + r0;
+          const uint32_t at_row = __shfl_sync(0xffffffffu, row, r);
+          const bool ok = at_row != 0xffffffffu;
+          copy16(to + tile_at<HD>(r, c), from + static_cast<size_t>(ok ? at_row : 0u) * HD, ok);
         }
       }
-      copy_commit();
-    };
+    }
+    copy_commit();
+  };
 
-    // the first copies are on their way while q is fetched
-    float2 sc_now, sc_next;
-    issue(0, page_of(0), sc_next);
-    int page_next = page_of(1);
+  // The copies of a unit are started as soon as the places of the one before are read, those
+  // of the next segment's first unit during this segment's last (6 us of waiting otherwise).
+  Piece next = piece_at(g_begin);
+  float2 sc_now, sc_next;
+  {
+    const uint32_t row = locate(next, 0, page_of(next, 0), sc_next);
+    issue(next.units > 0, row, 0);
+    issue(next.units > 0, row, 1);
+  }
+  for (int g = g_begin; g < g_end;) {
+    const Piece cur = next;
+    if (cur.x1 == 0) break;  // the stretch ends before the segment's first step
+    const int b = cur.b, kvh = cur.kvh, tile = cur.tile, len = cur.len, units = cur.units;
+    if (cur.x0 == 0 && t == 0 && a.seq_lens[b] > a.pages_per_seq * a.stride) atomicOr(a.status, DEV_ERR_BOUNDS);
+    int page_next = page_of(cur, 1), page_after = -1;
+    if (cur.end < g_end) {
+      next = piece_at(cur.end);
+      page_after = page_of(next, 0);
+    } else {
+      next.p_end = next.units = 0;
+    }
 
     // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two
     uint32_t qb[PARTS][NT][CH][2];
@@ -740,8 +891,6 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
 
     for (int u = 0; u < units; ++u) {
       sc_now = sc_next;
-      issue(u + 1, page_next, sc_next);
-      page_next = page_of(u + 2);
       {
         // dead positions (sc.y < 0: scales are never negative): weight 0 without touching the others
         const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f);  // 2^-100 in the place of 0
@@ -749,10 +898,10 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
         s_pos[warp][lane] =
             make_float4(sc_now.x, dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : rcp(vs), 0.f);
       }
-      copy_wait<AT_SLOTS - 1>();
+      copy_wait<1>();  // all but V of this unit
       __syncwarp();
-      const uint32_t kt = ring + (u % AT_SLOTS) * 2 * TILE, vt = kt + TILE;
-      const int p0 = p_begin + u * AT_STEP + warp * AT_UNIT;
+      const uint32_t kt = ring, vt = kt + TILE;
+      const int p0 = cur.p_begin + u * AT_STEP;
 
       // two accumulators for each 16 positions where there are no others to alternate with
       constexpr int ACC = NT == 1 ? 2 : 1;
@@ -785,6 +934,13 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
 #pragma unroll
           for (int k = 0; k < 4; ++k) s[h][n][k] = ACC == 2 ? acc[0][n][k] + acc[ACC - 1][n][k] : acc[0][n][k];
       }
+      __syncwarp();  // K is read: its place takes that of the next unit
+      const bool last = u + 1 == units;
+      const uint32_t row_next = locate(last ? next : cur, last ? 0 : u + 1, last ? page_after : page_next, sc_next);
+      page_next = page_of(cur, u + 2);
+      const bool unit_next = !last || next.units > 0;
+      issue(unit_next, row_next, 0);
+
       // scores of positions 16 h + 8 j + gid, columns 2 tig + e
       float top[NT][2];
 #pragma unroll
@@ -868,6 +1024,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
             }
           }
       }
+      copy_wait<1>();
+      __syncwarp();
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -885,12 +1043,16 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
               for (int n = 0; n < NT; ++n) mma(o[n][c + i], a0, a1, a2, a3, pb[p][n][h][0], pb[p][n][h][1]);
           }
         }
-      __syncwarp();  // the slot and s_pos are read: the next pass refills them
+      __syncwarp();  // V and s_pos are read
+      issue(unit_next, row_next, 1);
     }
-    copy_wait<0>();
-    __syncthreads();  // the ring is free
+    if (units == 0) {  // nothing of this segment for the warp: the next one's copies are started here
+      const uint32_t row = locate(next, 0, page_after, sc_next);
+      issue(next.units > 0, row, 0);
+      issue(next.units > 0, row, 1);
+    }
     // the four warps' states through shared memory
-    float* s_o = reinterpret_cast<float*>(smem);
+    __syncthreads();  // the last segment's are read
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -907,7 +1069,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
               make_float2(o[n][c][e], o[n][c][2 + e]);
       }
     __syncthreads();
-    const bool whole = x0 == 0 && x1 == steps;
+    const bool whole = cur.x0 == 0 && cur.x1 == cur.steps;
     float* part = a.partial + static_cast<size_t>(blockIdx.x * 2 + (g == g_begin ? 0 : 1)) * ROWS * (HD + 4);
     for (int i = t; i < ROWS * (HD / 4); i += AT_THREADS) {
       const int r = i / (HD / 4), d = i % (HD / 4) * 4, row = tile * ROWS + r;
@@ -935,49 +1097,59 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
         if (d == 0) *reinterpret_cast<float2*>(part + r * (HD + 4) + HD) = make_float2(top, den);
       }
     }
-    g = seg_begin + x1;
-    if (g == seg_first + steps * a.kv_heads * a.row_tiles) {
-      seg_first = g;
-      ++at.seq;
-    }
-    __syncthreads();  // s_o is read: the next segment's copies may land there
+    g = cur.end;
   }
 }
 
-// Joins the states of the segments that lie in several CTAs' stretches: a CTA per row, the
-// states shared out among its warps (up to some fifty for one long sequence: with one warp
-// per row their loads queued up, 22 us instead of 4).
+// Joins the states of the segments that lie in several CTAs' stretches: WPR warps per row,
+// eight per CTA.  A segment of the ordinary batch has two or three states, one of a single
+// long sequence some seventy: there one warp's loads would queue up (22 us instead of 3).
 constexpr int MG_WARPS = 8;
-template <int HD>
+template <int HD, int WPR>
 __global__ void __launch_bounds__(32 * MG_WARPS) kv8_attend_merge_kernel(const AttendArgs a, int tile_rows) {
   constexpr int N = HD / 32;
   __shared__ float s_o[MG_WARPS][HD];
   __shared__ float2 s_ml[MG_WARPS];
+  const int G = a.heads / a.kv_heads, rows = G * a.sl;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPR;
+  const int at = blockIdx.x * (MG_WARPS / WPR) + warp / WPR;
+  const int row = at % rows, kvh = at / rows % a.kv_heads, b = at / rows / a.kv_heads;
+  if (b >= a.bs) return;  // whole warps; with WPR > 1 the grid has no such rows
+  // The list once: its length, that of the sequences before this one, and this one's steps.
+  // The lengths may be read before the wait: this kernel starts when every CTA of the
+  // attention kernel has begun, that is after what came before it in the stream is complete.
+  const int per_step = a.kv_heads * a.row_tiles;
+  int real = 0, before = 0;
+  for (int i = lane; i < a.bs; i += 32) {
+    const int n = steps_of(live_positions(a, i)) * per_step;
+    real += n;
+    before += i < b ? n : 0;
+  }
+  const int steps = steps_of(live_positions(a, b));
+  real = __reduce_add_sync(0xffffffffu, real);
+  before = __reduce_add_sync(0xffffffffu, before);
+  const int start = start_steps(real, a.ctas), total = real + start * a.bs * per_step, ctas = min(a.ctas, total);
+  const int g0 = before + start * b * per_step + (kvh * a.row_tiles + row / tile_rows) * (start + steps);
+  const Stretches cut(total, ctas);
+  const int first = cut.cta_of(g0 + start), last = cut.cta_of(g0 + start + steps - 1);
   grid_dep_wait();
   grid_dep_launch();
-  const int G = a.heads / a.kv_heads, rows = G * a.sl;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.x % rows, kvh = blockIdx.x / rows % a.kv_heads, b = blockIdx.x / rows / a.kv_heads;
-  const int steps = steps_of(live_positions(a, b));
-  const int g0 = walk_list(a, lane, b, 0).before + (kvh * a.row_tiles + row / tile_rows) * steps;
-  const int total = walk_list(a, lane, a.bs, 0).before, ctas = min(a.ctas, total);
-  const int first = cta_of(g0, total, ctas), last = cta_of(g0 + steps - 1, total, ctas);
   if (first == last) return;  // finished by that CTA
   const size_t pitch = static_cast<size_t>(tile_rows) * (HD + 4);
   // the first CTA may have begun before this segment: its state is then its second; the others begin inside it
-  const float* in0 = a.partial + (2 * static_cast<size_t>(first) + (stretch_begin(first, total, ctas) < g0 ? 1 : 0)) * pitch +
+  const float* in0 = a.partial + (2 * static_cast<size_t>(first) + (cut.begin(first) < g0 ? 1 : 0)) * pitch +
                      row % tile_rows * (HD + 4);
   const float* in1 = a.partial + 2 * static_cast<size_t>(first) * pitch + row % tile_rows * (HD + 4);
   const int n = last - first + 1;
   float acc[N], top = -INFINITY, den = 0.f;
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
-  for (int s0 = warp; s0 < n; s0 += 4 * MG_WARPS) {
+  for (int s0 = part; s0 < n; s0 += 4 * WPR) {
     float v[4][N];
     float2 ml[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int s = s0 + k * MG_WARPS;
+      const int s = s0 + k * WPR;
       ml[k] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int j = 0; j < N; ++j) v[k][j] = 0.f;
@@ -1001,27 +1173,48 @@ __global__ void __launch_bounds__(32 * MG_WARPS) kv8_attend_merge_kernel(const A
       for (int j = 0; j < N; ++j) acc[j] = fmaf(v[k][j], f, acc[j]);
     }
   }
+  const size_t to = ((static_cast<size_t>(b) * a.sl + row / G) * a.heads + kvh * G + row % G) * HD;
+  if constexpr (WPR == 1) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) s_o[warp][lane * N + j] = acc[j];
-  if (lane == 0) s_ml[warp] = make_float2(top, den);
-  __syncthreads();
-  const int d = threadIdx.x * 2;
-  if (d >= HD) return;
-  top = -INFINITY;
+    for (int j = 0; j < N; ++j) acc[j] = den == 0.f ? 0.f : acc[j] / den;
+    store_as(a.out, a.out_dtype, to + lane * N, acc);
+  } else {
+    static_assert(WPR == 1 || WPR == MG_WARPS, "one row per CTA: all of its warps are here or none");
 #pragma unroll
-  for (int w = 0; w < MG_WARPS; ++w) top = fmaxf(top, s_ml[w].x);
-  float o[2] = {0.f, 0.f};
-  den = 0.f;
+    for (int j = 0; j < N; ++j) s_o[warp][lane * N + j] = acc[j];
+    if (lane == 0) s_ml[warp] = make_float2(top, den);
+    __syncthreads();
+    const int d = threadIdx.x * 2;
+    if (d >= HD) return;
+    top = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < MG_WARPS; ++w) {
-    const float f = state_weight(s_ml[w].x, top);
-    den = fmaf(s_ml[w].y, f, den);
-    o[0] = fmaf(s_o[w][d], f, o[0]);
-    o[1] = fmaf(s_o[w][d + 1], f, o[1]);
+    for (int w = 0; w < MG_WARPS; ++w) top = fmaxf(top, s_ml[w].x);
+    float o[2] = {0.f, 0.f};
+    den = 0.f;
+#pragma unroll
+    for (int w = 0; w < MG_WARPS; ++w) {
+      const float f = state_weight(s_ml[w].x, top);
+      den = fmaf(s_ml[w].y, f, den);
+      o[0] = fmaf(s_o[w][d], f, o[0]);
+      o[1] = fmaf(s_o[w][d + 1], f, o[1]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) o[j] = den == 0.f ? 0.f : o[j] / den;
+    store_as(a.out, a.out_dtype, to + d, o);
   }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) o[j] = den == 0.f ? 0.f : o[j] / den;
-  store_as(a.out, a.out_dtype, ((static_cast<size_t>(b) * a.sl + row / G) * a.heads + kvh * G + row % G) * HD + d, o);
+}
+
+template <int HD>
+int launch_merge(const AttendArgs& a, int tile_rows, cudaStream_t st) {
+  const int64_t rows = static_cast<int64_t>(a.bs) * a.heads * a.sl;
+  const bool many = a.ctas > 4 * a.bs * a.kv_heads * a.row_tiles;  // states of a segment, about
+  if (many)
+    B200_CHECK_CUDA(launch_dependent(kv8_attend_merge_kernel<HD, MG_WARPS>, dim3(static_cast<unsigned>(rows)),
+                                     dim3(32 * MG_WARPS), 0, st, a, tile_rows));
+  else
+    B200_CHECK_CUDA(launch_dependent(kv8_attend_merge_kernel<HD, 1>, dim3(static_cast<unsigned>((rows + MG_WARPS - 1) / MG_WARPS)),
+                                     dim3(32 * MG_WARPS), 0, st, a, tile_rows));
+  return B200MOE_OK;
 }
 
 // Rows of a CTA's tile; CTAs of a call: as many as are resident at once, or one for each
@@ -1037,8 +1230,7 @@ int attend_ctas(int bs, int kv_heads, int hd, int rows, int max_seq_len) {
 
 template <int HD, int CODE, int NT, bool SPLIT>
 int launch_attend(const AttendArgs& a, cudaStream_t st) {
-  constexpr int RING = AT_WARPS * AT_SLOTS * 2 * AT_UNIT * HD, MERGE = AT_WARPS * 8 * NT * (HD + 8) * 4;
-  constexpr int SMEM = RING > MERGE ? RING : MERGE;
+  constexpr int SMEM = AT_WARPS * 2 * AT_UNIT * HD + AT_WARPS * 8 * NT * (HD + 8) * 4;
   auto kern = kv8_attend_kernel<HD, CODE, NT, SPLIT>;
   static bool configured[16] = {};
   int dev = 0;
@@ -1127,26 +1319,22 @@ int b200moe_kv8_read(const void* slab, const float* scales, const b200moe_kv8_ca
                "%s: slab and outputs must be 16-byte aligned, scales 8-byte", who);
   ReadArgs a;
   a.slab = static_cast<const uint8_t*>(slab); a.scales = scales; a.page_ids = page_ids; a.seq_lens = seq_lens;
-  a.k_out = k_out; a.v_out = v_out; a.out_dtype = out_dtype; a.bs = bs; a.pages_per_seq = pages_per_seq;
+  a.k_out = k_out; a.v_out = v_out; a.bs = bs; a.pages_per_seq = pages_per_seq;
   a.page_count = cache->page_count; a.max_len = max_seq_len; a.kv_heads = cache->kv_heads; a.stride = cache->stride;
-  a.blocks = cache->blocks; a.block_index = block_index; a.scale_block = cache->scale_block;
+  a.blocks = cache->blocks; a.block_index = block_index; a.block_shift = log2_of(cache->scale_block);
   a.status = device_status_ptr();
   if (a.status == nullptr) return B200MOE_ERR_CUDA;
-  const size_t total = static_cast<size_t>(bs) * max_seq_len * cache->kv_heads * 2 * (cache->head_dim / 16);
-  const size_t ctas = (total + 255) / 256;
+  const int64_t ctas = static_cast<int64_t>((max_seq_len - 1) / RD_TILE + 1) * bs * cache->kv_heads;
   B200_REQUIRE(ctas <= 0x7fffffff, "%s: too many rows for one call", who);
   const unsigned grid = static_cast<unsigned>(ctas);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool i8 = cache->code == B200MOE_KV8_INT8;
-  if (cache->head_dim == 64) {
-    if (i8) kv8_read_kernel<64, B200MOE_KV8_INT8><<<grid, 256, 0, st>>>(a);
-    else kv8_read_kernel<64, B200MOE_KV8_E4M3><<<grid, 256, 0, st>>>(a);
-  } else {
-    if (i8) kv8_read_kernel<128, B200MOE_KV8_INT8><<<grid, 256, 0, st>>>(a);
-    else kv8_read_kernel<128, B200MOE_KV8_E4M3><<<grid, 256, 0, st>>>(a);
-  }
-  B200_CHECK_CUDA(cudaGetLastError());
-  return B200MOE_OK;
+  const bool h64 = cache->head_dim == 64;
+  if (out_dtype == B200MOE_DT_F32)
+    return h64 ? launch_read<float, 64>(a, cache->code, grid, st) : launch_read<float, 128>(a, cache->code, grid, st);
+  if (out_dtype == B200MOE_DT_F16)
+    return h64 ? launch_read<__half, 64>(a, cache->code, grid, st) : launch_read<__half, 128>(a, cache->code, grid, st);
+  return h64 ? launch_read<__nv_bfloat16, 64>(a, cache->code, grid, st)
+             : launch_read<__nv_bfloat16, 128>(a, cache->code, grid, st);
 }
 
 size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_t bs, int32_t new_tokens,
@@ -1189,15 +1377,12 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   a.page_ids = page_ids; a.seq_lens = seq_lens; a.out = out; a.partial = static_cast<float*>(scratch);
   a.out_dtype = out_dtype; a.bs = bs; a.sl = new_tokens;
   a.pages_per_seq = pages_per_seq; a.page_count = cache->page_count; a.heads = heads; a.kv_heads = cache->kv_heads;
-  a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index; a.scale_block = cache->scale_block;
+  a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index;
   const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows), hd = cache->head_dim;
   a.row_tiles = (rows + tile - 1) / tile;
   a.ctas = attend_ctas(bs, cache->kv_heads, hd, rows, max_seq_len);
-  a.stride_shift = a.block_shift = -1;
-  for (int i = 0; i < 31; ++i) {
-    if (a.stride == 1 << i) a.stride_shift = i;
-    if (a.scale_block == 1 << i) a.block_shift = i;
-  }
+  a.stride_shift = log2_of(a.stride);
+  a.block_shift = log2_of(cache->scale_block);
   B200_REQUIRE(static_cast<double>(bs) * a.kv_heads * a.row_tiles * (1.0 + pages_per_seq * static_cast<double>(a.stride) / AT_STEP) < 2147483647.0,
                "%s: too many positions for one call", who);
   a.scale = scale; a.softcap = softcap;
@@ -1216,10 +1401,7 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
             : launch_attend_rows<128, B200MOE_KV8_E4M3>(a, split, tile, st);
   if (rc) return rc;
   if (static_cast<int64_t>(pages_per_seq) * a.stride <= AT_STEP) return B200MOE_OK;  // no segment is longer than a step
-  const int64_t ctas = static_cast<int64_t>(bs) * a.kv_heads * rows;
-  auto merge = hd == 64 ? kv8_attend_merge_kernel<64> : kv8_attend_merge_kernel<128>;
-  B200_CHECK_CUDA(launch_dependent(merge, dim3(static_cast<unsigned>(ctas)), dim3(32 * MG_WARPS), 0, st, a, tile));
-  return B200MOE_OK;
+  return hd == 64 ? launch_merge<64>(a, tile, st) : launch_merge<128>(a, tile, st);
 }
 
 }  // extern "C"

@@ -337,6 +337,59 @@ def test_missing_pages_are_reported_and_skipped():
     assert _status() == 0
 
 
+@pytest.mark.parametrize("code", [I8, E4])
+def test_stretches_of_missing_pages_are_not_attended(code):
+    """Whole steps of positions without a page, in the middle and at the end, and the sequence behind them."""
+    from shark_platform_b200 import _cabi as C
+
+    A = _attention()
+    gen = torch.Generator().manual_seed(6)
+    cache = _cache(code, 2, 128, 16, 16)
+    state = _fill(cache, 90, gen)
+    ids = torch.stack([torch.arange(40), torch.arange(40, 80)]).to(torch.int32)
+    live = ids.clone()
+    ids[0, 10:30] = 90
+    ids[0, 36:] = -5
+    q = torch.randn(2, 1, 8, 128, generator=gen).to(BF)
+    o = A.kv_attend(q.cuda(), cache, state, block_index=0, seq_block_ids=ids.cuda(), seq_lens=torch.tensor([637, 640]).cuda())
+    with pytest.raises(C.B200MoeError, match="status word"):
+        _status()
+    codes, scales = ko.page_views(state, cache)
+    for b in range(2):
+        k, v = ko.gather(codes, scales, cache, 0, live[b], 637 + 3 * b)
+        if b == 0:
+            keep = [p for p in range(637) if not 160 <= p < 480 and p < 576]
+            k, v = k[keep], v[keep]
+        want = ko.attend(q[b], k, v, [k.shape[0]], 128 ** -0.5)
+        assert ((o[b].cpu().double() - want).abs() <= ko.attend_tolerance(q[b], k, v, 128 ** -0.5, 2.0 ** -11, EPS[BF], want)).all()
+
+
+def test_a_length_behind_the_page_table_is_reported():
+    from shark_platform_b200 import _cabi as C
+
+    A = _attention()
+    gen = torch.Generator().manual_seed(6)
+    cache = _cache(I8, 1, 64, 16, 16)
+    state = _fill(cache, 4, gen)
+    ids = torch.tensor([[1, 2]], dtype=torch.int32).cuda()
+    q = torch.randn(1, 1, 4, 64, generator=gen).cuda()
+    a = A.kv_attend(q, cache, state, block_index=0, seq_block_ids=ids, seq_lens=torch.tensor([32]).cuda())
+    assert _status() == 0
+    b = A.kv_attend(q, cache, state, block_index=0, seq_block_ids=ids, seq_lens=torch.tensor([33]).cuda())
+    with pytest.raises(C.B200MoeError, match="status word"):
+        _status()
+    assert torch.equal(a, b)
+    o = A.kv_attend(q, cache, state, block_index=0, seq_block_ids=ids, seq_lens=torch.tensor([-4]).cuda())
+    assert _status() == 0 and not o.any()
+
+
+@pytest.mark.parametrize("bs", [70, 200])
+def test_many_short_sequences(bs):
+    """More sequences than one look at the lengths takes, empty ones among them."""
+    _attend_case(I8, BF, 64, 8, 4, 16, 16, [(37 * i) % 150 for i in range(bs)])
+    _attend_case(E4, F32, 64, 8, 4, 16, 16, [(61 * i) % 300 if i % 7 else 0 for i in range(bs)], sl=2)
+
+
 # -------------------------------------------------------------------- read-back
 @pytest.mark.parametrize("code", [I8, E4])
 @pytest.mark.parametrize("dtype", [F32, HF, BF])
