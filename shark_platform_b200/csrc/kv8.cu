@@ -170,6 +170,9 @@ struct WriteArgs {
   const float* freqs;
   int order, bs, sl, pages_per_seq, page_count, heads, kv_heads, stride, blocks, block_index, scale_block;
   int tiles;                          // of a sequence
+  int stride_shift, block_shift;      // log2; -1 where the stride is no power of two
+  unsigned kv_ctas;                   // CTAs of K and V
+  int q_heads;                        // heads that a lane of the others takes
   int32_t* status;
 };
 
@@ -179,11 +182,64 @@ constexpr int WR_THREADS = 256;
 constexpr int WR_WARPS = WR_THREADS / 32;
 constexpr float QMAX[2] = {127.f, 448.f};
 
-// A lane's eight elements of a row, normed and rotated; LPR lanes have a row.  cs: the
-// row's cosines and sines.
-template <int LPR>
-__device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], bool norm, float eps, const float2* cs,
-                                            int order, int c) {
+// Cosine and sine of position * freq, the angle reduced to part of a turn first.
+// 32-bit rows: reduced in 64 bits, good to 2^-23 at any position.  16-bit rows: the position
+// (below 2^24) times freq / (2 pi) as the sum of two floats, their integer part dropped, and
+// the special-function unit, absolute error 2^-21: an eighth of a thousandth of half a step
+// of fp16.  (sincospif for both: 70 instead of ... us for 4 x 2048 tokens of 48 + 16 heads.)
+template <typename T>
+__device__ __forceinline__ float2 cos_sin(long long pos, float freq) {
+  float sn, cs;
+  if (sizeof(T) == 4 || pos >= 1 << 24) {
+    const double turns = static_cast<double>(pos) * (static_cast<double>(freq) * 0.31830988618379067154);  // halves
+    sincospif(static_cast<float>(turns - 2.0 * rint(0.5 * turns)), &sn, &cs);
+  } else {
+    constexpr double inv = 0.15915494309189533577;  // 1 / (2 pi)
+    constexpr float inv_hi = static_cast<float>(inv), inv_lo = static_cast<float>(inv - inv_hi);
+    const float p = static_cast<float>(static_cast<int>(pos));
+    const float g = freq * inv_hi, g_lo = fmaf(freq, inv_hi, -g) + freq * inv_lo;
+    const float u = p * g, u_lo = fmaf(p, g_lo, fmaf(p, g, -u));
+    const float angle = ((u - rintf(u)) + u_lo) * 6.2831853071795864769f;
+    sn = __sinf(angle);
+    cs = __cosf(angle);
+  }
+  return make_float2(cs, sn);
+}
+// max(m, |x|) for m >= 0, NaN where either is
+__device__ __forceinline__ float max_nan(float m, float x) {
+  float y;
+  asm("{.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;}" : "=f"(y) : "f"(m), "f"(x));
+  return y;
+}
+// What lane c of a row needs of the position's cosines and sines: of its four pairs, or in
+// the HuggingFace order of each of its eight elements.  There the other half of each pair is
+// LPR / 2 lanes away with the same angles: either lane computes four and they are exchanged.
+template <int ORDER>
+struct Turn { float2 t[ORDER == 0 ? 4 : 8]; };
+template <typename T, int LPR, int ORDER>
+__device__ __forceinline__ Turn<ORDER> turn_of(long long pos, const float* freqs, int c) {
+  Turn<ORDER> w;
+  const bool upper = c >= LPR / 2;
+  const int j0 = ORDER == 0 ? c * 4 : (c % (LPR / 2)) * 8 + (upper ? 4 : 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w.t[i] = cos_sin<T>(pos, freqs[j0 + i]);
+  if constexpr (ORDER != 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 mine = w.t[i];
+      float2 other;
+      other.x = __shfl_xor_sync(0xffffffffu, mine.x, LPR / 2);
+      other.y = __shfl_xor_sync(0xffffffffu, mine.y, LPR / 2);
+      w.t[i] = upper ? other : mine;
+      w.t[4 + i] = upper ? mine : other;
+    }
+  }
+  return w;
+}
+// A lane's eight elements of a row, normed and rotated; LPR lanes have a row.
+template <int LPR, int ORDER>
+__device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], bool norm, float eps,
+                                            const Turn<ORDER>& turn, int c) {
   if (norm) {
     float ss = 0.f;
 #pragma unroll
@@ -194,45 +250,117 @@ __device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], 
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = w[i] * (x[i] * r);
   }
-  if (order == 0) {
+  if constexpr (ORDER == 0) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 t = cs[c * 4 + i];
       const float re = x[2 * i], im = x[2 * i + 1];
-      x[2 * i] = re * t.x - im * t.y;
-      x[2 * i + 1] = im * t.x + re * t.y;
+      x[2 * i] = re * turn.t[i].x - im * turn.t[i].y;
+      x[2 * i + 1] = im * turn.t[i].x + re * turn.t[i].y;
     }
-  } else {  // the other half of the pair is LPR / 2 lanes away
+  } else {
     const float sign = c < LPR / 2 ? -1.f : 1.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 t = cs[(c % (LPR / 2)) * 8 + i];
       const float other = __shfl_xor_sync(0xffffffffu, x[i], LPR / 2);
-      x[i] = x[i] * t.x + sign * other * t.y;
+      x[i] = x[i] * turn.t[i].x + sign * other * turn.t[i].y;
     }
   }
 }
 
-// One CTA per (sequence, tile of TILE positions, kv head): K and V of the tile and the
-// queries of the heads that share the kv head.  Tiles are aligned in absolute positions, so
-// that a tile holds whole scale blocks.  HD / 8 lanes have a row (16-byte loads and stores
-// of 16-bit rows), a warp two or four rows at a time.  K and V stay in registers from their
-// load to their codes: one read of everything.
-template <typename T, int HD, int KIND, int TILE>
-__global__ void __launch_bounds__(WR_THREADS) norm_rope_write_kernel(const WriteArgs a) {
+// The scale of a block from the largest magnitude of its new rows (as bits) and, if it is
+// continued, the scale it had (else 0); 1 / scale; and what its earlier codes are multiplied
+// by: the scale grows by powers of two.
+struct BlockScale { float s, inv, shrink; };
+template <int KIND>
+__device__ __forceinline__ BlockScale block_scale(unsigned bits, float before) {
+  constexpr float qmax = QMAX[KIND], tiny = 7.888609052210118e-31f;  // 2^-100
+  const float amax = __uint_as_float(bits);
+  BlockScale r;
+  r.shrink = 1.f;
+  if (bits >= 0x7f800000u || before != before) {
+    r.s = __uint_as_float(0x7fc00000u);
+  } else if (before > 0.f) {
+    r.s = before;
+    const float ratio = amax / (before * qmax * (1.f + 0.0009765625f));
+    if (ratio > 1.f) {
+      int e;
+      const float m = frexpf(ratio, &e);
+      if (m == 0.5f) --e;
+      r.s = ldexpf(before, e);
+      r.shrink = ldexpf(1.f, -e);
+    }
+  } else {
+    r.s = amax < qmax * tiny ? 0.f : amax / qmax;
+  }
+  r.inv = r.s > 0.f ? 1.f / r.s : 0.f;
+  return r;
+}
+
+// Two kinds of CTAs.  kv_ctas of them have a (sequence, tile of TILE positions, kv head)
+// each: its K and V.  Tiles are aligned in absolute positions, so that a tile holds whole
+// scale blocks; K and V stay in registers from their load to their codes: one read of
+// everything.  The others have the queries: a lane keeps its position's cosines and sines
+// and takes four heads at once, q_heads in all.  HD / 8 lanes have a row (16-byte loads and
+// stores of 16-bit rows), a warp two or four rows.  (With K, V and the queries of a kv head
+// in one CTA, angles in shared memory: 79 instead of ... us for 4 x 2048 tokens of 48 + 16
+// heads, as the queries waited for the barriers of K and V.)
+template <typename T, int HD, int KIND, int TILE, int ORDER>
+__global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 2 ? 4 : 3) : 2) norm_rope_write_kernel(const WriteArgs a) {
   constexpr int LPR = HD / 8, RPW = 32 / LPR;                 // lanes per row, rows of a warp
   constexpr int RPP = WR_WARPS * RPW;                         // rows of a pass
   constexpr int PASSES = (TILE + RPP - 1) / RPP;
-  __shared__ float2 s_cs[TILE][HD / 2];
+  constexpr int QB = 4;                                       // heads that a lane takes at once
   __shared__ long long s_row[TILE];     // K row of each position in the slab, in rows of HD elements; -1: not written
   __shared__ unsigned s_amax[2][TILE];  // of each scale block, as bits
-  __shared__ float s_inv[2][TILE], s_shrink[2];
+  __shared__ uint32_t s_pair[TILE];     // scale pair of each position
+  __shared__ float2 s_before;           // scales of a continued block
   grid_dep_wait();
   grid_dep_launch();
-  const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads % a.tiles, b = blockIdx.x / a.kv_heads / a.tiles;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int sub = warp * RPW + lane / LPR, c = lane % LPR;    // row of a pass, chunk of eight elements
-  const int G = a.heads / a.kv_heads, B = a.scale_block;
+  const T *q = static_cast<const T*>(a.q), *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v);
+  // K and V's CTAs are spread evenly among the others
+  unsigned kv_before, rest;
+  if (gridDim.x < 65536) {
+    const unsigned x = blockIdx.x * a.kv_ctas;
+    kv_before = x / gridDim.x;
+    rest = x - kv_before * gridDim.x;
+  } else {
+    const unsigned long long x = static_cast<unsigned long long>(blockIdx.x) * a.kv_ctas;
+    kv_before = static_cast<unsigned>(x / gridDim.x);
+    rest = static_cast<unsigned>(x - static_cast<unsigned long long>(kv_before) * gridDim.x);
+  }
+  if (rest + a.kv_ctas < gridDim.x) {
+    const long long tokens = static_cast<long long>(a.bs) * a.sl, groups = (a.heads + a.q_heads - 1) / a.q_heads;
+    const long long mine = static_cast<long long>(blockIdx.x - kv_before) * RPP + sub;
+    const bool some = mine < tokens * groups;
+    const long long item = some ? mine : tokens * groups - 1;  // all lanes take part in the shuffles
+    const long long tok = item % tokens;
+    const int h0 = static_cast<int>(item / tokens) * a.q_heads, h1 = min(h0 + a.q_heads, a.heads);
+    const int b = static_cast<int>(tok / a.sl);
+    const T* from = q + tok * a.q_stride + c * 8;
+    T* to = static_cast<T*>(a.q_out) + tok * a.heads * HD + c * 8;
+    const long long pos = max(a.start_positions[b], 0) + (tok - static_cast<long long>(b) * a.sl);
+    const Turn<ORDER> turn = turn_of<T, LPR, ORDER>(pos, a.freqs, c);
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = a.q_norm != nullptr ? a.q_norm[c * 8 + i] : 1.f;
+    // every lane of a warp makes the same number of steps: heads behind the last are read again and not stored
+    for (int d = 0; d < a.q_heads; d += QB) {
+      Raw8<T> raw[QB];
+#pragma unroll
+      for (int g = 0; g < QB; ++g) raw[g].load(from + min(h0 + d + g, h1 - 1) * HD);
+#pragma unroll
+      for (int g = 0; g < QB; ++g) {
+        float x[8];
+        raw[g].get(x);
+        norm_rotate<LPR, ORDER>(x, w, a.q_norm != nullptr, a.eps, turn, c);
+        if (some && h0 + d + g < h1) store8(to + (h0 + d + g) * HD, x);
+      }
+    }
+    return;
+  }
+  const int kvh = kv_before % a.kv_heads, tile = kv_before / a.kv_heads % a.tiles, b = kv_before / a.kv_heads / a.tiles;
   const int start_in = a.start_positions[b];
   const long long start = start_in < 0 ? 0 : start_in;
   int count = start_in < 0 ? 0 : a.new_lens != nullptr ? a.new_lens[b] : a.sl;
@@ -246,7 +374,6 @@ __global__ void __launch_bounds__(WR_THREADS) norm_rope_write_kernel(const Write
 
   // K and V are on their way while the angles are computed
   const long long tok0 = static_cast<long long>(b) * a.sl + (p0 - start);  // token of row 0
-  const T *q = static_cast<const T*>(a.q), *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v);
   Raw8<T> kr[PASSES], vr[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
@@ -256,175 +383,143 @@ __global__ void __launch_bounds__(WR_THREADS) norm_rope_write_kernel(const Write
     if (r < hi) kr[i].load(k + (tok0 + r) * a.k_stride + kvh * HD + c * 8);
     if (r < whi) vr[i].load(v + (tok0 + r) * a.v_stride + kvh * HD + c * 8);
   }
-  float qw[8], kw[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    qw[i] = a.q_norm != nullptr ? a.q_norm[c * 8 + i] : 1.f;
-    kw[i] = a.k_norm != nullptr ? a.k_norm[c * 8 + i] : 1.f;
-  }
-  const int first = lo - lo % (KIND == CACHE_PLAIN ? 1 : B);  // earlier rows of a continued block included
+  const int first = KIND == CACHE_PLAIN ? lo : lo >> a.block_shift << a.block_shift;  // earlier rows of a continued block included
   for (int r = first + t; r < whi; r += WR_THREADS) {
-    const long long pos = p0 + r, slot = pos / a.stride;
+    const uint32_t pos = static_cast<uint32_t>(p0 + r), slot = a.stride_shift >= 0 ? pos >> a.stride_shift : pos / a.stride;
+    const uint32_t off = pos - slot * a.stride;
     long long row = -1;
-    const int off = static_cast<int>(pos - slot * a.stride);
-    const long long page = slot < a.pages_per_seq ? a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot] : -1;
+    const int page = slot < static_cast<uint32_t>(a.pages_per_seq) ? a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot] : -1;
     if (page < 0 || page >= a.page_count) {
       atomicOr(a.status, DEV_ERR_BOUNDS);
     } else if constexpr (KIND == CACHE_PLAIN) {
-      row = (((page * a.blocks + a.block_index) * 2) * a.stride + off) * a.kv_heads + kvh;
+      row = ((static_cast<long long>(page) * a.blocks + a.block_index) * 2 * a.stride + off) * a.kv_heads + kvh;
     } else {
-      row = ((page * a.blocks + a.block_index) * a.kv_heads + kvh) * 2 * a.stride + off;
+      const uint32_t head = (static_cast<uint32_t>(page) * a.blocks + a.block_index) * a.kv_heads + kvh;
+      row = head * 2u * a.stride + off;
+      s_pair[r] = head * static_cast<uint32_t>(a.stride >> a.block_shift) + (off >> a.block_shift);
+      if (r < lo && r == first) s_before = reinterpret_cast<const float2*>(a.scales)[s_pair[r]];
     }
     s_row[r] = row;
   }
   for (int i = t; i < 2 * TILE; i += WR_THREADS) (&s_amax[0][0])[i] = 0u;
-  for (int i = t; i < (hi - lo) * (HD / 2); i += WR_THREADS) {
-    const int r = lo + i / (HD / 2), j = i % (HD / 2);
-    // the angle in half turns, reduced in 64 bits: good to 2^-24 at any position
-    const double turns = static_cast<double>(p0 + r) * (static_cast<double>(a.freqs[j]) * 0.31830988618379067154);
-    float sn, cs;
-    sincospif(static_cast<float>(turns - 2.0 * rint(0.5 * turns)), &sn, &cs);
-    s_cs[r][j] = make_float2(cs, sn);
-  }
   __syncthreads();
-
-  float kx[PASSES][8];
-  // all lanes take part in the shuffles of the norm and the rotation; rows outside lo .. hi are zeros, unused
+  // the warps that have rows go on
+  const int kv_warps = min((hi - lo + RPW - 1) / RPW, WR_WARPS);
+  auto kv_sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(kv_warps * 32) : "memory"); };
+  if (warp < kv_warps) {
+    float w[8], kx[PASSES][8];
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = lo + i * RPP + sub;
-    if (lo + i * RPP >= hi) break;
-    kr[i].get(kx[i]);
-    norm_rotate<LPR>(kx[i], kw, a.k_norm != nullptr, a.eps, s_cs[min(r, hi - 1)], a.order, c);
-    if (r < hi && a.k_out != nullptr)
-      store8(static_cast<T*>(a.k_out) + ((tok0 + r) * a.kv_heads + kvh) * HD + c * 8, kx[i]);
-    if constexpr (KIND == CACHE_PLAIN) {
-      if (r < whi && s_row[r] >= 0) {
-        float y[8];
-        vr[i].get(y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) kx[i][j] = round_to<T>(kx[i][j]);
-        const size_t at = static_cast<size_t>(s_row[r]) * HD + c * 8, v_at = at + static_cast<size_t>(a.stride) * a.kv_heads * HD;
-        if (a.cache_dtype == B200MOE_DT_F32) {
-          store8(static_cast<float*>(a.slab) + at, kx[i]);
-          store8(static_cast<float*>(a.slab) + v_at, y);
-        } else if (a.cache_dtype == B200MOE_DT_F16) {
-          store8(static_cast<__half*>(a.slab) + at, kx[i]);
-          store8(static_cast<__half*>(a.slab) + v_at, y);
-        } else {
-          store8(static_cast<__nv_bfloat16*>(a.slab) + at, kx[i]);
-          store8(static_cast<__nv_bfloat16*>(a.slab) + v_at, y);
-        }
-      }
-    } else {
-      // the largest magnitude of the row, then of its scale block; as bits, so that NaN is the largest
-      float y[8];
-      vr[i].get(y);
-      unsigned mk = 0, mv = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        mk = max(mk, __float_as_uint(kx[i][j]) & 0x7fffffffu);
-        mv = max(mv, __float_as_uint(y[j]) & 0x7fffffffu);
-      }
-#pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) {
-        mk = max(mk, __shfl_xor_sync(0xffffffffu, mk, o));
-        mv = max(mv, __shfl_xor_sync(0xffffffffu, mv, o));
-      }
-      if (c == 0 && r < whi) {
-        atomicMax(&s_amax[0][r / B], mk);
-        atomicMax(&s_amax[1][r / B], mv);
-      }
-    }
-  }
-  if constexpr (KIND != CACHE_PLAIN) {
-    __syncthreads();
-    // the scale of each block: a thread for each block and K | V
-    constexpr float qmax = QMAX[KIND];
-    constexpr float tiny = 7.888609052210118e-31f;  // 2^-100
-    for (int i = t; i < 2 * (TILE / B); i += WR_THREADS) {
-      const int blk = i >> 1, kv = i & 1;
-      const int r0 = max(blk * B, lo), r1 = min(blk * B + B, whi);
-      if (r0 >= r1 || s_row[r0] < 0) continue;
-      const unsigned bits = s_amax[kv][blk];
-      const float amax = __uint_as_float(bits);
-      const long long row = s_row[r0];
-      const long long pair = (row / (2 * a.stride)) * (a.stride / B) + (row % a.stride) / B;
-      const bool continued = lo > blk * B;
-      const float before = continued ? a.scales[2 * pair + kv] : 0.f;
-      float s, shrink = 1.f;
-      if (bits >= 0x7f800000u || before != before) {
-        s = __uint_as_float(0x7fc00000u);
-      } else if (before > 0.f) {
-        s = before;
-        const float ratio = amax / (before * qmax * (1.f + 0.0009765625f));
-        if (ratio > 1.f) {
-          int e;
-          const float m = frexpf(ratio, &e);
-          if (m == 0.5f) --e;
-          s = ldexpf(before, e);
-          shrink = ldexpf(1.f, -e);
-        }
-      } else {
-        s = amax < qmax * tiny ? 0.f : amax / qmax;
-      }
-      if (!continued || s != before) a.scales[2 * pair + kv] = s;
-      s_inv[kv][blk] = s > 0.f ? 1.f / s : 0.f;
-      if (continued) s_shrink[kv] = s == s ? shrink : 1.f;
-    }
-    __syncthreads();
-    uint8_t* slab = static_cast<uint8_t*>(a.slab);
-    const size_t v_off = static_cast<size_t>(a.stride) * HD;
+    for (int i = 0; i < 8; ++i) w[i] = a.k_norm != nullptr ? a.k_norm[c * 8 + i] : 1.f;
+    // all lanes take part in the shuffles of the norm and the rotation; rows outside lo .. hi are zeros, unused
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int r = lo + i * RPP + sub;
-      if (r < whi && s_row[r] >= 0) {
-        uint8_t* at = slab + static_cast<size_t>(s_row[r]) * HD + c * 8;
-        *reinterpret_cast<uint2*>(at) = floats_to_codes<KIND>(kx[i], s_inv[0][r / B]);
+      if (lo + i * RPP >= hi) break;
+      kr[i].get(kx[i]);
+      norm_rotate<LPR, ORDER>(kx[i], w, a.k_norm != nullptr, a.eps, turn_of<T, LPR, ORDER>(p0 + r, a.freqs, c), c);
+      if (r < hi && a.k_out != nullptr)
+        store8(static_cast<T*>(a.k_out) + ((tok0 + r) * a.kv_heads + kvh) * HD + c * 8, kx[i]);
+      if constexpr (KIND == CACHE_PLAIN) {
+        if (r < whi && s_row[r] >= 0) {
+          float y[8];
+          vr[i].get(y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) kx[i][j] = round_to<T>(kx[i][j]);
+          const size_t at = static_cast<size_t>(s_row[r]) * HD + c * 8, v_at = at + static_cast<size_t>(a.stride) * a.kv_heads * HD;
+          if (a.cache_dtype == B200MOE_DT_F32) {
+            store8(static_cast<float*>(a.slab) + at, kx[i]);
+            store8(static_cast<float*>(a.slab) + v_at, y);
+          } else if (a.cache_dtype == B200MOE_DT_F16) {
+            store8(static_cast<__half*>(a.slab) + at, kx[i]);
+            store8(static_cast<__half*>(a.slab) + v_at, y);
+          } else {
+            store8(static_cast<__nv_bfloat16*>(a.slab) + at, kx[i]);
+            store8(static_cast<__nv_bfloat16*>(a.slab) + v_at, y);
+          }
+        }
+      } else {
+        // the largest magnitude of the row, then of its scale block; as bits, so that NaN is the largest
         float y[8];
         vr[i].get(y);
-        *reinterpret_cast<uint2*>(at + v_off) = floats_to_codes<KIND>(y, s_inv[1][r / B]);
+        float mk = 0.f, mv = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          mk = max_nan(mk, kx[i][j]);
+          mv = max_nan(mv, y[j]);
+        }
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) {
+          mk = max_nan(mk, __shfl_xor_sync(0xffffffffu, mk, o));
+          mv = max_nan(mv, __shfl_xor_sync(0xffffffffu, mv, o));
+        }
+        if (c == 0 && r < whi) {
+          atomicMax(&s_amax[0][r >> a.block_shift], __float_as_uint(mk));
+          atomicMax(&s_amax[1][r >> a.block_shift], __float_as_uint(mv));
+        }
       }
     }
-    // the live rows of a continued block whose scale has grown
-    if (first < lo && lo < whi && s_row[lo] >= 0) {
-      for (int i = sub; i < 2 * (lo - first); i += RPP) {
-        const int kv = i & 1, r = first + (i >> 1);
-        if (s_shrink[kv] == 1.f) continue;
-        uint2* at = reinterpret_cast<uint2*>(slab + static_cast<size_t>(s_row[r]) * HD + (kv ? v_off : 0) + c * 8);
+    if constexpr (KIND != CACHE_PLAIN) {
+      kv_sync();
+      uint8_t* slab = static_cast<uint8_t*>(a.slab);
+      const size_t v_off = static_cast<size_t>(a.stride) * HD;
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        const int r = lo + i * RPP + sub;
+        if (r >= whi || s_row[r] < 0) continue;
+        // every lane computes the scales of its row's block; the block's first new row stores them
+        const int blk = r >> a.block_shift, at_blk = max(blk << a.block_shift, lo);
+        const bool continued = lo > blk << a.block_shift;
+        const float2 before = continued ? s_before : make_float2(0.f, 0.f);
+        const BlockScale ks = block_scale<KIND>(s_amax[0][blk], before.x), vs = block_scale<KIND>(s_amax[1][blk], before.y);
+        if (r == at_blk && c == 0) reinterpret_cast<float2*>(a.scales)[s_pair[r]] = make_float2(ks.s, vs.s);
+        uint8_t* at = slab + static_cast<size_t>(s_row[r]) * HD + c * 8;
+        *reinterpret_cast<uint2*>(at) = floats_to_codes<KIND>(kx[i], ks.inv);
         float y[8];
-        codes_to_floats<KIND>(*at, y);
-        *at = floats_to_codes<KIND>(y, s_shrink[kv]);
+        vr[i].get(y);
+        *reinterpret_cast<uint2*>(at + v_off) = floats_to_codes<KIND>(y, vs.inv);
+      }
+      // the live rows of a continued block whose scale has grown
+      if (first < lo && lo < whi && s_row[lo] >= 0) {
+        const int blk = first >> a.block_shift;
+        const float k_shrink = block_scale<KIND>(s_amax[0][blk], s_before.x).shrink;
+        const float v_shrink = block_scale<KIND>(s_amax[1][blk], s_before.y).shrink;
+        for (int i = sub; i < 2 * (lo - first); i += kv_warps * RPW) {
+          const int kv = i & 1, r = first + (i >> 1);
+          const float shrink = kv ? v_shrink : k_shrink;
+          if (shrink == 1.f) continue;
+          uint2* at = reinterpret_cast<uint2*>(slab + static_cast<size_t>(s_row[r]) * HD + (kv ? v_off : 0) + c * 8);
+          float y[8];
+          codes_to_floats<KIND>(*at, y);
+          *at = floats_to_codes<KIND>(y, shrink);
+        }
       }
     }
-  }
-  // queries: rows (position, head) of the tile
-  const int q_rows = (hi - lo) * G;
-#pragma unroll 2
-  for (int i0 = 0; i0 < q_rows; i0 += RPP) {
-    const int i = min(i0 + sub, q_rows - 1);
-    const int r = lo + i / G, h = kvh * G + i % G;
-    Raw8<T> raw;
-    raw.load(q + (tok0 + r) * a.q_stride + static_cast<long long>(h) * HD + c * 8);
-    float x[8];
-    raw.get(x);
-    norm_rotate<LPR>(x, qw, a.q_norm != nullptr, a.eps, s_cs[r], a.order, c);
-    if (i0 + sub < q_rows) store8(static_cast<T*>(a.q_out) + ((tok0 + r) * a.heads + h) * HD + c * 8, x);
   }
 }
 
-template <typename T, int HD, int KIND, int TILE>
+template <typename T, int HD, int KIND, int TILE, int ORDER>
 int launch_write(WriteArgs& a, cudaStream_t st) {
   a.tiles = a.sl == 1 ? 1 : (a.sl - 1) / TILE + 2;
-  B200_CHECK_CUDA(launch_dependent(norm_rope_write_kernel<T, HD, KIND, TILE>,
-                                   dim3(static_cast<unsigned>(a.bs) * a.tiles * a.kv_heads), dim3(WR_THREADS), 0, st, a));
+  a.kv_ctas = static_cast<unsigned>(a.bs) * a.tiles * a.kv_heads;
+  // as many heads a lane as leave work for sixteen CTAs per SM: a position's angles are computed once for each group
+  constexpr int RPP = WR_THREADS / (HD / 8);
+  const int64_t tokens = static_cast<int64_t>(a.bs) * a.sl, want = static_cast<int64_t>(sm_count()) * 16 * RPP;
+  a.q_heads = 4;
+  while (a.q_heads < a.heads && tokens * ((a.heads - 1) / (2 * a.q_heads) + 1) >= want) a.q_heads *= 2;
+  const int64_t q_ctas = (tokens * ((a.heads - 1) / a.q_heads + 1) + RPP - 1) / RPP;
+  B200_CHECK_CUDA(launch_dependent(norm_rope_write_kernel<T, HD, KIND, TILE, ORDER>,
+                                   dim3(static_cast<unsigned>(a.kv_ctas + q_ctas)), dim3(WR_THREADS), 0, st, a));
   return B200MOE_OK;
+}
+template <typename T, int HD, int KIND>
+int launch_write_tile(WriteArgs& a, cudaStream_t st) {
+  if constexpr (KIND != CACHE_PLAIN)
+    if (a.scale_block > 32) return a.order ? launch_write<T, HD, KIND, 64, 1>(a, st) : launch_write<T, HD, KIND, 64, 0>(a, st);
+  return a.order ? launch_write<T, HD, KIND, 32, 1>(a, st) : launch_write<T, HD, KIND, 32, 0>(a, st);
 }
 template <typename T, int KIND>
 int launch_write_hd(WriteArgs& a, int hd, cudaStream_t st) {
-  if constexpr (KIND != CACHE_PLAIN)
-    if (a.scale_block > 32) return hd == 64 ? launch_write<T, 64, KIND, 64>(a, st) : launch_write<T, 128, KIND, 64>(a, st);
-  return hd == 64 ? launch_write<T, 64, KIND, 32>(a, st) : launch_write<T, 128, KIND, 32>(a, st);
+  return hd == 64 ? launch_write_tile<T, 64, KIND>(a, st) : launch_write_tile<T, 128, KIND>(a, st);
 }
 template <int KIND>
 int launch_write_io(WriteArgs& a, int io_dtype, int hd, cudaStream_t st) {
@@ -457,8 +552,10 @@ int check_write(const char* who, const WriteArgs& a, int io_dtype, int hd) {
   B200_REQUIRE(a.k_out != a.k && a.k_out != a.v && a.q_out != a.k && a.q_out != a.v && a.k_out != a.q && a.q_out != a.q &&
                    a.q_out != a.k_out,
                "%s: q_out and k_out must not be inputs", who);
-  const int64_t grid = static_cast<int64_t>(a.bs) * ((a.sl - 1) / 32 + 2) * a.kv_heads;
-  B200_REQUIRE(grid <= 0x7fffffff, "%s: %d sequences of %d tokens are too many for one call", who, a.bs, a.sl);
+  // CTAs of K and V, and at most one for each 16 heads of a token
+  const double grid = static_cast<double>(a.bs) * ((a.sl - 1) / 32 + 2) * a.kv_heads +
+                      static_cast<double>(a.bs) * a.sl * (a.heads / 4 + 1) / 16 + 1;
+  B200_REQUIRE(grid < 2147483647.0, "%s: %d sequences of %d tokens are too many for one call", who, a.bs, a.sl);
   return B200MOE_OK;
 }
 
@@ -708,7 +805,10 @@ struct Stretches {
 
 // CTAs per SM: shared memory of the ring, registers
 template <int HD, int NT, bool SPLIT>
-constexpr int attend_resident() { return HD == 128 ? (NT == 1 ? (SPLIT ? 3 : 4) : (SPLIT ? 2 : 3)) : (NT == 1 ? 5 : 4); }
+constexpr int attend_resident() {
+  if (NT == 4) return HD == 128 ? 2 : 3;
+  return HD == 128 ? (NT == 1 ? (SPLIT ? 3 : 4) : (SPLIT ? 2 : 3)) : (NT == 1 ? (SPLIT ? 4 : 5) : (SPLIT ? 3 : 4));
+}
 
 template <int HD, int CODE, int NT, bool SPLIT>
 __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())) kv8_attend_kernel(const AttendArgs a) {
@@ -722,6 +822,10 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
   float* s_o = reinterpret_cast<float*>(smem + AT_WARPS * 2 * TILE);
   __shared__ float4 s_pos[AT_WARPS][AT_UNIT];       // of each position: s_k, log2 s_v, 1 / s_v
   __shared__ float2 s_ml[AT_WARPS][ROWS];
+  constexpr bool Q_SHARED = NT == 4;
+  static_assert(!Q_SHARED || (AT_WARPS == NT && !SPLIT), "a warp prepares one tile of q");
+  __shared__ uint2 s_q[Q_SHARED ? CH : 1][NT][32];
+  __shared__ float s_fold[ROWS];
   grid_dep_wait();
   grid_dep_launch();
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gid = lane >> 2, tig = lane & 3;
@@ -835,12 +939,15 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
       next.p_end = next.units = 0;
     }
 
-    // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two
-    uint32_t qb[PARTS][NT][CH][2];
+    // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two.  Four
+    // columns' tiles do not fit in registers beside the output: there a warp prepares one, in
+    // the order of the fragments, and all read them from shared memory.
+    constexpr int QN = Q_SHARED ? 1 : NT;
+    uint32_t qb[PARTS][QN][CH][2];
     float fold[NT][2];  // of this lane's accumulator columns 2 tig, 2 tig + 1: back to to_score units
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = tile * ROWS + 8 * n + gid;
+    for (int n = 0; n < QN; ++n) {
+      const int r = tile * ROWS + 8 * (Q_SHARED ? warp : n) + gid;
       float x[CH][4], top = 0.f;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
@@ -861,8 +968,12 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
       if (__float_as_uint(top) == 0x7f800000u) e = 100;
       const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
       const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23) * to_score;
-      fold[n][0] = __shfl_sync(0xffffffffu, down, (2 * tig) * 4);
-      fold[n][1] = __shfl_sync(0xffffffffu, down, (2 * tig + 1) * 4);
+      if constexpr (Q_SHARED) {
+        if (tig == 0) s_fold[8 * warp + gid] = down;
+      } else {
+        fold[n][0] = __shfl_sync(0xffffffffu, down, (2 * tig) * 4);
+        fold[n][1] = __shfl_sync(0xffffffffu, down, (2 * tig + 1) * 4);
+      }
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -875,6 +986,17 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
             qb[PARTS - 1][n][c][i] = h2_as_u32(__floats2half2_rn(u - f.x, v - f.y));
           }
         }
+    }
+    if constexpr (Q_SHARED) {
+      // (the last segment's q is read: its end has a barrier)
+#pragma unroll
+      for (int c = 0; c < CH; ++c) s_q[c][warp][lane] = make_uint2(qb[0][0][c][0], qb[0][0][c][1]);
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        fold[n][0] = s_fold[8 * n + 2 * tig];
+        fold[n][1] = s_fold[8 * n + 2 * tig + 1];
+      }
     }
     // the first position that a column does not see
     const int all_see = len - a.sl + 1;
@@ -903,36 +1025,51 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
       const uint32_t kt = ring, vt = kt + TILE;
       const int p0 = cur.p_begin + u * AT_STEP;
 
-      // two accumulators for each 16 positions where there are no others to alternate with
-      constexpr int ACC = NT == 1 ? 2 : 1;
+      // two accumulators for each 16 positions where there are no others to alternate with;
+      // both halves of the unit at once where q comes from shared memory
+      constexpr int ACC = NT == 1 ? 2 : 1, HB = Q_SHARED ? 2 : 1;
       float s[2][NT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float acc[ACC][NT][4];
+      for (int h0 = 0; h0 < 2; h0 += HB) {
+        float acc[ACC][HB][NT][4];
 #pragma unroll
         for (int k = 0; k < ACC; ++k)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) acc[k][n][0] = acc[k][n][1] = acc[k][n][2] = acc[k][n][3] = 0.f;
+          for (int h = 0; h < HB; ++h)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[k][h][n][0] = acc[k][h][n][1] = acc[k][h][n][2] = acc[k][h][n][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; c += 2) {
-          uint32_t w[4];
-          ldsm_x4(kt + ld_at[c / 2] + 16 * h * HD, w);
+          uint32_t w[HB][4];
+#pragma unroll
+          for (int h = 0; h < HB; ++h) ldsm_x4(kt + ld_at[c / 2] + 16 * (h0 + h) * HD, w[h]);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t a0, a1, a2, a3;
-            widen4<CODE, false>(w[2 * i], a0, a2);
-            widen4<CODE, false>(w[2 * i + 1], a1, a3);
+            uint32_t f[HB][4];
+#pragma unroll
+            for (int h = 0; h < HB; ++h) {
+              widen4<CODE, false>(w[h][2 * i], f[h][0], f[h][2]);
+              widen4<CODE, false>(w[h][2 * i + 1], f[h][1], f[h][3]);
+            }
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
-                mma(acc[i % ACC][n], a0, a1, a2, a3, qb[p][n][c + i][0], qb[p][n][c + i][1]);
+              for (int n = 0; n < NT; ++n) {
+                uint2 y;
+                if constexpr (Q_SHARED) y = s_q[c + i][n][lane];
+                else y = make_uint2(qb[p][n][c + i][0], qb[p][n][c + i][1]);
+#pragma unroll
+                for (int h = 0; h < HB; ++h) mma(acc[i % ACC][h][n], f[h][0], f[h][1], f[h][2], f[h][3], y.x, y.y);
+              }
           }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int h = 0; h < HB; ++h)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[h][n][k] = ACC == 2 ? acc[0][n][k] + acc[ACC - 1][n][k] : acc[0][n][k];
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              s[h0 + h][n][k] = ACC == 2 ? acc[0][h][n][k] + acc[ACC - 1][h][n][k] : acc[0][h][n][k];
       }
       __syncwarp();  // K is read: its place takes that of the next unit
       const bool last = u + 1 == units;
@@ -1219,12 +1356,17 @@ int launch_merge(const AttendArgs& a, int tile_rows, cudaStream_t st) {
 
 // Rows of a CTA's tile; CTAs of a call: as many as are resident at once, or one for each
 // step of a full page table where those are fewer.
-inline int attend_tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
-int attend_ctas(int bs, int kv_heads, int hd, int rows, int max_seq_len) {
-  const int tile = attend_tile_rows(rows);
+inline int attend_tile_rows(int rows, bool split) { return rows <= 8 ? 8 : rows <= 16 || split ? 16 : 32; }
+template <int HD>
+int resident_ctas(int tile, bool split) {
+  if (tile == 32) return attend_resident<HD, 4, false>();
+  if (tile == 16) return split ? attend_resident<HD, 2, true>() : attend_resident<HD, 2, false>();
+  return split ? attend_resident<HD, 1, true>() : attend_resident<HD, 1, false>();
+}
+int attend_ctas(int bs, int kv_heads, int hd, int rows, bool split, int max_seq_len) {
+  const int tile = attend_tile_rows(rows, split);
   const int64_t steps = (static_cast<int64_t>(max_seq_len) + AT_STEP - 1) / AT_STEP * bs * kv_heads * ((rows + tile - 1) / tile);
-  const int64_t resident = static_cast<int64_t>(sm_count()) * (hd == 128 ? (tile == 8 ? attend_resident<128, 1, false>() : attend_resident<128, 2, false>())
-                                                                         : (tile == 8 ? attend_resident<64, 1, false>() : attend_resident<64, 2, false>()));
+  const int64_t resident = static_cast<int64_t>(sm_count()) * (hd == 128 ? resident_ctas<128>(tile, split) : resident_ctas<64>(tile, split));
   return static_cast<int>(steps < resident ? steps : resident);
 }
 
@@ -1244,6 +1386,7 @@ int launch_attend(const AttendArgs& a, cudaStream_t st) {
 }
 template <int HD, int CODE>
 int launch_attend_rows(const AttendArgs& a, bool split, int tile_rows, cudaStream_t st) {
+  if (tile_rows == 32) return launch_attend<HD, CODE, 4, false>(a, st);
   if (tile_rows == 8) return split ? launch_attend<HD, CODE, 1, true>(a, st) : launch_attend<HD, CODE, 1, false>(a, st);
   return split ? launch_attend<HD, CODE, 2, true>(a, st) : launch_attend<HD, CODE, 2, false>(a, st);
 }
@@ -1271,6 +1414,8 @@ int b200moe_attn_norm_rope_kv8_write(const void* q, const void* k, const void* v
   a.page_ids = page_ids; a.freqs = freqs; a.order = order; a.bs = bs; a.sl = tokens_per_seq;
   a.pages_per_seq = pages_per_seq; a.page_count = cache->page_count; a.heads = heads; a.kv_heads = cache->kv_heads;
   a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index; a.scale_block = cache->scale_block;
+  a.stride_shift = log2_of(a.stride);
+  a.block_shift = log2_of(a.scale_block);
   if (const int rc = check_write(who, a, io_dtype, cache->head_dim)) return rc;
   if (bs == 0) return B200MOE_OK;
   B200_REQUIRE(scales != nullptr && (reinterpret_cast<uintptr_t>(scales) & 7) == 0,
@@ -1299,6 +1444,7 @@ int b200moe_attn_norm_rope_kv_write(const void* q, const void* k, const void* v,
   a.page_ids = page_ids; a.freqs = freqs; a.order = order; a.bs = bs; a.sl = tokens_per_seq;
   a.pages_per_seq = pages_per_seq; a.page_count = cache->page_count; a.heads = heads; a.kv_heads = cache->kv_heads;
   a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index; a.scale_block = 1;
+  a.stride_shift = log2_of(a.stride);
   if (const int rc = check_write(who, a, io_dtype, cache->head_dim)) return rc;
   if (bs == 0) return B200MOE_OK;
   a.status = device_status_ptr();
@@ -1342,9 +1488,14 @@ size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_
   if (cache == nullptr || bs <= 0 || new_tokens <= 0 || new_tokens > MAX_NEW_TOKENS || heads <= 0 || max_seq_len <= 0 ||
       cache->kv_heads <= 0 || heads % cache->kv_heads != 0)
     return 0;
-  const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows);
-  const int ctas = attend_ctas(bs, cache->kv_heads, cache->head_dim, rows, max_seq_len);
-  return static_cast<size_t>(ctas) * 2 * tile * (cache->head_dim + 4) * sizeof(float);
+  const int rows = heads / cache->kv_heads * new_tokens;
+  size_t most = 0;  // the activations' type is not known here: enough for any
+  for (const bool split : {false, true}) {
+    const size_t n = static_cast<size_t>(attend_ctas(bs, cache->kv_heads, cache->head_dim, rows, split, max_seq_len)) * 2 *
+                     attend_tile_rows(rows, split) * (cache->head_dim + 4) * sizeof(float);
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void* slab, const float* scales,
@@ -1378,9 +1529,11 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   a.out_dtype = out_dtype; a.bs = bs; a.sl = new_tokens;
   a.pages_per_seq = pages_per_seq; a.page_count = cache->page_count; a.heads = heads; a.kv_heads = cache->kv_heads;
   a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index;
-  const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows), hd = cache->head_dim;
+  // 32-bit activations: 22 bits of q and of the probabilities
+  const bool split = q_dtype == B200MOE_DT_F32 || out_dtype == B200MOE_DT_F32;
+  const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows, split), hd = cache->head_dim;
   a.row_tiles = (rows + tile - 1) / tile;
-  a.ctas = attend_ctas(bs, cache->kv_heads, hd, rows, max_seq_len);
+  a.ctas = attend_ctas(bs, cache->kv_heads, hd, rows, split, max_seq_len);
   a.stride_shift = log2_of(a.stride);
   a.block_shift = log2_of(cache->scale_block);
   B200_REQUIRE(static_cast<double>(bs) * a.kv_heads * a.row_tiles * (1.0 + pages_per_seq * static_cast<double>(a.stride) / AT_STEP) < 2147483647.0,
@@ -1390,8 +1543,6 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   if (a.status == nullptr) return B200MOE_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool i8 = cache->code == B200MOE_KV8_INT8;
-  // 32-bit activations: 22 bits of q and of the probabilities
-  const bool split = q_dtype == B200MOE_DT_F32 || out_dtype == B200MOE_DT_F32;
   int rc;
   if (hd == 64)
     rc = i8 ? launch_attend_rows<64, B200MOE_KV8_INT8>(a, split, tile, st)
