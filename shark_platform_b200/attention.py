@@ -337,9 +337,11 @@ class B200PagedAttentionBlock(torch.nn.Module):
         self.rms_epsilon = rms_epsilon
         self.attention_kernel, self.attention_scale, self.softcap = attention_kernel, attention_scale, softcap
         if "kv_cache" in getattr(theta, "keys", ()):
-            raise C.B200MoeError("a quantized KV cache (kv_cache.quantizer) is not supported")
-        if head_count % head_count_kv != 0 or head_count // head_count_kv > 8:
-            raise C.B200MoeError("head_count must be 1..8 times head_count_kv")
+            raise C.B200MoeError("a quantized KV cache (kv_cache.quantizer) is not supported: its one scale per tensor "
+                                 "is replaced by PagedKVCache(dtype=torch.int8 or torch.float8_e4m3fn)")
+        self._quantized = bool(getattr(cache, "quantized", False))
+        if head_count % head_count_kv != 0 or (head_count // head_count_kv > 8 and not self._quantized):
+            raise C.B200MoeError("head_count must be 1..8 times head_count_kv (any multiple with an 8-bit cache)")
         if head_dim not in (64, 128):
             raise C.B200MoeError(f"head_dim {head_dim}: 64 and 128 are built")
         if cache.attn_head_count != head_count_kv or cache.attn_head_dim != head_dim:
@@ -350,6 +352,13 @@ class B200PagedAttentionBlock(torch.nn.Module):
         self._out_norm_w = None
         if theta.optional_tensor("attn_output_norm") is not None:
             self._out_norm_w = _moe._unbox(w("attn_output_norm")).to(torch.float32).contiguous()
+        # norms of every query and key head, before the rotation
+        self._q_norm_w, self._k_norm_w = (
+            _moe._unbox(w(n)).to(torch.float32).contiguous() if n in theta.keys else None
+            for n in ("attn_q_norm", "attn_k_norm"))
+        for x in (self._q_norm_w, self._k_norm_w):
+            if x is not None and x.shape != (head_dim,):
+                raise C.B200MoeError(f"attn_q_norm and attn_k_norm have one weight per element of a head ({head_dim})")
         wq, wk, wv, self._wo = w("attn_q"), w("attn_k"), w("attn_v"), w("attn_output")
         self._bias = {n: theta(n).optional_tensor("bias") if "bias" in theta(n).keys else None
                       for n in ("attn_q", "attn_k", "attn_v", "attn_output")}
@@ -386,8 +395,6 @@ class B200PagedAttentionBlock(torch.nn.Module):
 
     def _freq_table(self, embedding, device):
         if self._freqs is None or self._freqs.device != device:
-            if getattr(embedding, "use_hf", False):
-                raise C.B200MoeError("the HuggingFace rotary ordering (use_hf) is not supported")
             dim = embedding.rope_dimension_count
             if dim != self.head_dim:
                 raise C.B200MoeError("rope_dimension_count must equal head_dim")
@@ -402,22 +409,36 @@ class B200PagedAttentionBlock(torch.nn.Module):
                 start_index: Optional[int] = None, start_positions: Optional[torch.Tensor] = None,
                 attention_mask: Optional[torch.Tensor] = None, embedding_batch_mask: Optional[torch.Tensor] = None,
                 cache_state: list = None, xk_temp: Optional[torch.Tensor] = None,
-                xv_temp: Optional[torch.Tensor] = None) -> torch.Tensor:
+                xv_temp: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """`new_lens` [bs] (prefill; not in the reference): how many of each sequence's rows are
+        tokens; padding behind them is not written to the cache.  With an 8-bit cache a decode
+        step may bring up to 16 tokens per sequence (each attends the ones before it), a
+        negative start position marks a padding sequence, and a prefill with start_index > 0
+        attends the cached positions before it too (an attention_mask then covers the new
+        positions, or all of them)."""
         _moe._require_cuda(h, "h")
         if h.dtype not in _DT:
             raise C.B200MoeError(f"activations must be fp32, fp16 or bf16, got {h.dtype}")
         if (start_index is not None) == (start_positions is not None):
             raise C.B200MoeError("exactly one of start_index (prefill) and start_positions (decode) is given")
         slab = cache_state[0]
-        if slab.dtype not in _DT or not slab.is_contiguous():
+        if not self._quantized and (slab.dtype not in _DT or not slab.is_contiguous()):
             raise C.B200MoeError("the page slab must be a contiguous fp32, fp16 or bf16 tensor")
         dev = h.device
         bs, sl, d = h.shape
         H, Hkv, hd = self.head_count, self.head_count_kv, self.head_dim
         stride = self.cache.block_seq_stride
         decode = start_positions is not None
-        if decode and sl != 1:
+        if decode and sl != 1 and not self._quantized:
             raise C.B200MoeError("a decode step brings one token per sequence")
+        if decode and sl > MAX_NEW_TOKENS:
+            raise C.B200MoeError(f"a decode step brings at most {MAX_NEW_TOKENS} tokens per sequence")
+        if decode and new_lens is not None:
+            raise C.B200MoeError("new_lens is for prefill; a negative start position marks a padding sequence of a step")
+        use_hf = bool(getattr(embedding, "use_hf", False))
+        # norms, the HuggingFace order, padding and 8-bit codes: the one-pass write
+        one_pass = (self._quantized or use_hf or new_lens is not None or self._q_norm_w is not None or
+                    self._k_norm_w is not None)
         hc = h.contiguous()
         # the output projection with the residual, in one call
         fused_out = (self._fits_linear(self._wo) and [int(n) for n in self._wo.shape] == [d, H * hd] and
@@ -426,7 +447,8 @@ class B200PagedAttentionBlock(torch.nn.Module):
             x = self._norm(hc, self._norm_w)
             qkv = F.linear(x, self._wqkv.to(x.dtype))
             q, k, v = torch.split(qkv, [H * hd, Hkv * hd, Hkv * hd], dim=-1)
-            q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+            if not one_pass:
+                q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
         elif self._fits_linear(self._wq, self._wk, self._wv) and int(self._wq.shape[1]) == d:
             # norm and the three projections in one call
             q, k, v = _moe.linear_rows(hc.view(bs * sl, d), [_moe.prepare_linear(w) for w in (self._wq, self._wk, self._wv)],
@@ -441,28 +463,43 @@ class B200PagedAttentionBlock(torch.nn.Module):
         if self._wqkv is not None and any(self._bias[n] is not None for n in ("attn_q", "attn_k", "attn_v")):
             raise C.B200MoeError("projection biases are supported with unfused (quantized) weights only")
         tokens = bs * sl
-        if decode:
-            positions = start_positions.to(torch.int32).contiguous()
-        else:
-            positions = (torch.arange(sl, device=dev, dtype=torch.int32) + int(start_index)).repeat(bs)
         page_ids = seq_block_ids.to(torch.int32).contiguous()
         self._desc.page_count = slab.shape[0]
-        # prefill attends the fresh K and V: K is rotated in place, V is used as it is
-        k_out, v_out = (None, None) if decode else (k, v)
-        with torch.cuda.device(dev):
-            C.check(C.lib.b200moe_attn_rope_kv_write(
-                _p(q), _p(k), _p(v), _p(k_out), _p(v_out), _DT[q.dtype], _p(slab), _DT[slab.dtype],
-                ctypes.byref(self._desc), self.block_index, _p(positions), _p(page_ids),
-                _p(self._freq_table(embedding, dev)), tokens, sl, page_ids.shape[1], H, _moe._stream()),
-                "attn_rope_kv_write")
+        if one_pass:
+            start = (start_positions.to(torch.int32).contiguous() if decode else
+                     torch.full((bs,), int(start_index), device=dev, dtype=torch.int32))
+            q, k = norm_rope_kv_write(q.view(bs, sl, H, hd), k.view(bs, sl, Hkv, hd), v.view(bs, sl, Hkv, hd), self.cache,
+                                      cache_state, block_index=self.block_index, seq_block_ids=page_ids,
+                                      start_positions=start, new_lens=new_lens, freqs=self._freq_table(embedding, dev),
+                                      q_norm=self._q_norm_w, k_norm=self._k_norm_w, eps=float(self.rms_epsilon),
+                                      use_hf=use_hf)
+            positions = start
+        else:
+            if decode:
+                positions = start_positions.to(torch.int32).contiguous()
+            else:
+                positions = (torch.arange(sl, device=dev, dtype=torch.int32) + int(start_index)).repeat(bs)
+            # prefill attends the fresh K and V: K is rotated in place, V is used as it is
+            k_out, v_out = (None, None) if decode else (k, v)
+            with torch.cuda.device(dev):
+                C.check(C.lib.b200moe_attn_rope_kv_write(
+                    _p(q), _p(k), _p(v), _p(k_out), _p(v_out), _DT[q.dtype], _p(slab), _DT[slab.dtype],
+                    ctypes.byref(self._desc), self.block_index, _p(positions), _p(page_ids),
+                    _p(self._freq_table(embedding, dev)), tokens, sl, page_ids.shape[1], H, _moe._stream()),
+                    "attn_rope_kv_write")
         scale = self.attention_scale if self.attention_scale is not None else 1.0 / math.sqrt(hd)
-        if decode:
+        # a Q8_0 output projection reads fp16 rows: no cast in between
+        direct = fused_out and _moe._layout_name(self._wo) == "BlockScaledLayout"
+        if decode and self._quantized:
+            # a padding sequence (negative position) attends nothing
+            attn = kv_attend(q, self.cache, cache_state, block_index=self.block_index, seq_block_ids=page_ids,
+                             seq_lens=torch.where(positions < 0, 0, positions + sl), scale=float(scale),
+                             softcap=self.softcap, out_dtype=torch.float16 if direct else h.dtype).view(bs, sl, H * hd)
+        elif decode:
             # positions to attend: everything up to and including the new row (what the
             # reference's decode mask leaves unmasked)
             seq_lens = (positions + 1).contiguous()
             max_len = page_ids.shape[1] * stride
-            # a Q8_0 output projection reads fp16 rows: no cast in between
-            direct = fused_out and _moe._layout_name(self._wo) == "BlockScaledLayout"
             out = torch.empty(bs, H * hd, dtype=torch.float16 if direct else h.dtype, device=dev)
             nbytes = C.lib.b200moe_attn_decode_scratch_bytes(ctypes.byref(self._desc), bs, H, max_len)
             # per call, as the layer's workspace: other streams and captured graphs have their own
@@ -476,9 +513,20 @@ class B200PagedAttentionBlock(torch.nn.Module):
             attn = out.view(bs, 1, H * hd)
         else:
             qh = q.view(bs, sl, H, hd).transpose(1, 2)
-            kh = k.view(bs, sl, Hkv, hd).transpose(1, 2)
-            vh = v.view(bs, sl, Hkv, hd).transpose(1, 2)
+            kh = k.view(bs, sl, Hkv, hd)
+            vh = v.view(bs, sl, Hkv, hd)
             mask = None if attention_mask is None else attention_mask.to(q.dtype)
+            before = int(start_index) if self._quantized else 0
+            if before:  # a continued prompt: the cached positions, then the new ones as they are
+                kc, vc = kv_read(self.cache, cache_state, block_index=self.block_index, seq_block_ids=page_ids,
+                                 seq_lens=torch.full((bs,), before, device=dev, dtype=torch.int32), max_seq_len=before,
+                                 dtype=q.dtype)
+                kh, vh = torch.cat([kc, kh], dim=1), torch.cat([vc, vh], dim=1)
+                if mask is None:
+                    mask = torch.full((sl, before + sl), float("-inf"), device=dev, dtype=q.dtype).triu(before + 1)
+                elif mask.shape[-1] == sl:
+                    mask = F.pad(mask, (before, 0))
+            kh, vh = kh.transpose(1, 2), vh.transpose(1, 2)
             if self.softcap is None:
                 attn = F.scaled_dot_product_attention(qh, kh, vh, attn_mask=mask, is_causal=mask is None,
                                                       scale=scale, enable_gqa=H != Hkv)

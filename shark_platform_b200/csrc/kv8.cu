@@ -929,7 +929,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
   for (int g = g_begin; g < g_end;) {
     const Piece cur = next;
     if (cur.x1 == 0) break;  // the stretch ends before the segment's first step
-    const int b = cur.b, kvh = cur.kvh, tile = cur.tile, len = cur.len, units = cur.units;
+    const int b = cur.b, kvh = cur.kvh, tile = cur.tile, units = cur.units;
     if (cur.x0 == 0 && t == 0 && a.seq_lens[b] > a.pages_per_seq * a.stride) atomicOr(a.status, DEV_ERR_BOUNDS);
     int page_next = page_of(cur, 1), page_after = -1;
     if (cur.end < g_end) {
@@ -999,7 +999,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
       }
     }
     // the first position that a column does not see
-    const int all_see = len - a.sl + 1;
+    const int all_see = a.seq_lens[b] - a.sl + 1;
     auto seen = [&](int n, int j) { return all_see + (tile * ROWS + 8 * n + 2 * tig + j) / G; };
 
     float m[NT][2], l[NT][2], o[NT][CH][4];
