@@ -187,6 +187,27 @@ for _name, (_res, _args) in _PROTOS.items():
     _fn.argtypes = _args
 
 
+def _load_attention_ops():
+    """The compiled torch binding of attention.py's cache operators, on this library's entry points."""
+    import importlib.util
+
+    import torch  # noqa: F401  (the binding resolves its symbols in torch's libraries)
+
+    path = os.path.join(HERE, "lib", "_attention_ops.so")
+    if not os.path.exists(path):
+        raise B200MoeError(f"{path} is missing: build it with `python -m shark_platform_b200.build`")
+    spec = importlib.util.spec_from_file_location("_attention_ops", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.bind(B200MoeError, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
+        "b200moe_attn_norm_rope_kv8_write", "b200moe_attn_norm_rope_kv_write", "b200moe_kv8_read", "b200moe_kv8_attend",
+        "b200moe_kv8_attend_scratch_bytes", "b200moe_last_error")))
+    return module
+
+
+attention_ops = _load_attention_ops()
+
+
 def last_error() -> str:
     return lib.b200moe_last_error().decode()
 

@@ -96,6 +96,8 @@ class PagedKVCache:
             self.scale_block = None
             self.sub_page_dims = [transformer_block_count, 2, block_seq_stride, attn_head_count, attn_head_dim]
         self.page_slab_flat_dim = math.prod(self.sub_page_dims)
+        self._geometry = (transformer_block_count, block_seq_stride, attn_head_count, attn_head_dim,
+                          self.scale_block or 1, _KV8_CODES.get(dtype, -1))
 
     def allocate(self, page_count: int) -> list[torch.Tensor]:
         """[page slab], or [page slab, scales] for 8-bit codes: a row of each per page."""
@@ -106,63 +108,12 @@ class PagedKVCache:
 
 
 # ------------------------------------------------------------- cache operators
-# Called once per layer and token: messages are built only when raised, the device is
-# switched only where it is not the current one.
-def _int32(t: torch.Tensor) -> torch.Tensor:
-    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
-
-
-def _launch(what: str, dev: torch.device, fn, *args) -> None:
-    """fn(*args, stream) with `dev` current, on dev's current stream."""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    if rc:
-        C.check(rc, what)
-
-
-def _check_cache(cache, state, block_index: int, seq_block_ids: torch.Tensor, bs: int, dev) -> None:
-    slab = state[0]
-    if not 0 <= block_index < cache.transformer_block_count:
-        raise C.B200MoeError(f"block_index {block_index} is not one of the cache's {cache.transformer_block_count} "
-                             "transformer blocks")
-    if slab.dim() != 2 or slab.shape[1] != cache.page_slab_flat_dim or not slab.is_contiguous():
-        raise C.B200MoeError("the page slab must be contiguous, a row of the cache's page size per page")
-    if getattr(cache, "quantized", False):
-        if len(state) != 2:
-            raise C.B200MoeError("a cache of 8-bit codes is [page slab, scales], as allocate() gives it")
-        scales = state[1]
-        if slab.dtype is not cache.dtype:
-            raise C.B200MoeError(f"the page slab must be {cache.dtype}, got {slab.dtype}")
-        if (scales.dtype is not torch.float32 or scales.shape != (slab.shape[0], cache.scale_flat_dim) or
-                not scales.is_contiguous() or scales.device != dev):
-            raise C.B200MoeError("scales must be fp32, contiguous, beside the slab, a row per page")
-    elif slab.dtype not in _DT:
-        raise C.B200MoeError("the page slab must be a contiguous fp32, fp16 or bf16 tensor")
-    if seq_block_ids.dim() != 2 or seq_block_ids.shape[0] != bs or seq_block_ids.shape[1] < 1:
-        raise C.B200MoeError(f"seq_block_ids must be [{bs}, pages of a sequence], got {list(seq_block_ids.shape)}")
-    if slab.device != dev or seq_block_ids.device != dev:
-        raise C.B200MoeError("cache, page ids and activations must be on one device")
-
-
-def _kv8_desc(cache, pages: int):
-    return C.Kv8CacheDesc(cache.transformer_block_count, cache.block_seq_stride, cache.attn_head_count,
-                          cache.attn_head_dim, pages, cache.scale_block, _KV8_CODES[cache.dtype])
-
-
-def _rows(x: torch.Tensor):
-    """x [bs, sl, heads, hd] as rows of heads * hd elements one stride apart, 16-byte
-    aligned (a view of a fused projection is that already): (tensor, stride)."""
-    bs, sl, heads, hd = x.shape
-    s = x.stride()
-    if s[3] == 1 and (heads == 1 or s[2] == hd) and (bs == 1 or sl == 1 or s[0] == sl * s[1]):
-        stride = s[1] if sl > 1 else s[0] if bs > 1 else heads * hd
-        if stride >= heads * hd and stride * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0:
-            return x, stride
-    # a contiguous view that does not start on 16 bytes is copied too
-    return x.clone(memory_format=torch.contiguous_format), heads * hd
+# Checks, outputs and launches are in csrc/attention_ops.cpp: these are called once per layer
+# and token.
+def _geometry(cache) -> tuple:
+    g = getattr(cache, "_geometry", None)  # sharktank's own PagedKVCache: 16- or 32-bit
+    return g if g is not None else (cache.transformer_block_count, cache.block_seq_stride, cache.attn_head_count,
+                                    cache.attn_head_dim, 1, -1)
 
 
 def norm_rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, cache_state: list, *,
@@ -186,47 +137,8 @@ def norm_rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache:
     fit, else the scale grows by a power of two and the block's earlier codes are rounded
     to it.  Positions behind the last written one of a block are dead until written.  An
     infinity or NaN makes its block read as NaN."""
-    bs, sl, heads, hd = q.shape
-    kvh = cache.attn_head_count
-    dt = q.dtype
-    if dt not in _DT or k.dtype is not dt or v.dtype is not dt:
-        raise C.B200MoeError(f"q, k and v must be fp32, fp16 or bf16 alike, got {dt}, {k.dtype}, {v.dtype}")
-    if hd != cache.attn_head_dim or k.shape != (bs, sl, kvh, hd) or v.shape != k.shape or heads % kvh:
-        raise C.B200MoeError(f"q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} do not fit a cache of {kvh} "
-                             f"heads of {cache.attn_head_dim}")
-    if start_positions.shape != (bs,) or (new_lens is not None and new_lens.shape != (bs,)):
-        raise C.B200MoeError(f"start_positions and new_lens are [{bs}]")
-    if freqs.dtype is not torch.float32 or freqs.shape != (hd // 2,) or not freqs.is_contiguous():
-        raise C.B200MoeError(f"freqs must be fp32 [{hd // 2}]")
-    dev = q.device
-    for w in (q_norm, k_norm):
-        if w is not None and (w.dtype is not torch.float32 or w.shape != (hd,) or not w.is_contiguous() or
-                              w.device != dev):
-            raise C.B200MoeError(f"norm weights must be fp32 [{hd}], on q's device")
-    _check_cache(cache, cache_state, block_index, seq_block_ids, bs, dev)
-    if (k.device != dev or v.device != dev or start_positions.device != dev or freqs.device != dev or
-            (new_lens is not None and new_lens.device != dev)):
-        raise C.B200MoeError("all arguments must be on one device")
-    _moe._require_cuda(q, "q")
-    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
-    q_out = torch.empty((bs, sl, heads, hd), dtype=dt, device=dev)
-    k_out = torch.empty((bs, sl, kvh, hd), dtype=dt, device=dev)
-    if bs * sl == 0:
-        return q_out, k_out
-    start, ids = _int32(start_positions), _int32(seq_block_ids)
-    lens = None if new_lens is None else _int32(new_lens)
-    slab = cache_state[0]
-    head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[dt], qs, ks, vs, None if q_norm is None else q_norm.data_ptr(),
-            None if k_norm is None else k_norm.data_ptr(), eps, q_out.data_ptr(), k_out.data_ptr(), slab.data_ptr())
-    tail = (block_index, start.data_ptr(), None if lens is None else lens.data_ptr(), ids.data_ptr(), freqs.data_ptr(),
-            1 if use_hf else 0, bs, sl, ids.shape[1], heads)
-    if getattr(cache, "quantized", False):
-        _launch("attn_norm_rope_kv8_write", dev, C.lib.b200moe_attn_norm_rope_kv8_write, *head, cache_state[1].data_ptr(),
-                _kv8_desc(cache, slab.shape[0]), *tail)
-    else:
-        desc = C.KvCacheDesc(cache.transformer_block_count, cache.block_seq_stride, kvh, hd, slab.shape[0])
-        _launch("attn_norm_rope_kv_write", dev, C.lib.b200moe_attn_norm_rope_kv_write, *head, _DT[slab.dtype], desc, *tail)
-    return q_out, k_out
+    return C.attention_ops.write(q, k, v, cache_state, _geometry(cache), block_index, seq_block_ids, start_positions, new_lens,
+                                 freqs, q_norm, k_norm, eps, use_hf)
 
 
 def kv_read(cache: PagedKVCache, cache_state: list, *, block_index: int, seq_block_ids: torch.Tensor,
@@ -235,29 +147,7 @@ def kv_read(cache: PagedKVCache, cache_state: list, *, block_index: int, seq_blo
     """K and V of the listed pages of an 8-bit cache, [bs, max_seq_len, kv_heads, head_dim]
     each (`max_seq_len`: all of the listed pages by default); every value code * scale,
     rounded once to `dtype`.  Rows at and behind seq_lens[b] are zero."""
-    if not getattr(cache, "quantized", False):
-        raise C.B200MoeError("kv_read reads caches of 8-bit codes")
-    if dtype not in _DT:
-        raise C.B200MoeError(f"K and V are read as fp32, fp16 or bf16, not {dtype}")
-    slab = cache_state[0]
-    bs, dev = seq_block_ids.shape[0], slab.device
-    if seq_lens.shape != (bs,) or seq_lens.device != dev:
-        raise C.B200MoeError(f"seq_lens is [{bs}], on the cache's device")
-    _check_cache(cache, cache_state, block_index, seq_block_ids, bs, dev)
-    _moe._require_cuda(slab, "the page slab")
-    held = seq_block_ids.shape[1] * cache.block_seq_stride
-    n = held if max_seq_len is None else int(max_seq_len)
-    if not 0 <= n <= held:
-        raise C.B200MoeError(f"max_seq_len {n}: the listed pages hold {held} positions")
-    shape = (bs, n, cache.attn_head_count, cache.attn_head_dim)
-    k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
-    if bs * n == 0:
-        return k, v
-    ids, lens = _int32(seq_block_ids), _int32(seq_lens)
-    _launch("kv8_read", dev, C.lib.b200moe_kv8_read, slab.data_ptr(), cache_state[1].data_ptr(),
-            _kv8_desc(cache, slab.shape[0]), block_index, ids.data_ptr(), lens.data_ptr(), bs, ids.shape[1], n,
-            k.data_ptr(), v.data_ptr(), _DT[dtype])
-    return k, v
+    return C.attention_ops.read(cache_state, _geometry(cache), block_index, seq_block_ids, seq_lens, max_seq_len, dtype)
 
 
 def kv_attend(q: torch.Tensor, cache: PagedKVCache, cache_state: list, *, block_index: int,
@@ -270,41 +160,8 @@ def kv_attend(q: torch.Tensor, cache: PagedKVCache, cache_state: list, *, block_
     up to and including its own, seq_lens[b] - sl + i; where that leaves none its output is
     zero.  scale: 1 / sqrt(head_dim) by default; softcap: c * tanh(score / c).  Returns
     [bs, sl, heads, head_dim]."""
-    if not getattr(cache, "quantized", False):
-        raise C.B200MoeError("kv_attend reads caches of 8-bit codes")
-    bs, sl, heads, hd = q.shape
-    dt, dev, slab = q.dtype, q.device, cache_state[0]
-    if out_dtype is None:
-        out_dtype = dt
-    if dt not in _DT or out_dtype not in _DT:
-        raise C.B200MoeError(f"activations must be fp32, fp16 or bf16, got {dt}, {out_dtype}")
-    if hd != cache.attn_head_dim or heads % cache.attn_head_count:
-        raise C.B200MoeError(f"q {list(q.shape)} does not fit a cache of {cache.attn_head_count} heads of "
-                             f"{cache.attn_head_dim}")
-    if not 1 <= sl <= MAX_NEW_TOKENS:
-        raise C.B200MoeError(f"{sl} new tokens: 1 to {MAX_NEW_TOKENS}; longer stretches attend kv_read's K and V")
-    if softcap is not None and not softcap > 0:
-        raise C.B200MoeError("softcap must be positive")
-    if seq_lens.shape != (bs,) or seq_lens.device != dev:
-        raise C.B200MoeError(f"seq_lens is [{bs}], on q's device")
-    _check_cache(cache, cache_state, block_index, seq_block_ids, bs, dev)
-    _moe._require_cuda(q, "q")
-    q, qs = _rows(q)
-    out = torch.empty((bs, sl, heads, hd), dtype=out_dtype, device=dev)
-    if bs == 0:
-        return out
-    ids, lens = _int32(seq_block_ids), _int32(seq_lens)
-    per_seq = ids.shape[1]
-    max_len = per_seq * cache.block_seq_stride
-    desc = _kv8_desc(cache, slab.shape[0])
-    nbytes = C.lib.b200moe_kv8_attend_scratch_bytes(desc, bs, sl, heads, max_len)
-    # per call: other streams and captured graphs have their own
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch("kv8_attend", dev, C.lib.b200moe_kv8_attend, q.data_ptr(), _DT[dt], qs, slab.data_ptr(),
-            cache_state[1].data_ptr(), desc, block_index, ids.data_ptr(), lens.data_ptr(), bs, sl, per_seq, heads, max_len,
-            1.0 / math.sqrt(hd) if scale is None else scale, 0.0 if softcap is None else softcap, out.data_ptr(),
-            _DT[out_dtype], scratch.data_ptr(), nbytes)
-    return out
+    return C.attention_ops.attend(q, cache_state, _geometry(cache), block_index, seq_block_ids, seq_lens, scale, softcap,
+                                  out_dtype)
 
 
 class RotaryEmbeddingLayer:

@@ -1,4 +1,5 @@
-"""Builds the CUDA library in-tree: csrc/*.cu -> lib/libb200moe.so (sm_100a only).
+"""Builds the CUDA library in-tree: csrc/*.cu -> lib/libb200moe.so (sm_100a only), and the
+torch binding of the cache operators: csrc/attention_ops.cpp -> lib/_attention_ops.so.
 
 nvcc cross-compiles without a GPU.  Objects are rebuilt only when a source or
 header is newer.  Run as `python -m shark_platform_b200.build [--force] [--verbose]`.
@@ -15,9 +16,11 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libb200moe.so")
+OPS = os.path.join(LIBDIR, "_attention_ops.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+CXX = os.environ.get("CXX", "g++")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
@@ -37,6 +40,19 @@ def _headers_mtime():
     return max(os.path.getmtime(p) for p in paths)
 
 
+def _ops_command() -> list[str]:
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    return [CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", f"-I{root}/include",
+            f"-I{root}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", os.path.join(CSRC, "attention_ops.cpp"),
+            "-o", OPS, f"-L{root}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -53,6 +69,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
                 cmd.insert(1, "-Xptxas=-v")
             jobs.append(cmd)
 
+    src = os.path.join(CSRC, "attention_ops.cpp")
+    if force or not os.path.exists(OPS) or os.path.getmtime(OPS) < max(os.path.getmtime(src), hdr):
+        jobs.append(_ops_command())
+
     def run(cmd):
         r = subprocess.run(cmd, capture_output=True, text=True)
         return cmd, r
@@ -63,8 +83,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
                 if verbose or r.returncode != 0:
                     sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr + "\n")
                 if r.returncode != 0:
-                    raise RuntimeError(f"nvcc failed on {cmd[-3]}")
-    if jobs or not os.path.exists(LIB):
+                    raise RuntimeError(f"{os.path.basename(cmd[0])} failed: {' '.join(cmd)}")
+    if any(cmd[0] == NVCC for cmd in jobs) or not os.path.exists(LIB):
         cmd = [NVCC, "-shared", "-o", LIB, *objs, "-cudart", "static",
                "-gencode", "arch=compute_100a,code=sm_100a"]
         r = subprocess.run(cmd, capture_output=True, text=True)
