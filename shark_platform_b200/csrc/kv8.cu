@@ -67,7 +67,7 @@ __device__ __forceinline__ float round_to(float v) {
   else if constexpr (std::is_same<T, __half>::value) return __half2float(__float2half_rn(v));
   else return __bfloat162float(__float2bfloat16_rn(v));
 }
-// 2 or 4 consecutive elements of a type known at run time
+// 2 or 4 consecutive elements; stored as a type known at run time
 template <int N>
 __device__ __forceinline__ void load_elems(const float* p, float (&v)[N]) {
   if constexpr (N == 4) {
@@ -76,22 +76,6 @@ __device__ __forceinline__ void load_elems(const float* p, float (&v)[N]) {
   } else {
     const float2 a = *reinterpret_cast<const float2*>(p);
     v[0] = a.x; v[1] = a.y;
-  }
-}
-template <int N>
-__device__ __forceinline__ void load_elems(const __half* p, float (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float2 f = __half22float2(reinterpret_cast<const __half2*>(p)[i / 2]);
-    v[i] = f.x; v[i + 1] = f.y;
-  }
-}
-template <int N>
-__device__ __forceinline__ void load_elems(const __nv_bfloat16* p, float (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(p)[i / 2]);
-    v[i] = f.x; v[i + 1] = f.y;
   }
 }
 template <int N>
@@ -734,13 +718,6 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <int N>
-__device__ __forceinline__ void load_as(const void* p, int dtype, int64_t i, float (&v)[N]) {
-  if (dtype == B200MOE_DT_F32) load_elems(static_cast<const float*>(p) + i, v);
-  else if (dtype == B200MOE_DT_F16) load_elems(static_cast<const __half*>(p) + i, v);
-  else load_elems(static_cast<const __nv_bfloat16*>(p) + i, v);
-}
-
 // Byte offset of 16-byte chunk c of row r in a tile of rows of HD bytes: the eight chunks
 // that one ldmatrix phase reads (eight rows, one c) lie in eight different bank groups.
 template <int HD>
@@ -917,10 +894,50 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
     copy_commit();
   };
 
+  // q as it lies in memory: a lane's four elements of each chunk of its column's row
+  constexpr int QN = Q_SHARED ? 1 : NT;
+  uint32_t q_raw[QN][CH][SPLIT ? 4 : 2];
+  auto load_q = [&](const Piece& p) {
+#pragma unroll
+    for (int n = 0; n < QN; ++n) {
+      const int r = p.tile * ROWS + 8 * (Q_SHARED ? warp : n) + gid;
+      const int64_t from = (static_cast<int64_t>(p.b) * a.sl + r / G) * a.q_stride +
+                           static_cast<int64_t>(p.kvh * G + r % G) * HD + 4 * tig;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int i = 0; i < (SPLIT ? 4 : 2); ++i) q_raw[n][c][i] = 0u;
+        if (r < rows) {
+          if (SPLIT && a.q_dtype == B200MOE_DT_F32) {
+            const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.q) + from + 16 * c);
+            q_raw[n][c][0] = w.x; q_raw[n][c][1] = w.y;
+            if constexpr (SPLIT) { q_raw[n][c][2] = w.z; q_raw[n][c][3] = w.w; }
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const __half*>(a.q) + from + 16 * c);
+            q_raw[n][c][0] = w.x; q_raw[n][c][1] = w.y;
+          }
+        }
+      }
+    }
+  };
+  auto q_values = [&](const uint32_t (&w)[SPLIT ? 4 : 2], float (&x)[4]) {
+    if (SPLIT && a.q_dtype == B200MOE_DT_F32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(w[SPLIT ? e : 0]);
+    } else if (a.q_dtype == B200MOE_DT_F16) {
+      const float2 lo = __half22float2(u32_as_h2(w[0])), hi = __half22float2(u32_as_h2(w[1]));
+      x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
+    } else {
+      x[0] = __uint_as_float(w[0] << 16); x[1] = __uint_as_float(w[0] & 0xffff0000u);
+      x[2] = __uint_as_float(w[1] << 16); x[3] = __uint_as_float(w[1] & 0xffff0000u);
+    }
+  };
+
   // The copies of a unit are started as soon as the places of the one before are read, those
   // of the next segment's first unit during this segment's last (6 us of waiting otherwise).
   Piece next = piece_at(g_begin);
   float2 sc_now, sc_next;
+  load_q(next);  // before the first copies: behind all CTAs' of them it takes 4 us more
   {
     const uint32_t row = locate(next, 0, page_of(next, 0), sc_next);
     issue(next.units > 0, row, 0);
@@ -942,24 +959,18 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
     // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two.  Four
     // columns' tiles do not fit in registers beside the output: there a warp prepares one, in
     // the order of the fragments, and all read them from shared memory.
-    constexpr int QN = Q_SHARED ? 1 : NT;
+    if (g != g_begin) load_q(cur);
     uint32_t qb[PARTS][QN][CH][2];
     float fold[NT][2];  // of this lane's accumulator columns 2 tig, 2 tig + 1: back to to_score units
 #pragma unroll
     for (int n = 0; n < QN; ++n) {
-      const int r = tile * ROWS + 8 * (Q_SHARED ? warp : n) + gid;
       float x[CH][4], top = 0.f;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        x[c][0] = x[c][1] = x[c][2] = x[c][3] = 0.f;
-        if (r < rows)
-          load_as(a.q, a.q_dtype, (static_cast<int64_t>(b) * a.sl + r / G) * a.q_stride +
-                                      static_cast<int64_t>(kvh * G + r % G) * HD + 16 * c + 4 * tig, x[c]);
-      }
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
+        q_values(q_raw[n][c], x[c]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[c][e]));
+      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^e <= top < 2^(e + 1), so that the largest value lies in [2^14, 2^15)
