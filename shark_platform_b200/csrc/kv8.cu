@@ -737,9 +737,9 @@ __device__ __forceinline__ int live_positions(const AttendArgs& a, int b) {
 __device__ __forceinline__ int steps_of(int len) { return len > AT_STEP ? (len + AT_STEP - 1) / AT_STEP : 1; }
 
 // Joining a segment in the middle of a stretch (the barrier and the output of the last one,
-// q) takes a CTA as long as three steps (7 us): in long stretches a segment counts
+// q) takes a CTA as long as two to three steps (7 us): in long stretches a segment counts
 // START_STEPS more than it has, so that the CTAs that join one get fewer.
-constexpr int START_STEPS = 3;
+constexpr int START_STEPS = 2;
 __device__ __forceinline__ int start_steps(int steps, int ctas) { return steps >= 4 * ctas ? START_STEPS : 0; }
 
 // The list of steps, looked at by a whole warp: those of the sequences before `until` or,
@@ -781,14 +781,15 @@ struct Stretches {
 };
 
 // CTAs per SM: shared memory of the ring, registers
-template <int HD, int NT, bool SPLIT>
+template <int HD, int CODE, int NT, bool SPLIT>
 constexpr int attend_resident() {
   if (NT == 4) return HD == 128 ? 2 : 3;
-  return HD == 128 ? (NT == 1 ? (SPLIT ? 3 : 4) : (SPLIT ? 2 : 3)) : (NT == 1 ? (SPLIT ? 4 : 5) : (SPLIT ? 3 : 4));
+  if (HD == 128) return NT == 1 && !SPLIT ? 3 : 2;
+  return NT == 1 ? 4 : 3;
 }
 
 template <int HD, int CODE, int NT, bool SPLIT>
-__global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())) kv8_attend_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, CODE, NT, SPLIT>())) kv8_attend_kernel(const AttendArgs a) {
   constexpr int CH = HD / 16;                       // chunks of a row: MMA steps of q.k, row tiles of V^T
   constexpr int PARTS = SPLIT ? 2 : 1;
   constexpr int ROWS = 8 * NT;
@@ -937,7 +938,10 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
   // of the next segment's first unit during this segment's last (6 us of waiting otherwise).
   Piece next = piece_at(g_begin);
   float2 sc_now, sc_next;
-  load_q(next);  // before the first copies: behind all CTAs' of them it takes 4 us more
+  // before the first copies: behind all CTAs' of them it takes 4 us more (with two tiles of q or
+  // more the registers would have to wait in memory)
+  constexpr bool Q_FIRST = NT == 1;
+  if constexpr (Q_FIRST) load_q(next);
   {
     const uint32_t row = locate(next, 0, page_of(next, 0), sc_next);
     issue(next.units > 0, row, 0);
@@ -959,7 +963,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
     // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two.  Four
     // columns' tiles do not fit in registers beside the output: there a warp prepares one, in
     // the order of the fragments, and all read them from shared memory.
-    if (g != g_begin) load_q(cur);
+    if (!Q_FIRST || g != g_begin) load_q(cur);
     uint32_t qb[PARTS][QN][CH][2];
     float fold[NT][2];  // of this lane's accumulator columns 2 tig, 2 tig + 1: back to to_score units
 #pragma unroll
@@ -1368,16 +1372,21 @@ int launch_merge(const AttendArgs& a, int tile_rows, cudaStream_t st) {
 // Rows of a CTA's tile; CTAs of a call: as many as are resident at once, or one for each
 // step of a full page table where those are fewer.
 inline int attend_tile_rows(int rows, bool split) { return rows <= 8 ? 8 : rows <= 16 || split ? 16 : 32; }
-template <int HD>
+template <int HD, int CODE>
 int resident_ctas(int tile, bool split) {
-  if (tile == 32) return attend_resident<HD, 4, false>();
-  if (tile == 16) return split ? attend_resident<HD, 2, true>() : attend_resident<HD, 2, false>();
-  return split ? attend_resident<HD, 1, true>() : attend_resident<HD, 1, false>();
+  if (tile == 32) return attend_resident<HD, CODE, 4, false>();
+  if (tile == 16) return split ? attend_resident<HD, CODE, 2, true>() : attend_resident<HD, CODE, 2, false>();
+  return split ? attend_resident<HD, CODE, 1, true>() : attend_resident<HD, CODE, 1, false>();
 }
-int attend_ctas(int bs, int kv_heads, int hd, int rows, bool split, int max_seq_len) {
+int resident_ctas(int hd, int code, int tile, bool split) {
+  if (code == B200MOE_KV8_INT8)
+    return hd == 128 ? resident_ctas<128, B200MOE_KV8_INT8>(tile, split) : resident_ctas<64, B200MOE_KV8_INT8>(tile, split);
+  return hd == 128 ? resident_ctas<128, B200MOE_KV8_E4M3>(tile, split) : resident_ctas<64, B200MOE_KV8_E4M3>(tile, split);
+}
+int attend_ctas(const b200moe_kv8_cache_t& c, int bs, int rows, bool split, int max_seq_len) {
   const int tile = attend_tile_rows(rows, split);
-  const int64_t steps = (static_cast<int64_t>(max_seq_len) + AT_STEP - 1) / AT_STEP * bs * kv_heads * ((rows + tile - 1) / tile);
-  const int64_t resident = static_cast<int64_t>(sm_count()) * (hd == 128 ? resident_ctas<128>(tile, split) : resident_ctas<64>(tile, split));
+  const int64_t steps = (static_cast<int64_t>(max_seq_len) + AT_STEP - 1) / AT_STEP * bs * c.kv_heads * ((rows + tile - 1) / tile);
+  const int64_t resident = static_cast<int64_t>(sm_count()) * resident_ctas(c.head_dim, c.code, tile, split);
   return static_cast<int>(steps < resident ? steps : resident);
 }
 
@@ -1502,7 +1511,7 @@ size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_
   const int rows = heads / cache->kv_heads * new_tokens;
   size_t most = 0;  // the activations' type is not known here: enough for any
   for (const bool split : {false, true}) {
-    const size_t n = static_cast<size_t>(attend_ctas(bs, cache->kv_heads, cache->head_dim, rows, split, max_seq_len)) * 2 *
+    const size_t n = static_cast<size_t>(attend_ctas(*cache, bs, rows, split, max_seq_len)) * 2 *
                      attend_tile_rows(rows, split) * (cache->head_dim + 4) * sizeof(float);
     most = n > most ? n : most;
   }
@@ -1544,7 +1553,7 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   const bool split = q_dtype == B200MOE_DT_F32 || out_dtype == B200MOE_DT_F32;
   const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows, split), hd = cache->head_dim;
   a.row_tiles = (rows + tile - 1) / tile;
-  a.ctas = attend_ctas(bs, cache->kv_heads, hd, rows, split, max_seq_len);
+  a.ctas = attend_ctas(*cache, bs, rows, split, max_seq_len);
   a.stride_shift = log2_of(a.stride);
   a.block_shift = log2_of(cache->scale_block);
   B200_REQUIRE(static_cast<double>(bs) * a.kv_heads * a.row_tiles * (1.0 + pages_per_seq * static_cast<double>(a.stride) / AT_STEP) < 2147483647.0,
