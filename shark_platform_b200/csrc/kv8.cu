@@ -95,30 +95,42 @@ __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v & 0xffffu), __NV_E4M3);
   return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
 }
-// Four codes as two fp16 pairs, exact: bytes (0, 1), (2, 3), or with PAIRS_APART (0, 2), (1, 3).
-template <int CODE, bool PAIRS_APART>
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+// Four codes as two fp16 pairs for the MMAs, exact: bytes (0, 2) and (1, 3).
+// int8: 0x6400 | b is the fp16 number 1024 + b; the byte is biased to unsigned first.
+// e4m3: its exponent and mantissa moved to fp16's places are the value times 2^-8 (the two
+// biases differ by 8; subnormal codes become subnormal fp16 numbers), which goes into the
+// scale: E4M3_UNIT.  Seven integer instructions, against three or four with the conversion
+// instruction, which takes longer than they (47 and 45 us at 32 x 4000 positions).
+constexpr float E4M3_UNIT = 256.f;
+template <int CODE>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& even, uint32_t& odd) {
   if constexpr (CODE == B200MOE_KV8_INT8) {
-    // 0x6400 | b is the fp16 number 1024 + b; the byte is biased to unsigned first
     const uint32_t x = w ^ 0x80808080u;
     const __half2 bias = u32_as_h2(0x64806480u);
-    lo = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, PAIRS_APART ? 0x4240 : 0x4140)), bias));
-    hi = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, PAIRS_APART ? 0x4341 : 0x4342)), bias));
+    even = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, 0x4240)), bias));
+    odd = h2_as_u32(__hsub2(u32_as_h2(__byte_perm(x, 0x64646464u, 0x4341)), bias));
   } else {
-    if constexpr (PAIRS_APART) w = __byte_perm(w, 0, 0x3120);
-    lo = e4m3x2_to_h2(w);
-    hi = e4m3x2_to_h2(w >> 16);
+    even = ((w << 7) & 0x3f803f80u) | ((w << 8) & 0x80008000u);
+    odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
   }
 }
 template <int CODE>
 __device__ __forceinline__ void codes_to_floats(uint2 c, float (&v)[8]) {
-  uint32_t h[4];
-  widen4<CODE, false>(c.x, h[0], h[1]);
-  widen4<CODE, false>(c.y, h[2], h[3]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(u32_as_h2(h[i]));
-    v[2 * i] = f.x; v[2 * i + 1] = f.y;
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w = i ? c.y : c.x;
+    float2 f[2];
+    if constexpr (CODE == B200MOE_KV8_INT8) {
+      uint32_t even, odd;
+      widen4<CODE>(w, even, odd);
+      const float2 e = __half22float2(u32_as_h2(even)), o = __half22float2(u32_as_h2(odd));
+      f[0] = make_float2(e.x, o.x);
+      f[1] = make_float2(e.y, o.y);
+    } else {
+      f[0] = __half22float2(u32_as_h2(e4m3x2_to_h2(w)));
+      f[1] = __half22float2(u32_as_h2(e4m3x2_to_h2(w >> 16)));
+    }
+    v[4 * i] = f[0].x; v[4 * i + 1] = f[0].y; v[4 * i + 2] = f[1].x; v[4 * i + 3] = f[1].y;
   }
 }
 // v[i] * by, values / scale at most 2^-10 above qmax, to the nearest codes: without clamping
@@ -641,7 +653,8 @@ int launch_read(const ReadArgs& a, int code, unsigned grid, cudaStream_t st) {
 // several; NT = 2 takes sixteen).
 //   * K is the A operand as it lies: ldmatrix of 16-byte chunks gives a lane four
 //     consecutive bytes of a row, and the order of the 16 elements of an MMA is free as
-//     long as q's fragments have the same one (a lane holds q[16c + 4 tig .. + 3]).
+//     long as q's fragments have the same one (a lane holds q[16c + 4 tig .. + 3], the
+//     elements 0, 2 and 1, 3 as pairs).
 //   * V^T comes from ldmatrix.trans on pairs of bytes: a lane gets two elements of two
 //     positions, and taking bytes 0, 2 and 1, 3 apart makes rows 2 gid and 2 gid + 1 of V^T.
 //   * P^T is S^T's accumulator, packed and transposed within the warp (movmatrix).
@@ -993,7 +1006,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, CODE, NT, SPL
       for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float u = x[c][2 * i] * up, v = x[c][2 * i + 1] * up;
+          const float u = x[c][i] * up, v = x[c][i + 2] * up;  // the codes' bytes (0, 2), (1, 3)
           const __half2 h = __floats2half2_rn(u, v);
           qb[0][n][c][i] = h2_as_u32(h);
           if constexpr (SPLIT) {
@@ -1030,10 +1043,11 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, CODE, NT, SPL
       sc_now = sc_next;
       {
         // dead positions (sc.y < 0: scales are never negative): weight 0 without touching the others
-        const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f);  // 2^-100 in the place of 0
+        constexpr float unit = CODE == B200MOE_KV8_E4M3 ? E4M3_UNIT : 1.f;
+        const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f) * unit;  // 2^-100 in the place of 0
         const bool dead = sc_now.y < 0.f, bad = sc_now.y != sc_now.y;
         s_pos[warp][lane] =
-            make_float4(sc_now.x, dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : rcp(vs), 0.f);
+            make_float4(sc_now.x * unit, dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : rcp(vs), 0.f);
       }
       copy_wait<1>();  // all but V of this unit
       __syncwarp();
@@ -1063,8 +1077,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, CODE, NT, SPL
             uint32_t f[HB][4];
 #pragma unroll
             for (int h = 0; h < HB; ++h) {
-              widen4<CODE, false>(w[h][2 * i], f[h][0], f[h][2]);
-              widen4<CODE, false>(w[h][2 * i + 1], f[h][1], f[h][3]);
+              widen4<CODE>(w[h][2 * i], f[h][0], f[h][2]);
+              widen4<CODE>(w[h][2 * i + 1], f[h][1], f[h][3]);
             }
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
@@ -1187,8 +1201,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, CODE, NT, SPL
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             uint32_t a0, a1, a2, a3;
-            widen4<CODE, true>(w[2 * i], a0, a1);
-            widen4<CODE, true>(w[2 * i + 1], a2, a3);
+            widen4<CODE>(w[2 * i], a0, a1);
+            widen4<CODE>(w[2 * i + 1], a2, a3);
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
