@@ -1570,7 +1570,8 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   a.ctas = attend_ctas(*cache, bs, rows, split, max_seq_len);
   a.stride_shift = log2_of(a.stride);
   a.block_shift = log2_of(cache->scale_block);
-  B200_REQUIRE(static_cast<double>(bs) * a.kv_heads * a.row_tiles * (1.0 + pages_per_seq * static_cast<double>(a.stride) / AT_STEP) < 2147483647.0,
+  B200_REQUIRE(static_cast<double>(bs) * a.kv_heads * a.row_tiles *
+                       (2.0 + START_STEPS + pages_per_seq * static_cast<double>(a.stride) / AT_STEP) < 2147483647.0,
                "%s: too many positions for one call", who);
   a.scale = scale; a.softcap = softcap;
   a.status = device_status_ptr();

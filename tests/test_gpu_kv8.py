@@ -628,3 +628,76 @@ def test_captured_steps_and_other_streams():
         assert torch.equal(outs[g], ref[i]), i
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(ref_state, state))
     assert _status() == 0
+
+
+def test_a_slab_beyond_four_gigabytes():
+    """Pages whose codes lie behind 2^32 bytes, written, read and attended."""
+    A = _attention()
+    gen = torch.Generator().manual_seed(12)
+    cache = _cache(I8, 8, 128, 64, 16)
+    pages = (1 << 32) // cache.page_slab_flat_dim + 40
+    state = cache.allocate(pages)
+    w = Write(cache, 8, BF, gen)
+    ids = torch.tensor([[pages - 1, pages - 30], [pages - 2, 0]], dtype=torch.int32)
+    _, (q, k, v) = w.inputs(2, 90)
+    zero = torch.zeros(2, dtype=torch.int32)
+    got = w.call(state, ids, zero, q.cuda(), k.cuda(), v.cuda())
+    low = cache.allocate(4)
+    near = torch.tensor([[3, 2], [1, 0]], dtype=torch.int32)
+    w.call(low, near, zero, q.cuda(), k.cuda(), v.cuda())
+    lens = torch.tensor([90, 77]).cuda()
+    for f in (lambda st, i: A.kv_read(cache, st, block_index=1, seq_block_ids=i.cuda(), seq_lens=lens),
+              lambda st, i: [A.kv_attend(got[0][:, -1:], cache, st, block_index=1, seq_block_ids=i.cuda(), seq_lens=lens)]):
+        assert all(torch.equal(a, b) for a, b in zip(f(state, ids), f(low, near)))
+    assert _status() == 0
+
+
+def test_calls_on_two_streams_at_once():
+    """Long and short calls that overlap give what each gives alone."""
+    A = _attention()
+    gen = torch.Generator().manual_seed(13)
+    cache = _cache(E4, 4, 128, 32, 16, layers=1)
+    per = 130
+    state = _fill(cache, 4 * per + 2, gen)
+    ids = _ids(4, per, gen).cuda()
+    jobs = []
+    for i, (n, sl) in enumerate(((4100, 1), (300, 4), (33, 1), (2000, 8))):
+        q = torch.randn(4, sl, 16, 128, generator=gen).to(BF).cuda()
+        lens = torch.tensor([n, n // 2 + 8, n, 9]).cuda()
+        jobs.append(lambda q=q, lens=lens: A.kv_attend(q, cache, state, block_index=0, seq_block_ids=ids, seq_lens=lens))
+    alone = [j() for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for turn in range(6):
+        for i, j in enumerate(jobs):
+            with torch.cuda.stream(streams[(i + turn) % 2]):
+                got.append((i, j()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, alone[i]) for i, o in got)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("sl", [1, 4])
+def test_new_tokens_behind_the_page_table(sl):
+    """Drafted tokens that would not fit are reported; the tokens before them see what they should."""
+    from shark_platform_b200 import _cabi as C
+
+    A = _attention()
+    gen = torch.Generator().manual_seed(14)
+    cache = _cache(I8, 2, 64, 16, 16, layers=1)
+    state = _fill(cache, 4, gen)
+    ids = torch.tensor([[1, 3]], dtype=torch.int32).cuda()
+    q = torch.randn(1, sl, 4, 64, generator=gen).cuda()
+    o = A.kv_attend(q, cache, state, block_index=0, seq_block_ids=ids, seq_lens=torch.tensor([32 + sl - 1]).cuda())
+    if sl > 1:
+        with pytest.raises(C.B200MoeError, match="status word"):
+            _status()
+    first = A.kv_attend(q[:, :1], cache, state, block_index=0, seq_block_ids=ids, seq_lens=torch.tensor([32]).cuda())
+    assert _status() == 0
+    k, v = (t[0].cpu().double() for t in A.kv_read(cache, state, block_index=0, seq_block_ids=ids,
+                                                  seq_lens=torch.tensor([32]).cuda(), dtype=F32))
+    want = ko.attend(q[0, :1].cpu(), k, v, [32], 64 ** -0.5)
+    room = ko.attend_tolerance(q[0, :1].cpu(), k, v, 64 ** -0.5, 2.0 ** -21, EPS[F32], want)
+    for got in (o[0, :1], first[0]):
+        assert ((got.cpu().double() - want).abs() <= room).all()
