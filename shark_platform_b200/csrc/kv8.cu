@@ -497,9 +497,9 @@ template <typename T, int HD, int KIND, int TILE, int ORDER>
 int launch_write(WriteArgs& a, cudaStream_t st) {
   a.tiles = a.sl == 1 ? 1 : (a.sl - 1) / TILE + 2;
   a.kv_ctas = static_cast<unsigned>(a.bs) * a.tiles * a.kv_heads;
-  // as many heads a lane as leave work for sixteen CTAs per SM: a position's angles are computed once for each group
+  // as many heads a lane as leave work for eight CTAs per SM: a position's angles are computed once for each group
   constexpr int RPP = WR_THREADS / (HD / 8);
-  const int64_t tokens = static_cast<int64_t>(a.bs) * a.sl, want = static_cast<int64_t>(sm_count()) * 16 * RPP;
+  const int64_t tokens = static_cast<int64_t>(a.bs) * a.sl, want = static_cast<int64_t>(sm_count()) * 8 * RPP;
   a.q_heads = 4;
   while (a.q_heads < a.heads && tokens * ((a.heads - 1) / (2 * a.q_heads) + 1) >= want) a.q_heads *= 2;
   const int64_t q_ctas = (tokens * ((a.heads - 1) / a.q_heads + 1) + RPP - 1) / RPP;
@@ -581,9 +581,9 @@ struct ReadArgs {
   int32_t* status;
 };
 
-// One CTA per (sequence, kv head, 64 positions); a thread takes eight codes of a row (eight
+// One CTA per (sequence, kv head, 16 positions); a thread takes eight codes of a row (eight
 // bytes loaded, 16 stored in 16 bits: both whole sectors), K and V of several rows at once.
-constexpr int RD_THREADS = 256, RD_TILE = 64;
+constexpr int RD_THREADS = 128, RD_TILE = 16;
 template <typename T, int HD, int CODE>
 __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(const ReadArgs a) {
   constexpr int LPR = HD / 8, RPP = RD_THREADS / LPR, PASSES = RD_TILE / RPP;
