@@ -181,8 +181,8 @@ constexpr float QMAX[2] = {127.f, 448.f};
 // Cosine and sine of position * freq, the angle reduced to part of a turn first.
 // 32-bit rows: reduced in 64 bits, good to 2^-23 at any position.  16-bit rows: the position
 // (below 2^24) times freq / (2 pi) as the sum of two floats, their integer part dropped, and
-// the special-function unit, absolute error 2^-21: an eighth of a thousandth of half a step
-// of fp16.  (sincospif for both: 70 instead of ... us for 4 x 2048 tokens of 48 + 16 heads.)
+// the special-function unit, absolute error 2^-21: a thousandth of half a step of fp16.
+// (sincospif for both: 5 us of 71 for 4 x 2048 tokens of 48 + 16 heads.)
 template <typename T>
 __device__ __forceinline__ float2 cos_sin(long long pos, float freq) {
   float sn, cs;
@@ -297,9 +297,11 @@ __device__ __forceinline__ BlockScale block_scale(unsigned bits, float before) {
 // scale blocks; K and V stay in registers from their load to their codes: one read of
 // everything.  The others have the queries: a lane keeps its position's cosines and sines
 // and takes four heads at once, q_heads in all.  HD / 8 lanes have a row (16-byte loads and
-// stores of 16-bit rows), a warp two or four rows.  (With K, V and the queries of a kv head
-// in one CTA, angles in shared memory: 79 instead of ... us for 4 x 2048 tokens of 48 + 16
-// heads, as the queries waited for the barriers of K and V.)
+// stores of 16-bit rows), a warp two or four rows.  Bound by HBM, then by how much of it the
+// CTAs keep asking for: 4 x 2048 tokens of 48 + 16 heads (268 MB) take 50 us, 5.3 TB/s; with
+// K, V and the queries of a kv head in one CTA 79 (the queries waited for the barriers of K
+// and V), with three CTAs an SM instead of four 66, with K's and V's CTAs before the others
+// instead of among them 60.
 template <typename T, int HD, int KIND, int TILE, int ORDER>
 __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 2 ? 4 : 3) : 2) norm_rope_write_kernel(const WriteArgs a) {
   constexpr int LPR = HD / 8, RPW = 32 / LPR;                 // lanes per row, rows of a warp
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 2 ? 4 :
           }
         }
       } else {
-        // the largest magnitude of the row, then of its scale block; as bits, so that NaN is the largest
+        // the largest magnitude of the row, then of its scale block, NaN above all
         float y[8];
         vr[i].get(y);
         float mk = 0.f, mv = 0.f;
@@ -582,7 +584,10 @@ struct ReadArgs {
 };
 
 // One CTA per (sequence, kv head, 16 positions); a thread takes eight codes of a row (eight
-// bytes loaded, 16 stored in 16 bits: both whole sectors), K and V of several rows at once.
+// bytes loaded, 16 stored in 16 bits: both whole sectors), K and V of two rows (HD 128) at
+// once.  Bound by HBM: 32 sequences of up to 4000 positions, 8 heads of 128, to bf16 (723 MB)
+// take 119 us, 6.1 TB/s; in tiles of 32, 64, 128 positions 122, 137, 170; with 16 codes per
+// thread and 4-byte stores 310.
 constexpr int RD_THREADS = 128, RD_TILE = 16;
 template <typename T, int HD, int CODE>
 __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(const ReadArgs a) {
@@ -660,18 +665,26 @@ int launch_read(const ReadArgs& a, int code, unsigned grid, cudaStream_t st) {
 //   * P^T is S^T's accumulator, packed and transposed within the warp (movmatrix).
 // The scale of V joins the softmax: with t = S log2(e) + log2(s_v), P = 2^(t - max t) is at
 // most 1 whatever the scales are, the sum of P c_v is the numerator and that of P / s_v
-// the denominator.  P and q are fp16 with their largest value near 2^15, so that what is
-// rounded is 2^-11 of a value down to 2^-29 of the largest.  SPLIT (32-bit activations):
-// q and P are the sums of two fp16 parts, 2^-22, at twice the MMAs.
+// the denominator.  q is fp16 with its largest value in [2^14, 2^15), P with 2^7 where the
+// maximum is up to date (it is left behind by up to 2^8, so that the output is rescaled
+// rarely): what rounding loses is 2^-11 of a value down to 2^-28 and 2^-21 of the largest,
+// and 2^-32 of the largest P below.  SPLIT (32-bit activations): q and P are the sums of two
+// fp16 parts, 2^-22, at twice the MMAs.
 //
 // A warp owns units of 32 positions with its own softmax state and places for one unit's K
 // and V, filled by 16-byte cp.async, each again as soon as it is read: no barrier between
-// warps, and four CTAs an SM (with two units' places and three CTAs 51 instead of ... us); chunks are swizzled so that ldmatrix has no bank
-// conflicts.  A step of the CTA is 128 positions.  The steps of all (sequence, kv head, row
-// tile) segments form one list, cut into equal stretches, one for each resident CTA: ragged
-// lengths leave no SM idle, and the cut does not depend on how wide the page table is.  A
-// segment that lies within one stretch is finished there; of the others every CTA leaves a
-// state (at most two: its first and its last segment), which the merge kernel joins.
+// warps.  (Places for two units and fewer CTAs: the same time, 53 against 52 us when it was
+// tried.)  Chunks are swizzled so that ldmatrix has no bank conflicts.  A step of the CTA is
+// 128 positions.  The steps of all (sequence, kv head, row tile) segments form one list, cut
+// into equal stretches, one for each resident CTA: ragged lengths leave no SM idle, and the
+// cut does not depend on how wide the page table is.  A segment that lies within one stretch
+// is finished there; of the others every CTA leaves a state (at most two: its first and its
+// last segment), which the merge kernel joins.
+// 32 sequences of 2000 to 4000 positions, 8 kv heads of 128, 32 heads (200 MB): int8 41 us,
+// e4m3 43, 4.9 and 4.7 TB/s (a plain read of as much, by a reduction, 39 us); bound by HBM
+// once under way, before by the chain of lengths, page ids and first rows (6 us), after by the
+// merge (4 us).  With a CTA per position split of each sequence 68.  Several new tokens are
+// bound by the instructions around the MMAs: 16 rows 48 us, 32 rows 85 us of the same cache.
 struct AttendArgs {
   const void* q;
   int64_t q_stride;
@@ -750,8 +763,9 @@ __device__ __forceinline__ int live_positions(const AttendArgs& a, int b) {
 __device__ __forceinline__ int steps_of(int len) { return len > AT_STEP ? (len + AT_STEP - 1) / AT_STEP : 1; }
 
 // Joining a segment in the middle of a stretch (the barrier and the output of the last one,
-// q) takes a CTA as long as two to three steps (7 us): in long stretches a segment counts
-// START_STEPS more than it has, so that the CTAs that join one get fewer.
+// q) takes a CTA as long as a step or two: in long stretches a segment counts START_STEPS
+// more than it has, so that the CTAs that join one get fewer.  (0, 2, 3 at 32 x 4000
+// positions: 16 rows 51, 48, 49 us; 8 rows 40, 41, 42.)
 constexpr int START_STEPS = 2;
 __device__ __forceinline__ int start_steps(int steps, int ctas) { return steps >= 4 * ctas ? START_STEPS : 0; }
 
@@ -793,8 +807,11 @@ struct Stretches {
   }
 };
 
-// CTAs per SM: shared memory of the ring, registers
-template <int HD, int CODE, int NT, bool SPLIT>
+// CTAs per SM: as many as the registers allow without spilling in the loop.  (HD 128, one
+// more: NT = 1 44 instead of 41 us, NT = 2 61 instead of 48, at 32 x 4000 positions of int8;
+// one less: e4m3 51 instead of 48, int8 41 instead of 43, before the e4m3 codes were widened
+// as they are now.)
+template <int HD, int NT, bool SPLIT>
 constexpr int attend_resident() {
   if (NT == 4) return HD == 128 ? 2 : 3;
   if (HD == 128) return NT == 1 && !SPLIT ? 3 : 2;
@@ -802,7 +819,7 @@ constexpr int attend_resident() {
 }
 
 template <int HD, int CODE, int NT, bool SPLIT>
-__global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, CODE, NT, SPLIT>())) kv8_attend_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())) kv8_attend_kernel(const AttendArgs a) {
   constexpr int CH = HD / 16;                       // chunks of a row: MMA steps of q.k, row tiles of V^T
   constexpr int PARTS = SPLIT ? 2 : 1;
   constexpr int ROWS = 8 * NT;
@@ -948,7 +965,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, CODE, NT, SPL
   };
 
   // The copies of a unit are started as soon as the places of the one before are read, those
-  // of the next segment's first unit during this segment's last (6 us of waiting otherwise).
+  // of the next segment's first unit during this segment's last.
   Piece next = piece_at(g_begin);
   float2 sc_now, sc_next;
   // before the first copies: behind all CTAs' of them it takes 4 us more (with two tiles of q or
@@ -1386,21 +1403,17 @@ int launch_merge(const AttendArgs& a, int tile_rows, cudaStream_t st) {
 // Rows of a CTA's tile; CTAs of a call: as many as are resident at once, or one for each
 // step of a full page table where those are fewer.
 inline int attend_tile_rows(int rows, bool split) { return rows <= 8 ? 8 : rows <= 16 || split ? 16 : 32; }
-template <int HD, int CODE>
+template <int HD>
 int resident_ctas(int tile, bool split) {
-  if (tile == 32) return attend_resident<HD, CODE, 4, false>();
-  if (tile == 16) return split ? attend_resident<HD, CODE, 2, true>() : attend_resident<HD, CODE, 2, false>();
-  return split ? attend_resident<HD, CODE, 1, true>() : attend_resident<HD, CODE, 1, false>();
-}
-int resident_ctas(int hd, int code, int tile, bool split) {
-  if (code == B200MOE_KV8_INT8)
-    return hd == 128 ? resident_ctas<128, B200MOE_KV8_INT8>(tile, split) : resident_ctas<64, B200MOE_KV8_INT8>(tile, split);
-  return hd == 128 ? resident_ctas<128, B200MOE_KV8_E4M3>(tile, split) : resident_ctas<64, B200MOE_KV8_E4M3>(tile, split);
+  if (tile == 32) return attend_resident<HD, 4, false>();
+  if (tile == 16) return split ? attend_resident<HD, 2, true>() : attend_resident<HD, 2, false>();
+  return split ? attend_resident<HD, 1, true>() : attend_resident<HD, 1, false>();
 }
 int attend_ctas(const b200moe_kv8_cache_t& c, int bs, int rows, bool split, int max_seq_len) {
   const int tile = attend_tile_rows(rows, split);
   const int64_t steps = (static_cast<int64_t>(max_seq_len) + AT_STEP - 1) / AT_STEP * bs * c.kv_heads * ((rows + tile - 1) / tile);
-  const int64_t resident = static_cast<int64_t>(sm_count()) * resident_ctas(c.head_dim, c.code, tile, split);
+  const int64_t resident = static_cast<int64_t>(sm_count()) * 
+                           (c.head_dim == 128 ? resident_ctas<128>(tile, split) : resident_ctas<64>(tile, split));
   return static_cast<int>(steps < resident ? steps : resident);
 }
 
