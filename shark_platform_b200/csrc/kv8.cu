@@ -845,8 +845,10 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
   const int g_begin = cut.begin(blockIdx.x), g_end = cut.begin(blockIdx.x + 1);
   const ListSum at = walk_list(a, lane, -1, g_begin, start);
 
-  // scores in halvings; with a softcap c, c tanh(x / c) = c - 2 c / (2^(2 log2(e) x / c) + 1)
-  const float to_score = a.scale * LOG2E * (a.softcap > 0.f ? 2.f / a.softcap : 1.f), cap2 = a.softcap * LOG2E;
+  // Scores in halvings; with a softcap c, c tanh(x / c) = c - 2 c / (2^(2 log2(e) x / c) + 1):
+  // two special functions, good to c 2^-22.  32-bit activations take tanhf, 2^-22 of the value.
+  const float cap2 = a.softcap * LOG2E;
+  const float to_score = a.softcap > 0.f ? a.scale / a.softcap * (SPLIT ? 1.f : 2.f * LOG2E) : a.scale * LOG2E;
   const uint32_t ring = smem_u32(smem) + warp * (2 * TILE);
   const size_t v_off = static_cast<size_t>(a.stride) * HD;
   // byte offsets in a tile that this lane addresses with ldmatrix: rows 16 h + (lane & 15), chunks 2 i + (lane >> 4)
@@ -1141,8 +1143,12 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
             for (int e = 0; e < 2; ++e) {
               const float y = f.x * fold[n][e];
               float x;
-              if (a.softcap > 0.f) x = fmaf(-2.f * cap2, rcp(ex2(s[h][n][2 * j + e] * y) + 1.f), cap2 + f.y);
-              else x = fmaf(s[h][n][2 * j + e], y, f.y);
+              if (a.softcap > 0.f) {
+                if constexpr (SPLIT) x = fmaf(cap2, tanhf(s[h][n][2 * j + e] * y), f.y);
+                else x = fmaf(-2.f * cap2, rcp(ex2(s[h][n][2 * j + e] * y) + 1.f), cap2 + f.y);
+              } else {
+                x = fmaf(s[h][n][2 * j + e], y, f.y);
+              }
               s[h][n][2 * j + e] = x;
             }
         }
@@ -1209,23 +1215,52 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
       }
       copy_wait<1>();
       __syncwarp();
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
+      if constexpr (SPLIT) {
+        // the tensor cores cut off what a sum's last bit cannot hold: a unit's products are summed
+        // apart and added with rounding, or a long stretch would lose 2^-25 at every step
 #pragma unroll
         for (int c = 0; c < CH; c += 2) {
-          uint32_t w[4];
-          ldsm_x4_trans(vt + ld_at[c / 2] + 16 * h * HD, w);
+          uint32_t w[2][4];
+          ldsm_x4_trans(vt + ld_at[c / 2], w[0]);
+          ldsm_x4_trans(vt + ld_at[c / 2] + 16 * HD, w[1]);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t a0, a1, a2, a3;
-            widen4<CODE>(w[2 * i], a0, a1);
-            widen4<CODE>(w[2 * i + 1], a2, a3);
+            float unit_o[NT][4];
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
+            for (int n = 0; n < NT; ++n) unit_o[n][0] = unit_o[n][1] = unit_o[n][2] = unit_o[n][3] = 0.f;
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma(o[n][c + i], a0, a1, a2, a3, pb[p][n][h][0], pb[p][n][h][1]);
+            for (int h = 0; h < 2; ++h) {
+              uint32_t a0, a1, a2, a3;
+              widen4<CODE>(w[h][2 * i], a0, a1);
+              widen4<CODE>(w[h][2 * i + 1], a2, a3);
+#pragma unroll
+              for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma(unit_o[n], a0, a1, a2, a3, pb[p][n][h][0], pb[p][n][h][1]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) o[n][c + i][k] += unit_o[n][k];
           }
         }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < CH; c += 2) {
+            uint32_t w[4];
+            ldsm_x4_trans(vt + ld_at[c / 2] + 16 * h * HD, w);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t a0, a1, a2, a3;
+              widen4<CODE>(w[2 * i], a0, a1);
+              widen4<CODE>(w[2 * i + 1], a2, a3);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma(o[n][c + i], a0, a1, a2, a3, pb[0][n][h][0], pb[0][n][h][1]);
+            }
+          }
+      }
       __syncwarp();  // V and s_pos are read
       issue(unit_next, row_next, 1);
     }
