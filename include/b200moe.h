@@ -445,7 +445,8 @@ typedef struct {
  * smallest power of two that makes them fit, and the codes of the live rows are rounded
  * to the new scale (exact for e4m3 but for subnormal codes).  Rows of the block behind
  * the written ones keep their codes and are dead: no position behind the last written one
- * may be read before it is written.  A block whose new rows are all below qmax * 2^-100
+ * may be read before it is written.  (A drafted token that is taken back leaves its block's
+ * scale as it made it.)  A block whose new rows are all below qmax * 2^-100
  * counts as zero (scale 0); one with an infinity or NaN gets the scale NaN and reads as
  * NaN until it is fresh again.
  * The written pages of different sequences of a call have to be different pages.  A
@@ -483,9 +484,13 @@ int b200moe_kv8_read(const void* slab, const float* scales, const b200moe_kv8_ca
  * the positions in the cache, the new ones included; new token i attends the positions up
  * to and including seq_lens[seq] - new_tokens + i, and its output is zero where that
  * leaves none.  q [bs * new_tokens] rows of heads * head_dim elements, q_stride apart;
- * out [bs][new_tokens][heads][head_dim] contiguous.  Any heads / kv_heads; softcap <= 0
- * means none.  A missing page sets the bounds bit; its positions are not attended.
- * scratch: b200moe_kv8_attend_scratch_bytes(...) bytes, 16-byte aligned. */
+ * out [bs][new_tokens][heads][head_dim] contiguous.  Any heads / kv_heads; at most 65535
+ * sequences; softcap <= 0 means none.  A missing page, or a length that the page table does
+ * not hold, sets the bounds bit; such positions are not attended.  max_seq_len: the longest
+ * length to expect (only the number of CTAs and the scratch follow from it).  32-bit
+ * activations (q or out) keep 22 bits of q and of the probabilities, others 11.
+ * scratch: b200moe_kv8_attend_scratch_bytes(...) bytes, 16-byte aligned, not shared with a
+ * call that may run at the same time. */
 size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_t bs, int32_t new_tokens,
                                         int32_t heads, int32_t max_seq_len);
 int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void* slab, const float* scales,

@@ -135,8 +135,9 @@ def norm_rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache:
     8-bit codes: a scale block that the call begins has the scale amax / 127 (448 for
     e4m3) of the rows written; one that it continues keeps its scale while the new rows
     fit, else the scale grows by a power of two and the block's earlier codes are rounded
-    to it.  Positions behind the last written one of a block are dead until written.  An
-    infinity or NaN makes its block read as NaN."""
+    to it.  Positions behind the last written one of a block are dead until written (a
+    drafted token that is taken back leaves its block's scale as it made it).  An infinity
+    or NaN makes its block read as NaN until it is begun again."""
     return C.attention_ops.write(q, k, v, cache_state, _geometry(cache), block_index, seq_block_ids, start_positions, new_lens,
                                  freqs, q_norm, k_norm, eps, use_hf)
 

@@ -701,3 +701,62 @@ def test_new_tokens_behind_the_page_table(sl):
     room = ko.attend_tolerance(q[0, :1].cpu(), k, v, 64 ** -0.5, 2.0 ** -21, EPS[F32], want)
     for got in (o[0, :1], first[0]):
         assert ((got.cpu().double() - want).abs() <= room).all()
+
+
+def test_orders_and_alignments_of_the_inputs():
+    """Transposed, expanded, offset and sliced tensors, 64-bit and sliced index tensors, give
+    what contiguous ones give."""
+    A = _attention()
+    gen = torch.Generator().manual_seed(15)
+    cache = _cache(E4, 2, 64, 16, 8, layers=1)
+    ids = torch.tensor([[1, 4, 2], [5, 0, 3]], dtype=torch.int32).cuda()
+    q, k, v = (torch.randn(2, 20, h, 64, generator=gen).to(BF).cuda() for h in (8, 2, 2))
+    k = k[:1].expand(2, -1, -1, -1).contiguous()
+    start = torch.tensor([3, 0], dtype=torch.int32).cuda()
+    lens = torch.tensor([23, 20], dtype=torch.int32).cuda()
+
+    def off(t):  # starts two bytes behind a 16-byte boundary
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:]
+        return flat.copy_(t.reshape(-1)).view_as(t)
+
+    variants = {
+        "transposed": (lambda t: t.transpose(1, 2).contiguous().transpose(1, 2),) * 3,
+        "offset": (off, off, off),
+        "wide rows": (lambda t: torch.cat([t, t], dim=-1)[..., :64],) * 3,
+        "expanded": (lambda t: t, lambda t: t[:1].expand(2, -1, -1, -1), lambda t: t),
+        "padded rows": (lambda t: torch.cat([t.flatten(2), t.flatten(2)[..., :3]], dim=-1)[..., :-3].unflatten(-1, (-1, 64)),) * 3,
+    }
+
+    def go(q, k, v, ids, start, lens):
+        state = cache.allocate(6)
+        a, b = A.norm_rope_kv_write(q, k, v, cache, state, block_index=0, seq_block_ids=ids, start_positions=start,
+                                    freqs=_freqs(64).cuda())
+        o = A.kv_attend(q[:, :5], cache, state, block_index=0, seq_block_ids=ids, seq_lens=lens)
+        return [a, b, o, state[0].view(torch.int8), state[1], *A.kv_read(cache, state, block_index=0, seq_block_ids=ids, seq_lens=lens)]
+
+    want = go(q, k, v, ids, start, lens)
+    for name, fs in variants.items():
+        for x, y in zip(want, go(*(f(t) for f, t in zip(fs, (q, k, v))), ids, start, lens)):
+            assert torch.equal(x, y), name
+    wide = torch.cat([ids, ids], dim=1).long()[:, :3]
+    for x, y in zip(want, go(q, k, v, wide, start.long(), torch.stack([lens, lens], dim=1)[:, 0])):
+        assert torch.equal(x, y)
+    assert _status() == 0
+
+
+def test_rows_of_no_tokens():
+    A = _attention()
+    cache = _cache(I8, 2, 64, 16, layers=1)
+    state = cache.allocate(2)
+    e = lambda *s: torch.empty(*s, dtype=BF, device="cuda")
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    for bs, sl in ((0, 4), (2, 0)):
+        a, b = A.norm_rope_kv_write(e(bs, sl, 4, 64), e(bs, sl, 2, 64), e(bs, sl, 2, 64), cache, state, block_index=0,
+                                    seq_block_ids=i(bs, 1), start_positions=i(bs), freqs=_freqs(64).cuda())
+        assert a.shape == (bs, sl, 4, 64) and b.shape == (bs, sl, 2, 64)
+    assert A.kv_attend(e(0, 1, 4, 64), cache, state, block_index=0, seq_block_ids=i(0, 1), seq_lens=i(0)).shape == (0, 1, 4, 64)
+    k, v = A.kv_read(cache, state, block_index=0, seq_block_ids=i(2, 1), seq_lens=i(2), max_seq_len=0)
+    assert k.shape == v.shape == (2, 0, 2, 64)
+    k, v = A.kv_read(cache, state, block_index=0, seq_block_ids=i(2, 1), seq_lens=i(2))
+    assert not k.any() and not v.any()
+    assert _status() == 0
