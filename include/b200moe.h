@@ -474,7 +474,7 @@ int b200moe_attn_norm_rope_kv_write(const void* q, const void* k, const void* v,
  * listed pages' first seq_lens[seq] positions as contiguous k_out, v_out
  * [bs][max_seq_len][kv_heads][head_dim] of out_dtype, each c * s rounded once.  Rows at
  * and behind a sequence's length are zero.  A missing page sets the bounds bit and reads
- * as zeros. */
+ * as zeros.  At most 65535 sequences. */
 int b200moe_kv8_read(const void* slab, const float* scales, const b200moe_kv8_cache_t* cache, int32_t block_index,
                      const int32_t* page_ids, const int32_t* seq_lens, int32_t bs, int32_t pages_per_seq,
                      int32_t max_seq_len, void* k_out, void* v_out, int out_dtype, void* stream);

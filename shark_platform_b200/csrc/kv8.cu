@@ -114,11 +114,11 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& even, uint32_t& odd
     odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
   }
 }
-template <int CODE>
-__device__ __forceinline__ void codes_to_floats(uint2 c, float (&v)[8]) {
+template <int CODE, int N>
+__device__ __forceinline__ void codes_to_floats(const uint32_t (&c)[N / 4], float (&v)[N]) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t w = i ? c.y : c.x;
+  for (int i = 0; i < N / 4; ++i) {
+    const uint32_t w = c[i];
     float2 f[2];
     if constexpr (CODE == B200MOE_KV8_INT8) {
       uint32_t even, odd;
@@ -486,8 +486,10 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 2 ? 4 :
           const float shrink = kv ? v_shrink : k_shrink;
           if (shrink == 1.f) continue;
           uint2* at = reinterpret_cast<uint2*>(slab + static_cast<size_t>(s_row[r]) * HD + (kv ? v_off : 0) + c * 8);
+          const uint2 held = *at;
+          const uint32_t c8[2] = {held.x, held.y};
           float y[8];
-          codes_to_floats<KIND>(*at, y);
+          codes_to_floats<KIND>(c8, y);
           *at = floats_to_codes<KIND>(y, shrink);
         }
       }
@@ -579,43 +581,52 @@ struct ReadArgs {
   const float* scales;
   const int32_t *page_ids, *seq_lens;
   void *k_out, *v_out;
-  int bs, pages_per_seq, page_count, max_len, kv_heads, stride, blocks, block_index, block_shift;
+  int pages_per_seq, page_count, max_len, kv_heads, stride, blocks, block_index, stride_shift, block_shift;
   int32_t* status;
 };
 
-// One CTA per (sequence, kv head, 16 positions); a thread takes eight codes of a row (eight
-// bytes loaded, 16 stored in 16 bits: both whole sectors), K and V of two rows (HD 128) at
-// once.  Bound by HBM: 32 sequences of up to 4000 positions, 8 heads of 128, to bf16 (723 MB)
-// take 119 us, 6.1 TB/s; in tiles of 32, 64, 128 positions 122, 137, 170; with 16 codes per
-// thread and 4-byte stores 310.
+// One CTA per (sequence, kv head, 16 positions); a thread takes the codes of 16 bytes of
+// output (eight, or four for fp32: whole sectors are loaded and stored), K and V of several
+// rows at once.  Bound by HBM: 32 sequences of up to 4000 positions, 8 heads of 128, to bf16
+// (723 MB) take 114 us, 6.3 TB/s; with rows in tiles of 64 and 128 positions 137 and 170, with
+// the tile, head and sequence by division 119, with 16 codes per thread and 4-byte stores 310.
 constexpr int RD_THREADS = 128, RD_TILE = 16;
 template <typename T, int HD, int CODE>
 __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(const ReadArgs a) {
-  constexpr int LPR = HD / 8, RPP = RD_THREADS / LPR, PASSES = RD_TILE / RPP;
+  constexpr int E = 16 / static_cast<int>(sizeof(T)), W = E / 4;
+  constexpr int LPR = HD / E, RPP = RD_THREADS / LPR, PASSES = RD_TILE / RPP;
   grid_dep_wait();
   grid_dep_launch();
-  const int tiles = (a.max_len + RD_TILE - 1) / RD_TILE;
-  const int tile = blockIdx.x % tiles, h = blockIdx.x / tiles % a.kv_heads, b = blockIdx.x / tiles / a.kv_heads;
+  const int tile = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int sub = threadIdx.x / LPR, c = threadIdx.x % LPR;
   const int len = a.seq_lens[b];
   const size_t v_off = static_cast<size_t>(a.stride) * HD;
-  uint2 kc[PASSES], vc[PASSES];
+  uint32_t kc[PASSES][W], vc[PASSES][W];
   float2 sc[PASSES];
+  auto fetch = [](uint32_t (&to)[W], const uint8_t* from) {
+    if constexpr (W == 2) {
+      const uint2 w = *reinterpret_cast<const uint2*>(from);
+      to[0] = w.x; to[W - 1] = w.y;
+    } else {
+      to[0] = *reinterpret_cast<const uint32_t*>(from);
+    }
+  };
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int pos = tile * RD_TILE + i * RPP + sub;
-    kc[i] = vc[i] = make_uint2(0, 0);
+#pragma unroll
+    for (int j = 0; j < W; ++j) kc[i][j] = vc[i][j] = 0u;
     sc[i] = make_float2(0.f, 0.f);
     if (pos < len && pos < a.max_len) {
-      const int slot = pos / a.stride, off = pos - slot * a.stride;
+      const int slot = a.stride_shift >= 0 ? pos >> a.stride_shift : pos / a.stride, off = pos - slot * a.stride;
       const int page = slot < a.pages_per_seq ? a.page_ids[static_cast<size_t>(b) * a.pages_per_seq + slot] : -1;
       if (page < 0 || page >= a.page_count) {
         atomicOr(a.status, DEV_ERR_BOUNDS);
       } else {
         const size_t head = (static_cast<size_t>(page) * a.blocks + a.block_index) * a.kv_heads + h;
-        const uint8_t* at = a.slab + (head * 2 * a.stride + off) * HD + c * 8;
-        kc[i] = *reinterpret_cast<const uint2*>(at);
-        vc[i] = *reinterpret_cast<const uint2*>(at + v_off);
+        const uint8_t* at = a.slab + (head * 2 * a.stride + off) * HD + c * E;
+        fetch(kc[i], at);
+        fetch(vc[i], at + v_off);
         sc[i] = reinterpret_cast<const float2*>(a.scales)[head * (a.stride >> a.block_shift) + (off >> a.block_shift)];
       }
     }
@@ -624,25 +635,27 @@ __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(const ReadArgs a) 
   for (int i = 0; i < PASSES; ++i) {
     const int pos = tile * RD_TILE + i * RPP + sub;
     if (pos >= a.max_len) return;
-    const size_t to = ((static_cast<size_t>(b) * a.max_len + pos) * a.kv_heads + h) * HD + c * 8;
+    const size_t to = ((static_cast<size_t>(b) * a.max_len + pos) * a.kv_heads + h) * HD + c * E;
     const bool live = pos < len;  // a NaN scale shows in live rows only
-    float y[8];
-    codes_to_floats<CODE>(kc[i], y);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = live ? y[j] * sc[i].x : 0.f;
-    store8(static_cast<T*>(a.k_out) + to, y);
-    codes_to_floats<CODE>(vc[i], y);
+    for (int kv = 0; kv < 2; ++kv) {
+      float y[E];
+      codes_to_floats<CODE>(kv ? vc[i] : kc[i], y);
+      const float s = kv ? sc[i].y : sc[i].x;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = live ? y[j] * sc[i].y : 0.f;
-    store8(static_cast<T*>(a.v_out) + to, y);
+      for (int j = 0; j < E; ++j) y[j] = live ? y[j] * s : 0.f;
+      T* p = static_cast<T*>(kv ? a.v_out : a.k_out) + to;
+      if constexpr (E == 8) store8(p, y);
+      else *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
+    }
   }
 }
 
 template <typename T, int HD>
-int launch_read(const ReadArgs& a, int code, unsigned grid, cudaStream_t st) {
+int launch_read(const ReadArgs& a, int code, dim3 grid, cudaStream_t st) {
   B200_CHECK_CUDA(launch_dependent(code == B200MOE_KV8_INT8 ? kv8_read_kernel<T, HD, B200MOE_KV8_INT8>
                                                            : kv8_read_kernel<T, HD, B200MOE_KV8_E4M3>,
-                                   dim3(grid), dim3(RD_THREADS), 0, st, a));
+                                   grid, dim3(RD_THREADS), 0, st, a));
   return B200MOE_OK;
 }
 
@@ -1542,7 +1555,7 @@ int b200moe_kv8_read(const void* slab, const float* scales, const b200moe_kv8_ca
                      int32_t max_seq_len, void* k_out, void* v_out, int out_dtype, void* stream) {
   const char* who = "kv8_read";
   if (const int rc = check_kv8(who, cache, block_index)) return rc;
-  B200_REQUIRE(bs >= 0 && pages_per_seq >= 1 && max_seq_len >= 0, "%s: bad sizes", who);
+  B200_REQUIRE(bs >= 0 && bs <= 65535 && pages_per_seq >= 1 && max_seq_len >= 0, "%s: bad sizes", who);
   if (bs == 0 || max_seq_len == 0) return B200MOE_OK;
   B200_REQUIRE(slab && scales && page_ids && seq_lens && k_out && v_out, "%s: NULL buffer", who);
   B200_REQUIRE(dtype_ok(out_dtype), "%s: unknown dtype", who);
@@ -1550,14 +1563,12 @@ int b200moe_kv8_read(const void* slab, const float* scales, const b200moe_kv8_ca
                "%s: slab and outputs must be 16-byte aligned, scales 8-byte", who);
   ReadArgs a;
   a.slab = static_cast<const uint8_t*>(slab); a.scales = scales; a.page_ids = page_ids; a.seq_lens = seq_lens;
-  a.k_out = k_out; a.v_out = v_out; a.bs = bs; a.pages_per_seq = pages_per_seq;
+  a.k_out = k_out; a.v_out = v_out; a.pages_per_seq = pages_per_seq;
   a.page_count = cache->page_count; a.max_len = max_seq_len; a.kv_heads = cache->kv_heads; a.stride = cache->stride;
-  a.blocks = cache->blocks; a.block_index = block_index; a.block_shift = log2_of(cache->scale_block);
+  a.blocks = cache->blocks; a.block_index = block_index; a.stride_shift = log2_of(cache->stride); a.block_shift = log2_of(cache->scale_block);
   a.status = device_status_ptr();
   if (a.status == nullptr) return B200MOE_ERR_CUDA;
-  const int64_t ctas = static_cast<int64_t>((max_seq_len - 1) / RD_TILE + 1) * bs * cache->kv_heads;
-  B200_REQUIRE(ctas <= 0x7fffffff, "%s: too many rows for one call", who);
-  const unsigned grid = static_cast<unsigned>(ctas);
+  const dim3 grid((max_seq_len - 1) / RD_TILE + 1, cache->kv_heads, bs);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool h64 = cache->head_dim == 64;
   if (out_dtype == B200MOE_DT_F32)
