@@ -141,9 +141,11 @@ __device__ __forceinline__ uint2 floats_to_codes(const float (&v)[8], float by) 
   for (int i = 0; i < 2; ++i) {
     const float* x = v + 4 * i;
     if constexpr (CODE == B200MOE_KV8_INT8) {
-      const int a = __float2int_rn(x[0] * by), b = __float2int_rn(x[1] * by), e = __float2int_rn(x[2] * by),
-                f = __float2int_rn(x[3] * by);
-      c[i] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(e, f, 0x0040), 0x5410);
+      // in the last place of 1.5 * 2^23 + y stands y, rounded to even, in two's complement
+      uint32_t n[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) n[j] = __float_as_uint(fmaf(x[j], by, 12582912.f));
+      c[i] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
     } else {
       c[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * by, x[1] * by), __NV_SATFINITE, __NV_E4M3) |
              static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x[2] * by, x[3] * by), __NV_SATFINITE, __NV_E4M3)) << 16;
@@ -207,59 +209,75 @@ __device__ __forceinline__ float max_nan(float m, float x) {
   asm("{.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;}" : "=f"(y) : "f"(m), "f"(x));
   return y;
 }
-// What lane c of a row needs of the position's cosines and sines: of its four pairs, or in
-// the HuggingFace order of each of its eight elements.  There the other half of each pair is
-// LPR / 2 lanes away with the same angles: either lane computes four and they are exchanged.
-template <int ORDER>
-struct Turn { float2 t[ORDER == 0 ? 4 : 8]; };
-template <typename T, int LPR, int ORDER>
-__device__ __forceinline__ Turn<ORDER> turn_of(long long pos, const float* freqs, int c) {
-  Turn<ORDER> w;
-  const bool upper = c >= LPR / 2;
-  const int j0 = ORDER == 0 ? c * 4 : (c % (LPR / 2)) * 8 + (upper ? 4 : 0);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w.t[i] = cos_sin<T>(pos, freqs[j0 + i]);
-  if constexpr (ORDER != 0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 mine = w.t[i];
-      float2 other;
-      other.x = __shfl_xor_sync(0xffffffffu, mine.x, LPR / 2);
-      other.y = __shfl_xor_sync(0xffffffffu, mine.y, LPR / 2);
-      w.t[i] = upper ? other : mine;
-      w.t[4 + i] = upper ? mine : other;
-    }
+// The eight elements of a row that lane c of HD / 8 has, so that it has whole pairs: in order
+// 0 (pairs 2i, 2i + 1) elements 8c .. 8c + 7, in the HuggingFace order (pairs i, i + HD / 2)
+// 4c .. 4c + 3 and as many behind HD / 2.  Its pairs' frequencies are 4c .. 4c + 3 either way.
+template <int HD, int ORDER>
+__device__ __forceinline__ int element(int c, int i) {
+  return ORDER == 0 ? 8 * c + i : (i < 4 ? 4 * c + i : HD / 2 + 4 * c + i - 4);
+}
+template <typename T, int HD, int ORDER>
+__device__ __forceinline__ void load_row(Raw8<T>& x, const T* row, int c) {
+  if constexpr (ORDER == 0) {
+    x.load(row + 8 * c);
+  } else if constexpr (sizeof(T) == 4) {
+    x.w[0] = *reinterpret_cast<const uint4*>(row + 4 * c);
+    x.w[1] = *reinterpret_cast<const uint4*>(row + HD / 2 + 4 * c);
+  } else {
+    const uint2 lo = *reinterpret_cast<const uint2*>(row + 4 * c), hi = *reinterpret_cast<const uint2*>(row + HD / 2 + 4 * c);
+    x.w[0] = make_uint4(lo.x, lo.y, hi.x, hi.y);
   }
+}
+template <typename T, int HD, int ORDER>
+__device__ __forceinline__ void store_row(T* row, int c, const float (&v)[8]) {
+  if constexpr (ORDER == 0) {
+    store8(row + 8 * c, v);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(row + 4 * c) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(row + HD / 2 + 4 * c) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint2*>(row + 4 * c) = make_uint2(pack2(row, v[0], v[1]), pack2(row, v[2], v[3]));
+    *reinterpret_cast<uint2*>(row + HD / 2 + 4 * c) = make_uint2(pack2(row, v[4], v[5]), pack2(row, v[6], v[7]));
+  }
+}
+template <int HD, int ORDER>
+__device__ __forceinline__ void store_codes(uint8_t* row, int c, uint2 v) {
+  if constexpr (ORDER == 0) {
+    *reinterpret_cast<uint2*>(row + 8 * c) = v;
+  } else {
+    *reinterpret_cast<uint32_t*>(row + 4 * c) = v.x;
+    *reinterpret_cast<uint32_t*>(row + HD / 2 + 4 * c) = v.y;
+  }
+}
+
+// Cosines and sines of a lane's four pairs.
+struct Turn { float2 t[4]; };
+template <typename T>
+__device__ __forceinline__ Turn turn_of(long long pos, const float* freqs, int c) {
+  Turn w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w.t[i] = cos_sin<T>(pos, freqs[4 * c + i]);
   return w;
 }
 // A lane's eight elements of a row, normed and rotated; LPR lanes have a row.
 template <int LPR, int ORDER>
-__device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], bool norm, float eps,
-                                            const Turn<ORDER>& turn, int c) {
+__device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], bool norm, float eps, const Turn& turn) {
   if (norm) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = 1.0f / sqrtf(ss / (8 * LPR) + eps);
+    const float r = rsqrtf(ss * (1.f / (8 * LPR)) + eps);  // 2^-22; root and division cost a tenth of the kernel
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = w[i] * (x[i] * r);
   }
-  if constexpr (ORDER == 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float re = x[2 * i], im = x[2 * i + 1];
-      x[2 * i] = re * turn.t[i].x - im * turn.t[i].y;
-      x[2 * i + 1] = im * turn.t[i].x + re * turn.t[i].y;
-    }
-  } else {
-    const float sign = c < LPR / 2 ? -1.f : 1.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_xor_sync(0xffffffffu, x[i], LPR / 2);
-      x[i] = x[i] * turn.t[i].x + sign * other * turn.t[i].y;
-    }
+  for (int i = 0; i < 4; ++i) {
+    constexpr int STEP = ORDER == 0 ? 2 : 1, OTHER = ORDER == 0 ? 1 : 4;
+    const float re = x[STEP * i], im = x[STEP * i + OTHER];
+    x[STEP * i] = re * turn.t[i].x - im * turn.t[i].y;
+    x[STEP * i + OTHER] = im * turn.t[i].x + re * turn.t[i].y;
   }
 }
 
@@ -298,12 +316,14 @@ __device__ __forceinline__ BlockScale block_scale(unsigned bits, float before) {
 // everything.  The others have the queries: a lane keeps its position's cosines and sines
 // and takes four heads at once, q_heads in all.  HD / 8 lanes have a row (16-byte loads and
 // stores of 16-bit rows), a warp two or four rows.  Bound by HBM, then by how much of it the
-// CTAs keep asking for: 4 x 2048 tokens of 48 + 16 heads (268 MB) take 50 us, 5.3 TB/s; with
-// K, V and the queries of a kv head in one CTA 79 (the queries waited for the barriers of K
-// and V), with three CTAs an SM instead of four 66, with K's and V's CTAs before the others
-// instead of among them 60.
+// CTAs keep asking for: 4 x 2048 tokens of 48 + 16 heads (268 MB) take 47 us, 5.7 TB/s.  On
+// the way there: K, V and the queries of a kv head in one CTA 79 (the queries waited for the
+// barriers of K and V); CTAs of two kinds, three an SM 66, four 60 (five, registers in memory,
+// 54 instead of 47 later on; heads of 64 fit five: 13.9 instead of 14.7); K's and V's CTAs
+// among the others instead of before them 52; rounding of the codes by an addition and the
+// approximate reciprocal root 47.
 template <typename T, int HD, int KIND, int TILE, int ORDER>
-__global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 2 ? 4 : 3) : 2) norm_rope_write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 4 ? 3 : HD == 64 ? 5 : 4) : 2) norm_rope_write_kernel(const WriteArgs a) {
   constexpr int LPR = HD / 8, RPW = 32 / LPR;                 // lanes per row, rows of a warp
   constexpr int RPP = WR_WARPS * RPW;                         // rows of a pass
   constexpr int PASSES = (TILE + RPP - 1) / RPP;
@@ -336,24 +356,24 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 2 ? 4 :
     const long long tok = item % tokens;
     const int h0 = static_cast<int>(item / tokens) * a.q_heads, h1 = min(h0 + a.q_heads, a.heads);
     const int b = static_cast<int>(tok / a.sl);
-    const T* from = q + tok * a.q_stride + c * 8;
-    T* to = static_cast<T*>(a.q_out) + tok * a.heads * HD + c * 8;
+    const T* from = q + tok * a.q_stride;
+    T* to = static_cast<T*>(a.q_out) + tok * a.heads * HD;
     const long long pos = max(a.start_positions[b], 0) + (tok - static_cast<long long>(b) * a.sl);
-    const Turn<ORDER> turn = turn_of<T, LPR, ORDER>(pos, a.freqs, c);
+    const Turn turn = turn_of<T>(pos, a.freqs, c);
     float w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = a.q_norm != nullptr ? a.q_norm[c * 8 + i] : 1.f;
+    for (int i = 0; i < 8; ++i) w[i] = a.q_norm != nullptr ? a.q_norm[element<HD, ORDER>(c, i)] : 1.f;
     // every lane of a warp makes the same number of steps: heads behind the last are read again and not stored
     for (int d = 0; d < a.q_heads; d += QB) {
       Raw8<T> raw[QB];
 #pragma unroll
-      for (int g = 0; g < QB; ++g) raw[g].load(from + min(h0 + d + g, h1 - 1) * HD);
+      for (int g = 0; g < QB; ++g) load_row<T, HD, ORDER>(raw[g], from + min(h0 + d + g, h1 - 1) * HD, c);
 #pragma unroll
       for (int g = 0; g < QB; ++g) {
         float x[8];
         raw[g].get(x);
-        norm_rotate<LPR, ORDER>(x, w, a.q_norm != nullptr, a.eps, turn, c);
-        if (some && h0 + d + g < h1) store8(to + (h0 + d + g) * HD, x);
+        norm_rotate<LPR, ORDER>(x, w, a.q_norm != nullptr, a.eps, turn);
+        if (some && h0 + d + g < h1) store_row<T, HD, ORDER>(to + (h0 + d + g) * HD, c, x);
       }
     }
     return;
@@ -378,8 +398,8 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 2 ? 4 :
     const int r = lo + i * RPP + sub;
     kr[i].zero();
     vr[i].zero();
-    if (r < hi) kr[i].load(k + (tok0 + r) * a.k_stride + kvh * HD + c * 8);
-    if (r < whi) vr[i].load(v + (tok0 + r) * a.v_stride + kvh * HD + c * 8);
+    if (r < hi) load_row<T, HD, ORDER>(kr[i], k + (tok0 + r) * a.k_stride + kvh * HD, c);
+    if (r < whi) load_row<T, HD, ORDER>(vr[i], v + (tok0 + r) * a.v_stride + kvh * HD, c);
   }
   const int first = KIND == CACHE_PLAIN ? lo : lo >> a.block_shift << a.block_shift;  // earlier rows of a continued block included
   for (int r = first + t; r < whi; r += WR_THREADS) {
@@ -407,32 +427,32 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 2 ? 4 :
   if (warp < kv_warps) {
     float w[8], kx[PASSES][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = a.k_norm != nullptr ? a.k_norm[c * 8 + i] : 1.f;
+    for (int i = 0; i < 8; ++i) w[i] = a.k_norm != nullptr ? a.k_norm[element<HD, ORDER>(c, i)] : 1.f;
     // all lanes take part in the shuffles of the norm and the rotation; rows outside lo .. hi are zeros, unused
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int r = lo + i * RPP + sub;
       if (lo + i * RPP >= hi) break;
       kr[i].get(kx[i]);
-      norm_rotate<LPR, ORDER>(kx[i], w, a.k_norm != nullptr, a.eps, turn_of<T, LPR, ORDER>(p0 + r, a.freqs, c), c);
+      norm_rotate<LPR, ORDER>(kx[i], w, a.k_norm != nullptr, a.eps, turn_of<T>(p0 + r, a.freqs, c));
       if (r < hi && a.k_out != nullptr)
-        store8(static_cast<T*>(a.k_out) + ((tok0 + r) * a.kv_heads + kvh) * HD + c * 8, kx[i]);
+        store_row<T, HD, ORDER>(static_cast<T*>(a.k_out) + ((tok0 + r) * a.kv_heads + kvh) * HD, c, kx[i]);
       if constexpr (KIND == CACHE_PLAIN) {
         if (r < whi && s_row[r] >= 0) {
           float y[8];
           vr[i].get(y);
 #pragma unroll
           for (int j = 0; j < 8; ++j) kx[i][j] = round_to<T>(kx[i][j]);
-          const size_t at = static_cast<size_t>(s_row[r]) * HD + c * 8, v_at = at + static_cast<size_t>(a.stride) * a.kv_heads * HD;
+          const size_t at = static_cast<size_t>(s_row[r]) * HD, v_at = at + static_cast<size_t>(a.stride) * a.kv_heads * HD;
           if (a.cache_dtype == B200MOE_DT_F32) {
-            store8(static_cast<float*>(a.slab) + at, kx[i]);
-            store8(static_cast<float*>(a.slab) + v_at, y);
+            store_row<float, HD, ORDER>(static_cast<float*>(a.slab) + at, c, kx[i]);
+            store_row<float, HD, ORDER>(static_cast<float*>(a.slab) + v_at, c, y);
           } else if (a.cache_dtype == B200MOE_DT_F16) {
-            store8(static_cast<__half*>(a.slab) + at, kx[i]);
-            store8(static_cast<__half*>(a.slab) + v_at, y);
+            store_row<__half, HD, ORDER>(static_cast<__half*>(a.slab) + at, c, kx[i]);
+            store_row<__half, HD, ORDER>(static_cast<__half*>(a.slab) + v_at, c, y);
           } else {
-            store8(static_cast<__nv_bfloat16*>(a.slab) + at, kx[i]);
-            store8(static_cast<__nv_bfloat16*>(a.slab) + v_at, y);
+            store_row<__nv_bfloat16, HD, ORDER>(static_cast<__nv_bfloat16*>(a.slab) + at, c, kx[i]);
+            store_row<__nv_bfloat16, HD, ORDER>(static_cast<__nv_bfloat16*>(a.slab) + v_at, c, y);
           }
         }
       } else {
@@ -470,11 +490,11 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 2 ? 4 :
         const float2 before = continued ? s_before : make_float2(0.f, 0.f);
         const BlockScale ks = block_scale<KIND>(s_amax[0][blk], before.x), vs = block_scale<KIND>(s_amax[1][blk], before.y);
         if (r == at_blk && c == 0) reinterpret_cast<float2*>(a.scales)[s_pair[r]] = make_float2(ks.s, vs.s);
-        uint8_t* at = slab + static_cast<size_t>(s_row[r]) * HD + c * 8;
-        *reinterpret_cast<uint2*>(at) = floats_to_codes<KIND>(kx[i], ks.inv);
+        uint8_t* at = slab + static_cast<size_t>(s_row[r]) * HD;
+        store_codes<HD, ORDER>(at, c, floats_to_codes<KIND>(kx[i], ks.inv));
         float y[8];
         vr[i].get(y);
-        *reinterpret_cast<uint2*>(at + v_off) = floats_to_codes<KIND>(y, vs.inv);
+        store_codes<HD, ORDER>(at + v_off, c, floats_to_codes<KIND>(y, vs.inv));
       }
       // the live rows of a continued block whose scale has grown
       if (first < lo && lo < whi && s_row[lo] >= 0) {
