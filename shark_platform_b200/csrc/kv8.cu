@@ -717,7 +717,8 @@ int launch_read(const ReadArgs& a, int code, dim3 grid, cudaStream_t st) {
 // e4m3 43, 4.9 and 4.7 TB/s (a plain read of as much, by a reduction, 39 us); bound by HBM
 // once under way, before by the chain of lengths, page ids and first rows (6 us), after by the
 // merge (4 us).  With a CTA per position split of each sequence 68.  Several new tokens are
-// bound by the instructions around the MMAs: 16 rows 48 us, 32 rows 85 us of the same cache.
+// bound by the instructions around the MMAs: 16 rows 48 us, 32 rows, in two tiles that each
+// widen the codes, 88 us of the same cache (in one tile, q in shared memory, 86: not kept).
 struct AttendArgs {
   const void* q;
   int64_t q_stride;
@@ -846,7 +847,6 @@ struct Stretches {
 // as they are now.)
 template <int HD, int NT, bool SPLIT>
 constexpr int attend_resident() {
-  if (NT == 4) return HD == 128 ? 2 : 3;
   if (HD == 128) return NT == 1 && !SPLIT ? 3 : 2;
   return NT == 1 ? 4 : 3;
 }
@@ -863,10 +863,6 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
   float* s_o = reinterpret_cast<float*>(smem + AT_WARPS * 2 * TILE);
   __shared__ float4 s_pos[AT_WARPS][AT_UNIT];       // of each position: s_k, log2 s_v, 1 / s_v
   __shared__ float2 s_ml[AT_WARPS][ROWS];
-  constexpr bool Q_SHARED = NT == 4;
-  static_assert(!Q_SHARED || (AT_WARPS == NT && !SPLIT), "a warp prepares one tile of q");
-  __shared__ uint2 s_q[Q_SHARED ? CH : 1][NT][32];
-  __shared__ float s_fold[ROWS];
   grid_dep_wait();
   grid_dep_launch();
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gid = lane >> 2, tig = lane & 3;
@@ -961,12 +957,11 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
   };
 
   // q as it lies in memory: a lane's four elements of each chunk of its column's row
-  constexpr int QN = Q_SHARED ? 1 : NT;
-  uint32_t q_raw[QN][CH][SPLIT ? 4 : 2];
+  uint32_t q_raw[NT][CH][SPLIT ? 4 : 2];
   auto load_q = [&](const Piece& p) {
 #pragma unroll
-    for (int n = 0; n < QN; ++n) {
-      const int r = p.tile * ROWS + 8 * (Q_SHARED ? warp : n) + gid;
+    for (int n = 0; n < NT; ++n) {
+      const int r = p.tile * ROWS + 8 * n + gid;
       const int64_t from = (static_cast<int64_t>(p.b) * a.sl + r / G) * a.q_stride +
                            static_cast<int64_t>(p.kvh * G + r % G) * HD + 4 * tig;
 #pragma unroll
@@ -1025,14 +1020,12 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
       next.p_end = next.units = 0;
     }
 
-    // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two.  Four
-    // columns' tiles do not fit in registers beside the output: there a warp prepares one, in
-    // the order of the fragments, and all read them from shared memory.
+    // q: column gid of B is row tile * ROWS + 8 n + gid; its values times a power of two
     if (!Q_FIRST || g != g_begin) load_q(cur);
-    uint32_t qb[PARTS][QN][CH][2];
+    uint32_t qb[PARTS][NT][CH][2];
     float fold[NT][2];  // of this lane's accumulator columns 2 tig, 2 tig + 1: back to to_score units
 #pragma unroll
-    for (int n = 0; n < QN; ++n) {
+    for (int n = 0; n < NT; ++n) {
       float x[CH][4], top = 0.f;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
@@ -1048,12 +1041,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
       if (__float_as_uint(top) == 0x7f800000u) e = 100;
       const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
       const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23) * to_score;
-      if constexpr (Q_SHARED) {
-        if (tig == 0) s_fold[8 * warp + gid] = down;
-      } else {
-        fold[n][0] = __shfl_sync(0xffffffffu, down, (2 * tig) * 4);
-        fold[n][1] = __shfl_sync(0xffffffffu, down, (2 * tig + 1) * 4);
-      }
+      fold[n][0] = __shfl_sync(0xffffffffu, down, (2 * tig) * 4);
+      fold[n][1] = __shfl_sync(0xffffffffu, down, (2 * tig + 1) * 4);
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -1066,17 +1055,6 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
             qb[PARTS - 1][n][c][i] = h2_as_u32(__floats2half2_rn(u - f.x, v - f.y));
           }
         }
-    }
-    if constexpr (Q_SHARED) {
-      // (the last segment's q is read: its end has a barrier)
-#pragma unroll
-      for (int c = 0; c < CH; ++c) s_q[c][warp][lane] = make_uint2(qb[0][0][c][0], qb[0][0][c][1]);
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        fold[n][0] = s_fold[8 * n + 2 * tig];
-        fold[n][1] = s_fold[8 * n + 2 * tig + 1];
-      }
     }
     // the first position that a column does not see
     const int all_see = a.seq_lens[b] - a.sl + 1;
@@ -1106,51 +1084,36 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
       const uint32_t kt = ring, vt = kt + TILE;
       const int p0 = cur.p_begin + u * AT_STEP;
 
-      // two accumulators for each 16 positions where there are no others to alternate with;
-      // both halves of the unit at once where q comes from shared memory
-      constexpr int ACC = NT == 1 ? 2 : 1, HB = Q_SHARED ? 2 : 1;
+      // two accumulators for each 16 positions where there are no others to alternate with
+      constexpr int ACC = NT == 1 ? 2 : 1;
       float s[2][NT][4];
 #pragma unroll
-      for (int h0 = 0; h0 < 2; h0 += HB) {
-        float acc[ACC][HB][NT][4];
+      for (int h = 0; h < 2; ++h) {
+        float acc[ACC][NT][4];
 #pragma unroll
         for (int k = 0; k < ACC; ++k)
 #pragma unroll
-          for (int h = 0; h < HB; ++h)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) acc[k][h][n][0] = acc[k][h][n][1] = acc[k][h][n][2] = acc[k][h][n][3] = 0.f;
+          for (int n = 0; n < NT; ++n) acc[k][n][0] = acc[k][n][1] = acc[k][n][2] = acc[k][n][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; c += 2) {
-          uint32_t w[HB][4];
-#pragma unroll
-          for (int h = 0; h < HB; ++h) ldsm_x4(kt + ld_at[c / 2] + 16 * (h0 + h) * HD, w[h]);
+          uint32_t w[4];
+          ldsm_x4(kt + ld_at[c / 2] + 16 * h * HD, w);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t f[HB][4];
-#pragma unroll
-            for (int h = 0; h < HB; ++h) {
-              widen4<CODE>(w[h][2 * i], f[h][0], f[h][2]);
-              widen4<CODE>(w[h][2 * i + 1], f[h][1], f[h][3]);
-            }
+            uint32_t a0, a1, a2, a3;
+            widen4<CODE>(w[2 * i], a0, a2);
+            widen4<CODE>(w[2 * i + 1], a1, a3);
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                uint2 y;
-                if constexpr (Q_SHARED) y = s_q[c + i][n][lane];
-                else y = make_uint2(qb[p][n][c + i][0], qb[p][n][c + i][1]);
-#pragma unroll
-                for (int h = 0; h < HB; ++h) mma(acc[i % ACC][h][n], f[h][0], f[h][1], f[h][2], f[h][3], y.x, y.y);
-              }
+              for (int n = 0; n < NT; ++n)
+                mma(acc[i % ACC][n], a0, a1, a2, a3, qb[p][n][c + i][0], qb[p][n][c + i][1]);
           }
         }
 #pragma unroll
-        for (int h = 0; h < HB; ++h)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              s[h0 + h][n][k] = ACC == 2 ? acc[0][h][n][k] + acc[ACC - 1][h][n][k] : acc[0][h][n][k];
+          for (int k = 0; k < 4; ++k) s[h][n][k] = ACC == 2 ? acc[0][n][k] + acc[ACC - 1][n][k] : acc[0][n][k];
       }
       __syncwarp();  // K is read: its place takes that of the next unit
       const bool last = u + 1 == units;
@@ -1473,15 +1436,14 @@ int launch_merge(const AttendArgs& a, int tile_rows, cudaStream_t st) {
 
 // Rows of a CTA's tile; CTAs of a call: as many as are resident at once, or one for each
 // step of a full page table where those are fewer.
-inline int attend_tile_rows(int rows, bool split) { return rows <= 8 ? 8 : rows <= 16 || split ? 16 : 32; }
+inline int attend_tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
 template <int HD>
 int resident_ctas(int tile, bool split) {
-  if (tile == 32) return attend_resident<HD, 4, false>();
   if (tile == 16) return split ? attend_resident<HD, 2, true>() : attend_resident<HD, 2, false>();
   return split ? attend_resident<HD, 1, true>() : attend_resident<HD, 1, false>();
 }
 int attend_ctas(const b200moe_kv8_cache_t& c, int bs, int rows, bool split, int max_seq_len) {
-  const int tile = attend_tile_rows(rows, split);
+  const int tile = attend_tile_rows(rows);
   const int64_t steps = (static_cast<int64_t>(max_seq_len) + AT_STEP - 1) / AT_STEP * bs * c.kv_heads * ((rows + tile - 1) / tile);
   const int64_t resident = static_cast<int64_t>(sm_count()) * 
                            (c.head_dim == 128 ? resident_ctas<128>(tile, split) : resident_ctas<64>(tile, split));
@@ -1504,7 +1466,6 @@ int launch_attend(const AttendArgs& a, cudaStream_t st) {
 }
 template <int HD, int CODE>
 int launch_attend_rows(const AttendArgs& a, bool split, int tile_rows, cudaStream_t st) {
-  if (tile_rows == 32) return launch_attend<HD, CODE, 4, false>(a, st);
   if (tile_rows == 8) return split ? launch_attend<HD, CODE, 1, true>(a, st) : launch_attend<HD, CODE, 1, false>(a, st);
   return split ? launch_attend<HD, CODE, 2, true>(a, st) : launch_attend<HD, CODE, 2, false>(a, st);
 }
@@ -1608,7 +1569,7 @@ size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_
   size_t most = 0;  // the activations' type is not known here: enough for any
   for (const bool split : {false, true}) {
     const size_t n = static_cast<size_t>(attend_ctas(*cache, bs, rows, split, max_seq_len)) * 2 *
-                     attend_tile_rows(rows, split) * (cache->head_dim + 4) * sizeof(float);
+                     attend_tile_rows(rows) * (cache->head_dim + 4) * sizeof(float);
     most = n > most ? n : most;
   }
   return most;
@@ -1647,7 +1608,7 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index;
   // 32-bit activations: 22 bits of q and of the probabilities
   const bool split = q_dtype == B200MOE_DT_F32 || out_dtype == B200MOE_DT_F32;
-  const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows, split), hd = cache->head_dim;
+  const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows), hd = cache->head_dim;
   a.row_tiles = (rows + tile - 1) / tile;
   a.ctas = attend_ctas(*cache, bs, rows, split, max_seq_len);
   a.stride_shift = log2_of(a.stride);
