@@ -401,7 +401,8 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 4 ? 3 :
     if (r < hi) load_row<T, HD, ORDER>(kr[i], k + (tok0 + r) * a.k_stride + kvh * HD, c);
     if (r < whi) load_row<T, HD, ORDER>(vr[i], v + (tok0 + r) * a.v_stride + kvh * HD, c);
   }
-  const int first = KIND == CACHE_PLAIN ? lo : lo >> a.block_shift << a.block_shift;  // earlier rows of a continued block included
+  // earlier rows of a continued block included, if anything is written
+  const int first = KIND == CACHE_PLAIN || whi <= lo ? lo : lo >> a.block_shift << a.block_shift;
   for (int r = first + t; r < whi; r += WR_THREADS) {
     const uint32_t pos = static_cast<uint32_t>(p0 + r), slot = a.stride_shift >= 0 ? pos >> a.stride_shift : pos / a.stride;
     const uint32_t off = pos - slot * a.stride;
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 4 ? 3 :
         store_codes<HD, ORDER>(at + v_off, c, floats_to_codes<KIND>(y, vs.inv));
       }
       // the live rows of a continued block whose scale has grown
-      if (first < lo && lo < whi && s_row[lo] >= 0) {
+      if (first < lo && s_row[lo] >= 0) {
         const int blk = first >> a.block_shift;
         const float k_shrink = block_scale<KIND>(s_amax[0][blk], s_before.x).shrink;
         const float v_shrink = block_scale<KIND>(s_amax[1][blk], s_before.y).shrink;

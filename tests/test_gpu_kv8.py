@@ -300,6 +300,25 @@ def test_padding_rows_do_not_touch_the_cache():
     assert _status() == 0
 
 
+@pytest.mark.parametrize("code", [I8, E4, BF])
+def test_a_sequence_of_padding_needs_no_pages(code):
+    """new_lens 0 in the middle of a scale block: nothing is looked up, written or reported."""
+    A = _attention()
+    gen = torch.Generator().manual_seed(3)
+    cache = _cache(code, 2, 64, 32)
+    state = _fill(cache, 3, gen) if cache.quantized else cache.allocate(3)
+    before = [t.clone() for t in state]
+    x = torch.randn(2, 40, 2, 64, generator=gen).cuda()
+    for ids, start in (([[-1, 9], [7, -1]], [5, 37]), ([[0, 1], [1, 2]], [63, 1000])):
+        q, k = A.norm_rope_kv_write(x, x, x, cache, state, block_index=0, freqs=_freqs(64).cuda(),
+                                    seq_block_ids=torch.tensor(ids).cuda(), start_positions=torch.tensor(start).cuda(),
+                                    new_lens=torch.tensor([0, -3]).cuda())
+        assert _status() == 0
+        assert torch.equal(q, k) and q.isfinite().all()  # rotated all the same
+    for t, was in zip(state, before):
+        assert torch.equal(t.view(torch.uint8), was.view(torch.uint8))
+
+
 def test_missing_pages_are_reported_and_skipped():
     from shark_platform_b200 import _cabi as C
 
