@@ -295,11 +295,12 @@ __device__ __forceinline__ BlockScale block_scale(unsigned bits, float before) {
     r.s = __uint_as_float(0x7fc00000u);
   } else if (before > 0.f) {
     r.s = before;
-    const float ratio = amax / (before * qmax * (1.f + 0.0009765625f));
-    if (ratio > 1.f) {
-      int e;
-      const float m = frexpf(ratio, &e);
-      if (m == 0.5f) --e;
+    // the smallest e with amax <= fits * 2^e, from the two exponents: their quotient can be beyond 2^128
+    const float fits = before * qmax * (1.f + 0.0009765625f);
+    if (amax > fits) {
+      int ea, ef;
+      const float ma = frexpf(amax, &ea), mf = frexpf(fits, &ef);
+      const int e = ea - ef + (ma > mf);
       r.s = ldexpf(before, e);
       r.shrink = ldexpf(1.f, -e);
     }

@@ -1,0 +1,48 @@
+"""The operators of the 8-bit KV cache at the ends of their range, against their definition
+in 64 bits."""
+import pytest
+import torch
+
+import test_gpu_kv8 as base
+from oracle import kv8_oracle as ko
+
+pytestmark = pytest.mark.gpu
+
+I8, E4 = torch.int8, torch.float8_e4m3fn
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.parametrize("code", [I8, E4])
+@pytest.mark.parametrize("io", [BF, F32])
+@pytest.mark.parametrize("small,large", [(-88, 38), (-88, 39), (-88, 41), (-80, 50), (-88, 100), (-20, 107), (-20, 110)])
+def test_a_block_that_grows_by_any_power_of_two(code, io, small, large):
+    """Rows of size 2^small, then one of 2^large behind them in the same block: the quotient of
+    the two does not fit 32 bits where they are 2^128 apart."""
+    A = base._attention()
+    gen = torch.Generator().manual_seed(small - large)
+    cache = base._cache(code, 2, 64, 16, 16, layers=1)
+    state = cache.allocate(2)
+    ids = torch.tensor([[1]], dtype=torch.int32)
+    rows = [(torch.randn(1, n, 2, 64, generator=gen) * 2.0 ** size).to(io) for n, size in ((3, small), (1, large))]
+    kw = dict(block_index=0, seq_block_ids=ids.cuda(), freqs=base._freqs(64).cuda())
+    scales = []
+    for x, start in zip(rows, (0, 3)):
+        A.norm_rope_kv_write(x.cuda(), x.cuda(), x.cuda(), cache, state, start_positions=torch.tensor([start]).cuda(), **kw)
+        scales.append(ko.page_views(state, cache)[1][1, 0, :, 0])
+    codes = ko.page_views(state, cache)[0][1, 0]
+    assert base._status() == 0
+    qmax = ko.QMAX[code]
+    turned = [ko.turn(x, torch.arange(s, s + x.shape[1])[None], base._freqs(64)) for x, s in zip(rows, (0, 3))]
+    for h in range(2):
+        for slot, (first, new) in enumerate((turned, [x.double() for x in rows])):
+            new = new[0, 0, h]
+            old, s = float(scales[0][h, slot]), float(scales[1][h, slot])
+            # the rotation's error is at most 2^-19 of the largest value: nowhere near a border here
+            grow = ko.growth(float(new.abs().max()), old, qmax)
+            assert s == old * 2.0 ** grow
+            y = new / s
+            room = ko.half_step(y, code) * (1 + 2.0 ** -10) + y.abs().max() * 2.0 ** -18
+            assert ((codes[h, slot, 3] - y).abs() - room <= 0).all()
+            # what the earlier rows come to in steps of the new scale: the code they had, and its rounding
+            y = first[0, :, h] / s
+            assert ((codes[h, slot, :3] - y).abs() <= ko.half_step(y, code) * 2 + y.abs().max() * 2.0 ** -4).all()
