@@ -181,23 +181,29 @@ constexpr int WR_WARPS = WR_THREADS / 32;
 constexpr float QMAX[2] = {127.f, 448.f};
 
 // Cosine and sine of position * freq, the angle reduced to part of a turn first.
-// 32-bit rows: reduced in 64 bits, good to 2^-23 at any position.  16-bit rows: the position
-// (below 2^24) times freq / (2 pi) as the sum of two floats, their integer part dropped, and
-// the special-function unit, absolute error 2^-21: a thousandth of half a step of fp16.
-// (sincospif for both: 5 us of 71 for 4 x 2048 tokens of 48 + 16 heads.)
+// 32-bit rows, and far angles: reduced in 64 bits; the half turns are rounded by 2^-25, which
+// is pi 2^-25 of angle, and sincospif is good to an ulp or two: 2^-22 up to 2^25 turns (the
+// products in 64 bits are off by 2^-52 of the turns, which shows above).
+// 16-bit rows: the position (below 2^24, exact) times freq / (2 pi) as the sum of two floats
+// u + u_lo.  Below 2^22 turns u_lo is at most an eighth, so that the integer part is dropped
+// before and after the sum: the special-function unit's bounds hold within a turn only, 2^-21.4
+// (sine) and 2^-21.2.  The sum is rounded by 2^-25 of a turn, the product with 2 pi by 2^-23
+// and 2 pi itself by 2^-25 of it: 2^-20 in all, a 256th of half a step of fp16 just below one,
+// and 1e-4 of a step of int8.  (With power series, good to 2^-22: 49.0 instead of 47.4 us for
+// 4 x 2048 tokens of 48 + 16 heads, 8.0 instead of 7.2 for 777 of 32 + 8, and the same error of
+// q, k and K's codes against 64 bits in three digits; sincospif 48.4 and 8.0.)
 template <typename T>
 __device__ __forceinline__ float2 cos_sin(long long pos, float freq) {
+  constexpr double inv = 0.15915494309189533577;  // 1 / (2 pi)
+  constexpr float inv_hi = static_cast<float>(inv), inv_lo = static_cast<float>(inv - inv_hi);
+  const float p = static_cast<float>(static_cast<int>(pos)), g = freq * inv_hi, u = p * g;
   float sn, cs;
-  if (sizeof(T) == 4 || pos >= 1 << 24) {
-    const double turns = static_cast<double>(pos) * (static_cast<double>(freq) * 0.31830988618379067154);  // halves
+  if (sizeof(T) == 4 || pos >= 1 << 24 || !(fabsf(u) < 4194304.f)) {
+    const double turns = static_cast<double>(pos) * (static_cast<double>(freq) * (2.0 * inv));  // halves
     sincospif(static_cast<float>(turns - 2.0 * rint(0.5 * turns)), &sn, &cs);
   } else {
-    constexpr double inv = 0.15915494309189533577;  // 1 / (2 pi)
-    constexpr float inv_hi = static_cast<float>(inv), inv_lo = static_cast<float>(inv - inv_hi);
-    const float p = static_cast<float>(static_cast<int>(pos));
-    const float g = freq * inv_hi, g_lo = fmaf(freq, inv_hi, -g) + freq * inv_lo;
-    const float u = p * g, u_lo = fmaf(p, g_lo, fmaf(p, g, -u));
-    const float angle = ((u - rintf(u)) + u_lo) * 6.2831853071795864769f;
+    const float g_lo = fmaf(freq, inv_hi, -g) + freq * inv_lo, u_lo = fmaf(p, g_lo, fmaf(p, g, -u));
+    const float r = (u - rintf(u)) + u_lo, angle = (r - rintf(r)) * 6.2831853071795864769f;
     sn = __sinf(angle);
     cs = __cosf(angle);
   }

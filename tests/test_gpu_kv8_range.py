@@ -46,3 +46,35 @@ def test_a_block_that_grows_by_any_power_of_two(code, io, small, large):
             # what the earlier rows come to in steps of the new scale: the code they had, and its rounding
             y = first[0, :, h] / s
             assert ((codes[h, slot, :3] - y).abs() <= ko.half_step(y, code) * 2 + y.abs().max() * 2.0 ** -4).all()
+
+
+@pytest.mark.parametrize("io", [HF, BF])
+@pytest.mark.parametrize("hd,halves,stretch", [(128, False, 1.0), (64, True, 1.0), (64, False, 40.0)])
+@pytest.mark.parametrize("start", [0, 8000, 130_000, 1_047_000, 6_000_000, (1 << 24) - 2048, (1 << 30) + 12345])
+def test_angles_of_16_bit_rows(io, hd, halves, stretch, start):
+    """Rows are the 64-bit rotation rounded once, at any position and for frequencies above
+    one.  A value is re * cos - im * sin: with cosine and sine good to 2^-20, the angle's part of
+    its error is at most (|re| + |im|) 2^-20, and the product and the sum in 32 bits add 2^-24
+    of as much each.  Angles of many turns: the products of the definition and of the kernel in
+    64 bits are rounded by 2^-53 of the angle, four times in all."""
+    A = base._attention()
+    gen = torch.Generator().manual_seed(start % 1000)
+    cache = base._cache(BF, 1, hd, 32, layers=1)
+    sl, heads = 4096, 1024 // hd
+    q = (torch.rand(1, sl, heads, hd, generator=gen) * 2 - 1).to(io).cuda()
+    k = q[:, :, :1].contiguous()
+    freqs = (base._freqs(hd) * stretch).cuda()
+    got = A.norm_rope_kv_write(q, k, k, cache, cache.allocate(1), block_index=0, freqs=freqs, use_hf=halves,
+                               seq_block_ids=torch.zeros(1, 1, dtype=torch.int32).cuda(),
+                               start_positions=torch.tensor([start]).cuda(), new_lens=torch.tensor([0]).cuda())
+    assert base._status() == 0
+    pos = start + torch.arange(sl, device="cuda")[None]
+    for x, y in zip((q, k), got):
+        want = ko.turn(x, pos, freqs, halves=halves)
+        pair = x.double().abs().unflatten(-1, (2, hd // 2) if halves else (hd // 2, 2))
+        at = -2 if halves else -1
+        size = pair.sum(at, keepdim=True).expand_as(pair).flatten(-2)
+        half = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -14))) - (11 if io == HF else 8))
+        angle = (start + sl) * float(freqs.max())
+        over = (y.double() - want).abs() - half - size * (2.0 ** -20 + 2 * 2.0 ** -24 + angle * 2.0 ** -51)
+        assert over.max() <= 0, float(over.max())
