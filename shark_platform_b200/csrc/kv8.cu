@@ -133,22 +133,29 @@ __device__ __forceinline__ void codes_to_floats(const uint32_t (&c)[N / 4], floa
     v[4 * i] = f[0].x; v[4 * i + 1] = f[0].y; v[4 * i + 2] = f[1].x; v[4 * i + 3] = f[1].y;
   }
 }
-// v[i] * by, values / scale at most 2^-10 above qmax, to the nearest codes: without clamping
+// v[i] * (by + by_lo), values / scale at most 2^-10 above qmax, to the nearest codes: without
+// clamping.  The factor is the sum of two floats because quotients halfway between two codes
+// are common (half of the largest value of an int8 block is 63.5 steps): the product has to be
+// that number again, to go to the even code, and with a factor off by 2^-24 it falls to either
+// side.  (With one float the error of V against codes from 64-bit quotients is a tenth larger
+// for bf16 rows and three quarters for fp16, all of it from these.)
 template <int CODE>
-__device__ __forceinline__ uint2 floats_to_codes(const float (&v)[8], float by) {
+__device__ __forceinline__ uint2 floats_to_codes(const float (&v)[8], float by, float by_lo) {
   uint32_t c[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float* x = v + 4 * i;
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = fmaf(v[4 * i + j], by, v[4 * i + j] * by_lo);
     if constexpr (CODE == B200MOE_KV8_INT8) {
       // in the last place of 1.5 * 2^23 + y stands y, rounded to even, in two's complement
       uint32_t n[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) n[j] = __float_as_uint(fmaf(x[j], by, 12582912.f));
+      for (int j = 0; j < 4; ++j) n[j] = __float_as_uint(y[j] + 12582912.f);
       c[i] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
     } else {
-      c[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * by, x[1] * by), __NV_SATFINITE, __NV_E4M3) |
-             static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x[2] * by, x[3] * by), __NV_SATFINITE, __NV_E4M3)) << 16;
+      c[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3) |
+             static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3)) << 16;
     }
   }
   return make_uint2(c[0], c[1]);
@@ -287,15 +294,22 @@ __device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], 
   }
 }
 
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // The scale of a block from the largest magnitude of its new rows (as bits) and, if it is
-// continued, the scale it had (else 0); 1 / scale; and what its earlier codes are multiplied
-// by: the scale grows by powers of two.
-struct BlockScale { float s, inv, shrink; };
+// continued, the scale it had (else 0); the factor to codes, qmax / amax of a fresh block and
+// 1 / scale of a continued one, as an approximate reciprocal (scales are below 2^122) and what
+// it lacks; and what the earlier codes are multiplied by: the scale grows by powers of two.
+struct BlockScale { float s, inv, inv_lo, shrink; };
 template <int KIND>
 __device__ __forceinline__ BlockScale block_scale(unsigned bits, float before) {
   constexpr float qmax = QMAX[KIND], tiny = 7.888609052210118e-31f;  // 2^-100
   const float amax = __uint_as_float(bits);
   BlockScale r;
+  r.inv = r.inv_lo = 0.f;
   r.shrink = 1.f;
   if (bits >= 0x7f800000u || before != before) {
     r.s = __uint_as_float(0x7fc00000u);
@@ -310,10 +324,15 @@ __device__ __forceinline__ BlockScale block_scale(unsigned bits, float before) {
       r.s = ldexpf(before, e);
       r.shrink = ldexpf(1.f, -e);
     }
+    r.inv = rcp(r.s);
+    r.inv_lo = fmaf(-r.inv, r.s, 1.f) * r.inv;
+  } else if (amax < qmax * tiny) {
+    r.s = 0.f;
   } else {
-    r.s = amax < qmax * tiny ? 0.f : amax / qmax;
+    r.s = amax / qmax;
+    r.inv = rcp(r.s);
+    r.inv_lo = fmaf(-r.inv, amax, qmax) * (r.inv * (1.f / qmax));
   }
-  r.inv = r.s > 0.f ? 1.f / r.s : 0.f;
   return r;
 }
 
@@ -499,10 +518,10 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 4 ? 3 :
         const BlockScale ks = block_scale<KIND>(s_amax[0][blk], before.x), vs = block_scale<KIND>(s_amax[1][blk], before.y);
         if (r == at_blk && c == 0) reinterpret_cast<float2*>(a.scales)[s_pair[r]] = make_float2(ks.s, vs.s);
         uint8_t* at = slab + static_cast<size_t>(s_row[r]) * HD;
-        store_codes<HD, ORDER>(at, c, floats_to_codes<KIND>(kx[i], ks.inv));
+        store_codes<HD, ORDER>(at, c, floats_to_codes<KIND>(kx[i], ks.inv, ks.inv_lo));
         float y[8];
         vr[i].get(y);
-        store_codes<HD, ORDER>(at + v_off, c, floats_to_codes<KIND>(y, vs.inv));
+        store_codes<HD, ORDER>(at + v_off, c, floats_to_codes<KIND>(y, vs.inv, vs.inv_lo));
       }
       // the live rows of a continued block whose scale has grown
       if (first < lo && s_row[lo] >= 0) {
@@ -518,7 +537,7 @@ __global__ void __launch_bounds__(WR_THREADS, TILE == 32 ? (sizeof(T) == 4 ? 3 :
           const uint32_t c8[2] = {held.x, held.y};
           float y[8];
           codes_to_floats<KIND>(c8, y);
-          *at = floats_to_codes<KIND>(y, shrink);
+          *at = floats_to_codes<KIND>(y, shrink, 0.f);
         }
       }
     }
@@ -751,11 +770,6 @@ constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {

@@ -78,3 +78,38 @@ def test_angles_of_16_bit_rows(io, hd, halves, stretch, start):
         angle = (start + sl) * float(freqs.max())
         over = (y.double() - want).abs() - half - size * (2.0 ** -20 + 2 * 2.0 ** -24 + angle * 2.0 ** -51)
         assert over.max() <= 0, float(over.max())
+
+
+@pytest.mark.parametrize("code", [I8, E4])
+@pytest.mark.parametrize("io", [BF, HF, F32])
+def test_values_halfway_between_two_codes(code, io):
+    """V whose quotient by amax / qmax is exactly between two codes takes the even one.  16-bit
+    activations meet them often: half of the largest value is 63.5 steps of an int8 block."""
+    A = base._attention()
+    qmax = ko.QMAX[code]
+    rows = []
+    for m in range(1, 37):
+        if code == I8:  # v / amax * 127 = odd / 2: half of amax; of 127 / 64 also others
+            for top in range(64 + m, 128, 36):
+                rows.append([top / 64.0, top / 128.0, -top / 128.0] + ([j / 128.0 for j in range(1, 122, 2)] if top == 127 else []))
+        elif 7 * m < 256:  # v / amax * 448 with an odd five-bit number before the last place: odd * m of amax = 7 m
+            rows.append([7.0 * m] + [odd * m * 2.0 ** -e for odd in range(17, 32, 2) if odd * m < 256
+                                     for e in range(3, 9) if odd * m * 2.0 ** -e <= 7 * m])
+    v = torch.zeros(len(rows), 64)
+    for i, r in enumerate(rows):
+        v[i, :min(len(r), 64)] = torch.tensor(r[:64])
+    v = v.to(io)
+    n = len(rows)
+    cache = base._cache(code, 1, 64, 1, 1, layers=1)  # a block for each row
+    state = cache.allocate(n)
+    x = v[None, :, None].cuda()
+    A.norm_rope_kv_write(x, x, x, cache, state, block_index=0, seq_block_ids=torch.arange(n)[None].cuda(),
+                         start_positions=torch.tensor([0]).cuda(), freqs=base._freqs(64).cuda())
+    assert base._status() == 0
+    codes = ko.page_views(state, cache)[0][:, 0, 0, 1, 0]
+    amax = v.double().abs().amax(-1, keepdim=True)
+    y = v.double() * qmax / amax  # exact where it lies between two codes
+    step = 2 * ko.half_step(y, code)
+    tie = (y / step * 2) % 2 == 1
+    assert int(tie.sum()) >= (100 if code == I8 else 300)
+    assert torch.equal(codes, ko.to_code(y, code))
