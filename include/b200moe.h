@@ -487,8 +487,9 @@ int b200moe_kv8_read(const void* slab, const float* scales, const b200moe_kv8_ca
  * out [bs][new_tokens][heads][head_dim] contiguous.  Any heads / kv_heads; at most 65535
  * sequences; softcap <= 0 means none.  A missing page, or a length that the page table does
  * not hold, sets the bounds bit; such positions are not attended.  max_seq_len: the longest
- * length to expect (only the number of CTAs and the scratch follow from it).  32-bit
- * activations (q or out) keep 22 bits of q and of the probabilities, others 11.
+ * length to expect (only the number of CTAs and the scratch follow from it).  The
+ * probabilities keep 22 bits for fp32 and fp16 outputs and for fp32 q, 11 for bf16 outputs
+ * of 16-bit q; q is held as it is (fp32: 22 bits).
  * scratch: b200moe_kv8_attend_scratch_bytes(...) bytes, 16-byte aligned, not shared with a
  * call that may run at the same time. */
 size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_t bs, int32_t new_tokens,

@@ -160,7 +160,10 @@ def kv_attend(q: torch.Tensor, cache: PagedKVCache, cache_state: list, *, block_
     the sl new ones included (`norm_rope_kv_write` first).  Token i attends the positions
     up to and including its own, seq_lens[b] - sl + i; where that leaves none its output is
     zero.  scale: 1 / sqrt(head_dim) by default; softcap: c * tanh(score / c).  Returns
-    [bs, sl, heads, head_dim]."""
+    [bs, sl, heads, head_dim].
+
+    Sums and softmax statistics are 32-bit.  The probabilities are rounded to 22 bits where the
+    output is fp32 or fp16 or q is fp32, else (bf16) to 11, an eighth of the output's rounding."""
     return C.attention_ops.attend(q, cache_state, _geometry(cache), block_index, seq_block_ids, seq_lens, scale, softcap,
                                   out_dtype)
 

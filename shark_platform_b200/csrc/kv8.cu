@@ -728,8 +728,10 @@ int launch_read(const ReadArgs& a, int code, dim3 grid, cudaStream_t st) {
 // the denominator.  q is fp16 with its largest value in [2^14, 2^15), P with 2^7 where the
 // maximum is up to date (it is left behind by up to 2^8, so that the output is rescaled
 // rarely): what rounding loses is 2^-11 of a value down to 2^-28 and 2^-21 of the largest,
-// and 2^-32 of the largest P below.  SPLIT (32-bit activations): q and P are the sums of two
-// fp16 parts, 2^-22, at twice the MMAs.
+// and 2^-32 of the largest P below.  A bf16 output's own rounding is eight times that; an fp16
+// output would be off by a third more than its rounding, and P is the sum of two fp16 parts
+// for it, 2^-22, at one and a half times the MMAs (32 x 4000 positions int8 41 us instead of
+// 40, e4m3 46 instead of 42.5, four new tokens 53 instead of 48).  SPLIT (32-bit activations): q too.
 //
 // A warp owns units of 32 positions with its own softmax state and places for one unit's K
 // and V, filled by 16-byte cp.async, each again as soon as it is read: no barrier between
@@ -762,6 +764,9 @@ struct AttendArgs {
   int32_t* status;
 };
 
+// In how many fp16 parts the operands are: one; P in two (fp16 outputs); q and P in two (32-bit
+// activations).
+enum { BITS_ONE = 0, BITS_P = 1, BITS_BOTH = 2 };
 constexpr int AT_THREADS = 128, AT_WARPS = 4;
 constexpr int AT_UNIT = 32;   // positions of a warp's step
 constexpr int AT_STEP = AT_WARPS * AT_UNIT;
@@ -867,16 +872,17 @@ struct Stretches {
 // more: NT = 1 44 instead of 41 us, NT = 2 61 instead of 48, at 32 x 4000 positions of int8;
 // one less: e4m3 51 instead of 48, int8 41 instead of 43, before the e4m3 codes were widened
 // as they are now.)
-template <int HD, int NT, bool SPLIT>
+template <int HD, int NT, int BITS>
 constexpr int attend_resident() {
-  if (HD == 128) return NT == 1 && !SPLIT ? 3 : 2;
+  if (HD == 128) return NT == 1 && BITS != BITS_BOTH ? 3 : 2;
   return NT == 1 ? 4 : 3;
 }
 
-template <int HD, int CODE, int NT, bool SPLIT>
-__global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())) kv8_attend_kernel(const AttendArgs a) {
+template <int HD, int CODE, int NT, int BITS>
+__global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, BITS>())) kv8_attend_kernel(const AttendArgs a) {
   constexpr int CH = HD / 16;                       // chunks of a row: MMA steps of q.k, row tiles of V^T
-  constexpr int PARTS = SPLIT ? 2 : 1;
+  constexpr bool SPLIT = BITS == BITS_BOTH;
+  constexpr int PARTS = SPLIT ? 2 : 1, P_PARTS = BITS == BITS_ONE ? 1 : 2;
   constexpr int ROWS = 8 * NT;
   constexpr int TILE = AT_UNIT * HD;                // bytes of a unit's K (or V)
   constexpr int OPITCH = HD + 8;                    // floats
@@ -1211,7 +1217,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
             for (int c = 0; c < CH; ++c) { o[n][c][e] *= alpha; o[n][c][2 + e] *= alpha; }
           }
       }
-      uint32_t pb[PARTS][NT][2][2];
+      uint32_t pb[P_PARTS][NT][2][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float base0 = P_TOP - (m[n][0] == -INFINITY ? 0.f : m[n][0]);
@@ -1225,9 +1231,9 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
             l[n][1] = fmaf(u1, ivs[h][j], l[n][1]);
             const __half2 hp = __floats2half2_rn(u0, u1);
             pb[0][n][h][j] = transpose8x8(h2_as_u32(hp));
-            if constexpr (SPLIT) {
+            if constexpr (P_PARTS == 2) {
               const float2 f = __half22float2(hp);
-              pb[PARTS - 1][n][h][j] = transpose8x8(h2_as_u32(__floats2half2_rn(u0 - f.x, u1 - f.y)));
+              pb[P_PARTS - 1][n][h][j] = transpose8x8(h2_as_u32(__floats2half2_rn(u0 - f.x, u1 - f.y)));
             }
           }
       }
@@ -1275,7 +1281,9 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, SPLIT>())
               widen4<CODE>(w[2 * i], a0, a1);
               widen4<CODE>(w[2 * i + 1], a2, a3);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma(o[n][c + i], a0, a1, a2, a3, pb[0][n][h][0], pb[0][n][h][1]);
+              for (int p = 0; p < P_PARTS; ++p)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma(o[n][c + i], a0, a1, a2, a3, pb[p][n][h][0], pb[p][n][h][1]);
             }
           }
       }
@@ -1460,22 +1468,23 @@ int launch_merge(const AttendArgs& a, int tile_rows, cudaStream_t st) {
 // step of a full page table where those are fewer.
 inline int attend_tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
 template <int HD>
-int resident_ctas(int tile, bool split) {
-  if (tile == 16) return split ? attend_resident<HD, 2, true>() : attend_resident<HD, 2, false>();
-  return split ? attend_resident<HD, 1, true>() : attend_resident<HD, 1, false>();
+int resident_ctas(int tile, int bits) {
+  if (bits == BITS_BOTH) return tile == 16 ? attend_resident<HD, 2, BITS_BOTH>() : attend_resident<HD, 1, BITS_BOTH>();
+  if (bits == BITS_P) return tile == 16 ? attend_resident<HD, 2, BITS_P>() : attend_resident<HD, 1, BITS_P>();
+  return tile == 16 ? attend_resident<HD, 2, BITS_ONE>() : attend_resident<HD, 1, BITS_ONE>();
 }
-int attend_ctas(const b200moe_kv8_cache_t& c, int bs, int rows, bool split, int max_seq_len) {
+int attend_ctas(const b200moe_kv8_cache_t& c, int bs, int rows, int bits, int max_seq_len) {
   const int tile = attend_tile_rows(rows);
   const int64_t steps = (static_cast<int64_t>(max_seq_len) + AT_STEP - 1) / AT_STEP * bs * c.kv_heads * ((rows + tile - 1) / tile);
   const int64_t resident = static_cast<int64_t>(sm_count()) * 
-                           (c.head_dim == 128 ? resident_ctas<128>(tile, split) : resident_ctas<64>(tile, split));
+                           (c.head_dim == 128 ? resident_ctas<128>(tile, bits) : resident_ctas<64>(tile, bits));
   return static_cast<int>(steps < resident ? steps : resident);
 }
 
-template <int HD, int CODE, int NT, bool SPLIT>
+template <int HD, int CODE, int NT, int BITS>
 int launch_attend(const AttendArgs& a, cudaStream_t st) {
   constexpr int SMEM = AT_WARPS * 2 * AT_UNIT * HD + AT_WARPS * 8 * NT * (HD + 8) * 4;
-  auto kern = kv8_attend_kernel<HD, CODE, NT, SPLIT>;
+  auto kern = kv8_attend_kernel<HD, CODE, NT, BITS>;
   static bool configured[16] = {};
   int dev = 0;
   B200_CHECK_CUDA(cudaGetDevice(&dev));
@@ -1487,9 +1496,11 @@ int launch_attend(const AttendArgs& a, cudaStream_t st) {
   return B200MOE_OK;
 }
 template <int HD, int CODE>
-int launch_attend_rows(const AttendArgs& a, bool split, int tile_rows, cudaStream_t st) {
-  if (tile_rows == 8) return split ? launch_attend<HD, CODE, 1, true>(a, st) : launch_attend<HD, CODE, 1, false>(a, st);
-  return split ? launch_attend<HD, CODE, 2, true>(a, st) : launch_attend<HD, CODE, 2, false>(a, st);
+int launch_attend_rows(const AttendArgs& a, int bits, int tile_rows, cudaStream_t st) {
+  const bool one = tile_rows == 8;
+  if (bits == BITS_BOTH) return one ? launch_attend<HD, CODE, 1, BITS_BOTH>(a, st) : launch_attend<HD, CODE, 2, BITS_BOTH>(a, st);
+  if (bits == BITS_P) return one ? launch_attend<HD, CODE, 1, BITS_P>(a, st) : launch_attend<HD, CODE, 2, BITS_P>(a, st);
+  return one ? launch_attend<HD, CODE, 1, BITS_ONE>(a, st) : launch_attend<HD, CODE, 2, BITS_ONE>(a, st);
 }
 
 }  // namespace
@@ -1589,8 +1600,8 @@ size_t b200moe_kv8_attend_scratch_bytes(const b200moe_kv8_cache_t* cache, int32_
     return 0;
   const int rows = heads / cache->kv_heads * new_tokens;
   size_t most = 0;  // the activations' type is not known here: enough for any
-  for (const bool split : {false, true}) {
-    const size_t n = static_cast<size_t>(attend_ctas(*cache, bs, rows, split, max_seq_len)) * 2 *
+  for (const int bits : {BITS_ONE, BITS_P, BITS_BOTH}) {
+    const size_t n = static_cast<size_t>(attend_ctas(*cache, bs, rows, bits, max_seq_len)) * 2 *
                      attend_tile_rows(rows) * (cache->head_dim + 4) * sizeof(float);
     most = n > most ? n : most;
   }
@@ -1628,11 +1639,10 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   a.out_dtype = out_dtype; a.bs = bs; a.sl = new_tokens;
   a.pages_per_seq = pages_per_seq; a.page_count = cache->page_count; a.heads = heads; a.kv_heads = cache->kv_heads;
   a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index;
-  // 32-bit activations: 22 bits of q and of the probabilities
-  const bool split = q_dtype == B200MOE_DT_F32 || out_dtype == B200MOE_DT_F32;
+  const int bits = q_dtype == B200MOE_DT_F32 || out_dtype == B200MOE_DT_F32 ? BITS_BOTH : out_dtype == B200MOE_DT_F16 ? BITS_P : BITS_ONE;
   const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows), hd = cache->head_dim;
   a.row_tiles = (rows + tile - 1) / tile;
-  a.ctas = attend_ctas(*cache, bs, rows, split, max_seq_len);
+  a.ctas = attend_ctas(*cache, bs, rows, bits, max_seq_len);
   a.stride_shift = log2_of(a.stride);
   a.block_shift = log2_of(cache->scale_block);
   B200_REQUIRE(static_cast<double>(bs) * a.kv_heads * a.row_tiles *
@@ -1646,11 +1656,11 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   const bool i8 = cache->code == B200MOE_KV8_INT8;
   int rc;
   if (hd == 64)
-    rc = i8 ? launch_attend_rows<64, B200MOE_KV8_INT8>(a, split, tile, st)
-            : launch_attend_rows<64, B200MOE_KV8_E4M3>(a, split, tile, st);
+    rc = i8 ? launch_attend_rows<64, B200MOE_KV8_INT8>(a, bits, tile, st)
+            : launch_attend_rows<64, B200MOE_KV8_E4M3>(a, bits, tile, st);
   else
-    rc = i8 ? launch_attend_rows<128, B200MOE_KV8_INT8>(a, split, tile, st)
-            : launch_attend_rows<128, B200MOE_KV8_E4M3>(a, split, tile, st);
+    rc = i8 ? launch_attend_rows<128, B200MOE_KV8_INT8>(a, bits, tile, st)
+            : launch_attend_rows<128, B200MOE_KV8_E4M3>(a, bits, tile, st);
   if (rc) return rc;
   if (static_cast<int64_t>(pages_per_seq) * a.stride <= AT_STEP) return B200MOE_OK;  // no segment is longer than a step
   return hd == 64 ? launch_merge<64>(a, tile, st) : launch_merge<128>(a, tile, st);

@@ -113,3 +113,29 @@ def test_values_halfway_between_two_codes(code, io):
     tie = (y / step * 2) % 2 == 1
     assert int(tie.sum()) >= (100 if code == I8 else 300)
     assert torch.equal(codes, ko.to_code(y, code))
+
+
+@pytest.mark.parametrize("code", [I8, E4])
+@pytest.mark.parametrize("io,hd,heads,kvh,sl,softcap", [(HF, 128, 32, 8, 1, None), (HF, 64, 32, 8, 1, None), (BF, 128, 32, 8, 1, None),
+                                                        (HF, 128, 16, 4, 4, 30.0), (HF, 64, 48, 8, 5, None)])
+def test_fp16_outputs_lose_their_own_rounding_only(code, io, hd, heads, kvh, sl, softcap):
+    """fp16 outputs are off by what rounding the 64-bit result to fp16 costs.  Its errors are
+    uniform in a step: their 2-norm over N >= 8192 elements varies by sqrt(0.8 / N) / 2 = 0.5 %
+    at most, and what 32-bit sums, a 22-bit probability and the exponential add is 2^-20 of the
+    values, a two-hundredth of fp16's 2^-11 / sqrt(3): within 4 %.  Probabilities of 11 bits add a third."""
+    A = base._attention()
+    gen = torch.Generator().manual_seed(hd + heads)
+    cache = base._cache(code, kvh, hd, 32, 16, layers=1)
+    lens = [40, 333, 1200, 64, 200, 77]
+    state = base._fill(cache, 40, gen)
+    ids = torch.stack([torch.randperm(40, generator=gen)[:38] for _ in lens]).to(torch.int32)
+    q = torch.randn(len(lens), sl, heads, hd, generator=gen).to(io)
+    got = A.kv_attend(q.cuda(), cache, state, block_index=0, seq_block_ids=ids.cuda(), seq_lens=torch.tensor(lens).cuda(),
+                      softcap=softcap, out_dtype=HF)
+    assert base._status() == 0 and got.dtype == HF
+    codes, scales = ko.page_views(state, cache)
+    want = torch.stack([ko.attend(q[b], *ko.gather(codes, scales, cache, 0, ids[b], n), [n - sl + 1 + i for i in range(sl)],
+                                  hd ** -0.5, softcap) for b, n in enumerate(lens)])
+    assert want.numel() >= 8192
+    off, least = (got.cpu().double() - want).norm(), (want.half().double() - want).norm()
+    assert off <= 1.04 * least, float(off / least)
