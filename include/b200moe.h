@@ -485,7 +485,7 @@ int b200moe_kv8_read(const void* slab, const float* scales, const b200moe_kv8_ca
  * to and including seq_lens[seq] - new_tokens + i, and its output is zero where that
  * leaves none.  q [bs * new_tokens] rows of heads * head_dim elements, q_stride apart;
  * out [bs][new_tokens][heads][head_dim] contiguous.  Any heads / kv_heads; at most 65535
- * sequences; softcap <= 0 means none.  A missing page, or a length that the page table does
+ * sequences; softcap (finite) <= 0 means none.  A missing page, or a length that the page table does
  * not hold, sets the bounds bit; such positions are not attended.  max_seq_len: the longest
  * length to expect (only the number of CTAs and the scratch follow from it).  The
  * probabilities keep 22 bits for fp32 and fp16 outputs and for fp32 q, 11 for bf16 outputs

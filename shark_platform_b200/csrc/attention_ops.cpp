@@ -330,7 +330,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (sl < 1 || sl > 16) refuse(sl, " new tokens: 1 to 16; longer stretches attend kv_read's K and V");
   const double scale = a[6] == Py_None ? 1.0 / std::sqrt(static_cast<double>(hd)) : number(a[6]);
   const double softcap = a[7] == Py_None ? 0.0 : number(a[7]);
-  if (a[7] != Py_None && !(softcap > 0.0)) refuse("softcap must be positive");
+  if (a[7] != Py_None && !(softcap > 0.0 && std::isfinite(static_cast<float>(softcap)))) refuse("softcap must be positive and finite");
   const at::Device dev = q.device();
   const at::Tensor& lens = tensor(a[5], "seq_lens");
   need_vector(lens, bs, dev, "seq_lens is one whole number for each sequence, on q's device");

@@ -6,6 +6,8 @@
 // A code c stands for c * s.
 #include <cuda_fp8.h>
 
+#include <cmath>
+
 #include "kernels.h"
 
 namespace b200moe {
@@ -765,7 +767,9 @@ struct AttendArgs {
 };
 
 // In how many fp16 parts the operands are: one; P in two (fp16 outputs); q and P in two (32-bit
-// activations).
+// activations, and softcaps above CAP_FAST: there what the fast form of the softcap is off by,
+// CAP_FAST * 2^-22 = 2^-14 of a probability, would begin to show).
+constexpr float CAP_FAST = 256.f;
 enum { BITS_ONE = 0, BITS_P = 1, BITS_BOTH = 2 };
 constexpr int AT_THREADS = 128, AT_WARPS = 4;
 constexpr int AT_UNIT = 32;   // positions of a warp's step
@@ -903,7 +907,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, BITS>()))
   const ListSum at = walk_list(a, lane, -1, g_begin, start);
 
   // Scores in halvings; with a softcap c, c tanh(x / c) = c - 2 c / (2^(2 log2(e) x / c) + 1):
-  // two special functions, good to c 2^-22.  32-bit activations take tanhf, 2^-22 of the value.
+  // two special functions, good to c 2^-22.  32-bit activations and caps above CAP_FAST take
+  // tanhf, 2^-22 of the value.
   const float cap2 = a.softcap * LOG2E;
   const float to_score = a.softcap > 0.f ? a.scale / a.softcap * (SPLIT ? 1.f : 2.f * LOG2E) : a.scale * LOG2E;
   const uint32_t ring = smem_u32(smem) + warp * (2 * TILE);
@@ -1619,6 +1624,7 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   B200_REQUIRE(static_cast<int64_t>(pages_per_seq) * cache->stride <= 1 << 30, "%s: more than 2^30 positions", who);
   B200_REQUIRE(new_tokens >= 1 && new_tokens <= MAX_NEW_TOKENS, "%s: new_tokens %d (1 to %d)", who, new_tokens,
                MAX_NEW_TOKENS);
+  B200_REQUIRE(std::isfinite(softcap), "%s: softcap must be finite", who);
   if (bs == 0) return B200MOE_OK;
   B200_REQUIRE(q && slab && scales && page_ids && seq_lens && out && scratch, "%s: NULL buffer", who);
   B200_REQUIRE(dtype_ok(q_dtype) && dtype_ok(out_dtype), "%s: unknown dtype", who);
@@ -1639,7 +1645,8 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
   a.out_dtype = out_dtype; a.bs = bs; a.sl = new_tokens;
   a.pages_per_seq = pages_per_seq; a.page_count = cache->page_count; a.heads = heads; a.kv_heads = cache->kv_heads;
   a.stride = cache->stride; a.blocks = cache->blocks; a.block_index = block_index;
-  const int bits = q_dtype == B200MOE_DT_F32 || out_dtype == B200MOE_DT_F32 ? BITS_BOTH : out_dtype == B200MOE_DT_F16 ? BITS_P : BITS_ONE;
+  const bool f32 = q_dtype == B200MOE_DT_F32 || out_dtype == B200MOE_DT_F32;
+  const int bits = f32 || softcap > CAP_FAST ? BITS_BOTH : out_dtype == B200MOE_DT_F16 ? BITS_P : BITS_ONE;
   const int rows = heads / cache->kv_heads * new_tokens, tile = attend_tile_rows(rows), hd = cache->head_dim;
   a.row_tiles = (rows + tile - 1) / tile;
   a.ctas = attend_ctas(*cache, bs, rows, bits, max_seq_len);

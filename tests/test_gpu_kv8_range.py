@@ -139,3 +139,12 @@ def test_fp16_outputs_lose_their_own_rounding_only(code, io, hd, heads, kvh, sl,
     assert want.numel() >= 8192
     off, least = (got.cpu().double() - want).norm(), (want.half().double() - want).norm()
     assert off <= 1.04 * least, float(off / least)
+
+
+@pytest.mark.parametrize("code", [I8, E4])
+@pytest.mark.parametrize("io", [BF, HF, F32])
+@pytest.mark.parametrize("softcap", [200.0, 300.0, 1e4, 1e6, 1e20])
+def test_large_softcaps(code, io, softcap):
+    """A cap far above every score leaves the scores as they are."""
+    base._attend_case(code, io, 128, 8, 2, 32, 16, [90, 300], softcap=softcap)
+    base._attend_case(code, io, 64, 12, 2, 16, 16, [33], sl=3, softcap=softcap)
