@@ -1106,11 +1106,10 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, BITS>()))
       sc_now = sc_next;
       {
         // dead positions (sc.y < 0: scales are never negative): weight 0 without touching the others
-        constexpr float unit = CODE == B200MOE_KV8_E4M3 ? E4M3_UNIT : 1.f;
-        const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f) * unit;  // 2^-100 in the place of 0
+        const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f);  // 2^-100 in the place of 0
         const bool dead = sc_now.y < 0.f, bad = sc_now.y != sc_now.y;
         s_pos[warp][lane] =
-            make_float4(sc_now.x * unit, dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : rcp(vs), 0.f);
+            make_float4(sc_now.x * (CODE == B200MOE_KV8_E4M3 ? E4M3_UNIT : 1.f), dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : rcp(vs), 0.f);
       }
       copy_wait<1>();  // all but V of this unit
       __syncwarp();
@@ -1311,7 +1310,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, BITS>()))
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         v += __shfl_xor_sync(0xffffffffu, v, 16);
-        if (gid == 0) s_ml[warp][r] = make_float2(m[n][e], v);
+        // the unit of the e4m3 codes: here and not in s_v, whose reciprocal it would push out of 32 bits
+        if (gid == 0) s_ml[warp][r] = make_float2(m[n][e], CODE == B200MOE_KV8_E4M3 ? v * (1.f / E4M3_UNIT) : v);
 #pragma unroll
         for (int c = 0; c < CH; ++c)
           *reinterpret_cast<float2*>(&s_o[(warp * ROWS + r) * OPITCH + 16 * c + 2 * gid]) =

@@ -148,3 +148,31 @@ def test_large_softcaps(code, io, softcap):
     """A cap far above every score leaves the scores as they are."""
     base._attend_case(code, io, 128, 8, 2, 32, 16, [90, 300], softcap=softcap)
     base._attend_case(code, io, 64, 12, 2, 16, 16, [33], sl=3, softcap=softcap)
+
+
+def _attend_with_scales(code, io, change, lens=(90, 61)):
+    """One call over a cache whose V scales [page, layer, head, block] `change` has changed."""
+    A = base._attention()
+    gen = torch.Generator().manual_seed(21)
+    cache = base._cache(code, 2, 128, 32, 16, layers=1)
+    state = base._fill(cache, 8, gen)
+    sv = state[1].cpu().unflatten(1, cache.scale_page_dims)
+    change(sv[..., 1], gen)
+    state[1].copy_(sv.flatten(1))
+    ids = torch.tensor([[3, 2, 4], [5, 1, 7]], dtype=torch.int32)
+    q = torch.randn(2, 1, 8, 128, generator=gen).to(io)
+    got = A.kv_attend(q.cuda(), cache, state, block_index=0, seq_block_ids=ids.cuda(), seq_lens=torch.tensor(lens).cuda())
+    assert base._status() == 0
+    codes, scales = ko.page_views(state, cache)
+    for b, n in enumerate(lens):
+        k, v = ko.gather(codes, scales, cache, 0, ids[b], n)
+        want = ko.attend(q[b], k, v, [n], 128 ** -0.5)
+        room = ko.attend_tolerance(q[b], k, v, 128 ** -0.5, 2.0 ** -11 if io == BF else 2.0 ** -21, base.EPS[io], want)
+        assert ((got[b].cpu().double() - want).abs() <= room).all(), b
+
+
+@pytest.mark.parametrize("code", [I8, E4])
+@pytest.mark.parametrize("io", [BF, F32])
+def test_values_near_the_end_of_32_bits(code, io):
+    """V up to 1.9 * 2^127: 1 / s_v and what the codes are scaled by stay within 32 bits."""
+    _attend_with_scales(code, io, lambda s, gen: s.mul_(1.9 * 2.0 ** 127 / ko.QMAX[code] / s.max()))
