@@ -818,7 +818,10 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
 }
 
 // The sums of several states (max, denominator, numerator) of one row: weights 2^(m - M).
-__device__ __forceinline__ float state_weight(float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); }
+// Their roots are what is computed: where scales of V are far apart, 2^(m - M) can be below
+// 2^-126 while the denominator of a state of small scales is as large, and is multiplied by
+// one root after the other.
+__device__ __forceinline__ float state_root(float m, float top) { return m == -INFINITY ? 0.f : ex2(0.5f * (m - top)); }
 
 // Positions that a sequence's length names, and steps of its segments.
 __device__ __forceinline__ int live_positions(const AttendArgs& a, int b) {
@@ -1093,6 +1096,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, BITS>()))
     const int all_see = a.seq_lens[b] - a.sl + 1;
     auto seen = [&](int n, int j) { return all_see + (tile * ROWS + 8 * n + 2 * tig + j) / G; };
 
+    float top_v = 0.f;  // largest scale of V that this lane has met
     float m[NT][2], l[NT][2], o[NT][CH][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -1106,10 +1110,18 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, BITS>()))
       sc_now = sc_next;
       {
         // dead positions (sc.y < 0: scales are never negative): weight 0 without touching the others
-        const float vs = fmaxf(sc_now.y, 7.888609052210118e-31f);  // 2^-100 in the place of 0
         const bool dead = sc_now.y < 0.f, bad = sc_now.y != sc_now.y;
-        s_pos[warp][lane] =
-            make_float4(sc_now.x * (CODE == B200MOE_KV8_E4M3 ? E4M3_UNIT : 1.f), dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : rcp(vs), 0.f);
+        // A scale of 0 (codes all zero) may be any number: 2^-40 of the largest one that all columns
+        // have seen so far, so that such positions keep their weight in 2^t / s_v and do not become
+        // the maximum that the others' P are taken from.  At least 2^-100, as every other scale.
+        if (cur.p_begin + u * AT_STEP + lane < all_see) top_v = fmaxf(top_v, sc_now.y);
+        float vs = fmaxf(sc_now.y, 7.888609052210118e-31f);
+        if (__any_sync(0xffffffffu, sc_now.y == 0.f)) {
+          const int top = __reduce_max_sync(0xffffffffu, __float_as_int(top_v));
+          if (sc_now.y == 0.f) vs = fmaxf(vs, __int_as_float(top) * 9.0949470177292824e-13f);
+        }
+        s_pos[warp][lane] = make_float4(sc_now.x * (CODE == B200MOE_KV8_E4M3 ? E4M3_UNIT : 1.f),
+                                        dead ? -INFINITY : bad ? sc_now.y : __log2f(vs), dead ? 0.f : rcp(vs), 0.f);
       }
       copy_wait<1>();  // all but V of this unit
       __syncwarp();
@@ -1214,9 +1226,9 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, BITS>()))
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float m_new = fmaxf(m[n][e], top[n][e]);
-            const float alpha = m_new == -INFINITY ? 1.f : ex2(m[n][e] - m_new);
+            const float root = m_new == -INFINITY ? 1.f : state_root(m[n][e], m_new), alpha = root * root;
             m[n][e] = m_new;
-            l[n][e] *= alpha;
+            l[n][e] = l[n][e] * root * root;
 #pragma unroll
             for (int c = 0; c < CH; ++c) { o[n][c][e] *= alpha; o[n][c][2 + e] *= alpha; }
           }
@@ -1330,8 +1342,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, BITS>()))
 #pragma unroll
       for (int w = 0; w < AT_WARPS; ++w) {
         const float2 ml = s_ml[w][r];
-        const float f = state_weight(ml.x, top);
-        den = fmaf(ml.y, f, den);
+        const float root = state_root(ml.x, top), f = root * root;
+        den = fmaf(ml.y * root, root, den);
         const float4 v = *reinterpret_cast<const float4*>(&s_o[(w * ROWS + r) * OPITCH + d]);
         acc[0] = fmaf(v.x, f, acc[0]); acc[1] = fmaf(v.y, f, acc[1]);
         acc[2] = fmaf(v.z, f, acc[2]); acc[3] = fmaf(v.w, f, acc[3]);
@@ -1411,15 +1423,15 @@ __global__ void __launch_bounds__(32 * MG_WARPS) kv8_attend_merge_kernel(const A
     }
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) up = fmaxf(up, ml[k].x);
-    const float f0 = state_weight(top, up);
-    den *= f0;
+    const float root0 = state_root(top, up), f0 = root0 * root0;
+    den = den * root0 * root0;
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] *= f0;
     top = up;
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) {
-      const float f = state_weight(ml[k].x, top);
-      den = fmaf(ml[k].y, f, den);
+      const float root = state_root(ml[k].x, top), f = root * root;
+      den = fmaf(ml[k].y * root, root, den);
 #pragma unroll
       for (int j = 0; j < N; ++j) acc[j] = fmaf(v[k][j], f, acc[j]);
     }
@@ -1444,8 +1456,8 @@ __global__ void __launch_bounds__(32 * MG_WARPS) kv8_attend_merge_kernel(const A
     den = 0.f;
 #pragma unroll
     for (int w = 0; w < MG_WARPS; ++w) {
-      const float f = state_weight(s_ml[w].x, top);
-      den = fmaf(s_ml[w].y, f, den);
+      const float root = state_root(s_ml[w].x, top), f = root * root;
+      den = fmaf(s_ml[w].y * root, root, den);
       o[0] = fmaf(s_o[w][d], f, o[0]);
       o[1] = fmaf(s_o[w][d + 1], f, o[1]);
     }

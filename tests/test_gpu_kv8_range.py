@@ -176,3 +176,37 @@ def _attend_with_scales(code, io, change, lens=(90, 61)):
 def test_values_near_the_end_of_32_bits(code, io):
     """V up to 1.9 * 2^127: 1 / s_v and what the codes are scaled by stay within 32 bits."""
     _attend_with_scales(code, io, lambda s, gen: s.mul_(1.9 * 2.0 ** 127 / ko.QMAX[code] / s.max()))
+
+
+@pytest.mark.parametrize("code", [I8, E4])
+@pytest.mark.parametrize("io", [BF, F32])
+@pytest.mark.parametrize("size", [-60, -30, 0, 30, 48])
+def test_blocks_of_zeros_beside_others(code, io, size):
+    """Positions whose V is zero keep their weight, however large or small the other values are."""
+    def change(s, gen):
+        s *= 2.0 ** size
+        s[torch.rand(s.shape, generator=gen) < 0.5] = 0.0
+    _attend_with_scales(code, io, change)
+
+
+def test_zeros_and_large_values_in_different_warps():
+    """A long sequence: stretches of zeros in some CTAs, values of 2^60 or 2^-60 in others."""
+    A = base._attention()
+    gen = torch.Generator().manual_seed(22)
+    for code, io, size in ((I8, F32, 60), (E4, BF, 60), (E4, F32, -60), (I8, BF, -60)):
+        cache = base._cache(code, 1, 64, 32, 16, layers=1)
+        state = base._fill(cache, 300, gen)
+        sv = state[1].cpu().unflatten(1, cache.scale_page_dims)
+        sv[..., 1] *= 2.0 ** size
+        sv[:150, ..., 1] = 0.0
+        state[1].copy_(sv.flatten(1))
+        n = 9000
+        for ids in (torch.arange(300), torch.arange(300).flip(0), torch.randperm(300, generator=gen)):
+            ids = ids[None].to(torch.int32)
+            q = torch.randn(1, 1, 4, 64, generator=gen).to(io)
+            got = A.kv_attend(q.cuda(), cache, state, block_index=0, seq_block_ids=ids.cuda(), seq_lens=torch.tensor([n]).cuda())
+            assert base._status() == 0
+            k, v = ko.gather(*ko.page_views(state, cache), cache, 0, ids[0], n)
+            want = ko.attend(q[0], k, v, [n], 64 ** -0.5)
+            room = ko.attend_tolerance(q[0], k, v, 64 ** -0.5, 2.0 ** -11 if io == BF else 2.0 ** -21, base.EPS[io], want)
+            assert ((got[0].cpu().double() - want).abs() <= room).all(), (code, size)
