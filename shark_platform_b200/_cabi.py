@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import threading
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -187,25 +188,40 @@ for _name, (_res, _args) in _PROTOS.items():
     _fn.argtypes = _args
 
 
+# The compiled torch binding of attention.py's cache operators, linked against one version of
+# torch and Python: loaded when the first of them is called, so that the rest of the package
+# needs the plain C library alone.
+OPS_PATH = os.path.join(HERE, "lib", "_attention_ops.so")
+_ops_lock = threading.Lock()
+
+
 def _load_attention_ops():
-    """The compiled torch binding of attention.py's cache operators, on this library's entry points."""
     import importlib.util
 
     import torch  # noqa: F401  (the binding resolves its symbols in torch's libraries)
 
-    path = os.path.join(HERE, "lib", "_attention_ops.so")
-    if not os.path.exists(path):
-        raise B200MoeError(f"{path} is missing: build it with `python -m shark_platform_b200.build`")
-    spec = importlib.util.spec_from_file_location("_attention_ops", path)
-    module = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(module)
+    if not os.path.exists(OPS_PATH):
+        raise B200MoeError(f"{OPS_PATH} is missing: build it with `python -m shark_platform_b200.build`")
+    spec = importlib.util.spec_from_file_location("_attention_ops", OPS_PATH)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError as e:
+        raise B200MoeError(f"{OPS_PATH} does not load beside torch {torch.__version__} ({e}): build it again with "
+                           "`python -m shark_platform_b200.build`") from e
     module.bind(B200MoeError, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
         "b200moe_attn_norm_rope_kv8_write", "b200moe_attn_norm_rope_kv_write", "b200moe_kv8_read", "b200moe_kv8_attend",
         "b200moe_kv8_attend_scratch_bytes", "b200moe_last_error")))
     return module
 
 
-attention_ops = _load_attention_ops()
+def __getattr__(name: str):
+    if name != "attention_ops":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    with _ops_lock:
+        if "attention_ops" not in globals():
+            globals()["attention_ops"] = _load_attention_ops()
+    return globals()["attention_ops"]
 
 
 def last_error() -> str:
