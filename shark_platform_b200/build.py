@@ -2,7 +2,7 @@
 torch binding of the cache operators: csrc/attention_ops.cpp -> lib/_attention_ops.so.
 
 nvcc cross-compiles without a GPU.  Objects are rebuilt only when a source or
-header is newer.  Run as `python -m shark_platform_b200.build [--force] [--verbose]`.
+header is newer, the binding also when torch, Python or its command is another.  Run as `python -m shark_platform_b200.build [--force] [--verbose]`.
 """
 from __future__ import annotations
 
@@ -17,6 +17,7 @@ OBJ = os.path.join(HERE, "build")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libb200moe.so")
 OPS = os.path.join(LIBDIR, "_attention_ops.so")
+OPS_STAMP = os.path.join(OBJ, "attention_ops.stamp")  # what OPS was built with
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -53,6 +54,23 @@ def _ops_command() -> list[str]:
             "-o", OPS, f"-L{root}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
 
 
+def _ops_stamp() -> str:
+    import sysconfig
+
+    import torch
+
+    return "\n".join([torch.__version__, str(sysconfig.get_config_var("SOABI")), *_ops_command(), ""])
+
+
+def _ops_stale(headers: float) -> bool:
+    if not (os.path.exists(OPS) and os.path.exists(OPS_STAMP)):
+        return True
+    with open(OPS_STAMP) as f:
+        if f.read() != _ops_stamp():
+            return True
+    return os.path.getmtime(OPS) < max(os.path.getmtime(os.path.join(CSRC, "attention_ops.cpp")), headers)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -69,8 +87,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
                 cmd.insert(1, "-Xptxas=-v")
             jobs.append(cmd)
 
-    src = os.path.join(CSRC, "attention_ops.cpp")
-    if force or not os.path.exists(OPS) or os.path.getmtime(OPS) < max(os.path.getmtime(src), hdr):
+    ops = force or _ops_stale(hdr)
+    if ops:
         jobs.append(_ops_command())
 
     def run(cmd):
@@ -84,6 +102,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
                     sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr + "\n")
                 if r.returncode != 0:
                     raise RuntimeError(f"{os.path.basename(cmd[0])} failed: {' '.join(cmd)}")
+    if ops:
+        with open(OPS_STAMP, "w") as f:
+            f.write(_ops_stamp())
     if any(cmd[0] == NVCC for cmd in jobs) or not os.path.exists(LIB):
         cmd = [NVCC, "-shared", "-o", LIB, *objs, "-cudart", "static",
                "-gencode", "arch=compute_100a,code=sm_100a"]

@@ -55,3 +55,57 @@ def test_a_binding_that_does_not_load(what, monkeypatch, tmp_path):
         A.kv_read(cache, cache.allocate(1), block_index=0, seq_block_ids=torch.zeros(1, 1, dtype=torch.int32),
                   seq_lens=torch.zeros(1, dtype=torch.int32))
     assert "attention_ops" not in C.__dict__
+
+
+@pytest.fixture
+def commands(monkeypatch, tmp_path):
+    """What build() would run, with nothing run; everything but the binding is up to date."""
+    from shark_platform_b200 import build as B
+
+    ops, stamp = tmp_path / "_attention_ops.so", tmp_path / "attention_ops.stamp"
+    ops.write_bytes(b"")
+    monkeypatch.setattr(B, "OPS", str(ops))
+    stamp.write_text(B._ops_stamp())  # the command names the output
+    monkeypatch.setattr(B, "OPS_STAMP", str(stamp))
+    ran = []
+
+    def run(cmd, **kw):
+        ran.append(cmd)
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(B.subprocess, "run", run)
+
+    def build():
+        ran.clear()
+        B.build()
+        return [c for c in ran if any(str(a).endswith("attention_ops.cpp") for a in c)]
+
+    return build, stamp, monkeypatch
+
+
+def test_an_up_to_date_binding_is_kept(commands):
+    build, stamp, _ = commands
+    assert build() == []
+
+
+@pytest.mark.parametrize("what", ["torch", "python", "flags", "no stamp", "library"])
+def test_the_binding_is_built_again(commands, what):
+    from shark_platform_b200 import build as B
+
+    build, stamp, monkeypatch = commands
+    if what == "torch":
+        monkeypatch.setattr(torch, "__version__", "9.9.9")
+    elif what == "python":
+        import sysconfig
+
+        monkeypatch.setattr(sysconfig, "get_config_var", lambda name: "cpython-399")
+    elif what == "flags":
+        monkeypatch.setattr(B, "CXX", "another-compiler")
+    elif what == "no stamp":
+        stamp.unlink()
+    else:
+        os.unlink(B.OPS)
+    assert len(build()) == 1
+    assert stamp.read_text() == B._ops_stamp()
+    if what != "library":
+        assert build() == []  # and not a second time
