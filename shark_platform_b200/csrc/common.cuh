@@ -66,7 +66,9 @@ enum : int32_t {
 // (programmatic dependent launch).  The kernel calls grid_dep_wait() in every thread
 // before it touches anything an earlier kernel writes or reads: until then it sets up
 // barriers and tensor memory and at most prefetches weights into L2, so the start-up
-// of each kernel of a layer hides behind the tail of the one before.
+// of each kernel of a layer hides behind the tail of the one before.  (One kernel takes a
+// guess before it, kv8_attend_merge_kernel: what it reads is read again after the wait, and
+// nothing but when its loads start depends on the guess.)
 template <typename... P, typename... A>
 cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
   cudaLaunchAttribute attr{};

@@ -824,10 +824,11 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
 __device__ __forceinline__ float state_root(float m, float top) { return m == -INFINITY ? 0.f : ex2(0.5f * (m - top)); }
 
 // Positions that a sequence's length names, and steps of its segments.
-__device__ __forceinline__ int live_positions(const AttendArgs& a, int b) {
-  const int len = a.seq_lens[b], room = a.pages_per_seq * a.stride;
+__device__ __forceinline__ int clamp_length(const AttendArgs& a, int len) {
+  const int room = a.pages_per_seq * a.stride;
   return len < 0 ? 0 : len < room ? len : room;
 }
+__device__ __forceinline__ int live_positions(const AttendArgs& a, int b) { return clamp_length(a, a.seq_lens[b]); }
 __device__ __forceinline__ int steps_of(int len) { return len > AT_STEP ? (len + AT_STEP - 1) / AT_STEP : 1; }
 
 // Joining a segment in the middle of a stretch (the barrier and the output of the last one,
@@ -1377,50 +1378,70 @@ __global__ void __launch_bounds__(32 * MG_WARPS) kv8_attend_merge_kernel(const A
   const int row = at % rows, kvh = at / rows % a.kv_heads, b = at / rows / a.kv_heads;
   if (b >= a.bs) return;  // whole warps; with WPR > 1 the grid has no such rows
   // The list once: its length, that of the sequences before this one, and this one's steps.
-  // The lengths may be read before the wait: this kernel starts when every CTA of the
-  // attention kernel has begun, that is after what came before it in the stream is complete.
+  // Before the wait it is a guess, with which the states' loads can start as soon as the wait
+  // is over; the lengths are read again beside them (past L1, which may have kept the first
+  // look).  Lengths are clamped to the page table, so that any guess names states in scratch.
   const int per_step = a.kv_heads * a.row_tiles;
-  int real = 0, before = 0;
-  for (int i = lane; i < a.bs; i += 32) {
-    const int n = steps_of(live_positions(a, i)) * per_step;
-    real += n;
-    before += i < b ? n : 0;
-  }
-  const int steps = steps_of(live_positions(a, b));
-  real = __reduce_add_sync(0xffffffffu, real);
-  before = __reduce_add_sync(0xffffffffu, before);
-  const int start = start_steps(real, a.ctas), total = real + start * a.bs * per_step, ctas = min(a.ctas, total);
-  const int g0 = before + start * b * per_step + (kvh * a.row_tiles + row / tile_rows) * (start + steps);
-  const Stretches cut(total, ctas);
-  const int first = cut.cta_of(g0 + start), last = cut.cta_of(g0 + start + steps - 1);
-  grid_dep_wait();
-  grid_dep_launch();
-  if (first == last) return;  // finished by that CTA
+  struct List { int real, before, steps; };
+  auto look = [&] {
+    List l{0, 0, 0};
+    for (int i = lane; i < a.bs; i += 32) {
+      const int n = steps_of(clamp_length(a, __ldcg(a.seq_lens + i)));
+      l.real += n * per_step;
+      l.before += i < b ? n * per_step : 0;
+      l.steps += i == b ? n : 0;
+    }
+    l.real = __reduce_add_sync(0xffffffffu, l.real);
+    l.before = __reduce_add_sync(0xffffffffu, l.before);
+    l.steps = __reduce_add_sync(0xffffffffu, l.steps);
+    return l;
+  };
+  // where the row's states are: the first CTA may have begun before this segment, and its state
+  // is then its second; the others begin inside it
   const size_t pitch = static_cast<size_t>(tile_rows) * (HD + 4);
-  // the first CTA may have begun before this segment: its state is then its second; the others begin inside it
-  const float* in0 = a.partial + (2 * static_cast<size_t>(first) + (cut.begin(first) < g0 ? 1 : 0)) * pitch +
-                     row % tile_rows * (HD + 4);
-  const float* in1 = a.partial + 2 * static_cast<size_t>(first) * pitch + row % tile_rows * (HD + 4);
-  const int n = last - first + 1;
-  float acc[N], top = -INFINITY, den = 0.f;
-#pragma unroll
-  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  struct States { int n; const float *first, *others; };
+  auto find = [&](const List& l) {
+    const int start = start_steps(l.real, a.ctas), total = l.real + start * a.bs * per_step;
+    const int g0 = l.before + start * b * per_step + (kvh * a.row_tiles + row / tile_rows) * (start + l.steps);
+    const Stretches cut(total, min(a.ctas, total));
+    const int first = cut.cta_of(g0 + start), last = cut.cta_of(g0 + start + l.steps - 1);
+    const float* at = a.partial + 2 * static_cast<size_t>(first) * pitch + row % tile_rows * (HD + 4);
+    return States{last - first + 1, at + (cut.begin(first) < g0 ? pitch : 0), at};
+  };
   constexpr int AT_ONCE = WPR == 1 ? 4 : 8;
-  for (int s0 = part; s0 < n; s0 += AT_ONCE * WPR) {
-    float v[AT_ONCE][N], up = top;
-    float2 ml[AT_ONCE];
+  float v[AT_ONCE][N];
+  float2 ml[AT_ONCE];
+  auto load = [&](const States& in, int s0) {
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) {
       const int s = s0 + k * WPR;
       ml[k] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int j = 0; j < N; ++j) v[k][j] = 0.f;
-      if (s < n) {
-        const float* in = s == 0 ? in0 : in1 + 2 * s * pitch;
-        ml[k] = *reinterpret_cast<const float2*>(in + HD);
-        load_elems(in + lane * N, v[k]);
+      if (s < in.n) {
+        const float* from = s == 0 ? in.first : in.others + 2 * s * pitch;
+        ml[k] = *reinterpret_cast<const float2*>(from + HD);
+        load_elems(from + lane * N, v[k]);
       }
     }
+  };
+  const List guess = look();
+  States in = find(guess);
+  grid_dep_wait();
+  grid_dep_launch();
+  if (in.n > 1) load(in, part);
+  const List list = look();
+  if (list.real != guess.real || list.before != guess.before || list.steps != guess.steps) {
+    in = find(list);
+    if (in.n > 1) load(in, part);
+  }
+  if (in.n == 1) return;  // finished by that CTA
+  float acc[N], top = -INFINITY, den = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  for (int s0 = part; s0 < in.n; s0 += AT_ONCE * WPR) {
+    if (s0 != part) load(in, s0);
+    float up = top;
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) up = fmaxf(up, ml[k].x);
     const float root0 = state_root(top, up), f0 = root0 * root0;

@@ -210,3 +210,32 @@ def test_zeros_and_large_values_in_different_warps():
             want = ko.attend(q[0], k, v, [n], 64 ** -0.5)
             room = ko.attend_tolerance(q[0], k, v, 64 ** -0.5, 2.0 ** -11 if io == BF else 2.0 ** -21, base.EPS[io], want)
             assert ((got[0].cpu().double() - want).abs() <= room).all(), (code, size)
+
+
+def test_lengths_written_right_before_the_call():
+    """Lengths that the kernel in front of the call writes, in turn long and short ones, give
+    what they give on an idle stream: where the joined states are found follows from them."""
+    A = base._attention()
+    gen = torch.Generator().manual_seed(23)
+    cache = base._cache(I8, 2, 64, 16, 16, layers=1)
+    state = base._fill(cache, 200, gen)
+    bs, per = 5, 190
+    ids = torch.stack([torch.randperm(200, generator=gen)[:per] for _ in range(bs)]).to(torch.int32).cuda()
+    q = torch.randn(bs, 1, 8, 64, generator=gen).to(BF).cuda()
+    attend = lambda lens: A.kv_attend(q, cache, state, block_index=0, seq_block_ids=ids, seq_lens=lens)
+    sets = [torch.randint(0, 16 * per, (bs,), generator=gen).to(torch.int32).cuda() for _ in range(12)]
+    sets += [torch.full((bs,), n, dtype=torch.int32, device="cuda") for n in (0, 1, 128, 129, 16 * per)]
+    want = []
+    for x in sets:
+        torch.cuda.synchronize()
+        want.append(attend(x))
+    torch.cuda.synchronize()
+    lens = torch.zeros(bs, dtype=torch.int32, device="cuda")
+    got = []
+    for turn in range(4):
+        for i, x in enumerate(sets):
+            lens.copy_(x)
+            got.append((i, attend(lens)))
+            lens.fill_(7)
+    assert all(torch.equal(o, want[i]) for i, o in got)
+    assert base._status() == 0
