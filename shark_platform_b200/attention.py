@@ -276,7 +276,9 @@ class B200PagedAttentionBlock(torch.nn.Module):
         step may bring up to 16 tokens per sequence (each attends the ones before it), a
         negative start position marks a padding sequence, and a prefill with start_index > 0
         attends the cached positions before it too (an attention_mask then covers the new
-        positions, or all of them)."""
+        positions, or all of them).  With a 16- or 32-bit cache a prefill attends its new positions
+        only, as the reference's does; with norms, the HuggingFace order or `new_lens` such a
+        call with start_index > 0 is refused."""
         _moe._require_cuda(h, "h")
         if h.dtype not in _DT:
             raise C.B200MoeError(f"activations must be fp32, fp16 or bf16, got {h.dtype}")
@@ -300,6 +302,9 @@ class B200PagedAttentionBlock(torch.nn.Module):
         # norms, the HuggingFace order, padding and 8-bit codes: the one-pass write
         one_pass = (self._quantized or use_hf or new_lens is not None or self._q_norm_w is not None or
                     self._k_norm_w is not None)
+        if one_pass and not decode and (int(start_index) < 0 or (int(start_index) > 0 and not self._quantized)):
+            raise C.B200MoeError(f"a prefill from position {int(start_index)}: continued prompts are for 8-bit caches "
+                                 "(the positions before it would not be attended)")
         hc = h.contiguous()
         # the output projection with the residual, in one call
         fused_out = (self._fits_linear(self._wo) and [int(n) for n in self._wo.shape] == [d, H * hd] and
