@@ -50,3 +50,44 @@ def test_long_lists_of_steps(code, io, hd, heads, kvh, sl, bs):
         room = ko.attend_tolerance(q[b], k, v, hd ** -0.5, 2.0 ** -11 if io != F32 else 2.0 ** -21, base.EPS[io], want) + base.FLOOR[io]
         off = (got[b].cpu().double() - want).abs()
         assert bool((off <= room).all()), (b, n, float((off / room).max()))
+
+
+@pytest.mark.parametrize("io,hd,heads,kvh,bs,sl,at_once", [
+    (BF, 128, 48, 8, 4, 2048, 16), (BF, 128, 40, 4, 2, 5000, 32), (HF, 128, 42, 2, 2, 4096, 16), (F32, 128, 12, 2, 4, 2500, 8),
+    (HF, 64, 12, 4, 8, 2500, 8), (BF, 64, 36, 2, 5, 4001, 32)])
+@pytest.mark.parametrize("norm,halves", [(False, True), (True, False)])
+def test_queries_of_large_prompts(io, hd, heads, kvh, bs, sl, at_once, norm, halves):
+    """A lane takes 8, 16 or 32 heads of its position, the last group partly full."""
+    A = base._attention()
+    gen = torch.Generator(device="cuda").manual_seed(heads + sl)
+    cpu = torch.Generator().manual_seed(heads)
+    # the rule of the launch
+    want, groups = torch.cuda.get_device_properties(0).multi_processor_count * 8 * (256 // (hd // 8)), 4
+    while groups < heads and bs * sl * ((heads - 1) // (2 * groups) + 1) >= want:
+        groups *= 2
+    assert groups == at_once
+    cache = base._cache(io, kvh, hd, 32, layers=1)
+    per = -(-(sl + 9 * bs) // 32)
+    ids = torch.randperm(bs * per, generator=cpu).view(bs, per).to(torch.int32).cuda()
+    state = cache.allocate(bs * per)
+    w = base.Write(cache, heads, io, cpu, norm, halves)
+    q, k, v = (torch.randn(bs, sl, n, hd, generator=gen, device="cuda").to(io) for n in (heads, kvh, kvh))
+    start = torch.arange(bs) * 9
+    got = w.call(state, ids, start, q, k, v, layer=0)
+    assert base._status() == 0
+    slab = state[0].unflatten(1, cache.sub_page_dims)
+    for b in range(bs):
+        at = torch.cat([torch.randint(0, sl, (60,), generator=cpu), torch.tensor([0, 1, 31, 32, sl - 2, sl - 1])])
+        qb, kb, vb = (t[b, at.cuda()].cpu() for t in (q, k, v))
+        pos = int(start[b]) + at
+        for x, g, wt in ((qb, got[0], w.w[0]), (kb, got[1], w.w[1])):
+            y = ko.turn(x, pos, w.freqs, wt, halves=halves)
+            size = x.double().abs().amax(-1, keepdim=True)
+            if wt is not None:
+                size = size * wt.abs().max() / x.double().pow(2).mean(-1, keepdim=True).add(1e-5).sqrt()
+            d = size * 16 * 2.0 ** -23
+            off = (g[b, at.cuda()].cpu().double() - y).abs() - d - base.EPS[io] * (y.abs() + d) - base.FLOOR[io]
+            assert off.max() <= 0, float(off.max())
+        page = ids[b, (pos // 32).cuda()].long()
+        held = slab[page, 0, :, (pos % 32).cuda()]
+        assert torch.equal(held[:, 0], got[1][b, at.cuda()]) and torch.equal(held[:, 1].cpu(), vb)
