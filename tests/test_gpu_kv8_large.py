@@ -91,3 +91,38 @@ def test_queries_of_large_prompts(io, hd, heads, kvh, bs, sl, at_once, norm, hal
         page = ids[b, (pos // 32).cuda()].long()
         held = slab[page, 0, :, (pos % 32).cuda()]
         assert torch.equal(held[:, 0], got[1][b, at.cuda()]) and torch.equal(held[:, 1].cpu(), vb)
+
+
+@pytest.mark.parametrize("code", [I8, BF])
+def test_more_than_65535_ctas_of_keys_and_values(code):
+    """K and V of many short rows: their CTAs are found among the others in 64 bits."""
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    bs, heads, kvh, hd = 33_333, 4, 2, 64
+    cache = base._cache(code, kvh, hd, 4, layers=1)
+    state = cache.allocate(bs)
+    ids = torch.randperm(bs, generator=torch.Generator().manual_seed(18)).to(torch.int32)[:, None].cuda()
+    w = base.Write(cache, heads, BF, None)
+    q, k, v = (torch.randn(bs, 1, n, hd, generator=gen, device="cuda").to(BF) for n in (heads, kvh, kvh))
+    start = torch.arange(bs) % 4
+    got = w.call(state, ids, start, q, k, v, layer=0)
+    assert base._status() == 0
+    turned = [ko.turn(x.cpu(), start[:, None], w.freqs) for x in (q, k)]
+    for x, y, g in zip((q, k), turned, got):
+        d = x.cpu().double().abs().amax(-1, keepdim=True) * 16 * 2.0 ** -23
+        off = (g.cpu().double() - y).abs() - d - base.EPS[BF] * (y.abs() + d)
+        assert off.max() <= 0, float(off.max())
+    page, seq = ids[:, 0].long().cpu(), torch.arange(bs)
+    if code == BF:
+        held = state[0].unflatten(1, cache.sub_page_dims).cpu()
+        for slot, x in enumerate((got[1], v)):
+            assert torch.equal(held[page, 0, slot, start], x[:, 0].cpu())
+        held[page, 0, :, start] = 0
+        assert not held.any()
+        return
+    codes, scales = ko.page_views(state, cache)  # blocks of four positions; a fresh page's scale is 0
+    s, c = scales[page, 0, :, 0], codes[page, 0, :, :, start]
+    for slot, x in enumerate((turned[1][:, 0], v[:, 0].cpu().double())):
+        amax = x.abs().amax(-1)
+        assert ((s[..., slot] * 127 - amax).abs() <= amax * 2.0 ** -18).all()
+        y = x / s[..., slot, None]
+        assert ((c[:, :, slot] - y).abs() <= 0.5 * (1 + 2.0 ** -10) + 127 * 2.0 ** -18).all()
