@@ -102,7 +102,7 @@ __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {
 // e4m3: its exponent and mantissa moved to fp16's places are the value times 2^-8 (the two
 // biases differ by 8; subnormal codes become subnormal fp16 numbers), which goes into the
 // scale: E4M3_UNIT.  Seven integer instructions, against three or four with the conversion
-// instruction, which takes longer than they (47 and 45 us at 32 x 4000 positions).
+// instruction, which takes longer than they (42 us at 32 x 4000 positions, with it 51).
 constexpr float E4M3_UNIT = 256.f;
 template <int CODE>
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& even, uint32_t& odd) {
@@ -343,11 +343,14 @@ __device__ __forceinline__ BlockScale block_scale(unsigned bits, float before) {
 // scale blocks; K and V stay in registers from their load to their codes: one read of
 // everything.  The others have the queries: a lane keeps its position's cosines and sines
 // and takes four heads at once, q_heads in all.  HD / 8 lanes have a row (16-byte loads and
-// stores of 16-bit rows), a warp two or four rows.  Bound by HBM, then by how much of it the
-// CTAs keep asking for: 4 x 2048 tokens of 48 + 16 heads (268 MB) take 47 us, 5.7 TB/s.  On
+// stores of 16-bit rows), a warp two or four rows.  Bound by memory and by instructions alike
+// (63 % of the issue slots, and waits for the loads of four CTAs an SM): 4 x 2048 tokens of
+// 48 + 16 heads (268 MB) take 47 to 48 us, 5.6 TB/s.  On
 // the way there: K, V and the queries of a kv head in one CTA 79 (the queries waited for the
 // barriers of K and V); CTAs of two kinds, three an SM 66, four 60 (five, registers in memory,
-// 54 instead of 47 later on; heads of 64 fit five: 13.9 instead of 14.7); K's and V's CTAs
+// 54 instead of 47 later on; heads of 64 take five, 4 to 16 bytes of a thread's registers in
+// memory: 4 x 2048 tokens of 16 + 8 heads 12.8 instead of 13.7, 8 x 2048 of fp16 to e4m3 25.7
+// instead of 27.3, 4 x 1024 to a 16-bit cache and one of 777 as with four); K's and V's CTAs
 // among the others instead of before them 52; rounding of the codes by an addition and the
 // approximate reciprocal root 47.
 template <typename T, int HD, int KIND, int TILE, int ORDER>
@@ -744,8 +747,8 @@ int launch_read(const ReadArgs& a, int code, dim3 grid, cudaStream_t st) {
 // cut does not depend on how wide the page table is.  A segment that lies within one stretch
 // is finished there; of the others every CTA leaves a state (at most two: its first and its
 // last segment), which the merge kernel joins.
-// 32 sequences of 2000 to 4000 positions, 8 kv heads of 128, 32 heads (200 MB): int8 41 us,
-// e4m3 43, 4.9 and 4.7 TB/s (a plain read of as much, by a reduction, 39 us); bound by HBM
+// 32 sequences of 2000 to 4000 positions, 8 kv heads of 128, 32 heads (200 MB): int8 40 us,
+// e4m3 42, 5.0 and 4.7 TB/s (a plain read of as much, by a reduction, 39 us); bound by HBM
 // once under way, before by the chain of lengths, page ids and first rows (6 us), after by the
 // merge (4 us).  With a CTA per position split of each sequence 68.  Several new tokens are
 // bound by the instructions around the MMAs: 16 rows 48 us, 32 rows, in two tiles that each
@@ -876,10 +879,11 @@ struct Stretches {
   }
 };
 
-// CTAs per SM: as many as the registers allow without spilling in the loop.  (HD 128, one
-// more: NT = 1 44 instead of 41 us, NT = 2 61 instead of 48, at 32 x 4000 positions of int8;
-// one less: e4m3 51 instead of 48, int8 41 instead of 43, before the e4m3 codes were widened
-// as they are now.)
+// CTAs per SM, at 32 x 4000 positions against one less and one more.  HD 128: one row tile of
+// bf16, int8 39 us (41, 46), e4m3 42 (45, 47); two of bf16 48 (83, 55); one of fp32 46.5 (70,
+// 45.6) and 50.7 (69, 51.0).  HD 64, int8: bf16 17.3 (17.3, 17.7) and 21.8 with four tokens
+// (22.3, 25.4); fp32 20.5 (19.6, 21.7) and 26.8 (25.8, 32.4).  Some of the variants with P or
+// q in two parts keep 8 to 84 bytes of a thread's registers in memory.
 template <int HD, int NT, int BITS>
 constexpr int attend_resident() {
   if (HD == 128) return NT == 1 && BITS != BITS_BOTH ? 3 : 2;
