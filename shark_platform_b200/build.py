@@ -6,6 +6,7 @@ header is newer, the binding also when torch, Python or its command is another. 
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
@@ -87,7 +88,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
                 cmd.insert(1, "-Xptxas=-v")
             jobs.append(cmd)
 
-    ops = force or _ops_stale(hdr)
+    # without torch there is nothing to bind to: the C library alone
+    ops = importlib.util.find_spec("torch") is not None and (force or _ops_stale(hdr))
     if ops:
         jobs.append(_ops_command())
 

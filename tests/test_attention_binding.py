@@ -109,3 +109,15 @@ def test_the_binding_is_built_again(commands, what):
     assert stamp.read_text() == B._ops_stamp()
     if what != "library":
         assert build() == []  # and not a second time
+
+
+def test_the_c_library_is_built_without_torch(commands):
+    import importlib.util
+
+    build, stamp, monkeypatch = commands
+    stamp.unlink()
+    find = importlib.util.find_spec
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else find(name, *a))
+    monkeypatch.setitem(sys.modules, "torch", None)  # an import of it fails
+    assert build() == []
+    assert not stamp.exists()
