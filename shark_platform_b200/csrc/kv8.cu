@@ -140,7 +140,7 @@ __device__ __forceinline__ void codes_to_floats(const uint32_t (&c)[N / 4], floa
 // are common (half of the largest value of an int8 block is 63.5 steps): the product has to be
 // that number again, to go to the even code, and with a factor off by 2^-24 it falls to either
 // side.  (With one float the error of V against codes from 64-bit quotients is a tenth larger
-// for bf16 rows and three quarters for fp16, all of it from these.)
+// for bf16 rows and almost twice as large for fp16, all of it from these.)
 template <int CODE>
 __device__ __forceinline__ uint2 floats_to_codes(const float (&v)[8], float by, float by_lo) {
   uint32_t c[2];
