@@ -6,91 +6,12 @@
 // A code c stands for c * s.
 #include <cuda_fp8.h>
 
-#include <cmath>
-
-#include "kernels.h"
+#include "kv_attend.cuh"
 
 namespace b200moe {
 namespace {
 
 constexpr int MAX_SCALE_BLOCK = 64;
-constexpr int MAX_NEW_TOKENS = 16;
-
-inline bool dtype_ok(int dt) { return dt == B200MOE_DT_F32 || dt == B200MOE_DT_F16 || dt == B200MOE_DT_BF16; }
-inline size_t dt_bytes(int dt) { return dt == B200MOE_DT_F32 ? 4 : 2; }
-// log2 of a power of two, -1 of another number
-inline int log2_of(int n) {
-  for (int i = 0; i < 31; ++i)
-    if (n == 1 << i) return i;
-  return -1;
-}
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-// ------------------------------------------------------------- rows of 16 or 32 bits
-// Eight consecutive elements as they lie in memory: one or two 16-byte words.
-template <typename T>
-struct Raw8 {
-  uint4 w[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w[i] = make_uint4(0, 0, 0, 0);
-  }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    const T* e = reinterpret_cast<const T*>(w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (sizeof(T) == 4) v[i] = e[i];
-      else if constexpr (std::is_same<T, __half>::value) v[i] = __half2float(e[i]);
-      else v[i] = __bfloat162float(e[i]);
-    }
-  }
-};
-__device__ __forceinline__ uint32_t pack2(const __half*, float a, float b) { return h2_as_u32(__floats2half2_rn(a, b)); }
-__device__ __forceinline__ uint32_t pack2(const __nv_bfloat16*, float a, float b) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(p, v[0], v[1]), pack2(p, v[2], v[3]), pack2(p, v[4], v[5]), pack2(p, v[6], v[7]));
-  }
-}
-template <typename T>
-__device__ __forceinline__ float round_to(float v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(__float2half_rn(v));
-  else return __bfloat162float(__float2bfloat16_rn(v));
-}
-// 2 or 4 consecutive elements; stored as a type known at run time
-template <int N>
-__device__ __forceinline__ void load_elems(const float* p, float (&v)[N]) {
-  if constexpr (N == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  } else {
-    const float2 a = *reinterpret_cast<const float2*>(p);
-    v[0] = a.x; v[1] = a.y;
-  }
-}
-template <int N>
-__device__ __forceinline__ void store_as(void* p, int dtype, size_t i, const float (&v)[N]) {
-#pragma unroll
-  for (int j = 0; j < N; j += 2) {
-    if (dtype == B200MOE_DT_F32) *reinterpret_cast<float2*>(static_cast<float*>(p) + i + j) = make_float2(v[j], v[j + 1]);
-    else if (dtype == B200MOE_DT_F16)
-      *reinterpret_cast<__half2*>(static_cast<__half*>(p) + i + j) = __floats2half2_rn(v[j], v[j + 1]);
-    else
-      *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p) + i + j) = __floats2bfloat162_rn(v[j], v[j + 1]);
-  }
-}
 
 // ------------------------------------------------------------------------- codes
 __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t v) {
@@ -163,97 +84,17 @@ __device__ __forceinline__ uint2 floats_to_codes(const float (&v)[8], float by, 
   return make_uint2(c[0], c[1]);
 }
 
-// ------------------------------------------------------------------------- write
-struct WriteArgs {
-  const void *q, *k, *v;
-  int64_t q_stride, k_stride, v_stride;
-  const float *q_norm, *k_norm;
-  float eps;
-  void *q_out, *k_out;
-  void* slab;
-  float* scales;                      // 8-bit cache
-  int cache_dtype;                    // 16- or 32-bit cache
-  const int32_t *start_positions, *new_lens, *page_ids;
-  const float* freqs;
-  int order, bs, sl, pages_per_seq, page_count, heads, kv_heads, stride, blocks, block_index, scale_block;
-  int tiles;                          // of a sequence
-  int stride_shift, block_shift;      // log2; -1 where the stride is no power of two
-  unsigned kv_ctas;                   // CTAs of K and V
-  int q_heads;                        // heads that a lane of the others takes
-  int32_t* status;
-};
-
 enum { CACHE_INT8 = B200MOE_KV8_INT8, CACHE_E4M3 = B200MOE_KV8_E4M3, CACHE_PLAIN = 2 };
 
 constexpr int WR_THREADS = 256;
 constexpr int WR_WARPS = WR_THREADS / 32;
 constexpr float QMAX[2] = {127.f, 448.f};
 
-// Cosine and sine of position * freq, the angle reduced to part of a turn first.
-// 32-bit rows, and far angles: reduced in 64 bits; the half turns are rounded by 2^-25, which
-// is pi 2^-25 of angle, and sincospif is good to an ulp or two: 2^-22 up to 2^25 turns (the
-// products in 64 bits are off by 2^-52 of the turns, which shows above).
-// 16-bit rows: the position (below 2^24, exact) times freq / (2 pi) as the sum of two floats
-// u + u_lo.  Below 2^22 turns u_lo is at most an eighth, so that the integer part is dropped
-// before and after the sum: the special-function unit's bounds hold within a turn only, 2^-21.4
-// (sine) and 2^-21.2.  The sum is rounded by 2^-25 of a turn, the product with 2 pi by 2^-23
-// and 2 pi itself by 2^-25 of it: 2^-20 in all, a 256th of half a step of fp16 just below one,
-// and 1e-4 of a step of int8.  (With power series, good to 2^-22: 49.0 instead of 47.4 us for
-// 4 x 2048 tokens of 48 + 16 heads, 8.0 instead of 7.2 for 777 of 32 + 8, and the same error of
-// q, k and K's codes against 64 bits in three digits; sincospif 48.4 and 8.0.)
-template <typename T>
-__device__ __forceinline__ float2 cos_sin(long long pos, float freq) {
-  constexpr double inv = 0.15915494309189533577;  // 1 / (2 pi)
-  constexpr float inv_hi = static_cast<float>(inv), inv_lo = static_cast<float>(inv - inv_hi);
-  const float p = static_cast<float>(static_cast<int>(pos)), g = freq * inv_hi, u = p * g;
-  float sn, cs;
-  if (sizeof(T) == 4 || pos >= 1 << 24 || !(fabsf(u) < 4194304.f)) {
-    const double turns = static_cast<double>(pos) * (static_cast<double>(freq) * (2.0 * inv));  // halves
-    sincospif(static_cast<float>(turns - 2.0 * rint(0.5 * turns)), &sn, &cs);
-  } else {
-    const float g_lo = fmaf(freq, inv_hi, -g) + freq * inv_lo, u_lo = fmaf(p, g_lo, fmaf(p, g, -u));
-    const float r = (u - rintf(u)) + u_lo, angle = (r - rintf(r)) * 6.2831853071795864769f;
-    sn = __sinf(angle);
-    cs = __cosf(angle);
-  }
-  return make_float2(cs, sn);
-}
 // max(m, |x|) for m >= 0, NaN where either is
 __device__ __forceinline__ float max_nan(float m, float x) {
   float y;
   asm("{.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;}" : "=f"(y) : "f"(m), "f"(x));
   return y;
-}
-// The eight elements of a row that lane c of HD / 8 has, so that it has whole pairs: in order
-// 0 (pairs 2i, 2i + 1) elements 8c .. 8c + 7, in the HuggingFace order (pairs i, i + HD / 2)
-// 4c .. 4c + 3 and as many behind HD / 2.  Its pairs' frequencies are 4c .. 4c + 3 either way.
-template <int HD, int ORDER>
-__device__ __forceinline__ int element(int c, int i) {
-  return ORDER == 0 ? 8 * c + i : (i < 4 ? 4 * c + i : HD / 2 + 4 * c + i - 4);
-}
-template <typename T, int HD, int ORDER>
-__device__ __forceinline__ void load_row(Raw8<T>& x, const T* row, int c) {
-  if constexpr (ORDER == 0) {
-    x.load(row + 8 * c);
-  } else if constexpr (sizeof(T) == 4) {
-    x.w[0] = *reinterpret_cast<const uint4*>(row + 4 * c);
-    x.w[1] = *reinterpret_cast<const uint4*>(row + HD / 2 + 4 * c);
-  } else {
-    const uint2 lo = *reinterpret_cast<const uint2*>(row + 4 * c), hi = *reinterpret_cast<const uint2*>(row + HD / 2 + 4 * c);
-    x.w[0] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-  }
-}
-template <typename T, int HD, int ORDER>
-__device__ __forceinline__ void store_row(T* row, int c, const float (&v)[8]) {
-  if constexpr (ORDER == 0) {
-    store8(row + 8 * c, v);
-  } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(row + 4 * c) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(row + HD / 2 + 4 * c) = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    *reinterpret_cast<uint2*>(row + 4 * c) = make_uint2(pack2(row, v[0], v[1]), pack2(row, v[2], v[3]));
-    *reinterpret_cast<uint2*>(row + HD / 2 + 4 * c) = make_uint2(pack2(row, v[4], v[5]), pack2(row, v[6], v[7]));
-  }
 }
 template <int HD, int ORDER>
 __device__ __forceinline__ void store_codes(uint8_t* row, int c, uint2 v) {
@@ -265,42 +106,6 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int c, uint2 v) {
   }
 }
 
-// Cosines and sines of a lane's four pairs.
-struct Turn { float2 t[4]; };
-template <typename T>
-__device__ __forceinline__ Turn turn_of(long long pos, const float* freqs, int c) {
-  Turn w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w.t[i] = cos_sin<T>(pos, freqs[4 * c + i]);
-  return w;
-}
-// A lane's eight elements of a row, normed and rotated; LPR lanes have a row.
-template <int LPR, int ORDER>
-__device__ __forceinline__ void norm_rotate(float (&x)[8], const float (&w)[8], bool norm, float eps, const Turn& turn) {
-  if (norm) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(ss * (1.f / (8 * LPR)) + eps);  // 2^-22; root and division cost a tenth of the kernel
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = w[i] * (x[i] * r);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    constexpr int STEP = ORDER == 0 ? 2 : 1, OTHER = ORDER == 0 ? 1 : 4;
-    const float re = x[STEP * i], im = x[STEP * i + OTHER];
-    x[STEP * i] = re * turn.t[i].x - im * turn.t[i].y;
-    x[STEP * i + OTHER] = im * turn.t[i].x + re * turn.t[i].y;
-  }
-}
-
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // The scale of a block from the largest magnitude of its new rows (as bits) and, if it is
 // continued, the scale it had (else 0); the factor to codes, qmax / amax of a fresh block and
 // 1 / scale of a continued one, as an approximate reciprocal (scales are below 2^122) and what
@@ -580,36 +385,6 @@ int launch_write_io(WriteArgs& a, int io_dtype, int hd, cudaStream_t st) {
   return launch_write_hd<__nv_bfloat16, KIND>(a, hd, st);
 }
 
-// What both writes ask of their arguments.
-int check_write(const char* who, const WriteArgs& a, int io_dtype, int hd) {
-  B200_REQUIRE(a.bs >= 0 && a.sl >= 1 && a.pages_per_seq >= 1 && a.heads >= 1, "%s: bad sizes", who);
-  if (a.bs == 0) return B200MOE_OK;
-  B200_REQUIRE(a.q && a.k && a.v && a.q_out && a.slab && a.start_positions && a.page_ids && a.freqs, "%s: NULL buffer",
-               who);
-  B200_REQUIRE(dtype_ok(io_dtype), "%s: unknown dtype", who);
-  B200_REQUIRE(a.order == 0 || a.order == 1, "%s: rotation order %d (0 and 1 are known)", who, a.order);
-  B200_REQUIRE(hd == 64 || hd == 128, "%s: head_dim %d (64 and 128 are built)", who, hd);
-  B200_REQUIRE(a.kv_heads >= 1 && a.heads % a.kv_heads == 0, "%s: heads (%d) must be a multiple of the kv heads (%d)",
-               who, a.heads, a.kv_heads);
-  B200_REQUIRE(a.kv_heads <= 65535, "%s: kv_heads %d", who, a.kv_heads);
-  B200_REQUIRE(a.stride >= 1 && a.blocks >= 1 && a.block_index >= 0 && a.block_index < a.blocks && a.page_count >= 1,
-               "%s: bad cache geometry", who);
-  const int64_t per16 = 16 / static_cast<int64_t>(dt_bytes(io_dtype));
-  B200_REQUIRE(aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.q_out) && aligned16(a.k_out) &&
-                   aligned16(a.slab) && a.q_stride % per16 == 0 && a.k_stride % per16 == 0 && a.v_stride % per16 == 0,
-               "%s: buffers and row strides must be multiples of 16 bytes", who);
-  B200_REQUIRE(a.q_stride >= static_cast<int64_t>(a.heads) * hd && a.k_stride >= static_cast<int64_t>(a.kv_heads) * hd &&
-                   a.v_stride >= static_cast<int64_t>(a.kv_heads) * hd,
-               "%s: a row stride is shorter than the row", who);
-  B200_REQUIRE(a.k_out != a.k && a.k_out != a.v && a.q_out != a.k && a.q_out != a.v && a.k_out != a.q && a.q_out != a.q &&
-                   a.q_out != a.k_out,
-               "%s: q_out and k_out must not be inputs", who);
-  // CTAs of K and V, and at most one for each 16 heads of a token
-  const double grid = static_cast<double>(a.bs) * ((a.sl - 1) / 32 + 2) * a.kv_heads +
-                      static_cast<double>(a.bs) * a.sl * (a.heads / 4 + 1) / 16 + 1;
-  B200_REQUIRE(grid < 2147483647.0, "%s: %d sequences of %d tokens are too many for one call", who, a.bs, a.sl);
-  return B200MOE_OK;
-}
 
 int check_kv8(const char* who, const b200moe_kv8_cache_t* c, int32_t block_index) {
   B200_REQUIRE(c != nullptr, "%s: NULL cache geometry", who);
@@ -753,131 +528,6 @@ int launch_read(const ReadArgs& a, int code, dim3 grid, cudaStream_t st) {
 // merge (4 us).  With a CTA per position split of each sequence 68.  Several new tokens are
 // bound by the instructions around the MMAs: 16 rows 48 us, 32 rows, in two tiles that each
 // widen the codes, 88 us of the same cache (in one tile, q in shared memory, 86: not kept).
-struct AttendArgs {
-  const void* q;
-  int64_t q_stride;
-  int q_dtype;
-  const uint8_t* slab;
-  const float* scales;
-  const int32_t *page_ids, *seq_lens;
-  void* out;
-  float* partial;  // [CTA][2: its first, its last segment][rows of a tile][HD + 4]: numerator, max, denominator
-  int out_dtype, bs, sl, pages_per_seq, page_count, heads, kv_heads, stride, blocks, block_index;
-  int stride_shift, block_shift;  // log2; -1 where the stride is no power of two
-  int row_tiles, ctas;
-  float scale, softcap;
-  int32_t* status;
-};
-
-// In how many fp16 parts the operands are: one; P in two (fp16 outputs); q and P in two (32-bit
-// activations, and softcaps above CAP_FAST: there what the fast form of the softcap is off by,
-// CAP_FAST * 2^-22 = 2^-14 of a probability, would begin to show).
-constexpr float CAP_FAST = 256.f;
-enum { BITS_ONE = 0, BITS_P = 1, BITS_BOTH = 2 };
-constexpr int AT_THREADS = 128, AT_WARPS = 4;
-constexpr int AT_UNIT = 32;   // positions of a warp's step
-constexpr int AT_STEP = AT_WARPS * AT_UNIT;
-constexpr float LOG2E = 1.4426950408889634f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-// mma_16816 that the compiler may move between the loads of other tiles
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// Byte offset of 16-byte chunk c of row r in a tile of rows of HD bytes: the eight chunks
-// that one ldmatrix phase reads (eight rows, one c) lie in eight different bank groups.
-template <int HD>
-__device__ __forceinline__ uint32_t tile_at(int r, int c) {
-  if constexpr (HD == 128) return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4));
-  else return static_cast<uint32_t>((r >> 1) * 128 + ((((r & 1) * 4 + c) ^ ((r >> 1) & 3)) << 4));
-}
-
-// The sums of several states (max, denominator, numerator) of one row: weights 2^(m - M).
-// Their roots are what is computed: where scales of V are far apart, 2^(m - M) can be below
-// 2^-126 while the denominator of a state of small scales is as large, and is multiplied by
-// one root after the other.
-__device__ __forceinline__ float state_root(float m, float top) { return m == -INFINITY ? 0.f : ex2(0.5f * (m - top)); }
-
-// Positions that a sequence's length names, and steps of its segments.
-__device__ __forceinline__ int clamp_length(const AttendArgs& a, int len) {
-  const int room = a.pages_per_seq * a.stride;
-  return len < 0 ? 0 : len < room ? len : room;
-}
-__device__ __forceinline__ int live_positions(const AttendArgs& a, int b) { return clamp_length(a, a.seq_lens[b]); }
-__device__ __forceinline__ int steps_of(int len) { return len > AT_STEP ? (len + AT_STEP - 1) / AT_STEP : 1; }
-
-// Joining a segment in the middle of a stretch (the barrier and the output of the last one,
-// q) takes a CTA as long as a step or two: in long stretches a segment counts START_STEPS
-// more than it has, so that the CTAs that join one get fewer.  (0, 2, 3 at 32 x 4000
-// positions: 16 rows 51, 48, 49 us; 8 rows 40, 41, 42.)
-constexpr int START_STEPS = 2;
-__device__ __forceinline__ int start_steps(int steps, int ctas) { return steps >= 4 * ctas ? START_STEPS : 0; }
-
-// The list of steps, looked at by a whole warp: those of the sequences before `until` or,
-// with until < 0, before the sequence that holds step `want`; each segment with `start` more.
-struct ListSum { int before, seq; };
-__device__ __forceinline__ ListSum walk_list(const AttendArgs& a, int lane, int until, int want, int start) {
-  const int per_step = a.kv_heads * a.row_tiles, stop = until < 0 ? a.bs : until;
-  int before = 0;
-  for (int b0 = 0; b0 < stop; b0 += 32) {
-    const int b = b0 + lane;
-    const int own = b < stop ? (start + steps_of(live_positions(a, b))) * per_step : 0;
-    int sum = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
-    }
-    if (until < 0) {
-      const unsigned past = __ballot_sync(0xffffffffu, before + sum > want && own > 0);
-      if (past != 0) {
-        const int at = __ffs(past) - 1;
-        return {before + __shfl_sync(0xffffffffu, sum - own, at), b0 + at};
-      }
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  return {before, stop};
-}
-// First step of CTA i's stretch, and the CTA that holds step g: the first total % ctas
-// stretches are one step longer than the others.
-struct Stretches {
-  int each, longer;
-  __device__ Stretches(int total, int ctas) : each(total / ctas), longer(total - each * ctas) {}
-  __device__ int begin(int i) const { return i * each + min(i, longer); }
-  __device__ int cta_of(int g) const {
-    const int cut = longer * (each + 1);
-    return g < cut ? g / (each + 1) : longer + (g - cut) / each;
-  }
-};
 
 // CTAs per SM, at 32 x 4000 positions against one less and one more.  HD 128: one row tile of
 // bf16, int8 39 us (41, 46), e4m3 42 (45, 47); two of bf16 48 (83, 55); one of fp32 46.5 (70,
@@ -1367,148 +1017,9 @@ __global__ void __launch_bounds__(AT_THREADS, (attend_resident<HD, NT, BITS>()))
   }
 }
 
-// Joins the states of the segments that lie in several CTAs' stretches: WPR warps per row,
-// eight per CTA.  A segment of the ordinary batch has two or three states, one of a single
-// long sequence some seventy: there one warp's loads would queue up (22 us instead of 3).
-constexpr int MG_WARPS = 8;
-template <int HD, int WPR>
-__global__ void __launch_bounds__(32 * MG_WARPS) kv8_attend_merge_kernel(const AttendArgs a, int tile_rows) {
-  constexpr int N = HD / 32;
-  __shared__ float s_o[MG_WARPS][HD];
-  __shared__ float2 s_ml[MG_WARPS];
-  const int G = a.heads / a.kv_heads, rows = G * a.sl;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPR;
-  const int at = blockIdx.x * (MG_WARPS / WPR) + warp / WPR;
-  const int row = at % rows, kvh = at / rows % a.kv_heads, b = at / rows / a.kv_heads;
-  if (b >= a.bs) return;  // whole warps; with WPR > 1 the grid has no such rows
-  // The list once: its length, that of the sequences before this one, and this one's steps.
-  // Before the wait it is a guess, with which the states' loads can start as soon as the wait
-  // is over; the lengths are read again beside them (past L1, which may have kept the first
-  // look).  Lengths are clamped to the page table, so that any guess names states in scratch.
-  const int per_step = a.kv_heads * a.row_tiles;
-  struct List { int real, before, steps; };
-  auto look = [&] {
-    List l{0, 0, 0};
-    for (int i = lane; i < a.bs; i += 32) {
-      const int n = steps_of(clamp_length(a, __ldcg(a.seq_lens + i)));
-      l.real += n * per_step;
-      l.before += i < b ? n * per_step : 0;
-      l.steps += i == b ? n : 0;
-    }
-    l.real = __reduce_add_sync(0xffffffffu, l.real);
-    l.before = __reduce_add_sync(0xffffffffu, l.before);
-    l.steps = __reduce_add_sync(0xffffffffu, l.steps);
-    return l;
-  };
-  // where the row's states are: the first CTA may have begun before this segment, and its state
-  // is then its second; the others begin inside it
-  const size_t pitch = static_cast<size_t>(tile_rows) * (HD + 4);
-  struct States { int n; const float *first, *others; };
-  auto find = [&](const List& l) {
-    const int start = start_steps(l.real, a.ctas), total = l.real + start * a.bs * per_step;
-    const int g0 = l.before + start * b * per_step + (kvh * a.row_tiles + row / tile_rows) * (start + l.steps);
-    const Stretches cut(total, min(a.ctas, total));
-    const int first = cut.cta_of(g0 + start), last = cut.cta_of(g0 + start + l.steps - 1);
-    const float* at = a.partial + 2 * static_cast<size_t>(first) * pitch + row % tile_rows * (HD + 4);
-    return States{last - first + 1, at + (cut.begin(first) < g0 ? pitch : 0), at};
-  };
-  constexpr int AT_ONCE = WPR == 1 ? 4 : 8;
-  float v[AT_ONCE][N];
-  float2 ml[AT_ONCE];
-  auto load = [&](const States& in, int s0) {
-#pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      const int s = s0 + k * WPR;
-      ml[k] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[k][j] = 0.f;
-      if (s < in.n) {
-        const float* from = s == 0 ? in.first : in.others + 2 * s * pitch;
-        ml[k] = *reinterpret_cast<const float2*>(from + HD);
-        load_elems(from + lane * N, v[k]);
-      }
-    }
-  };
-  const List guess = look();
-  States in = find(guess);
-  grid_dep_wait();
-  grid_dep_launch();
-  if (in.n > 1) load(in, part);
-  const List list = look();
-  if (list.real != guess.real || list.before != guess.before || list.steps != guess.steps) {
-    in = find(list);
-    if (in.n > 1) load(in, part);
-  }
-  if (in.n == 1) return;  // finished by that CTA
-  float acc[N], top = -INFINITY, den = 0.f;
-#pragma unroll
-  for (int j = 0; j < N; ++j) acc[j] = 0.f;
-  for (int s0 = part; s0 < in.n; s0 += AT_ONCE * WPR) {
-    if (s0 != part) load(in, s0);
-    float up = top;
-#pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) up = fmaxf(up, ml[k].x);
-    const float root0 = state_root(top, up), f0 = root0 * root0;
-    den = den * root0 * root0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] *= f0;
-    top = up;
-#pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      const float root = state_root(ml[k].x, top), f = root * root;
-      den = fmaf(ml[k].y * root, root, den);
-#pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] = fmaf(v[k][j], f, acc[j]);
-    }
-  }
-  const size_t to = ((static_cast<size_t>(b) * a.sl + row / G) * a.heads + kvh * G + row % G) * HD;
-  if constexpr (WPR == 1) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = den == 0.f ? 0.f : acc[j] / den;
-    store_as(a.out, a.out_dtype, to + lane * N, acc);
-  } else {
-    static_assert(WPR == 1 || WPR == MG_WARPS, "one row per CTA: all of its warps are here or none");
-#pragma unroll
-    for (int j = 0; j < N; ++j) s_o[warp][lane * N + j] = acc[j];
-    if (lane == 0) s_ml[warp] = make_float2(top, den);
-    __syncthreads();
-    const int d = threadIdx.x * 2;
-    if (d >= HD) return;
-    top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < MG_WARPS; ++w) top = fmaxf(top, s_ml[w].x);
-    float o[2] = {0.f, 0.f};
-    den = 0.f;
-#pragma unroll
-    for (int w = 0; w < MG_WARPS; ++w) {
-      const float root = state_root(s_ml[w].x, top), f = root * root;
-      den = fmaf(s_ml[w].y * root, root, den);
-      o[0] = fmaf(s_o[w][d], f, o[0]);
-      o[1] = fmaf(s_o[w][d + 1], f, o[1]);
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) o[j] = den == 0.f ? 0.f : o[j] / den;
-    store_as(a.out, a.out_dtype, to + d, o);
-  }
-}
 
-template <int HD>
-int launch_merge(const AttendArgs& a, int tile_rows, cudaStream_t st) {
-  const int64_t rows = static_cast<int64_t>(a.bs) * a.heads * a.sl;
-  // states of a segment, about (8 x 8190 positions, 30 rows, 4.6 states: a warp per row 56 us in all, eight 64)
-  const bool many = a.ctas > 6 * a.bs * a.kv_heads * a.row_tiles;
-  if (many)
-    B200_CHECK_CUDA(launch_dependent(kv8_attend_merge_kernel<HD, MG_WARPS>, dim3(static_cast<unsigned>(rows)),
-                                     dim3(32 * MG_WARPS), 0, st, a, tile_rows));
-  else
-    B200_CHECK_CUDA(launch_dependent(kv8_attend_merge_kernel<HD, 1>, dim3(static_cast<unsigned>((rows + MG_WARPS - 1) / MG_WARPS)),
-                                     dim3(32 * MG_WARPS), 0, st, a, tile_rows));
-  return B200MOE_OK;
-}
-
-// Rows of a CTA's tile; CTAs of a call: as many as are resident at once, or one for each
+// CTAs of a call: as many as are resident at once, or one for each
 // step of a full page table where those are fewer.
-inline int attend_tile_rows(int rows) { return rows <= 8 ? 8 : 16; }
 template <int HD>
 int resident_ctas(int tile, int bits) {
   if (bits == BITS_BOTH) return tile == 16 ? attend_resident<HD, 2, BITS_BOTH>() : attend_resident<HD, 1, BITS_BOTH>();
