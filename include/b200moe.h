@@ -500,6 +500,55 @@ int b200moe_kv8_attend(const void* q, int q_dtype, int64_t q_stride, const void*
                        int32_t heads, int32_t max_seq_len, float scale, float softcap, void* out, int out_dtype,
                        void* scratch, size_t scratch_bytes, void* stream);
 
+/* A cache of 4-bit codes.  slab: [page][block][kv head][K | V][position in page][head_dim / 2]
+ * bytes of two codes each, the even element in the low half; scales: [page][block][kv head]
+ * [K | V][position in page][head_dim / 32] pairs of fp16, scale s and offset m of 32 values of a
+ * row.  A code c, 0 .. 15, stands for c * s + m (the form of Q4_1's blocks).  5 bits a value.
+ * Geometry: b200moe_kv_cache_t with head_dim 64 or 128 and page_count rows of both; fewer than
+ * 2^32 rows of positions in all.  Slab and scales are 16-byte aligned.
+ *
+ * The write is b200moe_attn_norm_rope_kv8_write's but for the quantisation: s is
+ * (max - min) / 15 and m min of the 32 values, each rounded to fp16, and c the integer nearest
+ * to (x - m) / s, the even one of two as near, within 0 .. 15 (0 where s is).  Rows are
+ * independent: any position may be written again at any time.  A group with an infinity or a
+ * NaN, or whose s or m is beyond fp16's range, has NaN in both and reads as NaN.  A position whose page
+ * is missing or out of range sets the bounds bit of the status word and is not written. */
+int b200moe_attn_norm_rope_kv4_write(const void* q, const void* k, const void* v, int io_dtype, int64_t q_stride,
+                                     int64_t k_stride, int64_t v_stride, const float* q_norm, const float* k_norm,
+                                     float eps, void* q_out, void* k_out, void* slab, void* scales,
+                                     const b200moe_kv_cache_t* cache, int32_t block_index,
+                                     const int32_t* start_positions, const int32_t* new_lens, const int32_t* page_ids,
+                                     const float* freqs, int order, int32_t bs, int32_t tokens_per_seq,
+                                     int32_t pages_per_seq, int32_t heads, void* stream);
+/* b200moe_kv8_read of a cache of 4-bit codes. */
+int b200moe_kv4_read(const void* slab, const void* scales, const b200moe_kv_cache_t* cache, int32_t block_index,
+                     const int32_t* page_ids, const int32_t* seq_lens, int32_t bs, int32_t pages_per_seq,
+                     int32_t max_seq_len, void* k_out, void* v_out, int out_dtype, void* stream);
+/* b200moe_kv8_attend over a cache of 4-bit codes. */
+size_t b200moe_kv4_attend_scratch_bytes(const b200moe_kv_cache_t* cache, int32_t bs, int32_t new_tokens, int32_t heads,
+                                        int32_t max_seq_len);
+int b200moe_kv4_attend(const void* q, int q_dtype, int64_t q_stride, const void* slab, const void* scales,
+                       const b200moe_kv_cache_t* cache, int32_t block_index, const int32_t* page_ids,
+                       const int32_t* seq_lens, int32_t bs, int32_t new_tokens, int32_t pages_per_seq, int32_t heads,
+                       int32_t max_seq_len, float scale, float softcap, void* out, int out_dtype, void* scratch,
+                       size_t scratch_bytes, void* stream);
+
+/* Attention of whole prompts, the attention core of PagedLlamaAttentionBlock's prefill
+ * (layers/paged_llama_attention_block.py:160-232) for packed sequences.  Sequence b has rows
+ * cu_q[b] .. cu_q[b + 1] - 1 of q and cu_k[b] .. cu_k[b + 1] - 1 of k and v (cu_k NULL: cu_q's);
+ * of its n and m rows, row i of q attends rows 0 .. m - n + i of k, and its output is zero where
+ * that leaves none.  q: q_rows rows of heads * head_dim elements, k and v: k_rows rows of
+ * kv_heads * head_dim, each q_stride, k_stride, v_stride elements apart, all of one dtype; out
+ * [q_rows][heads][head_dim] contiguous, of out_dtype.  Rows of q in no sequence (before cu_q[0],
+ * behind cu_q[bs]) give zeros.  Bounds that decrease or leave the rows set the bounds bit of the
+ * status word; such a sequence is cut to the rows there are.  Any heads / kv_heads; head_dim 64
+ * or 128; softcap (finite) <= 0 means none.  Infinities and NaN in k and v show in the rows that
+ * attend them only. */
+int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype, int64_t q_stride, int64_t k_stride,
+                          int64_t v_stride, const int32_t* cu_q, const int32_t* cu_k, int32_t bs, int64_t q_rows,
+                          int64_t k_rows, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, float softcap,
+                          void* out, int out_dtype, void* stream);
+
 /* A stream of batches from host memory (no reference counterpart: the
  * reference's eager layer takes whatever device its tensors are on).  The
  * pipeline keeps `depth` steps in flight: the host->device copy of a step's

@@ -20,6 +20,7 @@ LAYOUT_Q8_0, LAYOUT_Q4_K, LAYOUT_F16 = 0, 1, 2
 ACT_SILU, ACT_GELU = 0, 1
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 KV8_INT8, KV8_E4M3 = 0, 1
+KV4 = 2  # code of a cache geometry: 4-bit codes (attention.py, attention_ops.cpp)
 REGIME_AUTO, REGIME_STREAM, REGIME_TENSOR, REGIME_TENSOR_PAIR = 0, 1, 2, 3
 
 
@@ -169,6 +170,16 @@ _PROTOS = {
     "b200moe_kv8_attend_scratch_bytes": (c_size_t, [POINTER(Kv8CacheDesc), c_int32, c_int32, c_int32, c_int32]),
     "b200moe_kv8_attend": (c_int, [_P, c_int, c_int64, _P, _P, POINTER(Kv8CacheDesc), c_int32, _P, _P, c_int32, c_int32,
                                    c_int32, c_int32, c_int32, c_float, c_float, _P, c_int, _P, c_size_t, _P]),
+    "b200moe_attn_norm_rope_kv4_write": (c_int, [_P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, c_float, _P, _P, _P,
+                                                 _P, POINTER(KvCacheDesc), c_int32, _P, _P, _P, _P, c_int, c_int32,
+                                                 c_int32, c_int32, c_int32, _P]),
+    "b200moe_kv4_read": (c_int, [_P, _P, POINTER(KvCacheDesc), c_int32, _P, _P, c_int32, c_int32, c_int32, _P, _P, c_int,
+                                 _P]),
+    "b200moe_kv4_attend_scratch_bytes": (c_size_t, [POINTER(KvCacheDesc), c_int32, c_int32, c_int32, c_int32]),
+    "b200moe_kv4_attend": (c_int, [_P, c_int, c_int64, _P, _P, POINTER(KvCacheDesc), c_int32, _P, _P, c_int32, c_int32,
+                                   c_int32, c_int32, c_int32, c_float, c_float, _P, c_int, _P, c_size_t, _P]),
+    "b200moe_prompt_attend": (c_int, [_P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, c_int32, c_int64, c_int64,
+                                      c_int32, c_int32, c_int32, c_float, c_float, _P, c_int, _P]),
     "b200moe_pipeline_bytes": (c_size_t, [_L, c_int, c_int32, c_int32]),
     "b200moe_pipeline_create": (c_int, [_L, c_int, c_int32, c_int, c_int32, _P, c_size_t, POINTER(c_void_p)]),
     "b200moe_pipeline_submit": (c_int, [_P, _P, _P, c_int32, _P]),
@@ -211,7 +222,8 @@ def _load_attention_ops():
                            "`python -m shark_platform_b200.build`") from e
     module.bind(B200MoeError, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
         "b200moe_attn_norm_rope_kv8_write", "b200moe_attn_norm_rope_kv_write", "b200moe_kv8_read", "b200moe_kv8_attend",
-        "b200moe_kv8_attend_scratch_bytes", "b200moe_last_error")))
+        "b200moe_kv8_attend_scratch_bytes", "b200moe_attn_norm_rope_kv4_write", "b200moe_kv4_read", "b200moe_kv4_attend",
+        "b200moe_kv4_attend_scratch_bytes", "b200moe_prompt_attend", "b200moe_last_error")))
     return module
 
 

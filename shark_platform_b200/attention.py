@@ -14,6 +14,8 @@ kernel; they are public on their own:
   * `norm_rope_kv_write`: norms, rotation and the (quantising) cache write in one pass;
   * `kv_attend`: attention of one or a few new tokens over an 8-bit cache;
   * `kv_read`: the values of an 8-bit cache as plain K and V.
+All of them take caches of 4-bit codes as well (`PagedKVCache(dtype=torch.uint8)`).
+`prompt_attend` is the attention of whole prompts: packed sequences, causal, grouped heads.
 
 What runs where:
   * RMS norm, rotary embedding fused with the KV page write, and the decode
@@ -50,7 +52,8 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
-_KV8_CODES = {torch.int8: C.KV8_INT8, torch.float8_e4m3fn: C.KV8_E4M3}
+_CODES = {torch.int8: C.KV8_INT8, torch.float8_e4m3fn: C.KV8_E4M3, torch.uint8: C.KV4}
+KV4_GROUP = 32       # values of a row that share a scale and an offset, 4-bit codes
 MAX_NEW_TOKENS = 16  # of one kv_attend call
 
 
@@ -63,7 +66,10 @@ class PagedKVCache:
     scale for each `scale_block` consecutive positions of a page, kv head and K | V
     (a power of two up to 64 that divides `block_seq_stride`; by default the largest
     one up to 16): 1 + 4 / scale_block / head_dim bytes per value.  Small blocks follow
-    single large rows more closely, large ones have fewer scales to read."""
+    single large rows more closely, large ones have fewer scales to read.
+
+    `dtype` uint8 makes it a cache of 4-bit codes, two a byte, with an fp16 scale and offset
+    for each 32 values of a row: 5 / 8 bytes per value.  Rows are independent of each other."""
 
     def __init__(self, *, transformer_block_count: int, attn_head_count: int, attn_head_dim: int,
                  cache_partition_count: int = 2, block_seq_stride: int = 16,
@@ -78,8 +84,21 @@ class PagedKVCache:
         self.block_seq_stride = block_seq_stride
         self.shard_count = shard_count
         self.dtype, self.device = dtype, device
-        self.quantized = dtype in _KV8_CODES
-        if self.quantized:
+        self.quantized = dtype in _CODES
+        self.scale_dtype = None
+        if dtype == torch.uint8:
+            if scale_block is not None:
+                raise C.B200MoeError("scale_block is for caches of 8-bit codes, not 4-bit ones")
+            if attn_head_dim % KV4_GROUP:
+                raise C.B200MoeError(f"head_dim {attn_head_dim}: a cache of 4-bit codes has scales for {KV4_GROUP} values each")
+            self.scale_block = None
+            self.scale_dtype = torch.float16
+            # a head's rows of a page are one contiguous stretch; scales and offsets: the same rows
+            self.sub_page_dims = [transformer_block_count, attn_head_count, 2, block_seq_stride, attn_head_dim // 2]
+            self.scale_page_dims = [transformer_block_count, attn_head_count, 2, block_seq_stride, attn_head_dim // KV4_GROUP, 2]
+            self.scale_flat_dim = math.prod(self.scale_page_dims)
+        elif self.quantized:
+            self.scale_dtype = torch.float32
             # the largest power of two that divides the stride, up to 16
             self.scale_block = min(block_seq_stride & -block_seq_stride, 16) if scale_block is None else scale_block
             b = self.scale_block
@@ -97,13 +116,13 @@ class PagedKVCache:
             self.sub_page_dims = [transformer_block_count, 2, block_seq_stride, attn_head_count, attn_head_dim]
         self.page_slab_flat_dim = math.prod(self.sub_page_dims)
         self._geometry = (transformer_block_count, block_seq_stride, attn_head_count, attn_head_dim,
-                          self.scale_block or 1, _KV8_CODES.get(dtype, -1))
+                          self.scale_block or 1, _CODES.get(dtype, -1))
 
     def allocate(self, page_count: int) -> list[torch.Tensor]:
-        """[page slab], or [page slab, scales] for 8-bit codes: a row of each per page."""
+        """[page slab], or [page slab, scales] for 8- and 4-bit codes: a row of each per page."""
         state = [torch.zeros(page_count, self.page_slab_flat_dim, dtype=self.dtype, device=self.device)]
         if self.quantized:
-            state.append(torch.zeros(page_count, self.scale_flat_dim, dtype=torch.float32, device=self.device))
+            state.append(torch.zeros(page_count, self.scale_flat_dim, dtype=self.scale_dtype, device=self.device))
         return state
 
 
@@ -137,7 +156,12 @@ def norm_rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache:
     fit, else the scale grows by a power of two and the block's earlier codes are rounded
     to it.  Positions behind the last written one of a block are dead until written (a
     drafted token that is taken back leaves its block's scale as it made it).  An infinity
-    or NaN makes its block read as NaN until it is begun again."""
+    or NaN makes its block read as NaN until it is begun again.
+
+    4-bit codes: every 32 values of a row have the scale (max - min) / 15 and the offset min,
+    rounded to fp16, and the codes nearest to them.  Rows are independent: any position may be
+    written again at any time.  A group with an infinity or a NaN, or whose scale or offset
+    is beyond fp16's range, reads as NaN."""
     return C.attention_ops.write(q, k, v, cache_state, _geometry(cache), block_index, seq_block_ids, start_positions, new_lens,
                                  freqs, q_norm, k_norm, eps, use_hf)
 
@@ -145,16 +169,16 @@ def norm_rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache:
 def kv_read(cache: PagedKVCache, cache_state: list, *, block_index: int, seq_block_ids: torch.Tensor,
             seq_lens: torch.Tensor, max_seq_len: Optional[int] = None,
             dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
-    """K and V of the listed pages of an 8-bit cache, [bs, max_seq_len, kv_heads, head_dim]
-    each (`max_seq_len`: all of the listed pages by default); every value code * scale,
-    rounded once to `dtype`.  Rows at and behind seq_lens[b] are zero."""
+    """K and V of the listed pages of an 8- or 4-bit cache, [bs, max_seq_len, kv_heads, head_dim]
+    each (`max_seq_len`: all of the listed pages by default); every value code * scale
+    (+ offset), rounded once to `dtype`.  Rows at and behind seq_lens[b] are zero."""
     return C.attention_ops.read(cache_state, _geometry(cache), block_index, seq_block_ids, seq_lens, max_seq_len, dtype)
 
 
 def kv_attend(q: torch.Tensor, cache: PagedKVCache, cache_state: list, *, block_index: int,
               seq_block_ids: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
               softcap: Optional[float] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """Attention of the last sl (1 ... 16) positions of each sequence over an 8-bit cache.
+    """Attention of the last sl (1 ... 16) positions of each sequence over an 8- or 4-bit cache.
 
     q [bs, sl, heads, head_dim], rotated; seq_lens[b] counts the positions in the cache,
     the sl new ones included (`norm_rope_kv_write` first).  Token i attends the positions
@@ -166,6 +190,25 @@ def kv_attend(q: torch.Tensor, cache: PagedKVCache, cache_state: list, *, block_
     output is fp32 or fp16 or q is fp32, else (bf16) to 11, an eighth of the output's rounding."""
     return C.attention_ops.attend(q, cache_state, _geometry(cache), block_index, seq_block_ids, seq_lens, scale, softcap,
                                   out_dtype)
+
+
+def prompt_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: torch.Tensor,
+                  cu_seqlens_k: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                  softcap: Optional[float] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Causal attention of packed sequences of different lengths, without padding.
+
+    q [rows, heads, head_dim], k and v [rows, kv_heads, head_dim], rotated (views of one fused
+    projection are taken as they are).  Sequence b has q's rows cu_seqlens[b] ...
+    cu_seqlens[b + 1] - 1 (whole numbers on q's device, bs + 1 of them) and the rows of k and v
+    that cu_seqlens_k says, by default the same.  A continued prompt has more rows of k than of
+    q, its last ones being those of q: of n rows of q and m of k, row i attends rows 0 ...
+    m - n + i.  Where that leaves none the output is zero, as it is for rows of no sequence
+    (in front of the first and behind the last).  scale: 1 / sqrt(head_dim) by default; softcap:
+    c * tanh(score / c).  Returns [rows, heads, head_dim] of `out_dtype`, by default q's.
+
+    Sums and softmax statistics are 32-bit.  There is no gradient: inputs that want one are
+    refused."""
+    return C.attention_ops.prompt(q, k, v, cu_seqlens, cu_seqlens_k, scale, softcap, out_dtype)
 
 
 class RotaryEmbeddingLayer:

@@ -1,4 +1,4 @@
-// The cache operators of attention.py for torch tensors: argument checks, outputs and the
+// The cache operators and the prompt attention of attention.py for torch tensors: argument checks, outputs and the
 // call of the C ABI.  They run once per layer and token, beside kernels of a few
 // microseconds; the same work in Python and ctypes took the host 20 / 15 / 17 us a call
 // (write, read, attend).  The library's entry points come as addresses from the ctypes
@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -25,6 +26,11 @@ decltype(&b200moe_attn_norm_rope_kv_write) write_plain = nullptr;
 decltype(&b200moe_kv8_read) read8 = nullptr;
 decltype(&b200moe_kv8_attend) attend8 = nullptr;
 decltype(&b200moe_kv8_attend_scratch_bytes) attend8_scratch = nullptr;
+decltype(&b200moe_attn_norm_rope_kv4_write) write4 = nullptr;
+decltype(&b200moe_kv4_read) read4 = nullptr;
+decltype(&b200moe_kv4_attend) attend4 = nullptr;
+decltype(&b200moe_kv4_attend_scratch_bytes) attend4_scratch = nullptr;
+decltype(&b200moe_prompt_attend) attend_prompt = nullptr;
 decltype(&b200moe_last_error) last_error = nullptr;
 PyObject* error_class = nullptr;  // B200MoeError
 
@@ -79,7 +85,9 @@ at::Tensor as_int32(const at::Tensor& t) {
   return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
 }
 
-// (blocks, stride, kv_heads, head_dim, scale_block, code): code -1 is a 16- or 32-bit cache
+// (blocks, stride, kv_heads, head_dim, scale_block, code): code -1 is a 16- or 32-bit cache,
+// CODE4 one of 4-bit codes (no scale_block), others B200MOE_KV8_*
+constexpr int64_t CODE4 = 2;
 struct Geometry {
   int64_t blocks, stride, kv_heads, head_dim, scale_block, code;
   explicit Geometry(PyObject* t) {
@@ -88,10 +96,16 @@ struct Geometry {
     for (int i = 0; i < 6; ++i) *to[i] = integer(PyTuple_GET_ITEM(t, i));
     for (int i = 0; i < 4; ++i)
       if (*to[i] < 1 || *to[i] > 0x7fffffff) refuse("bad cache geometry");
-    if (code >= 0 && (scale_block < 1 || scale_block > 0x7fffffff)) refuse("bad cache geometry");
+    if (code > CODE4 || (code >= 0 && (scale_block < 1 || scale_block > 0x7fffffff)) || (four() && head_dim % 32 != 0))
+      refuse("bad cache geometry");
   }
   bool quantized() const { return code >= 0; }
-  at::ScalarType dtype() const { return code == B200MOE_KV8_INT8 ? at::kChar : at::kFloat8_e4m3fn; }
+  bool four() const { return code == CODE4; }
+  at::ScalarType dtype() const { return four() ? at::kByte : code == B200MOE_KV8_INT8 ? at::kChar : at::kFloat8_e4m3fn; }
+  // elements of a page in the slab, and scales (8-bit codes: fp32; 4-bit: fp16, with the offsets)
+  int64_t page() const { return blocks * 2 * stride * kv_heads * head_dim / (four() ? 2 : 1); }
+  int64_t page_scales() const { return blocks * kv_heads * 2 * (four() ? stride * (head_dim / 32) * 2 : stride / scale_block); }
+  at::ScalarType scale_type() const { return four() ? at::kHalf : at::kFloat; }
 };
 
 // The cache's tensors and page table, looked over.
@@ -107,17 +121,16 @@ struct State {
       refuse("block_index ", block_index, " is not one of the cache's ", g.blocks, " transformer blocks");
     if (n < 1) refuse("cache_state is a list of tensors, as allocate() gives it");
     slab = &tensor(items[0], "the page slab");
-    if (slab->dim() != 2 || slab->size(1) != g.blocks * 2 * g.stride * g.kv_heads * g.head_dim || !slab->is_contiguous())
+    if (slab->dim() != 2 || slab->size(1) != g.page() || !slab->is_contiguous())
       refuse("the page slab must be contiguous, a row of the cache's page size per page");
     if (g.quantized()) {
-      if (n != 2) refuse("a cache of 8-bit codes is [page slab, scales], as allocate() gives it");
+      if (n != 2) refuse("a cache of 8-bit codes (or of 4-bit ones) is [page slab, scales], as allocate() gives it");
       scales = &tensor(items[1], "scales");
       if (slab->scalar_type() != g.dtype())
         refuse("the page slab must be ", at::toString(g.dtype()), ", got ", at::toString(slab->scalar_type()));
-      if (scales->scalar_type() != at::kFloat || scales->dim() != 2 || scales->size(0) != slab->size(0) ||
-          scales->size(1) != g.blocks * g.kv_heads * (g.stride / g.scale_block) * 2 || !scales->is_contiguous() ||
-          scales->device() != dev)
-        refuse("scales must be fp32, contiguous, beside the slab, a row per page");
+      if (scales->scalar_type() != g.scale_type() || scales->dim() != 2 || scales->size(0) != slab->size(0) ||
+          scales->size(1) != g.page_scales() || !scales->is_contiguous() || scales->device() != dev)
+        refuse("scales must be ", g.four() ? "fp16" : "fp32", ", contiguous, beside the slab, a row per page");
     } else if (dtype_code(slab->scalar_type()) < 0) {
       refuse("the page slab must be a contiguous fp32, fp16 or bf16 tensor");
     }
@@ -132,6 +145,10 @@ struct State {
     return {static_cast<int32_t>(g.blocks), static_cast<int32_t>(g.stride), static_cast<int32_t>(g.kv_heads),
             static_cast<int32_t>(g.head_dim), static_cast<int32_t>(slab->size(0)), static_cast<int32_t>(g.scale_block),
             static_cast<int32_t>(g.code)};
+  }
+  b200moe_kv_cache_t desc(const Geometry& g) const {
+    return {static_cast<int32_t>(g.blocks), static_cast<int32_t>(g.stride), static_cast<int32_t>(g.kv_heads),
+            static_cast<int32_t>(g.head_dim), static_cast<int32_t>(slab->size(0))};
   }
 };
 
@@ -176,7 +193,7 @@ const void* data(const at::Tensor& t) { return t.const_data_ptr(); }
 // bind(error class, addresses): the library's entry points
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   OPS_BEGIN
-  if (n != 7) refuse("bind takes the error class and six addresses");
+  if (n != 12) refuse("bind takes the error class and eleven addresses");
   auto address = [&](int i) { return reinterpret_cast<void*>(static_cast<uintptr_t>(integer(a[i]))); };
   Py_INCREF(a[0]);
   error_class = a[0];
@@ -185,7 +202,12 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   read8 = reinterpret_cast<decltype(read8)>(address(3));
   attend8 = reinterpret_cast<decltype(attend8)>(address(4));
   attend8_scratch = reinterpret_cast<decltype(attend8_scratch)>(address(5));
-  last_error = reinterpret_cast<decltype(last_error)>(address(6));
+  write4 = reinterpret_cast<decltype(write4)>(address(6));
+  read4 = reinterpret_cast<decltype(read4)>(address(7));
+  attend4 = reinterpret_cast<decltype(attend4)>(address(8));
+  attend4_scratch = reinterpret_cast<decltype(attend4_scratch)>(address(9));
+  attend_prompt = reinterpret_cast<decltype(attend_prompt)>(address(10));
+  last_error = reinterpret_cast<decltype(last_error)>(address(11));
   Py_RETURN_NONE;
   OPS_END
 }
@@ -241,7 +263,17 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor ids = as_int32(s.ids), at0 = as_int32(start);
     const int32_t n_bs = i32(bs, "batch"), n_sl = i32(sl, "tokens"), n_heads = i32(heads, "heads");
     const int32_t* lens_p = lens ? static_cast<const int32_t*>(data(*lens)) : nullptr;
-    if (g.quantized()) {
+    if (g.four()) {
+      const b200moe_kv_cache_t desc = s.desc(g);
+      launch("attn_norm_rope_kv4_write", dev, [&](void* stream) {
+        return write4(data(qr.t), data(kr.t), data(vr.t), dt, qr.stride, kr.stride, vr.stride, norm[0], norm[1], eps,
+                      q_out.mutable_data_ptr(), k_out.mutable_data_ptr(), s.slab->mutable_data_ptr(),
+                      s.scales->mutable_data_ptr(), &desc, static_cast<int32_t>(block_index),
+                      static_cast<const int32_t*>(data(at0)), lens_p, static_cast<const int32_t*>(data(ids)),
+                      static_cast<const float*>(data(freqs)), hf, n_bs, n_sl, static_cast<int32_t>(ids.size(1)), n_heads,
+                      stream);
+      });
+    } else if (g.quantized()) {
       const b200moe_kv8_cache_t desc = s.desc8(g);
       launch("attn_norm_rope_kv8_write", dev, [&](void* stream) {
         return write8(data(qr.t), data(kr.t), data(vr.t), dt, qr.stride, kr.stride, vr.stride, norm[0], norm[1], eps,
@@ -252,9 +284,7 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       stream);
       });
     } else {
-      const b200moe_kv_cache_t desc = {static_cast<int32_t>(g.blocks), static_cast<int32_t>(g.stride),
-                                       static_cast<int32_t>(g.kv_heads), static_cast<int32_t>(hd),
-                                       static_cast<int32_t>(s.slab->size(0))};
+      const b200moe_kv_cache_t desc = s.desc(g);
       launch("attn_norm_rope_kv_write", dev, [&](void* stream) {
         return write_plain(data(qr.t), data(kr.t), data(vr.t), dt, qr.stride, kr.stride, vr.stride, norm[0], norm[1], eps,
                            q_out.mutable_data_ptr(), k_out.mutable_data_ptr(), s.slab->mutable_data_ptr(),
@@ -282,7 +312,7 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   OPS_BEGIN
   if (n != 7) refuse("read takes 7 arguments");
   const Geometry g(a[1]);
-  if (!g.quantized()) refuse("kv_read reads caches of 8-bit codes");
+  if (!g.quantized()) refuse("kv_read reads caches of 8-bit codes (or of 4-bit ones)");
   const at::ScalarType type = scalar_type(a[6], at::kBFloat16);
   if (dtype_code(type) < 0) refuse("K and V are read as fp32, fp16 or bf16, not ", at::toString(type));
   const at::Tensor &lens = tensor(a[4], "seq_lens"), &table = tensor(a[3], "seq_block_ids");
@@ -299,8 +329,14 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (bs * rows > 0) {
     const at::Tensor ids = as_int32(s.ids), len = as_int32(lens);
     const b200moe_kv8_cache_t desc = s.desc8(g);
+    const b200moe_kv_cache_t desc4 = s.desc(g);
     const int32_t n_bs = i32(bs, "batch"), n_rows = i32(rows, "max_seq_len");
-    launch("kv8_read", dev, [&](void* stream) {
+    launch(g.four() ? "kv4_read" : "kv8_read", dev, [&](void* stream) {
+      if (g.four())
+        return read4(data(*s.slab), data(*s.scales), &desc4, static_cast<int32_t>(block_index),
+                     static_cast<const int32_t*>(data(ids)), static_cast<const int32_t*>(data(len)), n_bs,
+                     static_cast<int32_t>(ids.size(1)), n_rows, k.mutable_data_ptr(), v.mutable_data_ptr(), dtype_code(type),
+                     stream);
       return read8(data(*s.slab), static_cast<const float*>(data(*s.scales)), &desc, static_cast<int32_t>(block_index),
                    static_cast<const int32_t*>(data(ids)), static_cast<const int32_t*>(data(len)), n_bs,
                    static_cast<int32_t>(ids.size(1)), n_rows, k.mutable_data_ptr(), v.mutable_data_ptr(), dtype_code(type),
@@ -319,7 +355,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 9) refuse("attend takes 9 arguments");
   const at::Tensor& q = tensor(a[0], "q");
   const Geometry g(a[2]);
-  if (!g.quantized()) refuse("kv_attend reads caches of 8-bit codes");
+  if (!g.quantized()) refuse("kv_attend reads caches of 8-bit codes (or of 4-bit ones)");
   const at::ScalarType type = scalar_type(a[8], q.scalar_type());
   const int dt = dtype_code(q.scalar_type()), out_dt = dtype_code(type);
   if (dt < 0 || out_dt < 0)
@@ -341,11 +377,19 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (bs > 0) {
     const at::Tensor ids = as_int32(s.ids), len = as_int32(lens);
     const b200moe_kv8_cache_t desc = s.desc8(g);
+    const b200moe_kv_cache_t desc4 = s.desc(g);
     const int32_t max_len = i32(ids.size(1) * g.stride, "positions"), n_bs = i32(bs, "batch"), n_heads = i32(heads, "heads");
-    launch("kv8_attend", dev, [&](void* stream) {
+    launch(g.four() ? "kv4_attend" : "kv8_attend", dev, [&](void* stream) {
       // per call: other streams and captured graphs have their own
-      const size_t bytes = attend8_scratch(&desc, n_bs, static_cast<int32_t>(sl), n_heads, max_len);
+      const size_t bytes = g.four() ? attend4_scratch(&desc4, n_bs, static_cast<int32_t>(sl), n_heads, max_len)
+                                    : attend8_scratch(&desc, n_bs, static_cast<int32_t>(sl), n_heads, max_len);
       at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte).memory_format(std::nullopt));
+      if (g.four())
+        return attend4(data(qr.t), dt, qr.stride, data(*s.slab), data(*s.scales), &desc4, static_cast<int32_t>(block_index),
+                       static_cast<const int32_t*>(data(ids)), static_cast<const int32_t*>(data(len)), n_bs,
+                       static_cast<int32_t>(sl), static_cast<int32_t>(ids.size(1)), n_heads, max_len,
+                       static_cast<float>(scale), static_cast<float>(softcap), out.mutable_data_ptr(), out_dt,
+                       scratch.mutable_data_ptr(), bytes, stream);
       return attend8(data(qr.t), dt, qr.stride, data(*s.slab), static_cast<const float*>(data(*s.scales)), &desc,
                      static_cast<int32_t>(block_index), static_cast<const int32_t*>(data(ids)),
                      static_cast<const int32_t*>(data(len)), n_bs, static_cast<int32_t>(sl),
@@ -357,11 +401,64 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   OPS_END
 }
 
+// prompt(q, k, v, cu_seqlens, cu_seqlens_k, scale, softcap, out_dtype) -> out
+PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  OPS_BEGIN
+  if (n != 8) refuse("prompt takes 8 arguments");
+  const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v");
+  const at::ScalarType type = scalar_type(a[7], q.scalar_type());
+  const int dt = dtype_code(q.scalar_type()), out_dt = dtype_code(type);
+  if (dt < 0 || out_dt < 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
+    refuse("q, k and v must be fp32, fp16 or bf16 alike and the output one of them, got ", at::toString(q.scalar_type()), ", ",
+           at::toString(k.scalar_type()), ", ", at::toString(v.scalar_type()), " and ", at::toString(type));
+  if (q.dim() != 3 || k.dim() != 3 || q.size(2) != k.size(2) || (q.size(2) != 64 && q.size(2) != 128) || k.size(1) < 1 ||
+      q.size(1) < 1 || q.size(1) % k.size(1) != 0 || v.sizes() != k.sizes())
+    refuse("q ", shape_of(q), ", k ", shape_of(k), ", v ", shape_of(v),
+           " must be [rows, heads, head_dim], heads a multiple of the kv heads, head_dim 64 or 128");
+  const at::Device dev = q.device();
+  auto bounds = [&](PyObject* o, const char* what) {
+    const at::Tensor& t = tensor(o, what);
+    if (t.dim() != 1 || t.size(0) < 1 || t.device() != dev || at::isFloatingType(t.scalar_type()))
+      refuse(what, " is one whole number for each sequence and one more, on q's device");
+    return as_int32(t);
+  };
+  const at::Tensor cu = bounds(a[3], "cu_seqlens");
+  std::optional<at::Tensor> cu_k;
+  if (a[4] != Py_None) {
+    cu_k = bounds(a[4], "cu_seqlens_k");
+    if (cu_k->size(0) != cu.size(0)) refuse("cu_seqlens_k is for other sequences than cu_seqlens");
+  } else if (k.size(0) != q.size(0)) {
+    refuse("k and v have ", k.size(0), " rows, q ", q.size(0), ": cu_seqlens_k says which are whose");
+  }
+  const int64_t rows = q.size(0), heads = q.size(1), hd = q.size(2);
+  const double scale = a[5] == Py_None ? 1.0 / std::sqrt(static_cast<double>(hd)) : number(a[5]);
+  const double softcap = a[6] == Py_None ? 0.0 : number(a[6]);
+  if (a[6] != Py_None && !(softcap > 0.0 && std::isfinite(static_cast<float>(softcap)))) refuse("softcap must be positive and finite");
+  if (k.device() != dev || v.device() != dev) refuse("all arguments must be on one device");
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    refuse("prompt_attend has no gradient: call it under torch.no_grad() or detach its inputs");
+  need_cuda(q, "q");
+  const Rows qr(q.unsqueeze(0)), kr(k.unsqueeze(0)), vr(v.unsqueeze(0));
+  at::Tensor out = at::empty({rows, heads, hd}, q.options().dtype(type).memory_format(std::nullopt));
+  if (rows > 0) {
+    const int32_t n_bs = i32(cu.size(0) - 1, "batch"), n_heads = i32(heads, "heads"), n_kv = i32(k.size(1), "kv heads");
+    launch("prompt_attend", dev, [&](void* stream) {
+      return attend_prompt(data(qr.t), data(kr.t), data(vr.t), dt, qr.stride, kr.stride, vr.stride,
+                           static_cast<const int32_t*>(data(cu)), cu_k ? static_cast<const int32_t*>(data(*cu_k)) : nullptr,
+                           n_bs, rows, k.size(0), n_heads, n_kv, static_cast<int32_t>(hd), static_cast<float>(scale),
+                           static_cast<float>(softcap), out.mutable_data_ptr(), out_dt, stream);
+    });
+  }
+  return THPVariable_Wrap(std::move(out));
+  OPS_END
+}
+
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, "the library's entry points"},
     {"write", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(write)), METH_FASTCALL, "attention.norm_rope_kv_write"},
     {"read", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(read)), METH_FASTCALL, "attention.kv_read"},
     {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attend)), METH_FASTCALL, "attention.kv_attend"},
+    {"prompt", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(prompt)), METH_FASTCALL, "attention.prompt_attend"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_attention_ops", nullptr, -1, methods};
 
