@@ -110,6 +110,29 @@ int make_tmap_2d_sw(CUtensorMap* out, const void* base, uint64_t rows, uint64_t 
   return B200MOE_OK;
 }
 
+int make_tmap_heads(CUtensorMap* out, const void* base, bool bf16, uint64_t rows, uint64_t heads, uint64_t head_dim,
+                    uint64_t row_stride, uint32_t box_rows, uint32_t box_heads) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from the driver");
+    return B200MOE_ERR_CUDA;
+  }
+  const cuuint64_t dims[3] = {head_dim, heads, rows};
+  const cuuint64_t strides[2] = {head_dim * 2, row_stride * 2};
+  const cuuint32_t box[3] = {64, box_heads, box_rows};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with %d (rows=%llu heads=%llu row stride=%llu box=%ux%u)", static_cast<int>(r),
+              static_cast<unsigned long long>(rows), static_cast<unsigned long long>(heads),
+              static_cast<unsigned long long>(row_stride), box_rows, box_heads);
+    return B200MOE_ERR_CUDA;
+  }
+  return B200MOE_OK;
+}
+
 int make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dt, uint32_t elem_bytes,
                  uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols,
                  bool swizzle128) {

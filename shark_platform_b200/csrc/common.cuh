@@ -45,6 +45,11 @@ int make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dt, uin
 int make_tmap_2d_sw(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes,
                     uint32_t box_rows, uint32_t box_bytes, int swizzle_bytes);
 
+// Tiled tensor map over [rows][heads][head_dim] of 16-bit elements, rows `row_stride` elements
+// apart, with the 128-byte swizzle: a box is box_rows x box_heads x 64 elements of a head.
+int make_tmap_heads(CUtensorMap* out, const void* base, bool bf16, uint64_t rows, uint64_t heads, uint64_t head_dim,
+                    uint64_t row_stride, uint32_t box_rows, uint32_t box_heads);
+
 // What a GEMM kernel of a layer call may prefetch into L2 while the kernel before it
 // still runs: nothing, the weights its first work item has if every expert turns out
 // to be active (the routing is not known yet), or those of the segments (known).

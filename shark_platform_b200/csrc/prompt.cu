@@ -13,6 +13,7 @@
 // they have the most keys, and the short ones fill the end.  It is made by every warp on its
 // own from the sequences' bounds on the device: the host does not know them.
 #include "kv_attend.cuh"
+#include "tcgen05.cuh"
 
 namespace b200moe {
 namespace {
@@ -26,6 +27,8 @@ struct PromptArgs {
   int out_dtype, bs, heads, kv_heads;
   int group, parts;       // heads of a tile; parts of a group of heads
   int tokens;             // of a tile
+  int splits;             // parts that the keys of a tile are cut into, at most
+  float* partial;         // [row of q][head][splits][HD + 4]: numerator, maximum, denominator
   float scale, softcap;
   int32_t* status;
 };
@@ -40,9 +43,16 @@ __device__ __forceinline__ Span span_of(const int32_t* cu, int b, int64_t rows, 
 }
 
 struct Item {
-  int seq, tile, kvh, part;
+  int seq, tile, kvh, part, chunk;
   bool some;
 };
+// Keys that the last of `toks` tokens from tok0 on sees, of a sequence of n tokens and m keys.
+__device__ __forceinline__ int keys_seen(int n, int m, int tok0, int toks) { return max(0, min(m, tok0 + toks + m - n)); }
+// Parts of a tile's keys, which are split between tiles of `step` keys; the first of them of part i.
+__device__ __forceinline__ int chunks_of(int keys, int step, int splits) { return max(1, min(splits, (keys + step - 1) / step)); }
+__device__ __forceinline__ int chunk_begin(int keys, int step, int chunks, int i) {
+  return static_cast<int>(static_cast<int64_t>((keys + step - 1) / step) * i / chunks) * step;
+}
 // The list of items, walked by a whole warp with rising indices.
 struct ItemWalk {
   int t;         // tiles with this place in their sequence are current
@@ -62,23 +72,39 @@ struct ItemWalk {
     }
     t = __reduce_max_sync(0xffffffffu, most) - 1;
   }
-  __device__ __forceinline__ Item find(const PromptArgs& a, int lane, long long i) {
+  // items of sequence b with tile t, apart from heads
+  __device__ __forceinline__ static int chunks(const PromptArgs& a, int b, int t, int step) {
+    if (b >= a.bs) return 0;
+    const int n = span_of(a.cu_q, b, a.q_rows, nullptr).len, tok0 = t * a.tokens;
+    if (tok0 >= n) return 0;
+    if (a.splits == 1) return 1;
+    const int m = span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, b, a.k_rows, nullptr).len;
+    return chunks_of(keys_seen(n, m, tok0, min(a.tokens, n - tok0)), step, a.splits);
+  }
+  __device__ __forceinline__ Item find(const PromptArgs& a, int lane, int step, long long i) {
     const int each = a.kv_heads * a.parts;
     for (; t >= 0; --t) {
       long long at = before;
       for (int b0 = 0; b0 < a.bs; b0 += 32) {
-        const unsigned has = __ballot_sync(0xffffffffu, tiles_of(a, b0 + lane) > t);
-        const int n = __popc(has);
-        if (i < at + static_cast<long long>(n) * each) {
-          const int r = static_cast<int>(i - at), which = r / each, h = r - which * each;
-          const int b = b0 + static_cast<int>(__fns(has, 0, which + 1));
-          return {b, t, h / a.parts, h % a.parts, true};
+        const int own = chunks(a, b0 + lane, t, step);
+        int sum = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += up;
         }
-        at += static_cast<long long>(n) * each;
+        const int all = __shfl_sync(0xffffffffu, sum, 31);
+        if (i < at + static_cast<long long>(all) * each) {
+          const int r = static_cast<int>(i - at), c = r / each, h = r - c * each;  // chunk c of those of 32 sequences
+          const int which = __ffs(__ballot_sync(0xffffffffu, sum > c)) - 1;
+          const int chunk = c - __shfl_sync(0xffffffffu, sum - own, which);
+          return {b0 + which, t, h / a.parts, h % a.parts, chunk, true};
+        }
+        at += static_cast<long long>(all) * each;
       }
       before = at;
     }
-    return {0, 0, 0, 0, false};
+    return {0, 0, 0, 0, 0, false};
   }
 };
 
@@ -97,20 +123,20 @@ __device__ __forceinline__ void zero_rest(const PromptArgs& a, int hd, int threa
   else zero_rest<__half>(a, hd, threads);
 }
 
-// ------------------------------------------------------------------ 32-bit products
+// ------------------------------------------------------------------ 32-bit rows
 // Tiles of 64 rows and 64 keys on the fp32 units: thread (ty, tx) of 16 x 16 has rows
 // 4 ty .. + 3, keys tx + 16 j of the scores and elements 4 tx + 64 j .. + 3 of the output.
 // Everything is fp32.
 constexpr int SP_ROWS = 64, SP_KEYS = 64, SP_THREADS = 256;
 
-template <typename T, int HD>
-__device__ __forceinline__ void load_tile(float* to, int pitch, const T* from, int64_t stride, int rows, int have) {
+template <int HD>
+__device__ __forceinline__ void load_tile(float* to, int pitch, const float* from, int64_t stride, int rows, int have) {
   constexpr int C = HD / 8;
   for (int i = threadIdx.x; i < rows * C; i += SP_THREADS) {
     const int r = i / C, c = i % C;
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (r < have) {
-      Raw8<T> raw;
+      Raw8<float> raw;
       raw.load(from + r * stride + c * 8);
       raw.get(x);
     }
@@ -118,7 +144,7 @@ __device__ __forceinline__ void load_tile(float* to, int pitch, const T* from, i
   }
 }
 
-template <typename T, int HD>
+template <int HD>
 __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const PromptArgs a) {
   constexpr int PITCH = HD + 4, PP = SP_KEYS + 4, NO = HD / 64;
   extern __shared__ __align__(16) float sp_smem[];
@@ -126,12 +152,12 @@ __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const Prom
   grid_dep_wait();
   grid_dep_launch();
   const int t = threadIdx.x, lane = t & 31, ty = t >> 4, tx = t & 15;
-  const T *q = static_cast<const T*>(a.q), *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v);
+  const float *q = static_cast<const float*>(a.q), *k = static_cast<const float*>(a.k), *v = static_cast<const float*>(a.v);
   const int G = a.heads / a.kv_heads;
   const float to_score = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E, cap2 = a.softcap * LOG2E;
   ItemWalk walk(a, lane);
   for (long long i = blockIdx.x;; i += gridDim.x) {
-    const Item it = walk.find(a, lane, i);
+    const Item it = walk.find(a, lane, SP_KEYS, i);
     if (!it.some) break;
     const Span qs = span_of(a.cu_q, it.seq, a.q_rows, nullptr), ks = span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, it.seq, a.k_rows, nullptr);
     const int tok0 = it.tile * a.tokens, toks = min(a.tokens, qs.len - tok0);
@@ -143,7 +169,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const Prom
       const int r = j / (HD / 8), c = j % (HD / 8);
       float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (r < rows) {
-        Raw8<T> raw;
+        Raw8<float> raw;
         raw.load(q + (static_cast<int64_t>(qs.begin) + tok0 + r / hs) * a.q_stride +
                  static_cast<int64_t>(it.kvh * G + h0 + r % hs) * HD + c * 8);
         raw.get(x);
@@ -164,7 +190,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const Prom
     for (int k0 = 0; k0 < keys; k0 += SP_KEYS) {
       const int have = min(SP_KEYS, keys - k0);
       __syncthreads();
-      load_tile<T, HD>(skv, PITCH, k + (static_cast<int64_t>(ks.begin) + k0) * a.k_stride + it.kvh * HD, a.k_stride, SP_KEYS, have);
+      load_tile<HD>(skv, PITCH, k + (static_cast<int64_t>(ks.begin) + k0) * a.k_stride + it.kvh * HD, a.k_stride, SP_KEYS, have);
       __syncthreads();
       float s[4][4] = {};
 #pragma unroll 4
@@ -185,7 +211,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const Prom
           }
       }
       __syncthreads();  // K is read: V takes its place
-      load_tile<T, HD>(skv, PITCH, v + (static_cast<int64_t>(ks.begin) + k0) * a.v_stride + it.kvh * HD, a.v_stride, SP_KEYS, have);
+      load_tile<HD>(skv, PITCH, v + (static_cast<int64_t>(ks.begin) + k0) * a.v_stride + it.kvh * HD, a.v_stride, SP_KEYS, have);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float top = -INFINITY;
@@ -263,23 +289,553 @@ __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const Prom
   zero_rest(a, HD, SP_THREADS);
 }
 
-template <typename T, int HD>
+template <int HD>
 int launch_prompt(PromptArgs& a, cudaStream_t st) {
   constexpr int SMEM = (2 * SP_ROWS * (HD + 4) + SP_ROWS * (SP_KEYS + 4)) * 4;
   const int G = a.heads / a.kv_heads;
   a.group = G < SP_ROWS ? G : SP_ROWS;
   a.parts = (G + a.group - 1) / a.group;
   a.tokens = SP_ROWS / a.group;
-  auto kern = prompt_attend_kernel<T, HD>;
+  a.splits = 1;
+  auto kern = prompt_attend_kernel<HD>;
   B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
   const int64_t items = (a.q_rows / a.tokens + a.bs) * a.kv_heads * a.parts + 1, resident = 2ll * sm_count();
   B200_CHECK_CUDA(launch_dependent(kern, dim3(static_cast<unsigned>(items < resident ? items : resident)), dim3(SP_THREADS), SMEM,
                                    st, a));
   return B200MOE_OK;
 }
+// ------------------------------------------------------------------ tensor cores
+// 16-bit rows: an item is two tiles of 128 rows, S = Q K^T and O += P V by tcgen05.mma with the
+// accumulators in tensor memory (S0, S1, O0, O1: all 512 columns at 128 elements a head).
+//   warps 0-3, 4-7  the softmax of tile 0, 1: a thread has a row.  S out of tensor memory, its
+//                   maximum, P = 2^(S - m) in the type of V back over S as the A operand of
+//                   the second product.  O is rescaled when the maximum has grown by more
+//                   than 2^8 (P stays below that), by the same threads.  The output at the end.
+//   warp 8          issues the MMAs: S0(0) S1(0) | P0V(j) S0(j+1) P1V(j) S1(j+1) ... : while one
+//                   tile's products run the other's softmax does.
+//   warp 9          loads: Q of an item, K and V tiles of 128 keys (128-byte swizzle; K is
+//                   K-major, V, whose keys are the reduction, MN-major)
+//   warp 10         looks at V tiles whose keys not all rows see: rows behind the sequence are
+//                   other data and become zeros, infinities and NaN too (a weight of zero does
+//                   not hide them from the product); where those are is noted, and they are
+//                   added at the end to the rows that see them.
+// Sums and statistics are fp32.  P is rounded to the type of V, as the output is after it.
+// An MMA reads P where a later one writes S: the tensor core executes a thread's MMAs in order.
+constexpr int TP_THREADS = 352, TP_ROWS = 128, TP_KEYS = 128, TP_SUB = 128 * 128;
+constexpr int TP_WARP_MMA = 8, TP_WARP_LOAD = 9, TP_WARP_CLEAN = 10;
+constexpr int TP_BAD = 4;  // items whose notes of bad values may be in use at once
+
+template <int HD>
+struct TpCfg {
+  static constexpr int SUBS = HD / 64, TILE = SUBS * TP_SUB;  // 128 rows of 64 elements each
+  static constexpr int OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_BAD = 6 * TILE, OFF_BAR = OFF_BAD + TP_BAD * 3 * HD * 4;
+  static constexpr int SMEM = 1024 + OFF_BAR + 256;
+  static_assert(SMEM <= 232448, "shared memory budget");
+};
+
+// V as the B operand: 64 elements a row of 128 bytes, eight keys 1024 bytes apart, the next 64
+// elements TP_SUB further.
+__device__ __forceinline__ uint64_t smem_desc_v(uint32_t addr) {
+  return smem_desc_sw128(addr) | static_cast<uint64_t>(TP_SUB >> 4) << 16;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tmap, int32_t x, int32_t y, int32_t z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+
+// What the roles of a CTA know of an item.
+struct Work {
+  int q0, toks, tok0;     // first row of q, tokens, first token of the item
+  int kvh, h0, hs;        // kv head; heads of its group: first, how many
+  int k0, begin, end;     // first row of k; keys of this item
+  int shift;              // token i sees keys up to i + shift
+  int n[2];               // tiles of keys of each tile of rows
+  int chunk, chunks;
+};
+__device__ __forceinline__ Work work_of(const PromptArgs& a, const Item& it) {
+  Work w;
+  const Span qs = span_of(a.cu_q, it.seq, a.q_rows, nullptr), ks = span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, it.seq, a.k_rows, nullptr);
+  const int G = a.heads / a.kv_heads, per = a.tokens / 2;
+  w.tok0 = it.tile * a.tokens;
+  w.toks = min(a.tokens, qs.len - w.tok0);
+  w.q0 = qs.begin + w.tok0;
+  w.kvh = it.kvh;
+  w.h0 = it.part * a.group;
+  w.hs = min(a.group, G - w.h0);
+  w.k0 = ks.begin;
+  w.shift = ks.len - qs.len;
+  const int keys = keys_seen(qs.len, ks.len, w.tok0, w.toks);
+  w.chunk = it.chunk;
+  w.chunks = a.splits == 1 ? 1 : chunks_of(keys, TP_KEYS, a.splits);
+  w.begin = w.chunks == 1 ? 0 : chunk_begin(keys, TP_KEYS, w.chunks, it.chunk);
+  w.end = w.chunks == 1 ? keys : min(keys, chunk_begin(keys, TP_KEYS, w.chunks, it.chunk + 1));
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int mine = min(per, w.toks - g * per);
+    const int last = mine > 0 ? min(w.end, keys_seen(qs.len, ks.len, w.tok0 + g * per, mine)) : 0;
+    w.n[g] = last > w.begin ? (last - w.begin + TP_KEYS - 1) / TP_KEYS : 0;
+  }
+  return w;
+}
+
 template <typename T>
-int launch_prompt_hd(PromptArgs& a, int hd, cudaStream_t st) {
-  return hd == 64 ? launch_prompt<T, 64>(a, st) : launch_prompt<T, 128>(a, st);
+__device__ __forceinline__ uint32_t pack16(float a, float b) { return pack2(static_cast<const T*>(nullptr), a, b); }
+
+template <typename T, int HD, bool CAP>
+__global__ void __launch_bounds__(TP_THREADS, 1)
+prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, const PromptArgs a) {
+  using C = TpCfg<HD>;
+  extern __shared__ uint8_t tp_smem[];
+  __shared__ int s_abort, s_any_bad[TP_BAD];
+  __shared__ uint32_t s_tmem;
+  const uint32_t base = (smem_u32(tp_smem) + 1023u) & ~1023u;
+  uint8_t* generic = tp_smem + (base - smem_u32(tp_smem));
+  int* s_bad = reinterpret_cast<int*>(generic + C::OFF_BAD);  // [item][NaN, +inf, -inf][element]: first key that has it
+  int nb = 0;
+  auto take = [&](int n) { const uint32_t b = base + C::OFF_BAR + 8u * nb; nb += n; return b; };
+  const uint32_t q_full = take(1), q_empty = take(1), k_full = take(2), k_empty = take(2), v_full = take(2), v_clean = take(2),
+                 v_empty = take(2), s_full = take(2), p_full = take(2), o_done = take(2), mma_done = take(1);
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  if (tid == 0) {
+    s_abort = 0;
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      for (const uint32_t b : {k_full, k_empty, v_full, v_clean, v_empty, s_full, o_done}) mbar_init(b + 8u * i, 1);
+      mbar_init(p_full + 8u * i, 4);  // one arrival per warp
+    }
+    mbar_init(mma_done, 1);
+    fence_mbar_init();
+  }
+  if (warp == TP_WARP_MMA) {
+    tmem_alloc(smem_u32(&s_tmem), 512);
+    tmem_relinquish();
+  }
+  grid_dep_wait();
+  grid_dep_launch();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  volatile int* abort_flag = &s_abort;
+  auto wait = [&](uint32_t bar, uint32_t n) { return mbar_wait_warp(bar, n & 1u, abort_flag, a.status); };  // for its phase n
+  const int per = a.tokens / 2, G = a.heads / a.kv_heads;
+  ItemWalk walk(a, lane);
+
+  if (warp == TP_WARP_LOAD) {
+    uint32_t items = 0, tiles = 0;
+    const uint32_t q_bytes = static_cast<uint32_t>(per * a.group) * HD * 2;
+    bool ok = true;
+    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+      const Item it = walk.find(a, lane, TP_KEYS, i);
+      if (!it.some) break;
+      const Work w = work_of(a, it);
+      const int n = max(w.n[0], w.n[1]);
+      if (n == 0) continue;
+      if (!(ok = wait(q_empty, items + 1))) break;
+      ++items;
+      if (elect_one()) {
+        const int both = w.n[1] > 0 ? 2 : 1;
+        mbar_expect_tx(q_full, both * q_bytes);
+        for (int g = 0; g < both; ++g)
+          for (int s = 0; s < C::SUBS; ++s)
+            tma_load_3d(base + g * C::TILE + s * TP_SUB, &tm_q, 64 * s, w.kvh * G + w.h0, w.q0 + g * per, q_full);
+      }
+      __syncwarp();
+      for (int j = 0; j < n; ++j) {
+        const uint32_t st = tiles & 1u, ph = tiles >> 1;
+        const int row = w.k0 + w.begin + j * TP_KEYS;
+        if (!(ok = wait(k_empty + 8u * st, ph + 1))) break;
+        if (elect_one()) {
+          mbar_expect_tx(k_full + 8u * st, C::TILE);
+          for (int s = 0; s < C::SUBS; ++s)
+            tma_load_3d(base + C::OFF_K + st * C::TILE + s * TP_SUB, &tm_k, 64 * s, w.kvh, row, k_full + 8u * st);
+        }
+        __syncwarp();
+        if (!(ok = wait(v_empty + 8u * st, ph + 1))) {  // V of this tile is not loaded: nobody waits for it any more
+          if (elect_one()) mbar_drain(k_full + 8u * st, ph & 1u, a.status);
+          __syncwarp();
+          break;
+        }
+        if (elect_one()) {
+          mbar_expect_tx(v_full + 8u * st, C::TILE);
+          for (int s = 0; s < C::SUBS; ++s)
+            tma_load_3d(base + C::OFF_V + st * C::TILE + s * TP_SUB, &tm_v, 64 * s, w.kvh, row, v_full + 8u * st);
+        }
+        __syncwarp();
+        ++tiles;
+      }
+    }
+    // do not leave while copies may still land in this CTA's shared memory
+    if (elect_one()) {
+      if (items > 0) mbar_drain(q_full, (items - 1) & 1u, a.status);
+      for (uint32_t i = tiles > 2 ? tiles - 2 : 0; i < tiles; ++i) {
+        mbar_drain(k_full + 8u * (i & 1u), (i >> 1) & 1u, a.status);
+        mbar_drain(v_full + 8u * (i & 1u), (i >> 1) & 1u, a.status);
+      }
+    }
+    __syncwarp();
+  } else if (warp == TP_WARP_MMA) {
+    constexpr uint32_t format = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+    constexpr uint32_t idesc_s = (1u << 4) | format | (TP_KEYS / 8u) << 17 | (TP_ROWS / 16u) << 24;
+    constexpr uint32_t idesc_o = (1u << 4) | format | 1u << 16 | (HD / 8u) << 17 | (TP_ROWS / 16u) << 24;  // B is MN-major
+    uint32_t items = 0, tiles = 0, given[2] = {0, 0};  // P tiles taken of each tile of rows
+    bool ok = true;
+    auto scores = [&](int g, uint32_t st) {
+      if (elect_one()) {
+        const uint64_t q = smem_desc_sw128(base + g * C::TILE), k = smem_desc_sw128(base + C::OFF_K + st * C::TILE);
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s) {
+          const uint64_t step = (s / 4) * (TP_SUB >> 4) + (s % 4) * 2;
+          mma_ss(tmem + g * TP_KEYS, q + step, k + step, idesc_s, s > 0);
+        }
+        tc_commit(s_full + 8u * g);
+      }
+      __syncwarp();
+    };
+    auto values = [&](int g, uint32_t st, bool first) {
+      if (elect_one()) {
+        const uint64_t v = smem_desc_v(base + C::OFF_V + st * C::TILE);
+#pragma unroll
+        for (int s = 0; s < TP_KEYS / 16; ++s)
+          mma_ts(tmem + 2 * TP_KEYS + g * HD, tmem + g * TP_KEYS + s * 8, v + s * (2048 >> 4), idesc_o, !first || s > 0);
+        tc_commit(o_done + 8u * g);
+      }
+      __syncwarp();
+    };
+    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+      const Item it = walk.find(a, lane, TP_KEYS, i);
+      if (!it.some) break;
+      const Work w = work_of(a, it);
+      const int n = max(w.n[0], w.n[1]);
+      if (n == 0) continue;
+      ok = wait(q_full, items) && wait(k_full + 8u * (tiles & 1u), tiles >> 1);
+      if (!ok) break;
+      ++items;
+      tc_fence_after();
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (w.n[g] > 0) scores(g, tiles & 1u);
+      if (elect_one()) tc_commit(k_empty + 8u * (tiles & 1u));
+      if (n == 1 && elect_one()) tc_commit(q_empty);
+      __syncwarp();
+      for (int j = 0; j < n && ok; ++j, ++tiles) {
+        const uint32_t st = tiles & 1u, next = (tiles + 1) & 1u;
+        ok = wait(v_full + 8u * st, tiles >> 1) && wait(v_clean + 8u * st, tiles >> 1);
+        if (ok && j + 1 < n) ok = wait(k_full + 8u * next, (tiles + 1) >> 1);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (!ok) break;
+          if (j < w.n[g]) {
+            if (!(ok = wait(p_full + 8u * g, given[g]))) break;
+            ++given[g];
+            tc_fence_after();
+            values(g, st, j == 0);
+          }
+          if (j + 1 < w.n[g]) scores(g, next);
+        }
+        if (ok && elect_one()) {
+          tc_commit(v_empty + 8u * st);
+          if (j + 1 < n) tc_commit(k_empty + 8u * next);
+          if (j + 2 == n) tc_commit(q_empty);
+        }
+        __syncwarp();
+      }
+    }
+    // after a wait that ran out nobody else waits for the last MMAs
+    if (elect_one()) tc_commit(mma_done);
+    __syncwarp();
+    mbar_drain(mma_done, 0, a.status);
+  } else if (warp == TP_WARP_CLEAN) {
+    constexpr uint32_t INF = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+    uint32_t items = 0, tiles = 0;
+    bool ok = true;
+    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+      const Item it = walk.find(a, lane, TP_KEYS, i);
+      if (!it.some) break;
+      const Work w = work_of(a, it);
+      const int n = max(w.n[0], w.n[1]);
+      if (n == 0) continue;
+      int* bad = s_bad + (items % TP_BAD) * 3 * HD;
+      bool fresh = true;
+      for (int j = 0; j < n; ++j, ++tiles) {
+        const uint32_t st = tiles & 1u;
+        if (!(ok = wait(v_full + 8u * st, tiles >> 1))) break;
+        const int first = w.begin + j * TP_KEYS;
+        if (first + TP_KEYS > w.tok0 + w.shift + 1) {
+          if (fresh) {
+            for (int e = lane; e < 3 * HD; e += 32) bad[e] = 0x7fffffff;
+            if (lane == 0) s_any_bad[items % TP_BAD] = 0;
+            fresh = false;
+            __syncwarp();
+          }
+          const int have = min(TP_KEYS, w.end - first);
+          const uint32_t tile = base + C::OFF_V + st * C::TILE;
+          uint32_t top = 0;
+          for (int s = 0; s < C::SUBS; ++s) {
+            const int full = have * 8;  // 16-byte pieces of the rows there are
+#pragma unroll 8
+            for (int e = lane; e < full; e += 32) {
+              uint32_t x[4];
+              lds128(tile + s * TP_SUB + e * 16, x);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) top = __vmaxu2(top, x[k] & 0x7fff7fffu);
+            }
+            const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+            for (int e = full + lane; e < TP_KEYS * 8; e += 32) sts128(tile + s * TP_SUB + e * 16, zero);
+          }
+          if (__any_sync(0xffffffffu, (top & 0xffffu) >= INF || (top >> 16) >= INF)) {
+            uint16_t* v = reinterpret_cast<uint16_t*>(generic + C::OFF_V + st * C::TILE);
+            for (int e = lane; e < have * HD; e += 32) {
+              const int row = e / HD, d = e % HD;
+              uint16_t* at = v + (d / 64) * (TP_SUB / 2) + row * 64 + ((d % 64 / 8) ^ (row & 7)) * 8 + d % 8;
+              const uint32_t x = *at, mag = x & 0x7fffu;
+              if (mag < INF) continue;
+              atomicMin(bad + (mag > INF ? 0 : x & 0x8000u ? 2 : 1) * HD + d, first + row);
+              *at = 0;
+            }
+            if (lane == 0) s_any_bad[items % TP_BAD] = 1;
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_clean + 8u * st);
+      }
+      ++items;
+    }
+  } else {
+    const int g = warp >> 2, row = (warp & 3) * 32 + lane;  // tile; row of it and lane of tensor memory
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, s_at = tmem + lanes + g * TP_KEYS, o_at = tmem + lanes + 2 * TP_KEYS + g * HD;
+    const float by = CAP ? fabsf(a.scale) / a.softcap * 2.f * LOG2E : fabsf(a.scale) * LOG2E, cap2 = a.softcap * LOG2E;
+    const uint32_t flip = a.scale < 0.f ? 0x80000000u : 0u;
+    uint32_t items = 0, tiles = 0;  // items with keys; S tiles taken
+    bool ok = true;
+    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+      const Item it = walk.find(a, lane, TP_KEYS, i);
+      if (!it.some) break;
+      const Work w = work_of(a, it);
+      const int tok = row / a.group, h = row - tok * a.group, mine = g * per + tok;
+      const bool live = tok < per && mine < w.toks && h < w.hs;
+      const int seen = w.tok0 + mine + w.shift + 1;        // keys that this row sees
+      const int all_see = w.tok0 + g * per + w.shift + 1;  // that all rows of the tile see
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < w.n[g]; ++j, ++tiles) {
+        if (!(ok = wait(s_full + 8u * g, tiles))) break;
+        tc_fence_after();
+        // twice through S, 64 and 32 columns at a time: its maximum, then the weights
+        const int first = w.begin + j * TP_KEYS, some = first + TP_KEYS > all_see ? seen - first : TP_KEYS;
+        const bool masked = first + TP_KEYS > all_see;
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          uint32_t v[2][32];
+          tmem_ld32(s_at + 32 * c, v[0]);
+          tmem_ld32(s_at + 32 * c + 32, v[1]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            float x = __uint_as_float(v[e / 32][e % 32] ^ flip);
+            if (masked && 32 * c + e >= some) x = -INFINITY;
+            top[e % 4] = fmaxf(top[e % 4], x);
+          }
+        }
+        float up = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * by;
+        if constexpr (CAP) up = up == -INFINITY ? up : fmaf(-2.f * cap2, rcp(ex2(up) + 1.f), cap2);
+        if (j == 0) {
+          m = up;
+        } else if (__any_sync(0xffffffffu, up > m + 8.f)) {
+          const float m_new = fmaxf(m, up), alpha = m_new == -INFINITY ? 1.f : ex2(m - m_new);
+          m = m_new;
+          l *= alpha;
+          if (!(ok = wait(o_done + 8u * g, tiles - 1))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_at + 32 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(o_at + 32 * c, o);
+          }
+        }
+        const float base2 = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32], p[16];
+          tmem_ld32(s_at + 32 * c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float x[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float y = __uint_as_float(v[e + k] ^ flip);
+              if constexpr (CAP) x[k] = fmaf(-2.f * cap2, rcp(ex2(y * by) + 1.f), cap2 - base2);
+              else x[k] = fmaf(y, by, -base2);
+              x[k] = masked && 32 * c + e + k >= some ? 0.f : ex2(x[k]);
+            }
+            sum[e / 2 % 4] += x[0] + x[1];
+            p[e / 2] = pack16<T>(x[0], x[1]);
+          }
+          tmem_st16(s_at + 16 * c, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 8u * g);
+      }
+      if (!ok) break;
+      const int n = max(w.n[0], w.n[1]);
+      if (w.n[g] > 0 && !(ok = wait(o_done + 8u * g, tiles - 1))) break;
+      tc_fence_after();
+      // the last tile of keys is one that was looked at: before it the notes may be older ones
+      const bool any_bad = w.n[g] > 0 && w.begin + w.n[g] * TP_KEYS > w.tok0 + w.shift + 1 && s_any_bad[items % TP_BAD] != 0;
+      const int* bad = s_bad + (items % TP_BAD) * 3 * HD;
+      const float f = w.chunks > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      const int64_t at = (static_cast<int64_t>(w.q0) + mine) * a.heads + w.kvh * G + w.h0 + h;
+      float* part = a.partial + (at * a.splits + w.chunk) * (HD + 4);
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t o[32];
+        if (w.n[g] > 0) {
+          tmem_ld32(o_at + 32 * c, o);
+          tmem_wait_ld();
+        }
+        if (live) {
+          float x[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            x[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * f;
+            if (any_bad) {
+              const int d = 32 * c + e;
+              if (bad[d] < seen) x[e] = __int_as_float(0x7fffffff);
+              if (bad[HD + d] < seen) x[e] += INFINITY;
+              if (bad[2 * HD + d] < seen) x[e] -= INFINITY;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = x[e + k];
+            if (w.chunks > 1) store8(part + 32 * c + e, y);
+            else if (a.out_dtype == B200MOE_DT_F32) store8(static_cast<float*>(a.out) + at * HD + 32 * c + e, y);
+            else if (a.out_dtype == B200MOE_DT_F16) store8(static_cast<__half*>(a.out) + at * HD + 32 * c + e, y);
+            else store8(static_cast<__nv_bfloat16*>(a.out) + at * HD + 32 * c + e, y);
+          }
+        }
+        __syncwarp();  // the next load of tensor memory is the whole warp's
+      }
+      if (w.chunks > 1 && live) *reinterpret_cast<float2*>(part + HD) = make_float2(m, l);
+      if (n > 0) ++items;
+    }
+  }
+  zero_rest(a, HD, TP_THREADS);
+  // everyone is done with tensor memory before it is freed
+  tc_fence_before();
+  __syncthreads();
+  if (warp == TP_WARP_MMA) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of the rows whose keys were split: a warp per row and head.
+template <int HD>
+__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptArgs a) {
+  constexpr int N = HD / 32;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t row = at / a.heads;
+  if (row >= a.q_rows) return;
+  int chunks = 0;
+  for (int b0 = 0; b0 < a.bs; b0 += 32) {
+    const int b = b0 + lane;
+    const Span qs = b < a.bs ? span_of(a.cu_q, b, a.q_rows, nullptr) : Span{0, 0};
+    const bool here = row >= qs.begin && row < qs.begin + qs.len;
+    const unsigned who = __ballot_sync(0xffffffffu, here);
+    if (who == 0) continue;
+    const int own = here ? ItemWalk::chunks(a, b, static_cast<int>(row - qs.begin) / a.tokens, TP_KEYS) : 0;
+    chunks = __shfl_sync(0xffffffffu, own, __ffs(who) - 1);
+    break;
+  }
+  if (chunks <= 1) return;  // the output is there
+  const float* part = a.partial + at * a.splits * (HD + 4);
+  float top = -INFINITY, den = 0.f, acc[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  for (int c = 0; c < chunks; ++c) top = fmaxf(top, part[c * (HD + 4) + HD]);
+  for (int c = 0; c < chunks; ++c) {
+    float v[N];
+    load_elems(part + c * (HD + 4) + lane * N, v);
+    const float2 ml = *reinterpret_cast<const float2*>(part + c * (HD + 4) + HD);
+    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+    den = fmaf(ml.y, f, den);
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] += ml.x == -INFINITY ? 0.f : v[j] * f;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = den == 0.f ? 0.f : acc[j] / den;
+  store_as(a.out, a.out_dtype, static_cast<size_t>(at) * HD + lane * N, acc);
+}
+
+template <typename T, int HD, bool CAP>
+int launch_prompt_tc(const PromptArgs& a, cudaStream_t st) {
+  CUtensorMap q, k, v;
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  if (const int rc = make_tmap_heads(&q, a.q, bf16, a.q_rows, a.heads, HD, a.q_stride, a.tokens / 2, a.group)) return rc;
+  if (const int rc = make_tmap_heads(&k, a.k, bf16, a.k_rows, a.kv_heads, HD, a.k_stride, TP_KEYS, 1)) return rc;
+  if (const int rc = make_tmap_heads(&v, a.v, bf16, a.k_rows, a.kv_heads, HD, a.v_stride, TP_KEYS, 1)) return rc;
+  auto kern = prompt_attend_tc_kernel<T, HD, CAP>;
+  static bool configured[16] = {};
+  int dev = 0;
+  B200_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev >= 16 || !configured[dev]) {
+    B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TpCfg<HD>::SMEM));
+    if (dev < 16) configured[dev] = true;
+  }
+  const int64_t items = (a.q_rows / a.tokens + a.bs) * a.kv_heads * a.parts * a.splits + 1, sms = sm_count();
+  B200_CHECK_CUDA(launch_dependent(kern, dim3(static_cast<unsigned>(items < sms ? items : sms)), dim3(TP_THREADS), TpCfg<HD>::SMEM, st,
+                                   q, k, v, a));
+  if (a.splits > 1)
+    B200_CHECK_CUDA(launch_dependent(prompt_merge_kernel<HD>, dim3(static_cast<unsigned>((a.q_rows * a.heads + 7) / 8)), dim3(256), 0, st, a));
+  return B200MOE_OK;
+}
+template <typename T>
+int launch_prompt_tc_hd(const PromptArgs& a, int hd, cudaStream_t st) {
+  if (a.softcap > 0.f) return hd == 64 ? launch_prompt_tc<T, 64, true>(a, st) : launch_prompt_tc<T, 128, true>(a, st);
+  return hd == 64 ? launch_prompt_tc<T, 64, false>(a, st) : launch_prompt_tc<T, 128, false>(a, st);
+}
+
+// The shape of a call's items on the tensor cores.
+struct PromptPlan { int group, parts, tokens, splits; };
+PromptPlan plan_prompt(int64_t q_rows, int64_t k_rows, int bs, int heads, int kv_heads) {
+  PromptPlan p;
+  const int G = heads / kv_heads;
+  p.group = G < TP_ROWS ? G : TP_ROWS;
+  p.parts = (G + p.group - 1) / p.group;
+  p.tokens = 2 * (TP_ROWS / p.group);
+  p.splits = 1;
+  return p;
 }
 
 }  // namespace
@@ -317,9 +873,14 @@ int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype
   a.status = device_status_ptr();
   if (a.status == nullptr) return B200MOE_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == B200MOE_DT_F32) return launch_prompt_hd<float>(a, head_dim, st);
-  if (dtype == B200MOE_DT_F16) return launch_prompt_hd<__half>(a, head_dim, st);
-  return launch_prompt_hd<__nv_bfloat16>(a, head_dim, st);
+  if (dtype == B200MOE_DT_F32) return head_dim == 64 ? launch_prompt<64>(a, st) : launch_prompt<128>(a, st);
+  if (k_rows == 0) {
+    B200_CHECK_CUDA(cudaMemsetAsync(out, 0, static_cast<size_t>(q_rows) * heads * head_dim * dt_bytes(out_dtype), st));
+    return B200MOE_OK;
+  }
+  const PromptPlan p = plan_prompt(q_rows, k_rows, bs, heads, kv_heads);
+  a.group = p.group; a.parts = p.parts; a.tokens = p.tokens; a.splits = p.splits;
+  return dtype == B200MOE_DT_F16 ? launch_prompt_tc_hd<__half>(a, head_dim, st) : launch_prompt_tc_hd<__nv_bfloat16>(a, head_dim, st);
 }
 
 }  // extern "C"
