@@ -55,43 +55,47 @@ __device__ __forceinline__ int chunk_begin(int keys, int step, int chunks, int i
 }
 // The list of items, walked by a whole warp with rising indices.
 struct ItemWalk {
-  int t;         // tiles with this place in their sequence are current
+  int t;             // tiles with this place in their sequence are current
   long long before;  // items before them
-  __device__ __forceinline__ static int tiles_of(const PromptArgs& a, int b) {
-    return b < a.bs ? (span_of(a.cu_q, b, a.q_rows, nullptr).len + a.tokens - 1) / a.tokens : 0;
+  int n, m;          // rows of q and k of sequence `lane`
+  __device__ __forceinline__ static void lengths(const PromptArgs& a, int b, int& n, int& m) {
+    n = b < a.bs ? span_of(a.cu_q, b, a.q_rows, nullptr).len : 0;
+    m = b < a.bs ? span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, b, a.k_rows, nullptr).len : 0;
   }
   __device__ __forceinline__ ItemWalk(const PromptArgs& a, int lane) : t(0), before(0) {
-    int most = 0;
-    int32_t* status = blockIdx.x == 0 && threadIdx.x < 32 ? a.status : nullptr;
-    for (int b = lane; b < a.bs; b += 32) {
-      most = max(most, tiles_of(a, b));
-      if (status != nullptr) {
-        span_of(a.cu_q, b, a.q_rows, status);
-        if (a.cu_k != nullptr) span_of(a.cu_k, b, a.k_rows, status);
-      }
-    }
+    lengths(a, lane, n, m);
+    int most = (n + a.tokens - 1) / a.tokens;
+    for (int b = lane + 32; b < a.bs; b += 32) most = max(most, (span_of(a.cu_q, b, a.q_rows, nullptr).len + a.tokens - 1) / a.tokens);
     t = __reduce_max_sync(0xffffffffu, most) - 1;
+    if (blockIdx.x == 0)
+      for (int b = lane; b < a.bs; b += 32) {
+        span_of(a.cu_q, b, a.q_rows, a.status);
+        if (a.cu_k != nullptr) span_of(a.cu_k, b, a.k_rows, a.status);
+      }
   }
-  // items of sequence b with tile t, apart from heads
-  __device__ __forceinline__ static int chunks(const PromptArgs& a, int b, int t, int step) {
-    if (b >= a.bs) return 0;
-    const int n = span_of(a.cu_q, b, a.q_rows, nullptr).len, tok0 = t * a.tokens;
+  // items of a sequence of n and m rows with tile t, apart from heads
+  __device__ __forceinline__ static int chunks(const PromptArgs& a, int n, int m, int t, int step) {
+    const int tok0 = t * a.tokens;
     if (tok0 >= n) return 0;
-    if (a.splits == 1) return 1;
-    const int m = span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, b, a.k_rows, nullptr).len;
-    return chunks_of(keys_seen(n, m, tok0, min(a.tokens, n - tok0)), step, a.splits);
+    return a.splits == 1 ? 1 : chunks_of(keys_seen(n, m, tok0, min(a.tokens, n - tok0)), step, a.splits);
   }
   __device__ __forceinline__ Item find(const PromptArgs& a, int lane, int step, long long i) {
     const int each = a.kv_heads * a.parts;
     for (; t >= 0; --t) {
       long long at = before;
       for (int b0 = 0; b0 < a.bs; b0 += 32) {
-        const int own = chunks(a, b0 + lane, t, step);
+        int nb = n, mb = m;
+        if (a.bs > 32) lengths(a, b0 + lane, nb, mb);
+        const int own = chunks(a, nb, mb, t, step);
         int sum = own;
+        if (a.splits == 1) {
+          sum = __popc(__ballot_sync(0xffffffffu, own) & (0xffffffffu >> (31 - lane)));
+        } else {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += up;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+          }
         }
         const int all = __shfl_sync(0xffffffffu, sum, 31);
         if (i < at + static_cast<long long>(all) * each) {
@@ -107,6 +111,10 @@ struct ItemWalk {
     return {0, 0, 0, 0, 0, false};
   }
 };
+// The r-th item of a CTA: there and back through the CTAs, so that none gets the largest of every round.
+__device__ __forceinline__ long long item_of(long long r) {
+  return r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
 
 // Rows of no sequence are zeros.
 template <typename T>
@@ -156,8 +164,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const Prom
   const int G = a.heads / a.kv_heads;
   const float to_score = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E, cap2 = a.softcap * LOG2E;
   ItemWalk walk(a, lane);
-  for (long long i = blockIdx.x;; i += gridDim.x) {
-    const Item it = walk.find(a, lane, SP_KEYS, i);
+  for (long long r = 0;; ++r) {
+    const Item it = walk.find(a, lane, SP_KEYS, item_of(r));
     if (!it.some) break;
     const Span qs = span_of(a.cu_q, it.seq, a.q_rows, nullptr), ks = span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, it.seq, a.k_rows, nullptr);
     const int tok0 = it.tile * a.tokens, toks = min(a.tokens, qs.len - tok0);
@@ -311,25 +319,27 @@ int launch_prompt(PromptArgs& a, cudaStream_t st) {
 //                   maximum, P = 2^(S - m) in the type of V back over S as the A operand of
 //                   the second product.  O is rescaled when the maximum has grown by more
 //                   than 2^8 (P stays below that), by the same threads.  The output at the end.
-//   warp 8          issues the MMAs: S0(0) S1(0) | P0V(j) S0(j+1) P1V(j) S1(j+1) ... : while one
-//                   tile's products run the other's softmax does.
-//   warp 9          loads: Q of an item, K and V tiles of 128 keys (128-byte swizzle; K is
-//                   K-major, V, whose keys are the reduction, MN-major)
-//   warp 10         looks at V tiles whose keys not all rows see: rows behind the sequence are
+//   warps 8, 9      issue the MMAs of tile 0, 1: S(0), then PV(j), S(j + 1) ...; while one tile's
+//                   products run the other's softmax does.
+//   warp 10         makes the list of items and loads: Q of an item, K and V tiles of 128 keys
+//                   (128-byte swizzle; K is K-major, V, whose keys are the reduction, MN-major)
+//   warp 11         looks at V tiles whose keys not all rows see: rows behind the sequence are
 //                   other data and become zeros, infinities and NaN too (a weight of zero does
 //                   not hide them from the product); where those are is noted, and they are
 //                   added at the end to the rows that see them.
 // Sums and statistics are fp32.  P is rounded to the type of V, as the output is after it.
 // An MMA reads P where a later one writes S: the tensor core executes a thread's MMAs in order.
-constexpr int TP_THREADS = 352, TP_ROWS = 128, TP_KEYS = 128, TP_SUB = 128 * 128;
-constexpr int TP_WARP_MMA = 8, TP_WARP_LOAD = 9, TP_WARP_CLEAN = 10;
-constexpr int TP_BAD = 4;  // items whose notes of bad values may be in use at once
+constexpr int TP_THREADS = 384, TP_ROWS = 128, TP_KEYS = 128, TP_SUB = 128 * 128;
+constexpr int TP_WARP_MMA = 8, TP_WARP_LOAD = 10, TP_WARP_CLEAN = 11;
+constexpr int TP_BAD = 4;   // items whose notes of bad values may be in use at once
+constexpr int TP_WORK = 4;  // items whose descriptions may be in use at once
 
 template <int HD>
 struct TpCfg {
   static constexpr int SUBS = HD / 64, TILE = SUBS * TP_SUB;  // 128 rows of 64 elements each
-  static constexpr int OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_BAD = 6 * TILE, OFF_BAR = OFF_BAD + TP_BAD * 3 * HD * 4;
-  static constexpr int SMEM = 1024 + OFF_BAR + 256;
+  static constexpr int OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_OUT = 6 * TILE, OFF_BAD = OFF_OUT + 8 * 2048;
+  static constexpr int OFF_WORK = OFF_BAD + TP_BAD * 3 * HD * 4, OFF_BAR = OFF_WORK + TP_WORK * 64;
+  static constexpr int SMEM = 1024 + OFF_BAR + 320;
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
@@ -358,13 +368,16 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tma
 
 // What the roles of a CTA know of an item.
 struct Work {
-  int q0, toks, tok0;     // first row of q, tokens, first token of the item
+  int q0, toks, tok0;     // first row of q, tokens (-1: no item, the list has ended), first token of the item
   int kvh, h0, hs;        // kv head; heads of its group: first, how many
   int k0, begin, end;     // first row of k; keys of this item
   int shift;              // token i sees keys up to i + shift
   int n[2];               // tiles of keys of each tile of rows
   int chunk, chunks;
+  int unused[2];
+  __device__ __forceinline__ int tiles() const { return max(n[0], n[1]); }
 };
+static_assert(sizeof(Work) == 64, "four 16-byte words");
 __device__ __forceinline__ Work work_of(const PromptArgs& a, const Item& it) {
   Work w;
   const Span qs = span_of(a.cu_q, it.seq, a.q_rows, nullptr), ks = span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, it.seq, a.k_rows, nullptr);
@@ -391,8 +404,72 @@ __device__ __forceinline__ Work work_of(const PromptArgs& a, const Item& it) {
   return w;
 }
 
+// two fp32 numbers of one 64-bit register, and their arithmetic
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// NaN where one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float a, float b) { return pack2(static_cast<const T*>(nullptr), a, b); }
+
+// 2^x for x <= 2^7 by the fp32 units: 2^n 2^f, n the nearest integer and |f| <= 1/2, 2^f by a
+// polynomial of degree 4 (minimax, off by 2^-18.5, an eightieth of half a step of fp16).
+__device__ __forceinline__ void ex2_pair(uint64_t v, float& x, float& y) {
+  constexpr float BIG = 12582912.f;  // 1.5 * 2^23: n in the last places
+  unpair(v, x, y);
+  v = pair(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const uint64_t t = add2(v, pair(BIG, BIG)), f = fma2(add2(t, pair(-BIG, -BIG)), pair(-1.f, -1.f), v);
+  uint64_t p = fma2(f, pair(0.009570096619427204f, 0.009570096619427204f), pair(0.05591786280274391f, 0.05591786280274391f));
+  p = fma2(f, p, pair(0.240247443318367f, 0.240247443318367f));
+  p = fma2(f, p, pair(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(f, p, pair(0.9999992847442627f, 0.9999992847442627f));
+  float tx, ty;
+  unpair(t, tx, ty);
+  unpair(p, x, y);
+  x = __uint_as_float(__float_as_uint(x) + (__float_as_uint(tx) << 23));
+  y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
+}
+// tanh(z) / z for |z| <= 1 as a polynomial in z^2 (minimax, off by 2^-20.7)
+__device__ __forceinline__ uint64_t tanh_pair(uint64_t z) {
+  const uint64_t u = mul2(z, z);
+  uint64_t p = fma2(u, pair(-0.0030670491978526115f, -0.0030670491978526115f), pair(0.016743090003728867f, 0.016743090003728867f));
+  p = fma2(u, p, pair(-0.05160565301775932f, -0.05160565301775932f));
+  p = fma2(u, p, pair(0.13281433284282684f, 0.13281433284282684f));
+  p = fma2(u, p, pair(-0.3332904279232025f, -0.3332904279232025f));
+  return fma2(u, p, pair(0.9999994039535522f, 0.9999994039535522f));
+}
+// Of 16 pairs of weights, how many the fp32 units compute: the special-function unit's 16 a
+// clock are as many as the MMAs need clocks for.
+constexpr int TP_POLY = 5;
 
 template <typename T, int HD, bool CAP>
 __global__ void __launch_bounds__(TP_THREADS, 1)
@@ -405,20 +482,26 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   const uint32_t base = (smem_u32(tp_smem) + 1023u) & ~1023u;
   uint8_t* generic = tp_smem + (base - smem_u32(tp_smem));
   int* s_bad = reinterpret_cast<int*>(generic + C::OFF_BAD);  // [item][NaN, +inf, -inf][element]: first key that has it
+  Work* s_work = reinterpret_cast<Work*>(generic + C::OFF_WORK);
   int nb = 0;
   auto take = [&](int n) { const uint32_t b = base + C::OFF_BAR + 8u * nb; nb += n; return b; };
   const uint32_t q_full = take(1), q_empty = take(1), k_full = take(2), k_empty = take(2), v_full = take(2), v_clean = take(2),
-                 v_empty = take(2), s_full = take(2), p_full = take(2), o_done = take(2), mma_done = take(1);
+                 v_empty = take(2), s_full = take(2), p_full = take(4), o_done = take(2), mma_done = take(2), w_full = take(TP_WORK),
+                 w_empty = take(TP_WORK);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     s_abort = 0;
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     for (int i = 0; i < 2; ++i) {
-      for (const uint32_t b : {k_full, k_empty, v_full, v_clean, v_empty, s_full, o_done}) mbar_init(b + 8u * i, 1);
-      mbar_init(p_full + 8u * i, 4);  // one arrival per warp
+      for (const uint32_t b : {k_full, v_full, v_clean, s_full, o_done, mma_done}) mbar_init(b + 8u * i, 1);
+      for (const uint32_t b : {k_empty, v_empty}) mbar_init(b + 8u * i, 2);                    // both issuers
+      for (const uint32_t b : {p_full, p_full + 16u}) mbar_init(b + 8u * i, 4);                // one arrival per warp
     }
-    mbar_init(mma_done, 1);
+    for (int i = 0; i < TP_WORK; ++i) {
+      mbar_init(w_full + 8u * i, 1);
+      mbar_init(w_empty + 8u * i, 11);  // all warps but the list's own
+    }
     fence_mbar_init();
   }
   if (warp == TP_WARP_MMA) {
@@ -433,228 +516,268 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
   auto wait = [&](uint32_t bar, uint32_t n) { return mbar_wait_warp(bar, n & 1u, abort_flag, a.status); };  // for its phase n
+  // item i of this CTA; false: there is none
+  auto next_work = [&](uint32_t i, Work& w) {
+    if (!wait(w_full + 8u * (i % TP_WORK), i / TP_WORK)) return false;
+    w = s_work[i % TP_WORK];
+    return w.toks >= 0;
+  };
+  auto done_work = [&](uint32_t i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(w_empty + 8u * (i % TP_WORK));
+  };
   const int per = a.tokens / 2, G = a.heads / a.kv_heads;
-  ItemWalk walk(a, lane);
 
-  if (warp == TP_WARP_LOAD) {
-    uint32_t items = 0, tiles = 0;
-    const uint32_t q_bytes = static_cast<uint32_t>(per * a.group) * HD * 2;
-    bool ok = true;
-    for (long long i = blockIdx.x; ok; i += gridDim.x) {
-      const Item it = walk.find(a, lane, TP_KEYS, i);
-      if (!it.some) break;
-      const Work w = work_of(a, it);
-      const int n = max(w.n[0], w.n[1]);
-      if (n == 0) continue;
-      if (!(ok = wait(q_empty, items + 1))) break;
-      ++items;
-      if (elect_one()) {
-        const int both = w.n[1] > 0 ? 2 : 1;
-        mbar_expect_tx(q_full, both * q_bytes);
-        for (int g = 0; g < both; ++g)
-          for (int s = 0; s < C::SUBS; ++s)
-            tma_load_3d(base + g * C::TILE + s * TP_SUB, &tm_q, 64 * s, w.kvh * G + w.h0, w.q0 + g * per, q_full);
-      }
-      __syncwarp();
-      for (int j = 0; j < n; ++j) {
-        const uint32_t st = tiles & 1u, ph = tiles >> 1;
-        const int row = w.k0 + w.begin + j * TP_KEYS;
-        if (!(ok = wait(k_empty + 8u * st, ph + 1))) break;
-        if (elect_one()) {
-          mbar_expect_tx(k_full + 8u * st, C::TILE);
-          for (int s = 0; s < C::SUBS; ++s)
-            tma_load_3d(base + C::OFF_K + st * C::TILE + s * TP_SUB, &tm_k, 64 * s, w.kvh, row, k_full + 8u * st);
+  // registers: 384 x 168 at launch = 128 x 88 + 256 x 208
+  if (warp >= TP_WARP_MMA) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == TP_WARP_LOAD) {
+      uint32_t loads = 0, tiles = 0;
+      const uint32_t q_bytes = static_cast<uint32_t>(per * a.group) * HD * 2;
+      ItemWalk walk(a, lane);
+      bool ok = true;
+      for (uint32_t i = 0; ok; ++i) {
+        const Item it = walk.find(a, lane, TP_KEYS, item_of(i));
+        Work w;
+        if (it.some) w = work_of(a, it);
+        else w.toks = -1;
+        if (!(ok = wait(w_empty + 8u * (i % TP_WORK), i / TP_WORK + 1))) break;
+        if (lane == 0) {
+          s_work[i % TP_WORK] = w;
+          mbar_arrive(w_full + 8u * (i % TP_WORK));
         }
         __syncwarp();
-        if (!(ok = wait(v_empty + 8u * st, ph + 1))) {  // V of this tile is not loaded: nobody waits for it any more
-          if (elect_one()) mbar_drain(k_full + 8u * st, ph & 1u, a.status);
+        if (!it.some) break;
+        const int n = w.tiles();
+        if (n == 0) continue;
+        if (!(ok = wait(q_empty, loads + 1))) break;
+        ++loads;
+        if (elect_one()) {
+          const int both = w.n[1] > 0 ? 2 : 1;
+          mbar_expect_tx(q_full, both * q_bytes);
+          for (int g = 0; g < both; ++g)
+            for (int s = 0; s < C::SUBS; ++s)
+              tma_load_3d(base + g * C::TILE + s * TP_SUB, &tm_q, 64 * s, w.kvh * G + w.h0, w.q0 + g * per, q_full);
+        }
+        __syncwarp();
+        for (int j = 0; j < n; ++j) {
+          const uint32_t st = tiles & 1u, ph = tiles >> 1;
+          const int row = w.k0 + w.begin + j * TP_KEYS;
+          if (!(ok = wait(k_empty + 8u * st, ph + 1))) break;
+          if (elect_one()) {
+            mbar_expect_tx(k_full + 8u * st, C::TILE);
+            for (int s = 0; s < C::SUBS; ++s)
+              tma_load_3d(base + C::OFF_K + st * C::TILE + s * TP_SUB, &tm_k, 64 * s, w.kvh, row, k_full + 8u * st);
+          }
           __syncwarp();
-          break;
-        }
-        if (elect_one()) {
-          mbar_expect_tx(v_full + 8u * st, C::TILE);
-          for (int s = 0; s < C::SUBS; ++s)
-            tma_load_3d(base + C::OFF_V + st * C::TILE + s * TP_SUB, &tm_v, 64 * s, w.kvh, row, v_full + 8u * st);
-        }
-        __syncwarp();
-        ++tiles;
-      }
-    }
-    // do not leave while copies may still land in this CTA's shared memory
-    if (elect_one()) {
-      if (items > 0) mbar_drain(q_full, (items - 1) & 1u, a.status);
-      for (uint32_t i = tiles > 2 ? tiles - 2 : 0; i < tiles; ++i) {
-        mbar_drain(k_full + 8u * (i & 1u), (i >> 1) & 1u, a.status);
-        mbar_drain(v_full + 8u * (i & 1u), (i >> 1) & 1u, a.status);
-      }
-    }
-    __syncwarp();
-  } else if (warp == TP_WARP_MMA) {
-    constexpr uint32_t format = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
-    constexpr uint32_t idesc_s = (1u << 4) | format | (TP_KEYS / 8u) << 17 | (TP_ROWS / 16u) << 24;
-    constexpr uint32_t idesc_o = (1u << 4) | format | 1u << 16 | (HD / 8u) << 17 | (TP_ROWS / 16u) << 24;  // B is MN-major
-    uint32_t items = 0, tiles = 0, given[2] = {0, 0};  // P tiles taken of each tile of rows
-    bool ok = true;
-    auto scores = [&](int g, uint32_t st) {
-      if (elect_one()) {
-        const uint64_t q = smem_desc_sw128(base + g * C::TILE), k = smem_desc_sw128(base + C::OFF_K + st * C::TILE);
-#pragma unroll
-        for (int s = 0; s < HD / 16; ++s) {
-          const uint64_t step = (s / 4) * (TP_SUB >> 4) + (s % 4) * 2;
-          mma_ss(tmem + g * TP_KEYS, q + step, k + step, idesc_s, s > 0);
-        }
-        tc_commit(s_full + 8u * g);
-      }
-      __syncwarp();
-    };
-    auto values = [&](int g, uint32_t st, bool first) {
-      if (elect_one()) {
-        const uint64_t v = smem_desc_v(base + C::OFF_V + st * C::TILE);
-#pragma unroll
-        for (int s = 0; s < TP_KEYS / 16; ++s)
-          mma_ts(tmem + 2 * TP_KEYS + g * HD, tmem + g * TP_KEYS + s * 8, v + s * (2048 >> 4), idesc_o, !first || s > 0);
-        tc_commit(o_done + 8u * g);
-      }
-      __syncwarp();
-    };
-    for (long long i = blockIdx.x; ok; i += gridDim.x) {
-      const Item it = walk.find(a, lane, TP_KEYS, i);
-      if (!it.some) break;
-      const Work w = work_of(a, it);
-      const int n = max(w.n[0], w.n[1]);
-      if (n == 0) continue;
-      ok = wait(q_full, items) && wait(k_full + 8u * (tiles & 1u), tiles >> 1);
-      if (!ok) break;
-      ++items;
-      tc_fence_after();
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (w.n[g] > 0) scores(g, tiles & 1u);
-      if (elect_one()) tc_commit(k_empty + 8u * (tiles & 1u));
-      if (n == 1 && elect_one()) tc_commit(q_empty);
-      __syncwarp();
-      for (int j = 0; j < n && ok; ++j, ++tiles) {
-        const uint32_t st = tiles & 1u, next = (tiles + 1) & 1u;
-        ok = wait(v_full + 8u * st, tiles >> 1) && wait(v_clean + 8u * st, tiles >> 1);
-        if (ok && j + 1 < n) ok = wait(k_full + 8u * next, (tiles + 1) >> 1);
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (!ok) break;
-          if (j < w.n[g]) {
-            if (!(ok = wait(p_full + 8u * g, given[g]))) break;
-            ++given[g];
-            tc_fence_after();
-            values(g, st, j == 0);
-          }
-          if (j + 1 < w.n[g]) scores(g, next);
-        }
-        if (ok && elect_one()) {
-          tc_commit(v_empty + 8u * st);
-          if (j + 1 < n) tc_commit(k_empty + 8u * next);
-          if (j + 2 == n) tc_commit(q_empty);
-        }
-        __syncwarp();
-      }
-    }
-    // after a wait that ran out nobody else waits for the last MMAs
-    if (elect_one()) tc_commit(mma_done);
-    __syncwarp();
-    mbar_drain(mma_done, 0, a.status);
-  } else if (warp == TP_WARP_CLEAN) {
-    constexpr uint32_t INF = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-    uint32_t items = 0, tiles = 0;
-    bool ok = true;
-    for (long long i = blockIdx.x; ok; i += gridDim.x) {
-      const Item it = walk.find(a, lane, TP_KEYS, i);
-      if (!it.some) break;
-      const Work w = work_of(a, it);
-      const int n = max(w.n[0], w.n[1]);
-      if (n == 0) continue;
-      int* bad = s_bad + (items % TP_BAD) * 3 * HD;
-      bool fresh = true;
-      for (int j = 0; j < n; ++j, ++tiles) {
-        const uint32_t st = tiles & 1u;
-        if (!(ok = wait(v_full + 8u * st, tiles >> 1))) break;
-        const int first = w.begin + j * TP_KEYS;
-        if (first + TP_KEYS > w.tok0 + w.shift + 1) {
-          if (fresh) {
-            for (int e = lane; e < 3 * HD; e += 32) bad[e] = 0x7fffffff;
-            if (lane == 0) s_any_bad[items % TP_BAD] = 0;
-            fresh = false;
+          if (!(ok = wait(v_empty + 8u * st, ph + 1))) {  // V of this tile is not loaded: nobody waits for it any more
+            if (elect_one()) mbar_drain(k_full + 8u * st, ph & 1u, a.status);
             __syncwarp();
+            break;
           }
-          const int have = min(TP_KEYS, w.end - first);
-          const uint32_t tile = base + C::OFF_V + st * C::TILE;
-          uint32_t top = 0;
-          for (int s = 0; s < C::SUBS; ++s) {
-            const int full = have * 8;  // 16-byte pieces of the rows there are
-#pragma unroll 8
-            for (int e = lane; e < full; e += 32) {
-              uint32_t x[4];
-              lds128(tile + s * TP_SUB + e * 16, x);
+          if (elect_one()) {
+            mbar_expect_tx(v_full + 8u * st, C::TILE);
+            for (int s = 0; s < C::SUBS; ++s)
+              tma_load_3d(base + C::OFF_V + st * C::TILE + s * TP_SUB, &tm_v, 64 * s, w.kvh, row, v_full + 8u * st);
+          }
+          __syncwarp();
+          ++tiles;
+        }
+      }
+      // do not leave while copies may still land in this CTA's shared memory
+      if (elect_one()) {
+        if (loads > 0) mbar_drain(q_full, (loads - 1) & 1u, a.status);
+        for (uint32_t i = tiles > 2 ? tiles - 2 : 0; i < tiles; ++i) {
+          mbar_drain(k_full + 8u * (i & 1u), (i >> 1) & 1u, a.status);
+          mbar_drain(v_full + 8u * (i & 1u), (i >> 1) & 1u, a.status);
+        }
+      }
+      __syncwarp();
+    } else if (warp != TP_WARP_CLEAN) {
+      const int g = warp - TP_WARP_MMA;
+      constexpr uint32_t format = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+      const uint32_t idesc_s = (1u << 4) | format | (TP_KEYS / 8u) << 17 | (TP_ROWS / 16u) << 24 | (a.scale < 0.f ? 1u << 13 : 0u);  // bit 13: -Q
+      constexpr uint32_t idesc_o = (1u << 4) | format | 1u << 16 | (HD / 8u) << 17 | (TP_ROWS / 16u) << 24;  // B is MN-major
+      uint32_t loads = 0, tiles = 0, given = 0;  // items with keys; their tiles of keys; tiles of P taken
+      bool ok = true;
+      auto scores = [&](uint32_t st) {
+        if (elect_one()) {
+          const uint64_t q = smem_desc_sw128(base + g * C::TILE), k = smem_desc_sw128(base + C::OFF_K + st * C::TILE);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) top = __vmaxu2(top, x[k] & 0x7fff7fffu);
-            }
-            const uint32_t zero[4] = {0u, 0u, 0u, 0u};
-            for (int e = full + lane; e < TP_KEYS * 8; e += 32) sts128(tile + s * TP_SUB + e * 16, zero);
+          for (int s = 0; s < HD / 16; ++s) {
+            const uint64_t step = (s / 4) * (TP_SUB >> 4) + (s % 4) * 2;
+            mma_ss(tmem + g * TP_KEYS, q + step, k + step, idesc_s, s > 0);
           }
-          if (__any_sync(0xffffffffu, (top & 0xffffu) >= INF || (top >> 16) >= INF)) {
-            uint16_t* v = reinterpret_cast<uint16_t*>(generic + C::OFF_V + st * C::TILE);
-            for (int e = lane; e < have * HD; e += 32) {
-              const int row = e / HD, d = e % HD;
-              uint16_t* at = v + (d / 64) * (TP_SUB / 2) + row * 64 + ((d % 64 / 8) ^ (row & 7)) * 8 + d % 8;
-              const uint32_t x = *at, mag = x & 0x7fffu;
-              if (mag < INF) continue;
-              atomicMin(bad + (mag > INF ? 0 : x & 0x8000u ? 2 : 1) * HD + d, first + row);
-              *at = 0;
-            }
-            if (lane == 0) s_any_bad[items % TP_BAD] = 1;
-          }
-          fence_proxy_async_smem();
+          tc_commit(s_full + 8u * g);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(v_clean + 8u * st);
+      };
+      // half of a tile's keys
+      auto values = [&](uint32_t st, int half, bool first) {
+        if (elect_one()) {
+          const uint64_t v = smem_desc_v(base + C::OFF_V + st * C::TILE);
+#pragma unroll
+          for (int i = 0; i < TP_KEYS / 32; ++i) {
+            const int s = half * (TP_KEYS / 32) + i;
+            mma_ts(tmem + 2 * TP_KEYS + g * HD, tmem + g * TP_KEYS + s * 8, v + s * (2048 >> 4), idesc_o, !first || s > 0);
+          }
+          if (half == 1) tc_commit(o_done + 8u * g);
+        }
+        __syncwarp();
+      };
+      Work w;
+      for (uint32_t i = 0; ok && (ok = next_work(i, w)); ++i) {
+        const int n = w.tiles(), own = w.n[g];
+        done_work(i);
+        if (n == 0) continue;
+        if (!(ok = wait(q_full, loads) && wait(k_full + 8u * (tiles & 1u), tiles >> 1))) break;
+        ++loads;
+        tc_fence_after();
+        if (own > 0) scores(tiles & 1u);
+        if (elect_one()) {
+          tc_commit(k_empty + 8u * (tiles & 1u));
+          if (n == 1) tc_commit(q_empty);
+        }
+        __syncwarp();
+        // both issuers wait for every tile, so that neither gives one back twice
+        for (int j = 0; j < n; ++j, ++tiles) {
+          const uint32_t st = tiles & 1u, next = (tiles + 1) & 1u;
+          if (!(ok = wait(v_full + 8u * st, tiles >> 1) && wait(v_clean + 8u * st, tiles >> 1))) break;
+          if (j < own) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (!(ok = wait(p_full + 16u * half + 8u * g, given))) break;
+              tc_fence_after();
+              values(st, half, j == 0);
+            }
+            if (!ok) break;
+            ++given;
+          }
+          if (j + 1 < n) {
+            if (!(ok = wait(k_full + 8u * next, (tiles + 1) >> 1))) break;
+            tc_fence_after();
+            if (j + 1 < own) scores(next);
+          }
+          if (elect_one()) {
+            tc_commit(v_empty + 8u * st);
+            if (j + 1 < n) tc_commit(k_empty + 8u * next);
+            if (j + 2 == n) tc_commit(q_empty);
+          }
+          __syncwarp();
+        }
       }
-      ++items;
+      // after a wait that ran out nobody else waits for the last MMAs
+      if (elect_one()) tc_commit(mma_done + 8u * g);
+      __syncwarp();
+      mbar_drain(mma_done + 8u * g, 0, a.status);
+    } else {
+      constexpr uint32_t INF = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+      uint32_t loads = 0, tiles = 0;
+      bool ok = true;
+      Work w;
+      for (uint32_t i = 0; ok && (ok = next_work(i, w)); ++i) {
+        const int n = w.tiles();
+        done_work(i);
+        if (n == 0) continue;
+        int* bad = s_bad + (loads % TP_BAD) * 3 * HD;
+        bool fresh = true;
+        for (int j = 0; j < n; ++j, ++tiles) {
+          const uint32_t st = tiles & 1u;
+          if (!(ok = wait(v_full + 8u * st, tiles >> 1))) break;
+          const int first = w.begin + j * TP_KEYS;
+          if (first + TP_KEYS > w.tok0 + w.shift + 1) {
+            if (fresh) {
+              for (int e = lane; e < 3 * HD; e += 32) bad[e] = 0x7fffffff;
+              if (lane == 0) s_any_bad[loads % TP_BAD] = 0;
+              fresh = false;
+              __syncwarp();
+            }
+            const int have = min(TP_KEYS, w.end - first);
+            const uint32_t tile = base + C::OFF_V + st * C::TILE;
+            uint32_t top = 0;
+            for (int s = 0; s < C::SUBS; ++s) {
+              const int full = have * 8;  // 16-byte pieces of the rows there are
+#pragma unroll 8
+              for (int e = lane; e < full; e += 32) {
+                uint32_t x[4];
+                lds128(tile + s * TP_SUB + e * 16, x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) top = __vmaxu2(top, x[k] & 0x7fff7fffu);
+              }
+              const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+              for (int e = full + lane; e < TP_KEYS * 8; e += 32) sts128(tile + s * TP_SUB + e * 16, zero);
+            }
+            if (__any_sync(0xffffffffu, (top & 0xffffu) >= INF || (top >> 16) >= INF)) {
+              uint16_t* v = reinterpret_cast<uint16_t*>(generic + C::OFF_V + st * C::TILE);
+              for (int e = lane; e < have * HD; e += 32) {
+                const int row = e / HD, d = e % HD;
+                uint16_t* at = v + (d / 64) * (TP_SUB / 2) + row * 64 + ((d % 64 / 8) ^ (row & 7)) * 8 + d % 8;
+                const uint32_t x = *at, mag = x & 0x7fffu;
+                if (mag < INF) continue;
+                atomicMin(bad + (mag > INF ? 0 : x & 0x8000u ? 2 : 1) * HD + d, first + row);
+                *at = 0;
+              }
+              if (lane == 0) s_any_bad[loads % TP_BAD] = 1;
+            }
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_clean + 8u * st);
+        }
+        ++loads;
+      }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int g = warp >> 2, row = (warp & 3) * 32 + lane;  // tile; row of it and lane of tensor memory
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, s_at = tmem + lanes + g * TP_KEYS, o_at = tmem + lanes + 2 * TP_KEYS + g * HD;
-    const float by = CAP ? fabsf(a.scale) / a.softcap * 2.f * LOG2E : fabsf(a.scale) * LOG2E, cap2 = a.softcap * LOG2E;
-    const uint32_t flip = a.scale < 0.f ? 0x80000000u : 0u;
-    uint32_t items = 0, tiles = 0;  // items with keys; S tiles taken
+    const float by = CAP ? fabsf(a.scale) / a.softcap : fabsf(a.scale) * LOG2E, cap2 = a.softcap * LOG2E;
+    const int tok = row / a.group, h = row - tok * a.group, mine = g * per + tok;
+    uint32_t loads = 0, tiles = 0;  // items with keys; S tiles taken
     bool ok = true;
-    for (long long i = blockIdx.x; ok; i += gridDim.x) {
-      const Item it = walk.find(a, lane, TP_KEYS, i);
-      if (!it.some) break;
-      const Work w = work_of(a, it);
-      const int tok = row / a.group, h = row - tok * a.group, mine = g * per + tok;
-      const bool live = tok < per && mine < w.toks && h < w.hs;
+    Work w;
+    for (uint32_t i = 0; ok && (ok = next_work(i, w)); ++i) {
       const int seen = w.tok0 + mine + w.shift + 1;        // keys that this row sees
       const int all_see = w.tok0 + g * per + w.shift + 1;  // that all rows of the tile see
+      const int begin = w.begin, own = w.n[g];
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < w.n[g]; ++j, ++tiles) {
+      for (int j = 0; j < own; ++j, ++tiles) {
         if (!(ok = wait(s_full + 8u * g, tiles))) break;
         tc_fence_after();
-        // twice through S, 64 and 32 columns at a time: its maximum, then the weights
-        const int first = w.begin + j * TP_KEYS, some = first + TP_KEYS > all_see ? seen - first : TP_KEYS;
+        uint32_t v[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, v[c]);
+        tmem_wait_ld();
+        const int first = begin + j * TP_KEYS;
         const bool masked = first + TP_KEYS > all_see;
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (masked) {
+          const int some = seen - first;
 #pragma unroll
-        for (int c = 0; c < 4; c += 2) {
-          uint32_t v[2][32];
-          tmem_ld32(s_at + 32 * c, v[0]);
-          tmem_ld32(s_at + 32 * c + 32, v[1]);
-          tmem_wait_ld();
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            float x = __uint_as_float(v[e / 32][e % 32] ^ flip);
-            if (masked && 32 * c + e >= some) x = -INFINITY;
-            top[e % 4] = fmaxf(top[e % 4], x);
-          }
+            for (int e = 0; e < 32; ++e)
+              if (32 * c + e >= some) v[c][e] = 0xff800000u;
         }
-        float up = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * by;
-        if constexpr (CAP) up = up == -INFINITY ? up : fmaf(-2.f * cap2, rcp(ex2(up) + 1.f), cap2);
+        float top[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          top[c] = max3(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]), __uint_as_float(v[c][0]));
+#pragma unroll
+          for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+        }
+        float up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * by;
+        bool wide = false;  // some score is beyond the polynomial of tanh (or masked, or no number)
+        if constexpr (CAP) {
+          float low[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            low[c] = fminf(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
+#pragma unroll
+            for (int e = 2; e < 32; e += 2) low[c] = min3(low[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+          }
+          wide = __any_sync(0xffffffffu, !(up <= 1.f && fminf(fminf(low[0], low[1]), fminf(low[2], low[3])) * by >= -1.f));
+          up = up == -INFINITY ? up : fmaf(-2.f * cap2, rcp(ex2(up * (2.f * LOG2E)) + 1.f), cap2);
+        }
         if (j == 0) {
           m = up;
         } else if (__any_sync(0xffffffffu, up > m + 8.f)) {
@@ -663,88 +786,155 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           l *= alpha;
           if (!(ok = wait(o_done + 8u * g, tiles - 1))) break;
           tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_at + 32 * c, o);
+#pragma unroll 1
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_at + 16 * c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32(o_at + 32 * c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(o_at + 16 * c, o);
           }
         }
-        const float base2 = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // an infinite score or none: NaN for the whole row, which the polynomial alone would not show
+        const float base2 = !(up < INFINITY) ? __int_as_float(0x7fffffff) : m == -INFINITY ? 0.f : m;
+        uint64_t sum[2] = {0ull, 0ull};
+        // P of 32 keys at a time; after 64 the first half of the product can start
+        auto weights = [&](auto poly, auto of) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32], p[16];
-          tmem_ld32(s_at + 32 * c, v);
-          tmem_wait_ld();
+          for (int c = 0; c < 4; ++c) {
+            uint32_t p[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float x[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float y = __uint_as_float(v[e + k] ^ flip);
-              if constexpr (CAP) x[k] = fmaf(-2.f * cap2, rcp(ex2(y * by) + 1.f), cap2 - base2);
-              else x[k] = fmaf(y, by, -base2);
-              x[k] = masked && 32 * c + e + k >= some ? 0.f : ex2(x[k]);
+            for (int e = 0; e < 16; ++e) {
+              float x, y;
+              const uint64_t z = of(v[c][2 * e], v[c][2 * e + 1]);
+              if (decltype(poly)::value && e * TP_POLY % 16 + TP_POLY >= 16) {
+                ex2_pair(z, x, y);
+              } else {
+                unpair(z, x, y);
+                x = ex2(x);
+                y = ex2(y);
+              }
+              sum[e % 2] = add2(sum[e % 2], pair(x, y));
+              p[e] = pack16<T>(x, y);
             }
-            sum[e / 2 % 4] += x[0] + x[1];
-            p[e / 2] = pack16<T>(x[0], x[1]);
+            tmem_st16(s_at + 16 * c, p);
+            if (c % 2) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_full + 16u * (c / 2) + 8u * g);
+            }
           }
-          tmem_st16(s_at + 16 * c, p);
+        };
+        if constexpr (CAP) {
+          if (!wide) {
+            const uint64_t by2 = pair(by, by), cc = pair(cap2, cap2), less = pair(-base2, -base2);
+            weights(std::true_type(), [&](uint32_t x, uint32_t y) {
+              const uint64_t z = mul2(pair(__uint_as_float(x), __uint_as_float(y)), by2);
+              return fma2(mul2(z, cc), tanh_pair(z), less);
+            });
+          } else {
+            const float by1 = by * (2.f * LOG2E);
+            auto one = [&](uint32_t x) {
+              const float f = __uint_as_float(x);
+              return f == -INFINITY ? f : fmaf(-2.f * cap2, rcp(ex2(f * by1) + 1.f), cap2 - base2);
+            };
+            weights(std::false_type(), [&](uint32_t x, uint32_t y) { return pair(one(x), one(y)); });
+          }
+        } else {
+          const uint64_t by2 = pair(by, by), less = pair(-base2, -base2);
+          auto of = [&](uint32_t x, uint32_t y) { return fma2(pair(__uint_as_float(x), __uint_as_float(y)), by2, less); };
+          if (masked) weights(std::false_type(), of);
+          else weights(std::true_type(), of);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + 8u * g);
+        {
+          float x, y;
+          unpair(add2(sum[0], sum[1]), x, y);
+          l += x + y;
+        }
       }
       if (!ok) break;
-      const int n = max(w.n[0], w.n[1]);
-      if (w.n[g] > 0 && !(ok = wait(o_done + 8u * g, tiles - 1))) break;
+      if (own > 0 && !(ok = wait(o_done + 8u * g, tiles - 1))) break;
       tc_fence_after();
+      w = s_work[i % TP_WORK];
       // the last tile of keys is one that was looked at: before it the notes may be older ones
-      const bool any_bad = w.n[g] > 0 && w.begin + w.n[g] * TP_KEYS > w.tok0 + w.shift + 1 && s_any_bad[items % TP_BAD] != 0;
-      const int* bad = s_bad + (items % TP_BAD) * 3 * HD;
-      const float f = w.chunks > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      const int64_t at = (static_cast<int64_t>(w.q0) + mine) * a.heads + w.kvh * G + w.h0 + h;
-      float* part = a.partial + (at * a.splits + w.chunk) * (HD + 4);
+      const bool any_bad = own > 0 && w.begin + own * TP_KEYS > w.tok0 + w.shift + 1 && s_any_bad[loads % TP_BAD] != 0;
+      const int* bad = s_bad + (loads % TP_BAD) * 3 * HD;
+      const bool parts = w.chunks > 1, wide_out = parts || a.out_dtype == B200MOE_DT_F32;
+      const float f = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      // 64 bytes of each row at a time through shared memory: four lanes then store them
+      const uint32_t stage = base + C::OFF_OUT + warp * 2048;
+      int64_t to[4];  // of the rows that this lane stores, 8 apart: their places in the output, -1: none
 #pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = (warp & 3) * 32 + 8 * k + lane / 4, rt = r / a.group, rh = r - rt * a.group;
+        const bool live = rt < per && g * per + rt < w.toks && rh < w.hs;
+        to[k] = live ? (static_cast<int64_t>(w.q0) + g * per + rt) * a.heads + w.kvh * G + w.h0 + rh : -1;
+      }
+      auto put = [&](const uint32_t (&x)[16], int byte) {  // byte: of the row, where these 64 go
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t y[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+          sts128(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4), y);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 8 * k + lane / 4, q = lane % 4;
+          uint32_t y[4];
+          lds128(stage + r * 64 + ((q ^ (r >> 1 & 3)) << 4), y);
+          if (to[k] < 0) continue;
+          uint8_t* at = parts ? reinterpret_cast<uint8_t*>(a.partial + (to[k] * a.splits + w.chunk) * (HD + 4))
+                              : static_cast<uint8_t*>(a.out) + to[k] * (wide_out ? HD * 4 : HD * 2);
+          *reinterpret_cast<uint4*>(at + byte + q * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+        __syncwarp();
+      };
+#pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t o[32];
-        if (w.n[g] > 0) {
+        if (own > 0) {
           tmem_ld32(o_at + 32 * c, o);
           tmem_wait_ld();
         }
-        if (live) {
-          float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
+        if (any_bad) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            x[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * f;
-            if (any_bad) {
-              const int d = 32 * c + e;
-              if (bad[d] < seen) x[e] = __int_as_float(0x7fffffff);
-              if (bad[HD + d] < seen) x[e] += INFINITY;
-              if (bad[2 * HD + d] < seen) x[e] -= INFINITY;
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            float y[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = x[e + k];
-            if (w.chunks > 1) store8(part + 32 * c + e, y);
-            else if (a.out_dtype == B200MOE_DT_F32) store8(static_cast<float*>(a.out) + at * HD + 32 * c + e, y);
-            else if (a.out_dtype == B200MOE_DT_F16) store8(static_cast<__half*>(a.out) + at * HD + 32 * c + e, y);
-            else store8(static_cast<__nv_bfloat16*>(a.out) + at * HD + 32 * c + e, y);
+            const int d = 32 * c + e;
+            float x = __uint_as_float(o[e]);
+            if (bad[d] < seen) x = __int_as_float(0x7fffffff);
+            if (bad[HD + d] < seen) x += INFINITY;
+            if (bad[2 * HD + d] < seen) x -= INFINITY;
+            o[e] = __float_as_uint(x);
           }
         }
-        __syncwarp();  // the next load of tensor memory is the whole warp's
+        uint32_t x[16];
+        if (wide_out) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = o[16 * half + e];
+            put(x, (32 * c + 16 * half) * 4);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float u = __uint_as_float(o[2 * e]), v = __uint_as_float(o[2 * e + 1]);
+            x[e] = a.out_dtype == B200MOE_DT_F16 ? pack16<__half>(u, v) : pack16<__nv_bfloat16>(u, v);
+          }
+          put(x, 64 * c);
+        }
       }
-      if (w.chunks > 1 && live) *reinterpret_cast<float2*>(part + HD) = make_float2(m, l);
-      if (n > 0) ++items;
+      if (parts) {
+        const bool live = tok < per && mine < w.toks && h < w.hs;
+        const int64_t at = (static_cast<int64_t>(w.q0) + mine) * a.heads + w.kvh * G + w.h0 + h;
+        if (live) *reinterpret_cast<float2*>(a.partial + (at * a.splits + w.chunk) * (HD + 4) + HD) = make_float2(m, l);
+      }
+      if (w.tiles() > 0) ++loads;
+      done_work(i);
     }
   }
   zero_rest(a, HD, TP_THREADS);
@@ -774,7 +964,8 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptArgs a) {
     const bool here = row >= qs.begin && row < qs.begin + qs.len;
     const unsigned who = __ballot_sync(0xffffffffu, here);
     if (who == 0) continue;
-    const int own = here ? ItemWalk::chunks(a, b, static_cast<int>(row - qs.begin) / a.tokens, TP_KEYS) : 0;
+    const int m = here ? span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, b, a.k_rows, nullptr).len : 0;
+    const int own = here ? ItemWalk::chunks(a, qs.len, m, static_cast<int>(row - qs.begin) / a.tokens, TP_KEYS) : 0;
     chunks = __shfl_sync(0xffffffffu, own, __ffs(who) - 1);
     break;
   }
