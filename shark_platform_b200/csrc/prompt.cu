@@ -26,6 +26,7 @@ struct PromptArgs {
   int64_t q_rows, k_rows;
   int out_dtype, bs, heads, kv_heads;
   int group, parts;       // heads of a tile; parts of a group of heads
+  uint32_t inv_group;     // 2^16 / group, rounded up: exact quotients of rows of a tile
   int tokens;             // of a tile
   int splits;             // parts that the keys of a tile are cut into, at most
   float* partial;         // [row of q][head][splits][HD + 4]: numerator, maximum, denominator
@@ -316,7 +317,7 @@ int launch_prompt(PromptArgs& a, cudaStream_t st) {
 // 16-bit rows: an item is two tiles of 128 rows, S = Q K^T and O += P V by tcgen05.mma with the
 // accumulators in tensor memory (S0, S1, O0, O1: all 512 columns at 128 elements a head).
 //   warps 0-3, 4-7  the softmax of tile 0, 1: a thread has a row.  S out of tensor memory, its
-//                   maximum, P = 2^(S - m) in the type of V back over S as the A operand of
+//                   maximum, P = 2^(S - m) in the type of V back over it as the A operand of
 //                   the second product.  O is rescaled when the maximum has grown by more
 //                   than 2^8 (P stays below that), by the same threads.  The output at the end.
 //   warps 8, 9      issue the MMAs of tile 0, 1: S(0), then PV(j), S(j + 1) ...; while one tile's
@@ -372,10 +373,11 @@ struct Work {
   int kvh, h0, hs;        // kv head; heads of its group: first, how many
   int k0, begin, end;     // first row of k; keys of this item
   int shift;              // token i sees keys up to i + shift
-  int n[2];               // tiles of keys of each tile of rows
+  int n0, n1;             // tiles of keys of each tile of rows
   int chunk, chunks;
   int unused[2];
-  __device__ __forceinline__ int tiles() const { return max(n[0], n[1]); }
+  __device__ __forceinline__ int tiles() const { return max(n0, n1); }
+  __device__ __forceinline__ int tiles_of(int g) const { return g == 0 ? n0 : n1; }
 };
 static_assert(sizeof(Work) == 64, "four 16-byte words");
 __device__ __forceinline__ Work work_of(const PromptArgs& a, const Item& it) {
@@ -395,12 +397,13 @@ __device__ __forceinline__ Work work_of(const PromptArgs& a, const Item& it) {
   w.chunks = a.splits == 1 ? 1 : chunks_of(keys, TP_KEYS, a.splits);
   w.begin = w.chunks == 1 ? 0 : chunk_begin(keys, TP_KEYS, w.chunks, it.chunk);
   w.end = w.chunks == 1 ? keys : min(keys, chunk_begin(keys, TP_KEYS, w.chunks, it.chunk + 1));
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
+  auto tiles = [&](int g) {
     const int mine = min(per, w.toks - g * per);
     const int last = mine > 0 ? min(w.end, keys_seen(qs.len, ks.len, w.tok0 + g * per, mine)) : 0;
-    w.n[g] = last > w.begin ? (last - w.begin + TP_KEYS - 1) / TP_KEYS : 0;
-  }
+    return last > w.begin ? (last - w.begin + TP_KEYS - 1) / TP_KEYS : 0;
+  };
+  w.n0 = tiles(0);
+  w.n1 = tiles(1);
   return w;
 }
 
@@ -441,23 +444,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float a, float b) { return pack2(static_cast<const T*>(nullptr), a, b); }
 
-// 2^x for x <= 2^7 by the fp32 units: 2^n 2^f, n the nearest integer and |f| <= 1/2, 2^f by a
-// polynomial of degree 4 (minimax, off by 2^-18.5, an eightieth of half a step of fp16).
-__device__ __forceinline__ void ex2_pair(uint64_t v, float& x, float& y) {
-  constexpr float BIG = 12582912.f;  // 1.5 * 2^23: n in the last places
-  unpair(v, x, y);
-  v = pair(fmaxf(x, -126.f), fmaxf(y, -126.f));
-  const uint64_t t = add2(v, pair(BIG, BIG)), f = fma2(add2(t, pair(-BIG, -BIG)), pair(-1.f, -1.f), v);
-  uint64_t p = fma2(f, pair(0.009570096619427204f, 0.009570096619427204f), pair(0.05591786280274391f, 0.05591786280274391f));
-  p = fma2(f, p, pair(0.240247443318367f, 0.240247443318367f));
-  p = fma2(f, p, pair(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(f, p, pair(0.9999992847442627f, 0.9999992847442627f));
-  float tx, ty;
-  unpair(t, tx, ty);
-  unpair(p, x, y);
-  x = __uint_as_float(__float_as_uint(x) + (__float_as_uint(tx) << 23));
-  y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
-}
 // tanh(z) / z for |z| <= 1 as a polynomial in z^2 (minimax, off by 2^-20.7)
 __device__ __forceinline__ uint64_t tanh_pair(uint64_t z) {
   const uint64_t u = mul2(z, z);
@@ -467,9 +453,6 @@ __device__ __forceinline__ uint64_t tanh_pair(uint64_t z) {
   p = fma2(u, p, pair(-0.3332904279232025f, -0.3332904279232025f));
   return fma2(u, p, pair(0.9999994039535522f, 0.9999994039535522f));
 }
-// Of 16 pairs of weights, how many the fp32 units compute: the special-function unit's 16 a
-// clock are as many as the MMAs need clocks for.
-constexpr int TP_POLY = 5;
 
 template <typename T, int HD, bool CAP>
 __global__ void __launch_bounds__(TP_THREADS, 1)
@@ -536,24 +519,30 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       const uint32_t q_bytes = static_cast<uint32_t>(per * a.group) * HD * 2;
       ItemWalk walk(a, lane);
       bool ok = true;
-      for (uint32_t i = 0; ok; ++i) {
+      auto publish = [&](uint32_t i, Work& w) {
         const Item it = walk.find(a, lane, TP_KEYS, item_of(i));
-        Work w;
         if (it.some) w = work_of(a, it);
         else w.toks = -1;
-        if (!(ok = wait(w_empty + 8u * (i % TP_WORK), i / TP_WORK + 1))) break;
+        if (!wait(w_empty + 8u * (i % TP_WORK), i / TP_WORK + 1)) return false;
         if (lane == 0) {
           s_work[i % TP_WORK] = w;
           mbar_arrive(w_full + 8u * (i % TP_WORK));
         }
         __syncwarp();
-        if (!it.some) break;
+        return true;
+      };
+      Work w, after;
+      ok = publish(0, w);
+      for (uint32_t i = 0; ok && w.toks >= 0; ++i, w = after) {
         const int n = w.tiles();
-        if (n == 0) continue;
+        if (n == 0) {
+          ok = publish(i + 1, after);
+          continue;
+        }
         if (!(ok = wait(q_empty, loads + 1))) break;
         ++loads;
         if (elect_one()) {
-          const int both = w.n[1] > 0 ? 2 : 1;
+          const int both = w.n1 > 0 ? 2 : 1;
           mbar_expect_tx(q_full, both * q_bytes);
           for (int g = 0; g < both; ++g)
             for (int s = 0; s < C::SUBS; ++s)
@@ -582,6 +571,7 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           }
           __syncwarp();
           ++tiles;
+          if (j == min(n, 2) - 1 && !(ok = publish(i + 1, after))) break;  // while both places are full
         }
       }
       // do not leave while copies may still land in this CTA's shared memory
@@ -613,21 +603,21 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         __syncwarp();
       };
       // half of a tile's keys
-      auto values = [&](uint32_t st, int half, bool first) {
+      auto values = [&](uint32_t st, int part, bool first) {
         if (elect_one()) {
           const uint64_t v = smem_desc_v(base + C::OFF_V + st * C::TILE);
 #pragma unroll
-          for (int i = 0; i < TP_KEYS / 32; ++i) {
-            const int s = half * (TP_KEYS / 32) + i;
-            mma_ts(tmem + 2 * TP_KEYS + g * HD, tmem + g * TP_KEYS + s * 8, v + s * (2048 >> 4), idesc_o, !first || s > 0);
+          for (int i = 0; i < 4; ++i) {
+            const int s = part * 4 + i;
+            mma_ts(tmem + 2 * TP_KEYS + g * HD, tmem + g * TP_KEYS + s * 8, v + s * (2048 >> 4), idesc_o, !first || part > 0 || i > 0);
           }
-          if (half == 1) tc_commit(o_done + 8u * g);
+          if (part == 1) tc_commit(o_done + 8u * g);
         }
         __syncwarp();
       };
       Work w;
       for (uint32_t i = 0; ok && (ok = next_work(i, w)); ++i) {
-        const int n = w.tiles(), own = w.n[g];
+        const int n = w.tiles(), own = w.tiles_of(g);
         done_work(i);
         if (n == 0) continue;
         if (!(ok = wait(q_full, loads) && wait(k_full + 8u * (tiles & 1u), tiles >> 1))) break;
@@ -645,10 +635,10 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           if (!(ok = wait(v_full + 8u * st, tiles >> 1) && wait(v_clean + 8u * st, tiles >> 1))) break;
           if (j < own) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              if (!(ok = wait(p_full + 16u * half + 8u * g, given))) break;
+            for (int part = 0; part < 2; ++part) {
+              if (!(ok = wait(p_full + 16u * part + 8u * g, given))) break;
               tc_fence_after();
-              values(st, half, j == 0);
+              values(st, part, j == 0);
             }
             if (!ok) break;
             ++given;
@@ -732,14 +722,15 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     const int g = warp >> 2, row = (warp & 3) * 32 + lane;  // tile; row of it and lane of tensor memory
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, s_at = tmem + lanes + g * TP_KEYS, o_at = tmem + lanes + 2 * TP_KEYS + g * HD;
     const float by = CAP ? fabsf(a.scale) / a.softcap : fabsf(a.scale) * LOG2E, cap2 = a.softcap * LOG2E;
-    const int tok = row / a.group, h = row - tok * a.group, mine = g * per + tok;
+    auto token_of = [&](int r) { return static_cast<int>((static_cast<uint32_t>(r) * a.inv_group) >> 16); };  // r / group
+    const int mine = g * per + token_of(row);
     uint32_t loads = 0, tiles = 0;  // items with keys; S tiles taken
     bool ok = true;
     Work w;
     for (uint32_t i = 0; ok && (ok = next_work(i, w)); ++i) {
       const int seen = w.tok0 + mine + w.shift + 1;        // keys that this row sees
       const int all_see = w.tok0 + g * per + w.shift + 1;  // that all rows of the tile see
-      const int begin = w.begin, own = w.n[g];
+      const int begin = w.begin, own = w.tiles_of(g);
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < own; ++j, ++tiles) {
         if (!(ok = wait(s_full + 8u * g, tiles))) break;
@@ -750,13 +741,43 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         tmem_wait_ld();
         const int first = begin + j * TP_KEYS;
         const bool masked = first + TP_KEYS > all_see;
+
+        if constexpr (CAP) {
+          // c tanh(x / c) in units of log 2, in place: the polynomial where no row of the warp has
+          // larger scores (or others than numbers), else by the exponential
+          float least = 0.f, most = 0.f;
+#pragma unroll
+          for (int e = 0; e < 128; e += 2) {
+            least = min3(least, __uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1]));
+            most = max3(most, __uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1]));
+          }
+          const bool small = __all_sync(0xffffffffu, most * by <= 1.f && least * by >= -1.f);
+          auto capped = [&](auto fast) {
+#pragma unroll
+            for (int e = 0; e < 128; e += 2) {
+              uint32_t &a0 = v[e / 32][e % 32], &a1 = v[e / 32][e % 32 + 1];
+              float x, y;
+              if constexpr (decltype(fast)::value) {
+                const uint64_t z = mul2(pair(__uint_as_float(a0), __uint_as_float(a1)), pair(by, by));
+                unpair(mul2(mul2(z, pair(cap2, cap2)), tanh_pair(z)), x, y);
+              } else {
+                x = fmaf(-2.f * cap2, rcp(ex2(__uint_as_float(a0) * (by * (2.f * LOG2E))) + 1.f), cap2);
+                y = fmaf(-2.f * cap2, rcp(ex2(__uint_as_float(a1) * (by * (2.f * LOG2E))) + 1.f), cap2);
+              }
+              a0 = __float_as_uint(x);
+              a1 = __float_as_uint(y);
+            }
+          };
+          if (small) capped(std::true_type());
+          else capped(std::false_type());
+        }
+        const float unit = CAP ? 1.f : by;
+
         if (masked) {
-          const int some = seen - first;
+          const int some = seen - first;  // of the tile's keys, how many the row sees
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * c + e >= some) v[c][e] = 0xff800000u;
+          for (int e = 0; e < 128; ++e)
+            if (e >= some) v[e / 32][e % 32] = 0xff800000u;
         }
         float top[4];
 #pragma unroll
@@ -765,23 +786,14 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 #pragma unroll
           for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
         }
-        float up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * by;
-        bool wide = false;  // some score is beyond the polynomial of tanh (or masked, or no number)
-        if constexpr (CAP) {
-          float low[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            low[c] = fminf(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
-#pragma unroll
-            for (int e = 2; e < 32; e += 2) low[c] = min3(low[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
-          }
-          wide = __any_sync(0xffffffffu, !(up <= 1.f && fminf(fminf(low[0], low[1]), fminf(low[2], low[3])) * by >= -1.f));
-          up = up == -INFINITY ? up : fmaf(-2.f * cap2, rcp(ex2(up * (2.f * LOG2E)) + 1.f), cap2);
-        }
+        const float up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * unit;
+        // The maximum is taken where it has grown by more than 2^8: what the weights are relative
+        // to from here on.  An infinite score or none makes it NaN: for the whole row.
         if (j == 0) {
-          m = up;
-        } else if (__any_sync(0xffffffffu, up > m + 8.f)) {
-          const float m_new = fmaxf(m, up), alpha = m_new == -INFINITY ? 1.f : ex2(m - m_new);
+          m = up < INFINITY ? up : __int_as_float(0x7fffffff);
+        } else if (__any_sync(0xffffffffu, !(up <= m + 8.f))) {
+          const float m_new = up < INFINITY ? fmaxf(m, up) : __int_as_float(0x7fffffff);
+          const float alpha = m_new == -INFINITY ? 1.f : ex2(m - m_new);
           m = m_new;
           l *= alpha;
           if (!(ok = wait(o_done + 8u * g, tiles - 1))) break;
@@ -796,57 +808,30 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             tmem_st16(o_at + 16 * c, o);
           }
         }
-        // an infinite score or none: NaN for the whole row, which the polynomial alone would not show
-        const float base2 = !(up < INFINITY) ? __int_as_float(0x7fffffff) : m == -INFINITY ? 0.f : m;
+        const float from = m == -INFINITY ? 0.f : m;
+        const uint64_t units = pair(unit, unit), less = pair(-from, -from);
         uint64_t sum[2] = {0ull, 0ull};
         // P of 32 keys at a time; after 64 the first half of the product can start
-        auto weights = [&](auto poly, auto of) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t p[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float x, y;
-              const uint64_t z = of(v[c][2 * e], v[c][2 * e + 1]);
-              if (decltype(poly)::value && e * TP_POLY % 16 + TP_POLY >= 16) {
-                ex2_pair(z, x, y);
-              } else {
-                unpair(z, x, y);
-                x = ex2(x);
-                y = ex2(y);
-              }
-              sum[e % 2] = add2(sum[e % 2], pair(x, y));
-              p[e] = pack16<T>(x, y);
-            }
-            tmem_st16(s_at + 16 * c, p);
-            if (c % 2) {
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(p_full + 16u * (c / 2) + 8u * g);
-            }
+          for (int e = 0; e < 16; ++e) {
+            float x, y;
+            const uint64_t s2 = pair(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1]));
+            unpair(CAP ? add2(s2, less) : fma2(s2, units, less), x, y);
+            x = ex2(x);
+            y = ex2(y);
+            sum[e % 2] = add2(sum[e % 2], pair(x, y));
+            p[e] = pack16<T>(x, y);
           }
-        };
-        if constexpr (CAP) {
-          if (!wide) {
-            const uint64_t by2 = pair(by, by), cc = pair(cap2, cap2), less = pair(-base2, -base2);
-            weights(std::true_type(), [&](uint32_t x, uint32_t y) {
-              const uint64_t z = mul2(pair(__uint_as_float(x), __uint_as_float(y)), by2);
-              return fma2(mul2(z, cc), tanh_pair(z), less);
-            });
-          } else {
-            const float by1 = by * (2.f * LOG2E);
-            auto one = [&](uint32_t x) {
-              const float f = __uint_as_float(x);
-              return f == -INFINITY ? f : fmaf(-2.f * cap2, rcp(ex2(f * by1) + 1.f), cap2 - base2);
-            };
-            weights(std::false_type(), [&](uint32_t x, uint32_t y) { return pair(one(x), one(y)); });
+          tmem_st16(s_at + 16 * c, p);
+          if (c % 2) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 16u * (c / 2) + 8u * g);
           }
-        } else {
-          const uint64_t by2 = pair(by, by), less = pair(-base2, -base2);
-          auto of = [&](uint32_t x, uint32_t y) { return fma2(pair(__uint_as_float(x), __uint_as_float(y)), by2, less); };
-          if (masked) weights(std::false_type(), of);
-          else weights(std::true_type(), of);
         }
         {
           float x, y;
@@ -862,15 +847,18 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       const bool any_bad = own > 0 && w.begin + own * TP_KEYS > w.tok0 + w.shift + 1 && s_any_bad[loads % TP_BAD] != 0;
       const int* bad = s_bad + (loads % TP_BAD) * 3 * HD;
       const bool parts = w.chunks > 1, wide_out = parts || a.out_dtype == B200MOE_DT_F32;
-      const float f = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      const float f = parts ? 1.f : l == 0.f ? 0.f : rcp(l);
       // 64 bytes of each row at a time through shared memory: four lanes then store them
       const uint32_t stage = base + C::OFF_OUT + warp * 2048;
-      int64_t to[4];  // of the rows that this lane stores, 8 apart: their places in the output, -1: none
+      const int64_t row0 = static_cast<int64_t>(w.q0) * a.heads + w.kvh * G + w.h0;
+      uint8_t* to[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int r = (warp & 3) * 32 + 8 * k + lane / 4, rt = r / a.group, rh = r - rt * a.group;
+        const int r = (warp & 3) * 32 + 8 * k + lane / 4, rt = token_of(r), rh = r - rt * a.group;
         const bool live = rt < per && g * per + rt < w.toks && rh < w.hs;
-        to[k] = live ? (static_cast<int64_t>(w.q0) + g * per + rt) * a.heads + w.kvh * G + w.h0 + rh : -1;
+        const int64_t at = row0 + (g * per + rt) * a.heads + rh;
+        to[k] = !live ? nullptr : parts ? reinterpret_cast<uint8_t*>(a.partial + (at * a.splits + w.chunk) * (HD + 4))
+                                        : static_cast<uint8_t*>(a.out) + at * (wide_out ? HD * 4 : HD * 2);
       }
       auto put = [&](const uint32_t (&x)[16], int byte) {  // byte: of the row, where these 64 go
 #pragma unroll
@@ -884,54 +872,51 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           const int r = 8 * k + lane / 4, q = lane % 4;
           uint32_t y[4];
           lds128(stage + r * 64 + ((q ^ (r >> 1 & 3)) << 4), y);
-          if (to[k] < 0) continue;
-          uint8_t* at = parts ? reinterpret_cast<uint8_t*>(a.partial + (to[k] * a.splits + w.chunk) * (HD + 4))
-                              : static_cast<uint8_t*>(a.out) + to[k] * (wide_out ? HD * 4 : HD * 2);
-          *reinterpret_cast<uint4*>(at + byte + q * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+          if (to[k] != nullptr) *reinterpret_cast<uint4*>(to[k] + byte + q * 16) = make_uint4(y[0], y[1], y[2], y[3]);
         }
         __syncwarp();
       };
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
+        uint32_t o[2][16];
         if (own > 0) {
-          tmem_ld32(o_at + 32 * c, o);
+          tmem_ld16(o_at + 32 * c, o[0]);
+          tmem_ld16(o_at + 32 * c + 16, o[1]);
           tmem_wait_ld();
-        }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * f);
+          for (int e = 0; e < 32; ++e) o[e / 16][e % 16] = __float_as_uint(__uint_as_float(o[e / 16][e % 16]) * f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e / 16][e % 16] = 0u;
+        }
         if (any_bad) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int d = 32 * c + e;
-            float x = __uint_as_float(o[e]);
+            float x = __uint_as_float(o[e / 16][e % 16]);
             if (bad[d] < seen) x = __int_as_float(0x7fffffff);
             if (bad[HD + d] < seen) x += INFINITY;
             if (bad[2 * HD + d] < seen) x -= INFINITY;
-            o[e] = __float_as_uint(x);
+            o[e / 16][e % 16] = __float_as_uint(x);
           }
         }
-        uint32_t x[16];
         if (wide_out) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = o[16 * half + e];
-            put(x, (32 * c + 16 * half) * 4);
-          }
+          put(o[0], 128 * c);
+          put(o[1], 128 * c + 64);
         } else {
+          uint32_t x[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float u = __uint_as_float(o[2 * e]), v = __uint_as_float(o[2 * e + 1]);
+            const float u = __uint_as_float(o[e / 8][2 * e % 16]), v = __uint_as_float(o[e / 8][2 * e % 16 + 1]);
             x[e] = a.out_dtype == B200MOE_DT_F16 ? pack16<__half>(u, v) : pack16<__nv_bfloat16>(u, v);
           }
           put(x, 64 * c);
         }
       }
       if (parts) {
-        const bool live = tok < per && mine < w.toks && h < w.hs;
-        const int64_t at = (static_cast<int64_t>(w.q0) + mine) * a.heads + w.kvh * G + w.h0 + h;
-        if (live) *reinterpret_cast<float2*>(a.partial + (at * a.splits + w.chunk) * (HD + 4) + HD) = make_float2(m, l);
+        const int h = row - token_of(row) * a.group;
+        if (mine - g * per < per && mine < w.toks && h < w.hs)
+          *reinterpret_cast<float2*>(a.partial + ((row0 + mine * a.heads + h) * a.splits + w.chunk) * (HD + 4) + HD) = make_float2(m, l);
       }
       if (w.tiles() > 0) ++loads;
       done_work(i);
@@ -1070,7 +1055,7 @@ int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype
     return B200MOE_OK;
   }
   const PromptPlan p = plan_prompt(q_rows, k_rows, bs, heads, kv_heads);
-  a.group = p.group; a.parts = p.parts; a.tokens = p.tokens; a.splits = p.splits;
+  a.group = p.group; a.inv_group = (65536 + p.group - 1) / p.group; a.parts = p.parts; a.tokens = p.tokens; a.splits = p.splits;
   return dtype == B200MOE_DT_F16 ? launch_prompt_tc_hd<__half>(a, head_dim, st) : launch_prompt_tc_hd<__nv_bfloat16>(a, head_dim, st);
 }
 
