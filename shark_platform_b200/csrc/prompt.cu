@@ -444,15 +444,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float a, float b) { return pack2(static_cast<const T*>(nullptr), a, b); }
 
-// tanh(z) / z for |z| <= 1 as a polynomial in z^2 (minimax, off by 2^-20.7)
-__device__ __forceinline__ uint64_t tanh_pair(uint64_t z) {
-  const uint64_t u = mul2(z, z);
-  uint64_t p = fma2(u, pair(-0.0030670491978526115f, -0.0030670491978526115f), pair(0.016743090003728867f, 0.016743090003728867f));
-  p = fma2(u, p, pair(-0.05160565301775932f, -0.05160565301775932f));
-  p = fma2(u, p, pair(0.13281433284282684f, 0.13281433284282684f));
-  p = fma2(u, p, pair(-0.3332904279232025f, -0.3332904279232025f));
-  return fma2(u, p, pair(0.9999994039535522f, 0.9999994039535522f));
-}
+// tanh(z) for |z| <= 1/2 is z times this polynomial in z^2 (minimax, off by 2^-20.8).
+constexpr float TANH[4] = {0.999999463558197f, -0.33326318860054016f, 0.13190296292304993f, -0.044402219355106354f};
 
 template <typename T, int HD, bool CAP>
 __global__ void __launch_bounds__(TP_THREADS, 1)
@@ -722,6 +715,9 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     const int g = warp >> 2, row = (warp & 3) * 32 + lane;  // tile; row of it and lane of tensor memory
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, s_at = tmem + lanes + g * TP_KEYS, o_at = tmem + lanes + 2 * TP_KEYS + g * HD;
     const float by = CAP ? fabsf(a.scale) / a.softcap : fabsf(a.scale) * LOG2E, cap2 = a.softcap * LOG2E;
+    // c log2(e) tanh(S by) as a polynomial in S, where its coefficients are within 32 bits
+    const float by3 = by * by * by, poly[4] = {TANH[0] * cap2 * by, TANH[1] * cap2 * by3, TANH[2] * cap2 * by3 * (by * by), TANH[3] * cap2 * by3 * (by3 * by)};
+    const bool usual = by > 1e-4f && by < 1e4f && cap2 > 1e-3f && cap2 < 1e4f;
     auto token_of = [&](int r) { return static_cast<int>((static_cast<uint32_t>(r) * a.inv_group) >> 16); };  // r / group
     const int mine = g * per + token_of(row);
     uint32_t loads = 0, tiles = 0;  // items with keys; S tiles taken
@@ -731,6 +727,7 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       const int seen = w.tok0 + mine + w.shift + 1;        // keys that this row sees
       const int all_see = w.tok0 + g * per + w.shift + 1;  // that all rows of the tile see
       const int begin = w.begin, own = w.tiles_of(g);
+      const bool live = mine - g * per < per && mine < w.toks;  // rows behind the tokens hold anything: no vote is theirs
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < own; ++j, ++tiles) {
         if (!(ok = wait(s_full + 8u * g, tiles))) break;
@@ -742,51 +739,52 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         const int first = begin + j * TP_KEYS;
         const bool masked = first + TP_KEYS > all_see;
 
+        const int some = masked ? seen - first : TP_KEYS;  // of the tile's keys, how many the row sees
+        float top[4], up;
+        bool small = true;  // softcap: the polynomial holds for all scores of the warp's rows
         if constexpr (CAP) {
-          // c tanh(x / c) in units of log 2, in place: the polynomial where no row of the warp has
-          // larger scores (or others than numbers), else by the exponential
-          float least = 0.f, most = 0.f;
+          // unseen scores are zeros, and their weights later
+          if (masked) {
 #pragma unroll
-          for (int e = 0; e < 128; e += 2) {
-            least = min3(least, __uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1]));
-            most = max3(most, __uint_as_float(v[e / 32][e % 32]), __uint_as_float(v[e / 32][e % 32 + 1]));
+            for (int e = 0; e < 128; ++e)
+              if (e >= some) v[e / 32][e % 32] = 0u;
           }
-          const bool small = __all_sync(0xffffffffu, most * by <= 1.f && least * by >= -1.f);
-          auto capped = [&](auto fast) {
+          float low[4];
 #pragma unroll
-            for (int e = 0; e < 128; e += 2) {
-              uint32_t &a0 = v[e / 32][e % 32], &a1 = v[e / 32][e % 32 + 1];
-              float x, y;
-              if constexpr (decltype(fast)::value) {
-                const uint64_t z = mul2(pair(__uint_as_float(a0), __uint_as_float(a1)), pair(by, by));
-                unpair(mul2(mul2(z, pair(cap2, cap2)), tanh_pair(z)), x, y);
-              } else {
-                x = fmaf(-2.f * cap2, rcp(ex2(__uint_as_float(a0) * (by * (2.f * LOG2E))) + 1.f), cap2);
-                y = fmaf(-2.f * cap2, rcp(ex2(__uint_as_float(a1) * (by * (2.f * LOG2E))) + 1.f), cap2);
-              }
-              a0 = __float_as_uint(x);
-              a1 = __float_as_uint(y);
+          for (int c = 0; c < 4; ++c) {
+            low[c] = top[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+            for (int e = 1; e < 31; e += 2) {
+              low[c] = min3(low[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+              top[c] = max3(top[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
             }
-          };
-          if (small) capped(std::true_type());
-          else capped(std::false_type());
-        }
-        const float unit = CAP ? 1.f : by;
-
-        if (masked) {
-          const int some = seen - first;  // of the tile's keys, how many the row sees
+            low[c] = min3(low[c], __uint_as_float(v[c][31]), low[c]);
+            top[c] = max3(top[c], __uint_as_float(v[c][31]), top[c]);
+          }
+          up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * by;
+          small = usual && __all_sync(0xffffffffu, !live || (up <= 0.5f && min3(min3(low[0], low[1], low[2]), low[3], low[3]) * by >= -0.5f));
+          if (masked) {
+            up = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (e >= some) v[e / 32][e % 32] = 0xff800000u;
-        }
-        float top[4];
+            for (int e = 0; e < 128; ++e) up = e < some ? max3(up, __uint_as_float(v[e / 32][e % 32]), up) : up;
+            up *= by;
+          }
+          up = up == -INFINITY ? up : fmaf(-2.f * cap2, rcp(ex2(up * (2.f * LOG2E)) + 1.f), cap2);
+        } else {
+          if (masked) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          top[c] = max3(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]), __uint_as_float(v[c][0]));
+            for (int e = 0; e < 128; ++e)
+              if (e >= some) v[e / 32][e % 32] = 0xff800000u;
+          }
 #pragma unroll
-          for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+          for (int c = 0; c < 4; ++c) {
+            top[c] = max3(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]), __uint_as_float(v[c][0]));
+#pragma unroll
+            for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+          }
+          up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * by;
         }
-        const float up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * unit;
+        up = live ? up : 0.f;
         // The maximum is taken where it has grown by more than 2^8: what the weights are relative
         // to from here on.  An infinite score or none makes it NaN: for the whole row.
         if (j == 0) {
@@ -809,29 +807,51 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           }
         }
         const float from = m == -INFINITY ? 0.f : m;
-        const uint64_t units = pair(unit, unit), less = pair(-from, -from);
+        const uint64_t by2 = pair(by, by), less = pair(-from, -from);
         uint64_t sum[2] = {0ull, 0ull};
         // P of 32 keys at a time; after 64 the first half of the product can start
+        auto weights = [&](auto cut, auto fast) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t p[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x, y;
-            const uint64_t s2 = pair(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1]));
-            unpair(CAP ? add2(s2, less) : fma2(s2, units, less), x, y);
-            x = ex2(x);
-            y = ex2(y);
-            sum[e % 2] = add2(sum[e % 2], pair(x, y));
-            p[e] = pack16<T>(x, y);
+            for (int e = 0; e < 16; ++e) {
+              const float s0 = __uint_as_float(v[c][2 * e]), s1 = __uint_as_float(v[c][2 * e + 1]);
+              float x, y;
+              if constexpr (!CAP) {
+                unpair(fma2(pair(s0, s1), by2, less), x, y);
+              } else if constexpr (decltype(fast)::value) {
+                const uint64_t s2 = pair(s0, s1), u = mul2(s2, s2);
+                const uint64_t t = fma2(u, fma2(u, fma2(u, pair(poly[3], poly[3]), pair(poly[2], poly[2])), pair(poly[1], poly[1])), pair(poly[0], poly[0]));
+                unpair(fma2(s2, t, less), x, y);
+              } else {
+                x = fmaf(-2.f * cap2, rcp(ex2(s0 * (by * (2.f * LOG2E))) + 1.f), cap2 - from);
+                y = fmaf(-2.f * cap2, rcp(ex2(s1 * (by * (2.f * LOG2E))) + 1.f), cap2 - from);
+              }
+              x = ex2(x);
+              y = ex2(y);
+              if constexpr (decltype(cut)::value) {
+                x = 32 * c + 2 * e < some ? x : 0.f;
+                y = 32 * c + 2 * e + 1 < some ? y : 0.f;
+              }
+              sum[e % 2] = add2(sum[e % 2], pair(x, y));
+              p[e] = pack16<T>(x, y);
+            }
+            tmem_st16(s_at + 16 * c, p);
+            if (c % 2) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_full + 16u * (c / 2) + 8u * g);
+            }
           }
-          tmem_st16(s_at + 16 * c, p);
-          if (c % 2) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 16u * (c / 2) + 8u * g);
-          }
+        };
+        if constexpr (!CAP) {
+          weights(std::false_type(), std::true_type());
+        } else {
+          if (!masked && small) weights(std::false_type(), std::true_type());
+          else if (small) weights(std::true_type(), std::true_type());
+          else weights(std::true_type(), std::false_type());
         }
         {
           float x, y;
