@@ -179,7 +179,8 @@ _PROTOS = {
     "b200moe_kv4_attend": (c_int, [_P, c_int, c_int64, _P, _P, POINTER(KvCacheDesc), c_int32, _P, _P, c_int32, c_int32,
                                    c_int32, c_int32, c_int32, c_float, c_float, _P, c_int, _P, c_size_t, _P]),
     "b200moe_prompt_attend": (c_int, [_P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, c_int32, c_int64, c_int64,
-                                      c_int32, c_int32, c_int32, c_float, c_float, _P, c_int, _P]),
+                                      c_int32, c_int32, c_int32, c_float, c_float, _P, c_int, _P, c_size_t, _P]),
+    "b200moe_prompt_attend_scratch_bytes": (c_size_t, [c_int, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32]),
     "b200moe_pipeline_bytes": (c_size_t, [_L, c_int, c_int32, c_int32]),
     "b200moe_pipeline_create": (c_int, [_L, c_int, c_int32, c_int, c_int32, _P, c_size_t, POINTER(c_void_p)]),
     "b200moe_pipeline_submit": (c_int, [_P, _P, _P, c_int32, _P]),
@@ -223,7 +224,8 @@ def _load_attention_ops():
     module.bind(B200MoeError, *(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
         "b200moe_attn_norm_rope_kv8_write", "b200moe_attn_norm_rope_kv_write", "b200moe_kv8_read", "b200moe_kv8_attend",
         "b200moe_kv8_attend_scratch_bytes", "b200moe_attn_norm_rope_kv4_write", "b200moe_kv4_read", "b200moe_kv4_attend",
-        "b200moe_kv4_attend_scratch_bytes", "b200moe_prompt_attend", "b200moe_last_error")))
+        "b200moe_kv4_attend_scratch_bytes", "b200moe_prompt_attend",
+        "b200moe_prompt_attend_scratch_bytes", "b200moe_last_error")))
     return module
 
 

@@ -31,6 +31,7 @@ decltype(&b200moe_kv4_read) read4 = nullptr;
 decltype(&b200moe_kv4_attend) attend4 = nullptr;
 decltype(&b200moe_kv4_attend_scratch_bytes) attend4_scratch = nullptr;
 decltype(&b200moe_prompt_attend) attend_prompt = nullptr;
+decltype(&b200moe_prompt_attend_scratch_bytes) attend_prompt_scratch = nullptr;
 decltype(&b200moe_last_error) last_error = nullptr;
 PyObject* error_class = nullptr;  // B200MoeError
 
@@ -193,7 +194,7 @@ const void* data(const at::Tensor& t) { return t.const_data_ptr(); }
 // bind(error class, addresses): the library's entry points
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   OPS_BEGIN
-  if (n != 12) refuse("bind takes the error class and eleven addresses");
+  if (n != 13) refuse("bind takes the error class and twelve addresses");
   auto address = [&](int i) { return reinterpret_cast<void*>(static_cast<uintptr_t>(integer(a[i]))); };
   Py_INCREF(a[0]);
   error_class = a[0];
@@ -207,7 +208,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   attend4 = reinterpret_cast<decltype(attend4)>(address(8));
   attend4_scratch = reinterpret_cast<decltype(attend4_scratch)>(address(9));
   attend_prompt = reinterpret_cast<decltype(attend_prompt)>(address(10));
-  last_error = reinterpret_cast<decltype(last_error)>(address(11));
+  attend_prompt_scratch = reinterpret_cast<decltype(attend_prompt_scratch)>(address(11));
+  last_error = reinterpret_cast<decltype(last_error)>(address(12));
   Py_RETURN_NONE;
   OPS_END
 }
@@ -443,10 +445,15 @@ PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (rows > 0) {
     const int32_t n_bs = i32(cu.size(0) - 1, "batch"), n_heads = i32(heads, "heads"), n_kv = i32(k.size(1), "kv heads");
     launch("prompt_attend", dev, [&](void* stream) {
+      // per call: other streams and captured graphs have their own
+      const size_t bytes = attend_prompt_scratch(dt, n_bs, rows, k.size(0), n_heads, n_kv, static_cast<int32_t>(hd));
+      at::Tensor scratch;
+      if (bytes > 0) scratch = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte).memory_format(std::nullopt));
       return attend_prompt(data(qr.t), data(kr.t), data(vr.t), dt, qr.stride, kr.stride, vr.stride,
                            static_cast<const int32_t*>(data(cu)), cu_k ? static_cast<const int32_t*>(data(*cu_k)) : nullptr,
                            n_bs, rows, k.size(0), n_heads, n_kv, static_cast<int32_t>(hd), static_cast<float>(scale),
-                           static_cast<float>(softcap), out.mutable_data_ptr(), out_dt, stream);
+                           static_cast<float>(softcap), out.mutable_data_ptr(), out_dt,
+                           bytes > 0 ? scratch.mutable_data_ptr() : nullptr, bytes, stream);
     });
   }
   return THPVariable_Wrap(std::move(out));

@@ -1022,8 +1022,13 @@ int launch_prompt_tc_hd(const PromptArgs& a, int hd, cudaStream_t st) {
   return hd == 64 ? launch_prompt_tc<T, 64, false>(a, st) : launch_prompt_tc<T, 128, false>(a, st);
 }
 
-// The shape of a call's items on the tensor cores.
+// The shape of a call's items on the tensor cores.  Where there are fewer items than SMs (few
+// rows, long keys) the keys of each are split: into as many parts as make the last SM finish
+// first, in units of a tile of keys (1.5 us), with two for an item's start and end and two for
+// the merge.  The lengths are on the device: all sequences are taken to be as long as the mean.
+// 4 x 60 tokens behind up to 16000, 32 heads (32 items): @SPLIT@.
 struct PromptPlan { int group, parts, tokens, splits; };
+constexpr int TP_MAX_SPLITS = 16;
 PromptPlan plan_prompt(int64_t q_rows, int64_t k_rows, int bs, int heads, int kv_heads) {
   PromptPlan p;
   const int G = heads / kv_heads;
@@ -1031,6 +1036,17 @@ PromptPlan plan_prompt(int64_t q_rows, int64_t k_rows, int bs, int heads, int kv
   p.parts = (G + p.group - 1) / p.group;
   p.tokens = 2 * (TP_ROWS / p.group);
   p.splits = 1;
+  const int64_t n = bs > 0 ? (q_rows + bs - 1) / bs : 0, m = bs > 0 ? (k_rows + bs - 1) / bs : 0;
+  const int64_t items = bs * ((n + p.tokens - 1) / p.tokens) * kv_heads * p.parts, tiles = (m + TP_KEYS - 1) / TP_KEYS;
+  if (items >= sm_count()) return p;
+  int64_t least = tiles + 2;
+  for (int s = 2; s <= TP_MAX_SPLITS && s <= tiles; ++s) {
+    const int64_t time = (items * s + sm_count() - 1) / sm_count() * ((tiles + s - 1) / s + 2) + 2;
+    if (time < least) {
+      least = time;
+      p.splits = s;
+    }
+  }
   return p;
 }
 
@@ -1041,10 +1057,19 @@ using namespace b200moe;
 
 extern "C" {
 
+size_t b200moe_prompt_attend_scratch_bytes(int dtype, int32_t bs, int64_t q_rows, int64_t k_rows, int32_t heads,
+                                           int32_t kv_heads, int32_t head_dim) {
+  if (dtype == B200MOE_DT_F32 || bs <= 0 || q_rows <= 0 || k_rows <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
+      heads % kv_heads != 0)
+    return 0;
+  const int splits = plan_prompt(q_rows, k_rows, bs, heads, kv_heads).splits;
+  return splits == 1 ? 0 : static_cast<size_t>(q_rows) * heads * splits * (head_dim + 4) * sizeof(float);
+}
+
 int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype, int64_t q_stride, int64_t k_stride,
                           int64_t v_stride, const int32_t* cu_q, const int32_t* cu_k, int32_t bs, int64_t q_rows,
                           int64_t k_rows, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, float softcap,
-                          void* out, int out_dtype, void* stream) {
+                          void* out, int out_dtype, void* scratch, size_t scratch_bytes, void* stream) {
   const char* who = "prompt_attend";
   B200_REQUIRE(bs >= 0 && q_rows >= 0 && k_rows >= 0 && heads >= 1 && kv_heads >= 1, "%s: bad sizes", who);
   B200_REQUIRE(q_rows < 0x7fffffff && k_rows < 0x7fffffff, "%s: more than 2^31 rows", who);
@@ -1062,7 +1087,14 @@ int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype
   B200_REQUIRE(q_stride >= static_cast<int64_t>(heads) * head_dim && k_stride >= static_cast<int64_t>(kv_heads) * head_dim &&
                    v_stride >= static_cast<int64_t>(kv_heads) * head_dim,
                "%s: a row stride is shorter than the row", who);
+  const size_t need = b200moe_prompt_attend_scratch_bytes(dtype, bs, q_rows, k_rows, heads, kv_heads, head_dim);
+  if (scratch_bytes < need) {
+    set_error("%s: scratch needs %zu bytes, got %zu", who, need, scratch_bytes);
+    return B200MOE_ERR_WORKSPACE;
+  }
+  B200_REQUIRE(need == 0 || (scratch != nullptr && aligned16(scratch)), "%s: scratch must be given and 16-byte aligned", who);
   PromptArgs a{};
+  a.partial = static_cast<float*>(scratch);
   a.q = q; a.k = k; a.v = v; a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
   a.cu_q = cu_q; a.cu_k = cu_k; a.out = out; a.q_rows = q_rows; a.k_rows = k_rows; a.out_dtype = out_dtype;
   a.bs = bs; a.heads = heads; a.kv_heads = kv_heads; a.scale = scale; a.softcap = softcap > 0.f ? softcap : 0.f;

@@ -197,6 +197,35 @@ def test_longer(dtype):
     _check(_call(q, k, v, cu), q, k, v, cu, cu_k)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (6, 1, 64), (130, 1, 64)])
+@pytest.mark.parametrize("lens,lens_k", [([1], [6000]), ([5, 90, 1, 0, 33], [5, 4000, 1, 700, 6500]), ([64, 2], [3500, 0]),
+                                         ([300], [2500]), ([40, 7], [20, 5000])], ids=str)
+def test_split_keys(lens, lens_k, heads, kvh, hd, dtype):
+    """Few rows, long keys: parts of the keys of a tile in several CTAs, joined; sequences of other lengths beside them."""
+    q, k, v, cu, cu_k = _inputs(lens, lens_k, heads, kvh, hd, dtype, seed=12, behind=3)
+    q[-3:], k[-3:], v[-3:] = math.nan, math.nan, math.nan
+    got = _call(q, k, v, cu, cu_k)
+    assert not got[-3:].any()
+    for t in (q, k, v):
+        t[-3:] = 0
+    _check(got, q, k, v, cu, cu_k)
+    _check(_call(q, k, v, cu, cu_k, softcap=30.0, out_dtype=F32), q, k, v, cu, cu_k, softcap=30.0, out_dtype=F32)
+    assert _status() == 0
+
+
+def test_split_keys_with_bad_values():
+    """An infinity in one part and a NaN in another: the rows that attend them."""
+    q, k, v, cu, cu_k = _inputs([60], [5000], 8, 2, 128, BF, seed=13)
+    clean = _call(q, k, v, cu, cu_k).cpu()
+    v[100, 0, 3], v[4980, 1, 7] = math.inf, math.nan
+    got = _call(q, k, v, cu, cu_k).cpu()
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    hit[:, :4, 3] = True
+    hit[40:, 4:, 7] = True  # row i attends keys up to 4940 + i
+    assert torch.equal(got[~hit], clean[~hit]) and not torch.isfinite(got[hit]).any()
+
+
 def test_nothing():
     A = _attention()
     e = lambda *s: torch.zeros(*s, dtype=BF, device="cuda")

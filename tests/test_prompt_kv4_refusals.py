@@ -84,8 +84,9 @@ def test_calls_without_work():
 
 # ------------------------------------------------------------------------ prompts
 def _prompt(q=DUMMY, k=DUMMY, v=DUMMY, dt=C.DT_BF16, qs=4096, ks=1024, vs=1024, cu=DUMMY, bs=2, rows=10, krows=10, heads=32, kvh=8,
-            hd=128, softcap=0.0, out=OUT, odt=C.DT_BF16):
-    return C.lib.b200moe_prompt_attend(q, k, v, dt, qs, ks, vs, cu, None, bs, rows, krows, heads, kvh, hd, 0.1, softcap, out, odt, None)
+            hd=128, softcap=0.0, out=OUT, odt=C.DT_BF16, scratch=DUMMY, nbytes=1 << 40):
+    return C.lib.b200moe_prompt_attend(q, k, v, dt, qs, ks, vs, cu, None, bs, rows, krows, heads, kvh, hd, 0.1, softcap, out, odt, scratch,
+                                       nbytes, None)
 
 
 @pytest.mark.parametrize("kw,message", [
@@ -96,6 +97,19 @@ def _prompt(q=DUMMY, k=DUMMY, v=DUMMY, dt=C.DT_BF16, qs=4096, ks=1024, vs=1024, 
     (dict(softcap=math.inf), "softcap"), (dict(heads=1 << 20, qs=1 << 27), "heads")])
 def test_prompt_refuses(kw, message):
     assert _prompt(**kw) == -1 and message in C.last_error()
+
+
+def test_prompt_asks_for_its_scratch():
+    """Few rows and long keys: the keys are split, and the parts need room."""
+    size = lambda *a: C.lib.b200moe_prompt_attend_scratch_bytes(*a)
+    need = size(C.DT_BF16, 1, 8, 20000, 32, 8, 128)
+    assert need > 0 and need % (8 * 32 * 132 * 4) == 0
+    kw = dict(bs=1, rows=8, krows=20000)
+    assert _prompt(**kw, nbytes=need - 1) == -3 and "scratch" in C.last_error()
+    assert _prompt(**kw, scratch=None) == -1 and "scratch" in C.last_error()
+    assert _prompt(**kw, scratch=ODD) == -1 and "scratch" in C.last_error()
+    assert size(C.DT_BF16, 1, 16384, 16384, 32, 8, 128) == 0 and size(C.DT_F32, 1, 8, 20000, 32, 8, 128) == 0
+    assert size(C.DT_BF16, 0, 8, 20000, 32, 8, 128) == 0 and size(C.DT_BF16, 1, 8, 0, 32, 8, 128) == 0
 
 
 def test_prompt_without_rows():
