@@ -311,11 +311,22 @@ __device__ __forceinline__ uint32_t tile4_at(int r, int c) {
   if constexpr (HD == 128) return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
   else return static_cast<uint32_t>(r * 32 + ((c ^ ((r >> 2) & 1)) << 4));
 }
-// mma with k = 8
-__device__ __forceinline__ void mma_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(b0));
+// the product alone: no sum to add to
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// the first of a sum (a constant once loops are unrolled), or one more
+__device__ __forceinline__ void mma_next(bool first, float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (first) mma_first(c, a0, a1, a2, a3, b0, b1);
+  else mma(c, a0, a1, a2, a3, b0, b1);
+}
+// mma_first with k = 8
+__device__ __forceinline__ void mma_first_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
 }
 // Codes as A operands, bits 0 .. 3 (HIGH: 4 .. 7, 16 times as large) of each half of w: as they
 // lie, subnormal numbers of 2^-24 (UNIT24), or CENTRED, less 8.  The MMAs align what they add by
@@ -327,6 +338,10 @@ __device__ __forceinline__ uint32_t codes_of(uint32_t w) {
   const uint32_t x = w & (HIGH ? 0x00f000f0u : 0x000f000fu);
   if constexpr (!CENTRED) return x;
   return h2_as_u32(__hsub2(u32_as_h2(x | 0x64006400u), u32_as_h2(HIGH ? 0x64806480u : 0x64086408u)));
+}
+__device__ __forceinline__ void sts_words(uint32_t to, const uint32_t (&v)[4]) { sts128(to, v); }
+__device__ __forceinline__ void sts_words(uint32_t to, const uint32_t (&v)[2]) {
+  asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to), "r"(v[0]), "r"(v[1]) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void copy_small(uint32_t dst, const void* src, bool valid) {
@@ -428,19 +443,33 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
         row = ((static_cast<uint32_t>(page) * a.blocks + a.block_index) * a.kv_heads + ahead.kvh) * 2u * a.stride + off;
       }
       live = __ballot_sync(0xffffffffu, ok);
-      const uint32_t to = ring + i * PLACE;
+      const uint32_t to = ring + i * PLACE, row0 = __shfl_sync(0xffffffffu, row, 0);
       constexpr int RPI = 32 / CH;  // rows of one pass of the warp
       const int r0 = lane / CH, c = lane % CH;
+      static_assert(RPI % 8 == 0, "passes are whole patterns of the swizzle apart");
+      if (__all_sync(0xffffffffu, ok && row == row0 + lane)) {  // within one page
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
+        for (int kv = 0; kv < 2; ++kv) {
+          const size_t first = static_cast<size_t>(row0) + (kv ? a.stride : 0);
+          const uint8_t* from = a.slab + (first + r0) * (HD / 2) + c * 16;
+          const uint32_t at = to + kv * TILE + tile4_at<HD>(r0, c);
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          const int r = j * RPI + r0;
-          const size_t from = static_cast<size_t>(__shfl_sync(0xffffffffu, row, r)) + (kv ? a.stride : 0);
-          copy16(to + kv * TILE + tile4_at<HD>(r, c), a.slab + from * (HD / 2) + c * 16, live >> r & 1);
+          for (int j = 0; j < CH; ++j) copy16(at + j * RPI * (HD / 2), from + j * RPI * (HD / 2), true);
+          copy_small<CH * 4>(to + 2 * TILE + kv * STILE + lane * (CH * 4),
+                             reinterpret_cast<const uint8_t*>(a.scales) + (first + lane) * (CH * 4), true);
         }
-        copy_small<CH * 4>(to + 2 * TILE + kv * STILE + lane * (CH * 4),
-                           reinterpret_cast<const uint8_t*>(a.scales) + (static_cast<size_t>(row) + (kv ? a.stride : 0)) * (CH * 4), ok);
+      } else {
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            const int r = j * RPI + r0;
+            const size_t from = static_cast<size_t>(__shfl_sync(0xffffffffu, row, r)) + (kv ? a.stride : 0);
+            copy16(to + kv * TILE + tile4_at<HD>(r, c), a.slab + from * (HD / 2) + c * 16, live >> r & 1);
+          }
+          copy_small<CH * 4>(to + 2 * TILE + kv * STILE + lane * (CH * 4),
+                             reinterpret_cast<const uint8_t*>(a.scales) + (static_cast<size_t>(row) + (kv ? a.stride : 0)) * (CH * 4), ok);
+        }
       }
       ++unit;
     }
@@ -563,26 +592,35 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
         for (int c = 0; c < CH; ++c) top = __vmaxu2(top, w[c] & 0x7fff7fffu);
         const bool bad = (top & 0xffffu) >= 0x7c00u || top >= 0x7c000000u, dead = !(live_now >> lane & 1);
         const float2 f = __half22float2(u32_as_h2(top));
-        const float most = fmaxf(fmaxf(f.x * 16.f, f.y), UNIT24);
-        const int e = bad ? 0 : static_cast<int>(__float_as_uint(most) >> 23) - 126;  // -23 .. 21
+        const float most = fmaxf(fmaxf(f.x * 16.f, f.y), 2.f * UNIT24);
+        const int e = bad ? 0 : static_cast<int>(__float_as_uint(most) >> 23) - 126;  // -22 .. 21
         const float shrink = bad ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
         s_pos[warp][lane] = make_float2(dead ? -INFINITY : bad ? __int_as_float(0x7fffffff) : static_cast<float>(e),
                                         dead ? 0.f : bad ? 1.f : shrink);
-        // even lanes put down the scales of two positions, odd ones their offsets
-        uint32_t* to = lane & 1 ? s_mv[0][warp][lane >> 1] : s_sv[warp][lane >> 1];
+        // Times 2^(4 - e) and 2^-e in two steps, each within fp16's range; a bad position's are zeros.
+        // Even lanes put down the scales of two positions, odd ones their offsets.
+        const int e1 = e >> 1, e2 = e - e1;
+        const uint32_t by1 = static_cast<uint32_t>((4 - e1 + 15) << 10 | (15 - e1) << 26), by_2 = bad ? 0u : static_cast<uint32_t>((15 - e2) << 10 | (15 - e2) << 26);
+        const uint32_t choose = lane & 1 ? 0x3276u : 0x5410u;
+        uint32_t both[CH], lower[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          float2 y = __half22float2(u32_as_h2(w[c]));
-          y = bad ? make_float2(0.f, 0.f) : make_float2(y.x * shrink, y.y * shrink);
-          if constexpr (SPLIT) y.y = fmaf(8.f, y.x, y.y);
-          const __half2 h = __floats2half2_rn(y.x * 16.f, y.y);
-          const uint32_t own = h2_as_u32(h), other = __shfl_xor_sync(0xffffffffu, own, 1);
-          to[c] = lane & 1 ? __byte_perm(other, own, 0x7632) : __byte_perm(own, other, 0x5410);
+          uint32_t own;
           if constexpr (SPLIT) {
-            const uint32_t low = h2_as_u32(__float2half2_rn(y.y - __high2float(h))), low_other = __shfl_xor_sync(0xffffffffu, low, 1);
-            if (lane & 1) s_mv[PARTS - 1][warp][lane >> 1][c] = __byte_perm(low_other, low, 0x5410);
+            float2 y = __half22float2(u32_as_h2(w[c]));
+            y = bad ? make_float2(0.f, 0.f) : make_float2(y.x * shrink, fmaf(8.f, y.x, y.y) * shrink);
+            const __half2 h = __floats2half2_rn(y.x * 16.f, y.y);
+            own = h2_as_u32(h);
+            const uint32_t low = h2_as_u32(__float2half2_rn(y.y - __high2float(h)));
+            lower[c] = __byte_perm(low, __shfl_xor_sync(0xffffffffu, low, 1), choose);
+          } else {
+            own = bad ? 0u : h2_as_u32(__hmul2(__hmul2(u32_as_h2(w[c]), u32_as_h2(by1)), u32_as_h2(by_2)));
           }
+          both[c] = __byte_perm(own, __shfl_xor_sync(0xffffffffu, own, 1), choose);
         }
+        sts_words(smem_u32(lane & 1 ? &s_mv[0][warp][lane >> 1][0] : &s_sv[warp][lane >> 1][0]), both);
+        if constexpr (SPLIT)
+          if (lane & 1) sts_words(smem_u32(&s_mv[PARTS - 1][warp][lane >> 1][0]), lower);
       }
       __syncwarp();
       const int p0 = cur.p_begin + u * AT_STEP;
@@ -617,9 +655,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
-            if constexpr (SPLIT) mma(s[h][n], a0, a1, b0, b1, qs[n], qs[n]);
-            else mma_k8(s[h][n], a0, a1, qs[n]);
+            if constexpr (SPLIT) mma_first(s[h][n], a0, a1, b0, b1, qs[n], qs[n]);
+            else mma_first_k8(s[h][n], a0, a1, qs[n]);
             if constexpr (!SPLIT) {
 #pragma unroll
               for (int k = 0; k < 4; ++k) s[h][n][k] *= UNIT24;
@@ -636,11 +673,10 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
             float acc[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 #pragma unroll
               for (int p = 0; p < PARTS; ++p) {
                 const uint32_t* q = qb[p][n][c + i];
-                mma(acc[n], codes_of<false, SPLIT>(x0), codes_of<false, SPLIT>(x1), codes_of<true, SPLIT>(x0), codes_of<true, SPLIT>(x1), q[0], q[1]);
+                mma_next(p == 0, acc[n], codes_of<false, SPLIT>(x0), codes_of<false, SPLIT>(x1), codes_of<true, SPLIT>(x0), codes_of<true, SPLIT>(x1), q[0], q[1]);
                 mma(acc[n], codes_of<false, SPLIT>(y0), codes_of<false, SPLIT>(y1), codes_of<true, SPLIT>(y0), codes_of<true, SPLIT>(y1), q[2], q[3]);
               }
               const float s0 = __low2float(u32_as_h2(w0[c + i])), s1 = __low2float(u32_as_h2(w1[c + i]));
@@ -697,20 +733,17 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float v = top[n][e];
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          top[n][e] = v;
-          moves |= v > m[n][e] + P_SLACK;
-        }
+        for (int e = 0; e < 2; ++e) moves |= top[n][e] > m[n][e] + P_SLACK;
       if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float m_new = fmaxf(m[n][e], top[n][e]);
+            float v = top[n][e];
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+            const float m_new = fmaxf(m[n][e], v);
             const float root = m_new == -INFINITY ? 1.f : state_root(m[n][e], m_new), alpha = root * root;
             m[n][e] = m_new;
             l[n][e] = l[n][e] * root * root;
@@ -745,8 +778,6 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
       {
         float unit[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) unit[n][0] = unit[n][1] = unit[n][2] = unit[n][3] = 0.f;
-#pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < PARTS; ++i) {
@@ -754,7 +785,8 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
 #pragma unroll
             for (int p = 0; p < P_PARTS - i; ++p)
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma(unit[n], a0, 0u, a2, 0u, pb[p][n][h][0], pb[p][n][h][1]);
+              for (int n = 0; n < NT; ++n)
+                mma_next(h + i + p == 0, unit[n], a0, 0u, a2, 0u, pb[p][n][h][0], pb[p][n][h][1]);
           }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -762,6 +794,16 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
           om[n][1] += unit[n][1];
         }
       }
+      // scales of the positions 2 tig, + 1 and eight behind them, of both halves
+      uint32_t sv[2][2][CH];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t at = smem_u32(&s_sv[warp][8 * h + 4 * j + tig][0]);
+          if constexpr (CH == 4) lds128(at, sv[h][j]);
+          else lds64(at, sv[h][j]);
+        }
 #pragma unroll
       for (int c = 0; c < CH; c += 2) {
         uint32_t w[2][4];
@@ -771,24 +813,20 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
         for (int i = 0; i < 2; ++i) {
           float unit[NT][2][4];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) unit[n][0][k] = unit[n][1][k] = 0.f;
-#pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t x0 = w[h][2 * i], x1 = w[h][2 * i + 1], y0 = x0 >> 8, y1 = x1 >> 8;
-            const __half2 s0 = u32_as_h2(s_sv[warp][8 * h + tig][c + i]), s1 = u32_as_h2(s_sv[warp][8 * h + 4 + tig][c + i]);
-            auto products = [&](int n, uint32_t b0, uint32_t b1) {
-              mma(unit[n][0], codes_of<false, SPLIT>(x0), codes_of<true, SPLIT>(x0), codes_of<false, SPLIT>(x1), codes_of<true, SPLIT>(x1), b0, b1);
-              mma(unit[n][1], codes_of<false, SPLIT>(y0), codes_of<true, SPLIT>(y0), codes_of<false, SPLIT>(y1), codes_of<true, SPLIT>(y1), b0, b1);
+            const __half2 s0 = u32_as_h2(sv[h][0][c + i]), s1 = u32_as_h2(sv[h][1][c + i]);
+            auto products = [&](bool first, int n, uint32_t b0, uint32_t b1) {
+              mma_next(first, unit[n][0], codes_of<false, SPLIT>(x0), codes_of<true, SPLIT>(x0), codes_of<false, SPLIT>(x1), codes_of<true, SPLIT>(x1), b0, b1);
+              mma_next(first, unit[n][1], codes_of<false, SPLIT>(y0), codes_of<true, SPLIT>(y0), codes_of<false, SPLIT>(y1), codes_of<true, SPLIT>(y1), b0, b1);
             };
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const __half2 p0 = u32_as_h2(pb[0][n][h][0]), p1 = u32_as_h2(pb[0][n][h][1]);
               const __half2 b0 = __hmul2(p0, s0), b1 = __hmul2(p1, s1);
-              products(n, h2_as_u32(b0), h2_as_u32(b1));
+              products(h == 0, n, h2_as_u32(b0), h2_as_u32(b1));
               if constexpr (P_PARTS == 2)  // what the product lost, and the lower part's
-                products(n, h2_as_u32(__hfma2(u32_as_h2(pb[P_PARTS - 1][n][h][0]), s0, __hfma2(p0, s0, __hneg2(b0)))),
+                products(false, n, h2_as_u32(__hfma2(u32_as_h2(pb[P_PARTS - 1][n][h][0]), s0, __hfma2(p0, s0, __hneg2(b0)))),
                          h2_as_u32(__hfma2(u32_as_h2(pb[P_PARTS - 1][n][h][1]), s1, __hfma2(p1, s1, __hneg2(b1)))));
             }
           }
