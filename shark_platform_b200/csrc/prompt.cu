@@ -133,31 +133,25 @@ __device__ __forceinline__ void zero_rest(const PromptArgs& a, int hd, int threa
 }
 
 // ------------------------------------------------------------------ 32-bit rows
-// Tiles of 64 rows and 64 keys on the fp32 units: thread (ty, tx) of 16 x 16 has rows
-// 4 ty .. + 3, keys tx + 16 j of the scores and elements 4 tx + 64 j .. + 3 of the output.
-// Everything is fp32.
-constexpr int SP_ROWS = 64, SP_KEYS = 64, SP_THREADS = 256;
+// Tiles of 64 (heads of 64) or 128 rows and 64 keys on the fp32 units: thread (ty, tx) of 8 or
+// 16 by 16 has rows 8 ty .. + 7, keys tx + 16 j of the scores and elements 4 tx + 64 n .. + 3 of the output, so
+// that 16 bytes from shared memory serve eight or four products.  K of the next tile is on its
+// way while the softmax and V's products of this one run, V during the scores.  Everything is
+// fp32.
+constexpr int SP_KEYS = 64, SP_R = 8;
+template <int HD>
+struct SpCfg {
+  // as many CTAs as shared memory and registers hold: 3 of 128 threads, 1 of 256
+  static constexpr int ROWS = HD == 64 ? 64 : 128, THREADS = 2 * ROWS, RESIDENT = HD == 64 ? 3 : 1;
+  static constexpr int PITCH = HD + 4, PP = SP_KEYS + 4;
+  static constexpr int SMEM = ((ROWS + 2 * SP_KEYS) * PITCH + ROWS * PP) * 4;
+};
 
 template <int HD>
-__device__ __forceinline__ void load_tile(float* to, int pitch, const float* from, int64_t stride, int rows, int have) {
-  constexpr int C = HD / 8;
-  for (int i = threadIdx.x; i < rows * C; i += SP_THREADS) {
-    const int r = i / C, c = i % C;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (r < have) {
-      Raw8<float> raw;
-      raw.load(from + r * stride + c * 8);
-      raw.get(x);
-    }
-    store8(to + r * pitch + c * 8, x);
-  }
-}
-
-template <int HD>
-__global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const PromptArgs a) {
-  constexpr int PITCH = HD + 4, PP = SP_KEYS + 4, NO = HD / 64;
+__global__ void __launch_bounds__(SpCfg<HD>::THREADS, SpCfg<HD>::RESIDENT) prompt_attend_kernel(const PromptArgs a) {
+  constexpr int SP_ROWS = SpCfg<HD>::ROWS, SP_THREADS = SpCfg<HD>::THREADS, PITCH = SpCfg<HD>::PITCH, PP = SpCfg<HD>::PP, NO = HD / 64, C = HD / 4;
   extern __shared__ __align__(16) float sp_smem[];
-  float *sq = sp_smem, *skv = sq + SP_ROWS * PITCH, *sp = skv + SP_KEYS * PITCH;
+  float *sq = sp_smem, *sk = sq + SP_ROWS * PITCH, *sv = sk + SP_KEYS * PITCH, *sp = sv + SP_KEYS * PITCH;
   grid_dep_wait();
   grid_dep_launch();
   const int t = threadIdx.x, lane = t & 31, ty = t >> 4, tx = t & 15;
@@ -172,107 +166,115 @@ __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const Prom
     const int tok0 = it.tile * a.tokens, toks = min(a.tokens, qs.len - tok0);
     const int h0 = it.part * a.group, hs = min(a.group, G - h0), rows = toks * hs;
     const int shift = ks.len - qs.len;  // row i sees keys up to i + shift
-    const int keys = max(0, min(ks.len, tok0 + toks + shift));
-    __syncthreads();  // the last item's tiles are read
-    for (int j = t; j < SP_ROWS * (HD / 8); j += SP_THREADS) {
-      const int r = j / (HD / 8), c = j % (HD / 8);
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (r < rows) {
-        Raw8<float> raw;
-        raw.load(q + (static_cast<int64_t>(qs.begin) + tok0 + r / hs) * a.q_stride +
-                 static_cast<int64_t>(it.kvh * G + h0 + r % hs) * HD + c * 8);
-        raw.get(x);
+    const int keys = keys_seen(qs.len, ks.len, tok0, toks);
+    // 64 rows of K or V from key k0 on, zeros behind the last key; one group of copies
+    auto fetch = [&](float* to, const float* from, int64_t stride, int k0) {
+      from += (static_cast<int64_t>(ks.begin) + k0) * stride + it.kvh * HD;
+#pragma unroll
+      for (int i = 0; i < SP_KEYS * C / SP_THREADS; ++i) {
+        const int e = i * SP_THREADS + t, j = e / C, c = e % C * 4;
+        const bool some = k0 + j < keys;
+        copy16(smem_u32(to + j * PITCH + c), some ? from + j * stride + c : from, some);
       }
-      store8(sq + r * PITCH + c * 8, x);
+      copy_commit();
+    };
+    __syncthreads();  // the last item's tiles are read
+    if (keys > 0) fetch(sk, k, a.k_stride, 0);
+    for (int e = t; e < SP_ROWS * C; e += SP_THREADS) {
+      const int j = e / C, c = e % C * 4;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j < rows)
+        x = *reinterpret_cast<const float4*>(q + (static_cast<int64_t>(qs.begin) + tok0 + j / hs) * a.q_stride +
+                                             static_cast<int64_t>(it.kvh * G + h0 + j % hs) * HD + c);
+      *reinterpret_cast<float4*>(sq + j * PITCH + c) = x;
     }
-    int seen[4];  // keys that this thread's rows see
+    float m[SP_R], l[SP_R], o[SP_R][NO][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) seen[r] = min(ks.len, tok0 + (4 * ty + r) / hs + shift + 1);
-    float m[4], l[4], o[4][NO][4];
+    for (int i = 0; i < SP_R; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      m[r] = -INFINITY;
-      l[r] = 0.f;
-#pragma unroll
-      for (int n = 0; n < NO; ++n) o[r][n][0] = o[r][n][1] = o[r][n][2] = o[r][n][3] = 0.f;
+      for (int n = 0; n < NO; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
     }
     for (int k0 = 0; k0 < keys; k0 += SP_KEYS) {
-      const int have = min(SP_KEYS, keys - k0);
-      __syncthreads();
-      load_tile<HD>(skv, PITCH, k + (static_cast<int64_t>(ks.begin) + k0) * a.k_stride + it.kvh * HD, a.k_stride, SP_KEYS, have);
-      __syncthreads();
-      float s[4][4] = {};
-#pragma unroll 4
+      copy_wait<0>();
+      __syncthreads();  // K is there, V of the last tile is read
+      fetch(sv, v, a.v_stride, k0);
+      float s[SP_R][4] = {};
+#pragma unroll 2
       for (int d = 0; d < HD; d += 4) {
-        float4 x[4], y[4];
+        float4 y[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const float4*>(sq + (4 * ty + r) * PITCH + d);
+        for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * PITCH + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(skv + (tx + 16 * j) * PITCH + d);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int i = 0; i < SP_R; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(sq + (SP_R * ty + i) * PITCH + d);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            s[r][j] = fmaf(x[r].x, y[j].x, s[r][j]);
-            s[r][j] = fmaf(x[r].y, y[j].y, s[r][j]);
-            s[r][j] = fmaf(x[r].z, y[j].z, s[r][j]);
-            s[r][j] = fmaf(x[r].w, y[j].w, s[r][j]);
+            s[i][j] = fmaf(x.x, y[j].x, s[i][j]);
+            s[i][j] = fmaf(x.y, y[j].y, s[i][j]);
+            s[i][j] = fmaf(x.z, y[j].z, s[i][j]);
+            s[i][j] = fmaf(x.w, y[j].w, s[i][j]);
           }
+        }
       }
-      __syncthreads();  // K is read: V takes its place
-      load_tile<HD>(skv, PITCH, v + (static_cast<int64_t>(ks.begin) + k0) * a.v_stride + it.kvh * HD, a.v_stride, SP_KEYS, have);
+      __syncthreads();  // K is read: the next one takes its place
+      if (k0 + SP_KEYS < keys) fetch(sk, k, a.k_stride, k0 + SP_KEYS);
+      // where not all rows see all keys, a weight of zero leaves infinities and NaN out
+      const bool masked = k0 + SP_KEYS > tok0 + shift + 1;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int i = 0; i < SP_R; ++i) {
+        const int seen = masked ? min(ks.len, tok0 + (SP_R * ty + i) / hs + shift + 1) - k0 : SP_KEYS;
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float x = s[r][j] * to_score;
+          float x = s[i][j] * to_score;
           if (a.softcap > 0.f) x = cap2 * tanhf(x);
-          s[r][j] = k0 + tx + 16 * j < seen[r] ? x : -INFINITY;
-          top = fmaxf(top, s[r][j]);
+          s[i][j] = tx + 16 * j < seen ? x : -INFINITY;
+          top = fmaxf(top, s[i][j]);
         }
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        const float m_new = fmaxf(m[r], top), base = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = exp2f(m[r] - base);
-        m[r] = m_new;
+        const float m_new = fmaxf(m[i], top), from = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2f(m[i] - from);
+        m[i] = m_new;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float p = exp2f(s[r][j] - base);
+          const float p = exp2f(s[i][j] - from);
           sum += p;
-          sp[(4 * ty + r) * PP + tx + 16 * j] = p;
+          sp[(SP_R * ty + i) * PP + tx + 16 * j] = p;
         }
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        l[r] = fmaf(l[r], alpha, sum);
+        l[i] = fmaf(l[i], alpha, sum);
 #pragma unroll
         for (int n = 0; n < NO; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[r][n][e] *= alpha;
+          for (int e = 0; e < 4; ++e) o[i][n][e] *= alpha;
       }
-      __syncthreads();
-      // where not all rows see all keys, a weight of zero leaves infinities and NaN out
-      const bool masked = k0 + SP_KEYS > tok0 + shift + 1;
+      if (k0 + SP_KEYS < keys) copy_wait<1>();
+      else copy_wait<0>();
+      __syncthreads();  // V is there, and the weights
       auto products = [&](auto some) {
-#pragma unroll 2
+#pragma unroll 1
         for (int j = 0; j < SP_KEYS; j += 4) {
-          float4 p[4];
+          float4 p[SP_R];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(sp + (4 * ty + r) * PP + j);
+          for (int i = 0; i < SP_R; ++i) p[i] = *reinterpret_cast<const float4*>(sp + (SP_R * ty + i) * PP + j);
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
             for (int n = 0; n < NO; ++n) {
-              const float4 y = *reinterpret_cast<const float4*>(skv + (j + jj) * PITCH + 4 * tx + 64 * n);
+              const float4 y = *reinterpret_cast<const float4*>(sv + (j + jj) * PITCH + 4 * tx + 64 * n);
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float w = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
+              for (int i = 0; i < SP_R; ++i) {
+                const float w = jj == 0 ? p[i].x : jj == 1 ? p[i].y : jj == 2 ? p[i].z : p[i].w;
                 if (decltype(some)::value && w == 0.f) continue;
-                o[r][n][0] = fmaf(w, y.x, o[r][n][0]);
-                o[r][n][1] = fmaf(w, y.y, o[r][n][1]);
-                o[r][n][2] = fmaf(w, y.z, o[r][n][2]);
-                o[r][n][3] = fmaf(w, y.w, o[r][n][3]);
+                o[i][n][0] = fmaf(w, y.x, o[i][n][0]);
+                o[i][n][1] = fmaf(w, y.y, o[i][n][1]);
+                o[i][n][2] = fmaf(w, y.z, o[i][n][2]);
+                o[i][n][3] = fmaf(w, y.w, o[i][n][3]);
               }
             }
         }
@@ -281,16 +283,16 @@ __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const Prom
       else products(std::false_type());
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 4 * ty + r;
+    for (int i = 0; i < SP_R; ++i) {
+      const int row = SP_R * ty + i;
       if (row >= rows) continue;
-      const float f = l[r] == 0.f ? 0.f : 1.f / l[r];
+      const float f = l[i] == 0.f ? 0.f : 1.f / l[i];
       const size_t to = ((static_cast<size_t>(qs.begin) + tok0 + row / hs) * a.heads + it.kvh * G + h0 + row % hs) * HD + 4 * tx;
 #pragma unroll
       for (int n = 0; n < NO; ++n) {
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = l[r] == 0.f ? 0.f : o[r][n][e] * f;
+        for (int e = 0; e < 4; ++e) y[e] = l[i] == 0.f ? 0.f : o[i][n][e] * f;
         store_as(a.out, a.out_dtype, to + 64 * n, y);
       }
     }
@@ -300,19 +302,20 @@ __global__ void __launch_bounds__(SP_THREADS, 2) prompt_attend_kernel(const Prom
 
 template <int HD>
 int launch_prompt(PromptArgs& a, cudaStream_t st) {
-  constexpr int SMEM = (2 * SP_ROWS * (HD + 4) + SP_ROWS * (SP_KEYS + 4)) * 4;
   const int G = a.heads / a.kv_heads;
-  a.group = G < SP_ROWS ? G : SP_ROWS;
+  constexpr int ROWS = SpCfg<HD>::ROWS;
+  a.group = G < ROWS ? G : ROWS;
   a.parts = (G + a.group - 1) / a.group;
-  a.tokens = SP_ROWS / a.group;
+  a.tokens = ROWS / a.group;
   a.splits = 1;
   auto kern = prompt_attend_kernel<HD>;
-  B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-  const int64_t items = (a.q_rows / a.tokens + a.bs) * a.kv_heads * a.parts + 1, resident = 2ll * sm_count();
-  B200_CHECK_CUDA(launch_dependent(kern, dim3(static_cast<unsigned>(items < resident ? items : resident)), dim3(SP_THREADS), SMEM,
-                                   st, a));
+  B200_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SpCfg<HD>::SMEM));
+  const int64_t items = (a.q_rows / a.tokens + a.bs) * a.kv_heads * a.parts + 1, resident = static_cast<int64_t>(sm_count()) * SpCfg<HD>::RESIDENT;
+  B200_CHECK_CUDA(launch_dependent(kern, dim3(static_cast<unsigned>(items < resident ? items : resident)), dim3(SpCfg<HD>::THREADS),
+                                   SpCfg<HD>::SMEM, st, a));
   return B200MOE_OK;
 }
+
 // ------------------------------------------------------------------ tensor cores
 // 16-bit rows: an item is two tiles of 128 rows, S = Q K^T and O += P V by tcgen05.mma with the
 // accumulators in tensor memory (S0, S1, O0, O1: all 512 columns at 128 elements a head).
