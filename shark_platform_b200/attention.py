@@ -26,10 +26,11 @@ What runs where:
   * the four projections: one dense product each (q, k and v fused into one) —
     a library GEMM for dense weights, this library's quantized linear for Q8_0 /
     Q4_K / Q4_1 weights;
-  * the prefill attention core over the freshly computed K/V: torch's fused
-    scaled-dot-product attention, which the reference also offers as
-    `attention_kernel="torch"` (:215-224); with a softcap (Grok) the decomposed
-    torch operators, since the fused kernel has no cap.
+  * the prefill attention core over the freshly computed K/V: with
+    `attention_kernel="b200"` this library's `prompt_attend`, as with a cache of 4-bit
+    codes and no mask; else torch's fused scaled-dot-product attention, which the
+    reference also offers as `attention_kernel="torch"` (:215-224); with a softcap (Grok)
+    the decomposed torch operators, since the fused kernel has no cap.
 
 There is no CPU path: CPU tensors are rejected.
 """
@@ -229,7 +230,11 @@ def _is_quantized(t) -> bool:
 
 class B200PagedAttentionBlock(torch.nn.Module):
     """Drop-in for PagedLlamaAttentionBlock (same constructor keywords, same
-    `forward` keywords)."""
+    `forward` keywords).
+
+    `attention_kernel="b200"` takes `prompt_attend` for prompts.  It is causal by itself: of
+    an `attention_mask` it takes for granted that it is the causal one, with any padding
+    behind a sequence's tokens (the rows of padding are attended too and mean nothing)."""
 
     def __init__(self, theta, *, block_index: int, cache, head_count: int, head_dim: int, head_count_kv: int,
                  rms_epsilon: float, attention_kernel: str = "decomposed", attention_scale: Optional[float] = None,
@@ -242,10 +247,10 @@ class B200PagedAttentionBlock(torch.nn.Module):
         self.attention_kernel, self.attention_scale, self.softcap = attention_kernel, attention_scale, softcap
         if "kv_cache" in getattr(theta, "keys", ()):
             raise C.B200MoeError("a quantized KV cache (kv_cache.quantizer) is not supported: its one scale per tensor "
-                                 "is replaced by PagedKVCache(dtype=torch.int8 or torch.float8_e4m3fn)")
+                                 "is replaced by PagedKVCache(dtype=torch.int8, torch.float8_e4m3fn or torch.uint8)")
         self._quantized = bool(getattr(cache, "quantized", False))
         if head_count % head_count_kv != 0 or (head_count // head_count_kv > 8 and not self._quantized):
-            raise C.B200MoeError("head_count must be 1..8 times head_count_kv (any multiple with an 8-bit cache)")
+            raise C.B200MoeError("head_count must be 1..8 times head_count_kv (any multiple with an 8- or 4-bit cache)")
         if head_dim not in (64, 128):
             raise C.B200MoeError(f"head_dim {head_dim}: 64 and 128 are built")
         if cache.attn_head_count != head_count_kv or cache.attn_head_dim != head_dim:
@@ -308,6 +313,32 @@ class B200PagedAttentionBlock(torch.nn.Module):
             self._freqs = freqs[0::2].contiguous().to(device)
         return self._freqs
 
+    def _torch_attention(self, q, k, v, attention_mask, before, scale):
+        """Prefill by torch's operators: q [bs, sl, heads, hd], k and v [bs, before + sl, kv_heads, hd]."""
+        bs, sl, H, hd = q.shape
+        Hkv = k.shape[2]
+        qh, kh, vh = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+        mask = None if attention_mask is None else attention_mask.to(q.dtype)
+        if before:
+            if mask is None:
+                mask = torch.full((sl, before + sl), float("-inf"), device=q.device, dtype=q.dtype).triu(before + 1)
+            elif mask.shape[-1] == sl:
+                mask = F.pad(mask, (before, 0))
+        if self.softcap is None:
+            attn = F.scaled_dot_product_attention(qh, kh, vh, attn_mask=mask, is_causal=mask is None, scale=scale,
+                                                  enable_gqa=H != Hkv)
+        else:
+            rep = H // Hkv
+            kh, vh = kh.repeat_interleave(rep, dim=1), vh.repeat_interleave(rep, dim=1)
+            w = torch.matmul(qh, kh.transpose(2, 3)) * scale
+            w = self.softcap * torch.tanh(w / self.softcap)
+            if mask is not None:
+                w = w + mask
+            else:
+                w = w + torch.full((sl, sl), float("-inf"), device=q.device, dtype=w.dtype).triu(1)
+            attn = torch.matmul(torch.softmax(w.float(), dim=-1).to(qh.dtype), vh)
+        return attn.transpose(1, 2)
+
     # --------------------------------------------------------------- forward
     def forward(self, h: torch.Tensor, *, embedding, seq_block_ids: torch.Tensor,
                 start_index: Optional[int] = None, start_positions: Optional[torch.Tensor] = None,
@@ -315,7 +346,7 @@ class B200PagedAttentionBlock(torch.nn.Module):
                 cache_state: list = None, xk_temp: Optional[torch.Tensor] = None,
                 xv_temp: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """`new_lens` [bs] (prefill; not in the reference): how many of each sequence's rows are
-        tokens; padding behind them is not written to the cache.  With an 8-bit cache a decode
+        tokens; padding behind them is not written to the cache.  With an 8- or 4-bit cache a decode
         step may bring up to 16 tokens per sequence (each attends the ones before it), a
         negative start position marks a padding sequence, and a prefill with start_index > 0
         attends the cached positions before it too (an attention_mask then covers the new
@@ -346,7 +377,7 @@ class B200PagedAttentionBlock(torch.nn.Module):
         one_pass = (self._quantized or use_hf or new_lens is not None or self._q_norm_w is not None or
                     self._k_norm_w is not None)
         if one_pass and not decode and (int(start_index) < 0 or (int(start_index) > 0 and not self._quantized)):
-            raise C.B200MoeError(f"a prefill from position {int(start_index)}: continued prompts are for 8-bit caches "
+            raise C.B200MoeError(f"a prefill from position {int(start_index)}: continued prompts are for 8- and 4-bit caches "
                                  "(the positions before it would not be attended)")
         hc = h.contiguous()
         # the output projection with the residual, in one call
@@ -421,35 +452,24 @@ class B200PagedAttentionBlock(torch.nn.Module):
                     _p(scratch), nbytes, _moe._stream()), "attn_decode")
             attn = out.view(bs, 1, H * hd)
         else:
-            qh = q.view(bs, sl, H, hd).transpose(1, 2)
             kh = k.view(bs, sl, Hkv, hd)
             vh = v.view(bs, sl, Hkv, hd)
-            mask = None if attention_mask is None else attention_mask.to(q.dtype)
             before = int(start_index) if self._quantized else 0
+            own = self.attention_kernel == "b200" or (getattr(self.cache, "dtype", None) == torch.uint8 and attention_mask is None)
             if before:  # a continued prompt: the cached positions, then the new ones as they are
                 kc, vc = kv_read(self.cache, cache_state, block_index=self.block_index, seq_block_ids=page_ids,
                                  seq_lens=torch.full((bs,), before, device=dev, dtype=torch.int32), max_seq_len=before,
                                  dtype=q.dtype)
                 kh, vh = torch.cat([kc, kh], dim=1), torch.cat([vc, vh], dim=1)
-                if mask is None:
-                    mask = torch.full((sl, before + sl), float("-inf"), device=dev, dtype=q.dtype).triu(before + 1)
-                elif mask.shape[-1] == sl:
-                    mask = F.pad(mask, (before, 0))
-            kh, vh = kh.transpose(1, 2), vh.transpose(1, 2)
-            if self.softcap is None:
-                attn = F.scaled_dot_product_attention(qh, kh, vh, attn_mask=mask, is_causal=mask is None,
-                                                      scale=scale, enable_gqa=H != Hkv)
+            if own:
+                cu = torch.arange(bs + 1, device=dev, dtype=torch.int32)
+                rows = lambda x, heads: x.detach().reshape(-1, heads, hd)
+                attn = prompt_attend(rows(q, H), rows(kh, Hkv), rows(vh, Hkv), cu_seqlens=cu * sl,
+                                     cu_seqlens_k=cu * (before + sl) if before else None, scale=float(scale),
+                                     softcap=self.softcap, out_dtype=torch.float16 if direct else q.dtype)
             else:
-                rep = H // Hkv
-                kh, vh = kh.repeat_interleave(rep, dim=1), vh.repeat_interleave(rep, dim=1)
-                w = torch.matmul(qh, kh.transpose(2, 3)) * scale
-                w = self.softcap * torch.tanh(w / self.softcap)
-                if mask is not None:
-                    w = w + mask
-                else:
-                    w = w + torch.full((sl, sl), float("-inf"), device=dev, dtype=w.dtype).triu(1)
-                attn = torch.matmul(torch.softmax(w.float(), dim=-1).to(qh.dtype), vh)
-            attn = attn.transpose(1, 2).reshape(bs, sl, H * hd)
+                attn = self._torch_attention(q.view(bs, sl, H, hd), kh, vh, attention_mask, before, scale)
+            attn = attn.reshape(bs, sl, H * hd)
         if fused_out:
             y, = _moe.linear_rows(attn.reshape(bs * sl, H * hd), [_moe.prepare_linear(self._wo)],
                                   residual=hc.view(bs * sl, d), out_dtype=h.dtype)
@@ -460,11 +480,12 @@ class B200PagedAttentionBlock(torch.nn.Module):
         return h + y
 
 
-def patch_attention_blocks(model) -> int:
+def patch_attention_blocks(model, attention_kernel: Optional[str] = None) -> int:
     """Replaces every PagedLlamaAttentionBlock-shaped child of `model` (anything
     with `.theta`, `.cache`, `.head_count_kv` and `.block_index`) by a
-    B200PagedAttentionBlock built from the same theta and cache.  Returns the
-    number of blocks replaced."""
+    B200PagedAttentionBlock built from the same theta and cache, with the child's
+    `attention_kernel` or the one given ("b200").  Returns the number of blocks
+    replaced."""
     replaced = 0
     for parent in list(model.modules()):
         for name, child in list(parent.named_children()):
@@ -475,7 +496,7 @@ def patch_attention_blocks(model) -> int:
             new = B200PagedAttentionBlock(
                 child.theta, block_index=child.block_index, cache=child.cache, head_count=child.head_count,
                 head_dim=child.head_dim, head_count_kv=child.head_count_kv, rms_epsilon=child.attn_norm.epsilon,
-                attention_kernel=getattr(child, "attention_kernel", "decomposed"),
+                attention_kernel=attention_kernel or getattr(child, "attention_kernel", "decomposed"),
                 attention_scale=getattr(child, "attention_scale", None), softcap=getattr(child, "softcap", None))
             setattr(parent, name, new)
             replaced += 1
