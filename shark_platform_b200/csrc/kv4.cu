@@ -40,20 +40,24 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[8], int first, __h
     lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  held = __halves2half2(__float2half_rn(__fdiv_rn(hi - lo, 15.f)), __float2half_rn(lo));
+  // (hi - lo) / 15, rounded: the quotient by the rounded reciprocal, then by what it leaves
+  const float range = hi - lo, near = range * (1.f / 15.f), fifteenth = fmaf(fmaf(-15.f, near, range), 1.f / 15.f, near);
+  held = __halves2half2(__float2half_rn(fifteenth), __float2half_rn(lo));
   const uint32_t bits = h2_as_u32(held);
   if ((bits & 0x7c00u) == 0x7c00u || (bits & 0x7c000000u) == 0x7c000000u) held = u32_as_h2(0x7fff7fffu);
   const float s = __low2float(held), m = __high2float(held);
   const float inv = s > 0.f ? rcp(s) : 0.f, inv_lo = fmaf(-inv, s, 1.f) * inv;
-  uint32_t codes = 0;
+  // in the last place of 1.5 * 2^23 + y stands y, rounded to even (NaN gives 0); the upper bits
+  // are the same for all and are taken off at once
+  uint32_t codes = 0, all = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float d = x[first + i] - m;
-    // in the last place of 1.5 * 2^23 + y stands y, rounded to even; NaN gives 0
     const float y = fminf(fmaxf(fmaf(d, inv, d * inv_lo), 0.f), 15.f);
-    codes |= (__float_as_uint(y + 12582912.f) & 15u) << (4 * i);
+    codes += __float_as_uint(y + 12582912.f) << (4 * i);
+    all += 0x4b400000u << (4 * i);
   }
-  return codes;
+  return codes - all;
 }
 // The codes of a row's eight elements of lane c, and the scales of its groups.
 template <int HD, int ORDER>
@@ -92,30 +96,48 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) norm_rope_write4_
   const bool some = mine < tokens;
   const long long tok = some ? mine : tokens - 1;  // all lanes take part in the shuffles
   const int b = static_cast<int>(tok / a.sl), i = static_cast<int>(tok - static_cast<long long>(b) * a.sl);
-  const int start = a.start_positions[b];
-  const long long pos = static_cast<long long>(max(start, 0)) + i;
-  const Turn turn = turn_of<T>(pos, a.freqs, c);
-  float w[8];
+  // the first rows are on their way while the angles are computed
   if (grp >= kv_groups) {
     const int h0 = (grp - kv_groups) * a.q_heads, h1 = min(h0 + a.q_heads, a.heads);
     const T* from = static_cast<const T*>(a.q) + tok * a.q_stride;
     T* to = static_cast<T*>(a.q_out) + tok * a.heads * HD;
+    Raw8<T> raw[QB];
+    auto fetch = [&](int h) {
+#pragma unroll
+      for (int g = 0; g < QB; ++g) load_row<T, HD, ORDER>(raw[g], from + min(h + g, h1 - 1) * HD, c);
+    };
+    fetch(h0);
+    float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = a.q_norm != nullptr ? a.q_norm[element<HD, ORDER>(c, e)] : 1.f;
-    for (int d = 0; h0 + d < h1; d += QB) {
-      Raw8<T> raw[QB];
-#pragma unroll
-      for (int g = 0; g < QB; ++g) load_row<T, HD, ORDER>(raw[g], from + min(h0 + d + g, h1 - 1) * HD, c);
+    // to 2^-22 for all types: a step of a code is far above the rows' own
+    const Turn turn = turn_of<float>(static_cast<long long>(max(a.start_positions[b], 0)) + i, a.freqs, c);
+    for (int h = h0; h < h1; h += QB) {
+      if (h > h0) fetch(h);
 #pragma unroll
       for (int g = 0; g < QB; ++g) {
         float x[8];
         raw[g].get(x);
         norm_rotate<LPR, ORDER>(x, w, a.q_norm != nullptr, a.eps, turn);
-        if (some && h0 + d + g < h1) store_row<T, HD, ORDER>(to + (h0 + d + g) * HD, c, x);
+        if (some && h + g < h1) store_row<T, HD, ORDER>(to + (h + g) * HD, c, x);
       }
     }
     return;
   }
+  const int h0 = grp * a.tiles, h1 = min(h0 + a.tiles, a.kv_heads);
+  const T *k = static_cast<const T*>(a.k) + tok * a.k_stride, *v = static_cast<const T*>(a.v) + tok * a.v_stride;
+  Raw8<T> kr[KB], vr[KB];
+  auto fetch = [&](int first) {
+#pragma unroll
+    for (int g = 0; g < KB; ++g) {
+      const int h = min(first + g, h1 - 1);
+      load_row<T, HD, ORDER>(kr[g], k + h * HD, c);
+      load_row<T, HD, 0>(vr[g], v + h * HD, c);
+    }
+  };
+  fetch(h0);
+  const int start = a.start_positions[b];
+  const long long pos = static_cast<long long>(max(start, 0)) + i;
   // where the token's rows are in the cache; -1: not written
   const int count = start < 0 ? 0 : a.new_lens != nullptr ? min(a.new_lens[b], a.sl) : a.sl;
   long long page_row = -1;
@@ -126,24 +148,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) norm_rope_write4_
     else
       page_row = (static_cast<long long>(page) * a.blocks + a.block_index) * a.kv_heads * 2 * a.stride + (pos - slot * a.stride);
   }
-  const int h0 = grp * a.tiles, h1 = min(h0 + a.tiles, a.kv_heads);
-  const T *k = static_cast<const T*>(a.k) + tok * a.k_stride, *v = static_cast<const T*>(a.v) + tok * a.v_stride;
   T* k_out = a.k_out == nullptr ? nullptr : static_cast<T*>(a.k_out) + tok * a.kv_heads * HD;
   uint8_t* slab = static_cast<uint8_t*>(a.slab);
   __half2* scales = reinterpret_cast<__half2*>(a.scales);
+  float w[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = a.k_norm != nullptr ? a.k_norm[element<HD, ORDER>(c, e)] : 1.f;
-  for (int d = 0; h0 + d < h1; d += KB) {
-    Raw8<T> kr[KB], vr[KB];
+  const Turn turn = turn_of<float>(pos, a.freqs, c);
+  for (int first = h0; first < h1; first += KB) {
+    if (first > h0) fetch(first);
 #pragma unroll
     for (int g = 0; g < KB; ++g) {
-      const int h = min(h0 + d + g, h1 - 1);
-      load_row<T, HD, ORDER>(kr[g], k + h * HD, c);
-      load_row<T, HD, 0>(vr[g], v + h * HD, c);
-    }
-#pragma unroll
-    for (int g = 0; g < KB; ++g) {
-      const int h = h0 + d + g;
+      const int h = first + g;
       const bool live = some && h < h1, put = live && page_row >= 0;
       const size_t at = static_cast<size_t>(max(page_row, 0ll)) + static_cast<size_t>(min(h, h1 - 1)) * 2 * a.stride, v_at = at + a.stride;
       float x[8];
