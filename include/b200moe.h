@@ -538,8 +538,9 @@ int b200moe_kv4_attend(const void* q, int q_dtype, int64_t q_stride, const void*
  * cu_q[b] .. cu_q[b + 1] - 1 of q and cu_k[b] .. cu_k[b + 1] - 1 of k and v (cu_k NULL: cu_q's);
  * of its n and m rows, row i of q attends rows 0 .. m - n + i of k, and its output is zero where
  * that leaves none.  q: q_rows rows of heads * head_dim elements, k and v: k_rows rows of
- * kv_heads * head_dim, each q_stride, k_stride, v_stride elements apart, all of one dtype; out
- * [q_rows][heads][head_dim] contiguous, of out_dtype.  Rows of q in no sequence (before cu_q[0],
+ * kv_heads * head_dim, each q_stride, k_stride, v_stride elements apart, all of one dtype (buffers
+ * and strides multiples of 16 bytes); out [q_rows][heads][head_dim] contiguous, of out_dtype,
+ * 32-byte aligned.  Rows of q in no sequence (before cu_q[0],
  * behind cu_q[bs]) give zeros.  Bounds that decrease or leave the rows set the bounds bit of the
  * status word; such a sequence is cut to the rows there are.  Any heads / kv_heads; head_dim 64
  * or 128; softcap (finite) <= 0 means none.  Infinities and NaN in k and v show in the rows that

@@ -341,7 +341,7 @@ constexpr int TP_WORK = 4;  // items whose descriptions may be in use at once
 template <int HD>
 struct TpCfg {
   static constexpr int SUBS = HD / 64, TILE = SUBS * TP_SUB;  // 128 rows of 64 elements each
-  static constexpr int OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_OUT = 6 * TILE, OFF_BAD = OFF_OUT + 8 * 2048;
+  static constexpr int OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_BAD = 6 * TILE;
   static constexpr int OFF_WORK = OFF_BAD + TP_BAD * 3 * HD * 4, OFF_BAR = OFF_WORK + TP_WORK * 64;
   static constexpr int SMEM = 1024 + OFF_BAR + 320;
   static_assert(SMEM <= 232448, "shared memory budget");
@@ -444,6 +444,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+__device__ __forceinline__ void store_sector(void* to, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float a, float b) { return pack2(static_cast<const T*>(nullptr), a, b); }
 
@@ -749,8 +753,12 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           // unseen scores are zeros, and their weights later
           if (masked) {
 #pragma unroll
-            for (int e = 0; e < 128; ++e)
-              if (e >= some) v[e / 32][e % 32] = 0u;
+            for (int c = 0; c < 4; ++c)
+              if (__any_sync(0xffffffffu, 32 * c + 32 > some)) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (32 * c + e >= some) v[c][e] = 0u;
+              }
           }
           float low[4];
 #pragma unroll
@@ -776,8 +784,12 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         } else {
           if (masked) {
 #pragma unroll
-            for (int e = 0; e < 128; ++e)
-              if (e >= some) v[e / 32][e % 32] = 0xff800000u;
+            for (int c = 0; c < 4; ++c)
+              if (__any_sync(0xffffffffu, 32 * c + 32 > some)) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (32 * c + e >= some) v[c][e] = 0xff800000u;
+              }
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -869,78 +881,65 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       // the last tile of keys is one that was looked at: before it the notes may be older ones
       const bool any_bad = own > 0 && w.begin + own * TP_KEYS > w.tok0 + w.shift + 1 && s_any_bad[loads % TP_BAD] != 0;
       const int* bad = s_bad + (loads % TP_BAD) * 3 * HD;
-      const bool parts = w.chunks > 1, wide_out = parts || a.out_dtype == B200MOE_DT_F32;
+      const bool parts = w.chunks > 1;
       const float f = parts ? 1.f : l == 0.f ? 0.f : rcp(l);
-      // 64 bytes of each row at a time through shared memory: four lanes then store them
-      const uint32_t stage = base + C::OFF_OUT + warp * 2048;
-      const int64_t row0 = static_cast<int64_t>(w.q0) * a.heads + w.kvh * G + w.h0;
-      uint8_t* to[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = (warp & 3) * 32 + 8 * k + lane / 4, rt = token_of(r), rh = r - rt * a.group;
-        const bool live = rt < per && g * per + rt < w.toks && rh < w.hs;
-        const int64_t at = row0 + (g * per + rt) * a.heads + rh;
-        to[k] = !live ? nullptr : parts ? reinterpret_cast<uint8_t*>(a.partial + (at * a.splits + w.chunk) * (HD + 4))
-                                        : static_cast<uint8_t*>(a.out) + at * (wide_out ? HD * 4 : HD * 2);
-      }
-      auto put = [&](const uint32_t (&x)[16], int byte) {  // byte: of the row, where these 64 go
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t y[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
-          sts128(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4), y);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = 8 * k + lane / 4, q = lane % 4;
-          uint32_t y[4];
-          lds128(stage + r * 64 + ((q ^ (r >> 1 & 3)) << 4), y);
-          if (to[k] != nullptr) *reinterpret_cast<uint4*>(to[k] + byte + q * 16) = make_uint4(y[0], y[1], y[2], y[3]);
-        }
-        __syncwarp();
-      };
+      const int h = row - (mine - g * per) * a.group;
+      const bool stored = live && h < w.hs;
+      const int64_t at = (static_cast<int64_t>(w.q0) + mine) * a.heads + w.kvh * G + w.h0 + h;
+      float* part = a.partial + (at * a.splits + w.chunk) * (HD + 4);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[2][16];
+        uint32_t o[32];
         if (own > 0) {
-          tmem_ld16(o_at + 32 * c, o[0]);
-          tmem_ld16(o_at + 32 * c + 16, o[1]);
+          tmem_ld32(o_at + 32 * c, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e / 16][e % 16] = __float_as_uint(__uint_as_float(o[e / 16][e % 16]) * f);
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e / 16][e % 16] = 0u;
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
         }
         if (any_bad) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int d = 32 * c + e;
-            float x = __uint_as_float(o[e / 16][e % 16]);
+            float x = __uint_as_float(o[e]);
             if (bad[d] < seen) x = __int_as_float(0x7fffffff);
             if (bad[HD + d] < seen) x += INFINITY;
             if (bad[2 * HD + d] < seen) x -= INFINITY;
-            o[e / 16][e % 16] = __float_as_uint(x);
+            o[e] = __float_as_uint(x);
           }
         }
-        if (wide_out) {
-          put(o[0], 128 * c);
-          put(o[1], 128 * c + 64);
-        } else {
-          uint32_t x[16];
+        if (stored) {  // whole sectors of 32 bytes
+          if (parts) {  // (its rows are 16 bytes from those)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float u = __uint_as_float(o[e / 8][2 * e % 16]), v = __uint_as_float(o[e / 8][2 * e % 16 + 1]);
-            x[e] = a.out_dtype == B200MOE_DT_F16 ? pack16<__half>(u, v) : pack16<__nv_bfloat16>(u, v);
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(part + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          } else if (a.out_dtype == B200MOE_DT_F32) {
+            float* to = static_cast<float*>(a.out) + at * HD + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              const uint32_t y[8] = {o[e], o[e + 1], o[e + 2], o[e + 3], o[e + 4], o[e + 5], o[e + 6], o[e + 7]};
+              store_sector(to + e, y);
+            }
+          } else {
+            uint16_t* to = static_cast<uint16_t*>(a.out) + at * HD + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 16) {
+              uint32_t y[8];
+              auto pack = [&](auto type) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = pack16<decltype(type)>(__uint_as_float(o[e + 2 * k]), __uint_as_float(o[e + 2 * k + 1]));
+              };
+              if (a.out_dtype == B200MOE_DT_F16) pack(__half());
+              else pack(__nv_bfloat16());
+              store_sector(to + e, y);
+            }
           }
-          put(x, 64 * c);
         }
+        __syncwarp();  // the next load of tensor memory is the whole warp's
       }
-      if (parts) {
-        const int h = row - token_of(row) * a.group;
-        if (mine - g * per < per && mine < w.toks && h < w.hs)
-          *reinterpret_cast<float2*>(a.partial + ((row0 + mine * a.heads + h) * a.splits + w.chunk) * (HD + 4) + HD) = make_float2(m, l);
-      }
+      if (parts && stored) *reinterpret_cast<float2*>(part + HD) = make_float2(m, l);
       if (w.tiles() > 0) ++loads;
       done_work(i);
     }
@@ -1087,6 +1086,7 @@ int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype
   B200_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && q_stride % per16 == 0 &&
                    k_stride % per16 == 0 && v_stride % per16 == 0,
                "%s: buffers and row strides must be multiples of 16 bytes", who);
+  B200_REQUIRE((reinterpret_cast<uintptr_t>(out) & 31) == 0, "%s: out must be 32-byte aligned", who);
   B200_REQUIRE(q_stride >= static_cast<int64_t>(heads) * head_dim && k_stride >= static_cast<int64_t>(kv_heads) * head_dim &&
                    v_stride >= static_cast<int64_t>(kv_heads) * head_dim,
                "%s: a row stride is shorter than the row", who);

@@ -93,7 +93,7 @@ def _prompt(q=DUMMY, k=DUMMY, v=DUMMY, dt=C.DT_BF16, qs=4096, ks=1024, vs=1024, 
     (dict(heads=30), "multiple of the kv heads"), (dict(dt=3), "dtype"), (dict(odt=9), "dtype"), (dict(hd=80), "head_dim"),
     (dict(q=ODD), "16 bytes"), (dict(qs=4100), "16 bytes"), (dict(vs=1028), "16 bytes"), (dict(qs=2048), "shorter than the row"),
     (dict(ks=512), "shorter than the row"), (dict(q=None), "NULL"), (dict(v=None), "NULL"), (dict(cu=None), "NULL"),
-    (dict(out=None), "NULL"), (dict(bs=-1), "sizes"), (dict(rows=-1), "sizes"), (dict(rows=1 << 31), "2^31"),
+    (dict(out=None), "NULL"), (dict(out=ctypes.c_void_p(8208)), "32-byte"), (dict(bs=-1), "sizes"), (dict(rows=-1), "sizes"), (dict(rows=1 << 31), "2^31"),
     (dict(softcap=math.inf), "softcap"), (dict(heads=1 << 20, qs=1 << 27), "heads")])
 def test_prompt_refuses(kw, message):
     assert _prompt(**kw) == -1 and message in C.last_error()
