@@ -81,7 +81,8 @@ __device__ __forceinline__ void write_codes(const float (&x)[8], int c, bool som
 
 // Rows are written alone: a CTA has tokens and either a few query heads or a few kv heads of
 // each.  HD / 8 lanes have a row; a lane keeps its position's cosines and sines for all of its
-// heads.  Bound by memory and instructions alike.
+// heads.  3 x 777 tokens of 32 + 16 heads (55 MB) 15.6 us, 4 x 2048 of 48 + 16 (272 MB) 55 us, 4.9 TB/s,
+// 64 x 1 3.5 us: as the 8-bit cache's write.
 template <typename T, int HD, int ORDER>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) norm_rope_write4_kernel(const WriteArgs a) {
   constexpr int LPR = HD / 8, RPW = 32 / LPR, RPP = 8 * RPW;  // lanes per row; rows of a warp, of the CTA
@@ -225,7 +226,8 @@ __device__ __forceinline__ void values_of(uint32_t codes, __half2 held, float (&
 }
 
 // One CTA per (sequence, kv head, 16 positions); a thread takes the codes of 16 bytes of
-// output, K and V of several rows at once.
+// output, K and V of several rows at once.  Bound by HBM: 32 sequences of up to 4000 positions, 8
+// heads of 128, to bf16 (648 MB) 115 us, 5.6 TB/s.
 constexpr int RD4_THREADS = 128, RD4_TILE = 16;
 template <typename T, int HD>
 __global__ void __launch_bounds__(RD4_THREADS) kv4_read_kernel(const Read4Args a) {
@@ -315,6 +317,15 @@ int launch_read4(const Read4Args& a, int hd, dim3 grid, cudaStream_t st) {
 // A warp owns units of 32 positions with its own softmax state and two places for a unit's K
 // and V, filled by cp.async while the other is worked on.  The list of steps, its stretches
 // and the merge are those of the 8-bit cache.
+//
+// 32 sequences of 2000 to 4000 positions, 8 kv heads of 128, 32 heads (125 MB): bf16 36 us (int8
+// codes, 200 MB: 40), fp16 41, fp32 57; one of 32768 20 us; 8 x 8190, 48 heads, five new tokens, in two
+// tiles of 16 rows: bf16 50 us, fp16 61.  What bounds it: before the first rows 6 us, the merge 4 us, in
+// between the chain of dependent instructions of a unit (700 of a warp, issued every second clock;
+// 8 and 12 warps an SM take the same time within a tenth).
+// CTAs per SM at 32 x 4000: two 38.8 us, three 36.1, four (128 registers, the warps' states joined
+// in two halves) 43.9.  q loaded before the first copies, which helps over the 8-bit cache, costs
+// registers that wait in memory: 37.5 us.
 template <int HD, int NT, int BITS>
 constexpr int attend4_resident() {
   return NT == 1 && BITS != BITS_BOTH ? 3 : 2;
@@ -946,8 +957,6 @@ int launch_attend4_rows(const AttendArgs& a, int bits, int tile_rows, cudaStream
   return one ? launch_attend4<HD, 1, BITS_ONE>(a, st) : launch_attend4<HD, 2, BITS_ONE>(a, st);
 }
 
-inline bool aligned_scales(const void* p) { return aligned16(p); }
-
 }  // namespace
 }  // namespace b200moe
 
@@ -974,7 +983,7 @@ int b200moe_attn_norm_rope_kv4_write(const void* q, const void* k, const void* v
   a.stride_shift = log2_of(a.stride);
   if (const int rc = check_write(who, a, io_dtype, cache->head_dim)) return rc;
   if (bs == 0) return B200MOE_OK;
-  B200_REQUIRE(scales != nullptr && aligned_scales(scales), "%s: scales must be given and 16-byte aligned", who);
+  B200_REQUIRE(scales != nullptr && aligned16(scales), "%s: scales must be given and 16-byte aligned", who);
   a.status = device_status_ptr();
   if (a.status == nullptr) return B200MOE_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -992,7 +1001,7 @@ int b200moe_kv4_read(const void* slab, const void* scales, const b200moe_kv_cach
   if (bs == 0 || max_seq_len == 0) return B200MOE_OK;
   B200_REQUIRE(slab && scales && page_ids && seq_lens && k_out && v_out, "%s: NULL buffer", who);
   B200_REQUIRE(dtype_ok(out_dtype), "%s: unknown dtype", who);
-  B200_REQUIRE(aligned16(slab) && aligned16(k_out) && aligned16(v_out) && aligned_scales(scales),
+  B200_REQUIRE(aligned16(slab) && aligned16(k_out) && aligned16(v_out) && aligned16(scales),
                "%s: slab, scales and outputs must be 16-byte aligned", who);
   Read4Args a;
   a.slab = static_cast<const uint8_t*>(slab); a.scales = static_cast<const __half2*>(scales); a.page_ids = page_ids;
@@ -1038,7 +1047,7 @@ int b200moe_kv4_attend(const void* q, int q_dtype, int64_t q_stride, const void*
                cache->kv_heads);
   B200_REQUIRE(q_stride >= static_cast<int64_t>(heads) * cache->head_dim &&
                    q_stride % (16 / static_cast<int64_t>(dt_bytes(q_dtype))) == 0 && aligned16(q) && aligned16(out) &&
-                   aligned16(slab) && aligned16(scratch) && aligned_scales(scales),
+                   aligned16(slab) && aligned16(scratch) && aligned16(scales),
                "%s: q, its row stride, out, slab, scales and scratch must be multiples of 16 bytes", who);
   const size_t need = b200moe_kv4_attend_scratch_bytes(cache, bs, new_tokens, heads, max_seq_len);
   if (scratch_bytes < need) {

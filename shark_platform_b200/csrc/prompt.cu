@@ -137,7 +137,9 @@ __device__ __forceinline__ void zero_rest(const PromptArgs& a, int hd, int threa
 // 16 by 16 has rows 8 ty .. + 7, keys tx + 16 j of the scores and elements 4 tx + 64 n .. + 3 of the output, so
 // that 16 bytes from shared memory serve eight or four products.  K of the next tile is on its
 // way while the softmax and V's products of this one run, V during the scores.  Everything is
-// fp32.
+// fp32.  6 x 777 tokens of 16 heads over 4 of 64 191 us, 25 TFLOP/s; 2048 of 32 over 8 of 128 968 us, 36:
+// bound by shared memory (12 loads of 16 bytes for 128 products a thread) and by the few warps that
+// fit.  (Four rows a thread 205, with K and V loaded in between 258 us.)
 constexpr int SP_KEYS = 64, SP_R = 8;
 template <int HD>
 struct SpCfg {
@@ -331,8 +333,23 @@ int launch_prompt(PromptArgs& a, cudaStream_t st) {
 //                   other data and become zeros, infinities and NaN too (a weight of zero does
 //                   not hide them from the product); where those are is noted, and they are
 //                   added at the end to the rows that see them.
-// Sums and statistics are fp32.  P is rounded to the type of V, as the output is after it.
+// Sums and statistics are fp32.  P is rounded to the type of V, as the output is after it: the
+// error against 64 bits is at most sqrt(2) of what rounding the output alone costs (2.1e-3 of 1.6e-3
+// for bf16; P in two parts would cost half again as many MMAs).
 // An MMA reads P where a later one writes S: the tensor core executes a thread's MMAs in order.
+//
+// A step (128 keys of both tiles) needs 2048 clocks of the tensor core (4096 products a clock) and
+// as many of the special-function unit (16 exponentials a clock), side by side; it takes about 3100:
+// S out of tensor memory, the maximum and the way from the last P to the next S are in no other
+// unit's shadow when both tiles wait.  One B200, 32 heads over 8 of 128, bf16: 8192 tokens 418 us,
+// 1.31 PFLOP/s, 4096 118 us, 1.16; 16 x 1024 of 48 heads 264 us, with a softcap 407 (a polynomial of
+// seven products a pair of scores, and a minimum beside the maximum).  An item costs about two steps
+// beside its own (start, last product, output).
+// On the way there, 8192 tokens: every role walking the list itself 545 us; descriptions of items
+// with a run-time index, which puts them into local memory, 474; rows stored through shared memory
+// 434.  Not kept: two threads a row, 16 warps (both tiles then wait and compute at the same time)
+// 572 for 545; 3 to 8 of 16 pairs of exponentials as polynomials of degree 4 by the fp32 units 474 for
+// 444; weights computed with the old maximum while the new one is found 499 for 446 (more live registers).
 constexpr int TP_THREADS = 384, TP_ROWS = 128, TP_KEYS = 128, TP_SUB = 128 * 128;
 constexpr int TP_WARP_MMA = 8, TP_WARP_LOAD = 10, TP_WARP_CLEAN = 11;
 constexpr int TP_BAD = 4;   // items whose notes of bad values may be in use at once
@@ -1028,7 +1045,8 @@ int launch_prompt_tc_hd(const PromptArgs& a, int hd, cudaStream_t st) {
 // rows, long keys) the keys of each are split: into as many parts as make the last SM finish
 // first, in units of a tile of keys (1.5 us), with two for an item's start and end and two for
 // the merge.  The lengths are on the device: all sequences are taken to be as long as the mean.
-// 4 x 60 tokens behind up to 16000, 32 heads (32 items): @SPLIT@.
+// 4 x 60 tokens behind 12000, 32 heads (32 items): 4 parts 63 us, 5 95, 6 90, 9 74, 13 87; 16 tokens
+// behind 30000 (8 items): 16 parts 40 us, 13 44, 9 54, 4 99; unsplit 208 for 4 x 60 behind up to 16000.
 struct PromptPlan { int group, parts, tokens, splits; };
 constexpr int TP_MAX_SPLITS = 16;
 PromptPlan plan_prompt(int64_t q_rows, int64_t k_rows, int bs, int heads, int kv_heads) {
