@@ -56,14 +56,14 @@ __device__ __forceinline__ int chunk_begin(int keys, int step, int chunks, int i
 }
 // The list of items, walked by a whole warp with rising indices.
 struct ItemWalk {
-  int t;             // tiles with this place in their sequence are current
-  long long before;  // items before them
+  int t, b0;         // tiles with this place in their sequence are current, in 32 sequences from b0 on
+  long long before;  // items before those
   int n, m;          // rows of q and k of sequence `lane`
   __device__ __forceinline__ static void lengths(const PromptArgs& a, int b, int& n, int& m) {
     n = b < a.bs ? span_of(a.cu_q, b, a.q_rows, nullptr).len : 0;
     m = b < a.bs ? span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, b, a.k_rows, nullptr).len : 0;
   }
-  __device__ __forceinline__ ItemWalk(const PromptArgs& a, int lane) : t(0), before(0) {
+  __device__ __forceinline__ ItemWalk(const PromptArgs& a, int lane) : t(0), b0(0), before(0) {
     lengths(a, lane, n, m);
     int most = (n + a.tokens - 1) / a.tokens;
     for (int b = lane + 32; b < a.bs; b += 32) most = max(most, (span_of(a.cu_q, b, a.q_rows, nullptr).len + a.tokens - 1) / a.tokens);
@@ -82,9 +82,8 @@ struct ItemWalk {
   }
   __device__ __forceinline__ Item find(const PromptArgs& a, int lane, int step, long long i) {
     const int each = a.kv_heads * a.parts;
-    for (; t >= 0; --t) {
-      long long at = before;
-      for (int b0 = 0; b0 < a.bs; b0 += 32) {
+    for (; t >= 0; --t, b0 = 0) {
+      for (; b0 < a.bs; b0 += 32) {
         int nb = n, mb = m;
         if (a.bs > 32) lengths(a, b0 + lane, nb, mb);
         const int own = chunks(a, nb, mb, t, step);
@@ -98,16 +97,15 @@ struct ItemWalk {
             if (lane >= o) sum += up;
           }
         }
-        const int all = __shfl_sync(0xffffffffu, sum, 31);
-        if (i < at + static_cast<long long>(all) * each) {
-          const int r = static_cast<int>(i - at), c = r / each, h = r - c * each;  // chunk c of those of 32 sequences
+        const long long all = static_cast<long long>(__shfl_sync(0xffffffffu, sum, 31)) * each;
+        if (i < before + all) {
+          const int r = static_cast<int>(i - before), c = r / each, h = r - c * each;  // chunk c of those of 32 sequences
           const int which = __ffs(__ballot_sync(0xffffffffu, sum > c)) - 1;
           const int chunk = c - __shfl_sync(0xffffffffu, sum - own, which);
           return {b0 + which, t, h / a.parts, h % a.parts, chunk, true};
         }
-        at += static_cast<long long>(all) * each;
+        before += all;
       }
-      before = at;
     }
     return {0, 0, 0, 0, 0, false};
   }
@@ -738,7 +736,8 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int g = warp >> 2, row = (warp & 3) * 32 + lane;  // tile; row of it and lane of tensor memory
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, s_at = tmem + lanes + g * TP_KEYS, o_at = tmem + lanes + 2 * TP_KEYS + g * HD;
-    const float by = CAP ? fabsf(a.scale) / a.softcap : fabsf(a.scale) * LOG2E, cap2 = a.softcap * LOG2E;
+    // (never zero: an unseen score is -infinity times it)
+    const float by = fmaxf(CAP ? fabsf(a.scale) / a.softcap : fabsf(a.scale) * LOG2E, 1e-37f), cap2 = a.softcap * LOG2E;
     // c log2(e) tanh(S by) as a polynomial in S, where its coefficients are within 32 bits
     const float by3 = by * by * by, poly[4] = {TANH[0] * cap2 * by, TANH[1] * cap2 * by3, TANH[2] * cap2 * by3 * (by * by), TANH[3] * cap2 * by3 * (by3 * by)};
     const bool usual = by > 1e-4f && by < 1e4f && cap2 > 1e-3f && cap2 < 1e4f;

@@ -190,6 +190,25 @@ def test_many_sequences():
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_thousands_of_sequences(dtype):
+    """More sequences than a warp looks at in one go, at one and at several places of the list."""
+    g = torch.Generator().manual_seed(15)
+    lens = torch.randint(0, 4, (3500,), generator=g)
+    lens[1234], lens[3400] = 200, 131
+    q, k, v, cu, cu_k = _inputs(lens.tolist(), None, 4, 2, 64, dtype, seed=16)
+    _check(_call(q, k, v, cu), q, k, v, cu, cu_k)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("scale,softcap", [(-0.125, None), (-0.125, 20.0), (0.0, None), (0.0, 20.0), (1e-6, 0.1), (40.0, 0.01)])
+def test_scales_of_any_sign_and_size(dtype, scale, softcap):
+    q, k, v, cu, cu_k = _inputs([150, 20], None, 4, 2, 64, dtype, seed=17)
+    got = _call(q, k, v, cu, scale=scale, softcap=softcap)
+    want, room = po.packed(q, k, v, cu, cu_k, scale, softcap, 0.0 if dtype == F32 else EPS[dtype], EPS[dtype])
+    assert ((got.cpu().double() - want).abs() - room).max() <= 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_longer(dtype):
     """More items than SMs, several tiles of keys: the list of items and the rings go round."""
     lens = [1300, 900, 2050]
