@@ -81,8 +81,8 @@ __device__ __forceinline__ void write_codes(const float (&x)[8], int c, bool som
 
 // Rows are written alone: a CTA has tokens and either a few query heads or a few kv heads of
 // each.  HD / 8 lanes have a row; a lane keeps its position's cosines and sines for all of its
-// heads.  3 x 777 tokens of 32 + 16 heads (55 MB) 15.6 us, 4 x 2048 of 48 + 16 (272 MB) 55 us, 4.9 TB/s,
-// 64 x 1 3.5 us: as the 8-bit cache's write.
+// heads.  3 x 777 tokens of 32 + 16 heads (55 MB) 14.6 us, 4 x 2048 of 48 + 16 (272 MB) 51 us, 5.3 TB/s,
+// 64 x 1 3.5 us.
 template <typename T, int HD, int ORDER>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) norm_rope_write4_kernel(const WriteArgs a) {
   constexpr int LPR = HD / 8, RPW = 32 / LPR, RPP = 8 * RPW;  // lanes per row; rows of a warp, of the CTA
@@ -176,9 +176,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) norm_rope_write4_
 
 template <typename T, int HD>
 int launch_write4(WriteArgs& a, cudaStream_t st) {
-  // as many heads a lane as leave work for eight CTAs per SM: a position's angles are computed once for each group
+  // as many heads a lane as leave work for two CTAs per SM: a position's angles are computed once for
+  // each group (eight CTAs: 4 x 2048 55 instead of 51 us, 3 x 777 15.7 instead of 14.6; one: 1 x 1500
+  // 12.1 instead of 9.9)
   constexpr int RPP = 8 * (32 / (HD / 8));
-  const int64_t tokens = static_cast<int64_t>(a.bs) * a.sl, tok_ctas = (tokens + RPP - 1) / RPP, want = sm_count() * 8ll;
+  const int64_t tokens = static_cast<int64_t>(a.bs) * a.sl, tok_ctas = (tokens + RPP - 1) / RPP, want = sm_count() * 2ll;
   a.q_heads = 4;
   a.tiles = 2;  // kv heads of a lane
   while (a.q_heads < a.heads && tok_ctas * ((a.heads - 1) / (2 * a.q_heads) + 1) >= want) a.q_heads *= 2;

@@ -340,8 +340,8 @@ int launch_prompt(PromptArgs& a, cudaStream_t st) {
 // as many of the special-function unit (16 exponentials a clock), side by side; it takes about 3100:
 // S out of tensor memory, the maximum and the way from the last P to the next S are in no other
 // unit's shadow when both tiles wait.  One B200, 32 heads over 8 of 128, bf16: 8192 tokens 418 us,
-// 1.31 PFLOP/s, 4096 118 us, 1.16; 16 x 1024 of 48 heads 264 us, with a softcap 407 (a polynomial of
-// seven products a pair of scores, and a minimum beside the maximum).  An item costs about two steps
+// 1.31 PFLOP/s, 4096 118 us, 1.16; 16 x 1024 of 48 heads 256 us, with a softcap 404 (a polynomial of
+// five products a pair of scores, and a minimum beside the maximum).  An item costs about two steps
 // beside its own (start, last product, output).
 // On the way there, 8192 tokens: every role walking the list itself 545 us; descriptions of items
 // with a run-time index, which puts them into local memory, 474; rows stored through shared memory
@@ -766,16 +766,20 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         float top[4], up;
         bool small = true;  // softcap: the polynomial holds for all scores of the warp's rows
         if constexpr (CAP) {
-          // unseen scores are zeros, and their weights later
-          if (masked) {
+          // the polynomial's range is looked at with zeros for unseen scores; then they become so
+          // large that it falls (odd, its last coefficient negative) and their weights are zero
+          auto unseen = [&](uint32_t value) {
+            if (masked) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (__any_sync(0xffffffffu, 32 * c + 32 > some)) {
+              for (int c = 0; c < 4; ++c)
+                if (__any_sync(0xffffffffu, 32 * c + 32 > some)) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (32 * c + e >= some) v[c][e] = 0u;
-              }
-          }
+                  for (int e = 0; e < 32; ++e)
+                    if (32 * c + e >= some) v[c][e] = value;
+                }
+            }
+          };
+          unseen(0u);
           float low[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -790,11 +794,17 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           }
           up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * by;
           small = usual && __all_sync(0xffffffffu, !live || (up <= 0.5f && min3(min3(low[0], low[1], low[2]), low[3], low[3]) * by >= -0.5f));
-          if (masked) {
-            up = -INFINITY;
+          if (masked) {  // the zeros are no scores
 #pragma unroll
-            for (int e = 0; e < 128; ++e) up = e < some ? max3(up, __uint_as_float(v[e / 32][e % 32]), up) : up;
-            up *= by;
+            for (int c = 0; c < 4; ++c)
+              if (__any_sync(0xffffffffu, 32 * c + 32 > some)) {
+                top[c] = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (32 * c + e < some) top[c] = max3(top[c], __uint_as_float(v[c][e]), top[c]);
+              }
+            up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * by;
+            unseen(__float_as_uint(100.f / by));
           }
           up = up == -INFINITY ? up : fmaf(-2.f * cap2, rcp(ex2(up * (2.f * LOG2E)) + 1.f), cap2);
         } else {
@@ -841,48 +851,56 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         const uint64_t by2 = pair(by, by), less = pair(-from, -from);
         uint64_t sum[2] = {0ull, 0ull};
         // P of 32 keys at a time; after 64 the first half of the product can start
-        auto weights = [&](auto cut, auto fast) {
+        auto give = [&](int c, const uint32_t (&p)[16]) {
+          tmem_st16(s_at + 16 * c, p);
+          if (c % 2) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 16u * (c / 2) + 8u * g);
+          }
+        };
+        if (!CAP || small) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t p[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float s0 = __uint_as_float(v[c][2 * e]), s1 = __uint_as_float(v[c][2 * e + 1]);
+              const uint64_t s2 = pair(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1]));
               float x, y;
-              if constexpr (!CAP) {
-                unpair(fma2(pair(s0, s1), by2, less), x, y);
-              } else if constexpr (decltype(fast)::value) {
-                const uint64_t s2 = pair(s0, s1), u = mul2(s2, s2);
+              if constexpr (CAP) {
+                const uint64_t u = mul2(s2, s2);
                 const uint64_t t = fma2(u, fma2(u, fma2(u, pair(poly[3], poly[3]), pair(poly[2], poly[2])), pair(poly[1], poly[1])), pair(poly[0], poly[0]));
                 unpair(fma2(s2, t, less), x, y);
               } else {
-                x = fmaf(-2.f * cap2, rcp(ex2(s0 * (by * (2.f * LOG2E))) + 1.f), cap2 - from);
-                y = fmaf(-2.f * cap2, rcp(ex2(s1 * (by * (2.f * LOG2E))) + 1.f), cap2 - from);
+                unpair(fma2(s2, by2, less), x, y);
               }
               x = ex2(x);
               y = ex2(y);
-              if constexpr (decltype(cut)::value) {
-                x = 32 * c + 2 * e < some ? x : 0.f;
-                y = 32 * c + 2 * e + 1 < some ? y : 0.f;
-              }
               sum[e % 2] = add2(sum[e % 2], pair(x, y));
               p[e] = pack16<T>(x, y);
             }
-            tmem_st16(s_at + 16 * c, p);
-            if (c % 2) {
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(p_full + 16u * (c / 2) + 8u * g);
-            }
+            give(c, p);
           }
-        };
-        if constexpr (!CAP) {
-          weights(std::false_type(), std::true_type());
-        } else {
-          if (!masked && small) weights(std::false_type(), std::true_type());
-          else if (small) weights(std::true_type(), std::true_type());
-          else weights(std::true_type(), std::false_type());
+        } else if constexpr (CAP) {  // by the exponential; S once more from tensor memory (P takes the part that is read)
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t z[32], p[16];
+            tmem_ld32(s_at + 32 * c, z);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float x[2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float f = fmaf(-2.f * cap2, rcp(ex2(__uint_as_float(z[2 * e + k]) * (by * (2.f * LOG2E))) + 1.f), cap2 - from);
+                x[k] = 32 * c + 2 * e + k < some ? ex2(f) : 0.f;
+              }
+              sum[e % 2] = add2(sum[e % 2], pair(x[0], x[1]));
+              p[e] = pack16<T>(x[0], x[1]);
+            }
+            give(c, p);
+          }
         }
         {
           float x, y;
