@@ -234,7 +234,8 @@ class B200PagedAttentionBlock(torch.nn.Module):
 
     `attention_kernel="b200"` takes `prompt_attend` for prompts.  It is causal by itself: of
     an `attention_mask` it takes for granted that it is the causal one, with any padding
-    behind a sequence's tokens (the rows of padding are attended too and mean nothing)."""
+    behind a sequence's tokens (the rows of padding are attended too and mean nothing); one
+    whose last two dimensions cannot be that is refused."""
 
     def __init__(self, theta, *, block_index: int, cache, head_count: int, head_dim: int, head_count_kv: int,
                  rms_epsilon: float, attention_kernel: str = "decomposed", attention_scale: Optional[float] = None,
@@ -372,6 +373,11 @@ class B200PagedAttentionBlock(torch.nn.Module):
             raise C.B200MoeError(f"a decode step brings at most {MAX_NEW_TOKENS} tokens per sequence")
         if decode and new_lens is not None:
             raise C.B200MoeError("new_lens is for prefill; a negative start position marks a padding sequence of a step")
+        if not decode and self.attention_kernel == "b200" and attention_mask is not None:
+            seen = {sl, int(start_index) + sl} if self._quantized else {sl}
+            if attention_mask.dim() < 2 or attention_mask.shape[-2] != sl or attention_mask.shape[-1] not in seen:
+                raise C.B200MoeError('attention_kernel="b200" is causal by itself: an attention_mask of '
+                                     f"{list(attention_mask.shape)} is not the causal one of {sl} tokens")
         use_hf = bool(getattr(embedding, "use_hf", False))
         # norms, the HuggingFace order, padding and 8-bit codes: the one-pass write
         one_pass = (self._quantized or use_hf or new_lens is not None or self._q_norm_w is not None or

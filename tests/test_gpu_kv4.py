@@ -84,8 +84,10 @@ def _check_write(cache, before, state, ids, start, q, k, v, got, norms, halves, 
             over = (z - 15).clamp(min=0) + (-z).clamp(min=0)
             assert ((code - z).abs() - 0.5 - step - over - 2.0 ** -19).max() <= 0
             # a scale rounded down leaves the largest value 2^-11 of 15 steps above the last code, a
-            # scale among fp16's subnormal numbers more
-            assert ((over - step) * s - 15 * (s * 2.0 ** -11 + 2.0 ** -25) - x.abs() * 2.0 ** -10 - 2.0 ** -23).max() <= 0
+            # scale among fp16's subnormal numbers more; so does an offset rounded by 2^-11 of itself:
+            # hi - offset = 15 (hi - lo) / 15 + lo - offset
+            least = lo.abs().repeat_interleave(k4.GROUP, -1)
+            assert ((over - step) * s - 15 * (s * 2.0 ** -11 + 2.0 ** -25) * 1.001 - least * 2.0 ** -11 - 2.0 ** -23).max() <= 0
             c0[at[0], layer, :, slot, p % stride], h0[at[0], layer, :, slot, p % stride] = code, held
     # nothing else has changed
     assert torch.equal(c0, c1) and torch.equal(h0.nan_to_num(7e5), h1.nan_to_num(7e5))

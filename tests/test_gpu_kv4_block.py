@@ -92,6 +92,21 @@ def test_padded_prompts_in_the_block():
         assert torch.equal(again[0], y[0]) and torch.equal(again[1, :19], y[1, :19])
 
 
+@pytest.mark.parametrize("dtype", [torch.uint8, I8])
+def test_masks_that_are_not_causal_ones(dtype):
+    """A mask of padding alone, or of other lengths, is refused before anything is written."""
+    from shark_platform_b200 import moe
+
+    m = (Model4 if dtype == torch.uint8 else Model)(dtype)
+    m.block.attention_kernel = "b200"
+    before = [t.clone() for t in m.state]
+    h = m.rows(20)
+    for shape in ((2, 1, 1, 20), (2, 1, 20, 1), (2, 1, 20, 24), (2, 1, 24, 20), (20,)):
+        with pytest.raises(moe.C.B200MoeError, match="is causal by itself"):
+            m.call(h, start_index=0, attention_mask=torch.zeros(shape).cuda())
+    assert all(torch.equal(a, b) for a, b in zip(before, m.state))
+
+
 def test_patching_takes_the_kernel():
     from shark_platform_b200 import attention as A
 

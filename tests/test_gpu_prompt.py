@@ -199,6 +199,20 @@ def test_thousands_of_sequences(dtype):
     _check(_call(q, k, v, cu), q, k, v, cu, cu_k)
 
 
+@pytest.mark.parametrize("dtype,rows", [(BF, 300000), (F32, 150000)])
+def test_rows_beyond_32_bits_of_elements(dtype, rows):
+    """q of more than 2^32 bytes, k and v rows of a tensor of more than 2^32 bytes: the last sequences."""
+    q, k, v, cu, _ = _inputs([100, 100], None, 64, 1, 128, dtype, seed=18)
+    full = torch.zeros(rows, 64, 128, dtype=dtype, device="cuda")
+    wide = torch.zeros(rows, 16384, dtype=dtype, device="cuda")
+    kk, vv = (wide[:, at:at + 128].unflatten(1, (1, 128)) for at in (128, 16000))
+    for to, x in ((full, q), (kk, k), (vv, v)):
+        to[-200:] = x.cuda()
+    got = _call(full, kk, vv, torch.arange(0, rows + 1, 100))
+    _check(got[-200:], q, k, v, cu, cu)
+    assert got[:-200].abs().max() == 0
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 @pytest.mark.parametrize("scale,softcap", [(-0.125, None), (-0.125, 20.0), (0.0, None), (0.0, 20.0), (1e-6, 0.1), (40.0, 0.01)])
 def test_scales_of_any_sign_and_size(dtype, scale, softcap):
