@@ -137,7 +137,8 @@ __device__ __forceinline__ void zero_rest(const PromptArgs& a, int hd, int threa
 // way while the softmax and V's products of this one run, V during the scores.  Everything is
 // fp32.  6 x 777 tokens of 16 heads over 4 of 64 191 us, 25 TFLOP/s; 2048 of 32 over 8 of 128 968 us, 36:
 // bound by shared memory (12 loads of 16 bytes for 128 products a thread) and by the few warps that
-// fit.  (Four rows a thread 205, with K and V loaded in between 258 us.)
+// fit.  (Four rows a thread 205, with K and V loaded in between 258 us; heads of 64 by 8 lanes a row and
+// 64 threads, with a third fewer loads for a product, 276.)
 constexpr int SP_KEYS = 64, SP_R = 8;
 template <int HD>
 struct SpCfg {
@@ -339,8 +340,8 @@ int launch_prompt(PromptArgs& a, cudaStream_t st) {
 // A step (128 keys of both tiles) needs 2048 clocks of the tensor core (4096 products a clock) and
 // as many of the special-function unit (16 exponentials a clock), side by side; it takes about 3100:
 // S out of tensor memory, the maximum and the way from the last P to the next S are in no other
-// unit's shadow when both tiles wait.  One B200, 32 heads over 8 of 128, bf16: 8192 tokens 418 us,
-// 1.31 PFLOP/s, 4096 118 us, 1.16; 16 x 1024 of 48 heads 256 us, with a softcap 404 (a polynomial of
+// unit's shadow when both tiles wait.  One B200, 32 heads over 8 of 128, bf16: 8192 tokens 420 us,
+// 1.31 PFLOP/s, 4096 118 us, 1.16; 16 x 1024 of 48 heads 257 us, with a softcap 408 (a polynomial of
 // five products a pair of scores, and a minimum beside the maximum).  An item costs about two steps
 // beside its own (start, last product, output).
 // On the way there, 8192 tokens: every role walking the list itself 545 us; descriptions of items
