@@ -29,7 +29,9 @@ struct PromptArgs {
   uint32_t inv_group;     // 2^16 / group, rounded up: exact quotients of rows of a tile
   int tokens;             // of a tile
   int splits;             // parts that the keys of a tile are cut into, at most
-  float* partial;         // [row of q][head][splits][HD + 4]: numerator, maximum, denominator
+  unsigned units;         // parts of one kv head that should come out
+  float cut;              // parts for each tile of keys, where the sequences are not looked at
+  float* partial;         // [row of q][head][splits][HD + 4]: numerator, maximum, denominator; the first: cut
   float scale, softcap;
   int32_t* status;
 };
@@ -49,8 +51,10 @@ struct Item {
 };
 // Keys that the last of `toks` tokens from tok0 on sees, of a sequence of n tokens and m keys.
 __device__ __forceinline__ int keys_seen(int n, int m, int tok0, int toks) { return max(0, min(m, tok0 + toks + m - n)); }
-// Parts of a tile's keys, which are split between tiles of `step` keys; the first of them of part i.
-__device__ __forceinline__ int chunks_of(int keys, int step, int splits) { return max(1, min(splits, (keys + step - 1) / step)); }
+// Parts of a tile's keys, `cut` of them for each tile of `step` keys; the first of the keys of part i.
+__device__ __forceinline__ int chunks_of(int keys, int step, float cut, int splits) {
+  return max(1, min(splits, __float2int_ru(fmaf(static_cast<float>((keys + step - 1) / step), cut, -1e-4f))));
+}
 __device__ __forceinline__ int chunk_begin(int keys, int step, int chunks, int i) {
   return static_cast<int>(static_cast<int64_t>((keys + step - 1) / step) * i / chunks) * step;
 }
@@ -75,18 +79,30 @@ struct ItemWalk {
       }
   }
   // items of a sequence of n and m rows with tile t, apart from heads
-  __device__ __forceinline__ static int chunks(const PromptArgs& a, int n, int m, int t, int step) {
+  __device__ __forceinline__ static int chunks(const PromptArgs& a, int n, int m, int t, int step, float cut) {
     const int tok0 = t * a.tokens;
     if (tok0 >= n) return 0;
-    return a.splits == 1 ? 1 : chunks_of(keys_seen(n, m, tok0, min(a.tokens, n - tok0)), step, a.splits);
+    return a.splits == 1 ? 1 : chunks_of(keys_seen(n, m, tok0, min(a.tokens, n - tok0)), step, cut, a.splits);
   }
-  __device__ __forceinline__ Item find(const PromptArgs& a, int lane, int step, long long i) {
+  // Parts for each tile of keys, so that there are no more than a.units: the sum of ceil(x cut) over
+  // tiles of x tiles of keys is at most the sum of x cut, and one for each.  (The largest cut, by a
+  // search, ends the longest part 2 tiles of 28 earlier, and its code took 2 us to fetch and run.)
+  __device__ __forceinline__ float cut(const PromptArgs& a, int step) const {
+    if (a.splits == 1 || a.bs > 32) return a.cut;
+    const unsigned count = (n + a.tokens - 1) / a.tokens, most = (m + step - 1) / step;
+    const unsigned items = __reduce_add_sync(0xffffffffu, count), tiles = __reduce_add_sync(0xffffffffu, count * most);
+    const unsigned longest = __reduce_max_sync(0xffffffffu, count > 0 ? most : 0);
+    if (items >= a.units || tiles == 0) return 0.f;
+    return fminf(__fdividef(static_cast<float>(a.units - items), static_cast<float>(tiles)),
+                 __fdividef(static_cast<float>(a.splits), static_cast<float>(longest)));
+  }
+  __device__ __forceinline__ Item find(const PromptArgs& a, int lane, int step, float cut, long long i) {
     const int each = a.kv_heads * a.parts;
     for (; t >= 0; --t, b0 = 0) {
       for (; b0 < a.bs; b0 += 32) {
         int nb = n, mb = m;
         if (a.bs > 32) lengths(a, b0 + lane, nb, mb);
-        const int own = chunks(a, nb, mb, t, step);
+        const int own = chunks(a, nb, mb, t, step, cut);
         int sum = own;
         if (a.splits == 1) {
           sum = __popc(__ballot_sync(0xffffffffu, own) & (0xffffffffu >> (31 - lane)));
@@ -161,7 +177,7 @@ __global__ void __launch_bounds__(SpCfg<HD>::THREADS, SpCfg<HD>::RESIDENT) promp
   const float to_score = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E, cap2 = a.softcap * LOG2E;
   ItemWalk walk(a, lane);
   for (long long r = 0;; ++r) {
-    const Item it = walk.find(a, lane, SP_KEYS, item_of(r));
+    const Item it = walk.find(a, lane, SP_KEYS, 0.f, item_of(r));
     if (!it.some) break;
     const Span qs = span_of(a.cu_q, it.seq, a.q_rows, nullptr), ks = span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, it.seq, a.k_rows, nullptr);
     const int tok0 = it.tile * a.tokens, toks = min(a.tokens, qs.len - tok0);
@@ -399,7 +415,7 @@ struct Work {
   __device__ __forceinline__ int tiles_of(int g) const { return g == 0 ? n0 : n1; }
 };
 static_assert(sizeof(Work) == 64, "four 16-byte words");
-__device__ __forceinline__ Work work_of(const PromptArgs& a, const Item& it) {
+__device__ __forceinline__ Work work_of(const PromptArgs& a, const Item& it, float cut) {
   Work w;
   const Span qs = span_of(a.cu_q, it.seq, a.q_rows, nullptr), ks = span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, it.seq, a.k_rows, nullptr);
   const int G = a.heads / a.kv_heads, per = a.tokens / 2;
@@ -413,7 +429,7 @@ __device__ __forceinline__ Work work_of(const PromptArgs& a, const Item& it) {
   w.shift = ks.len - qs.len;
   const int keys = keys_seen(qs.len, ks.len, w.tok0, w.toks);
   w.chunk = it.chunk;
-  w.chunks = a.splits == 1 ? 1 : chunks_of(keys, TP_KEYS, a.splits);
+  w.chunks = a.splits == 1 ? 1 : chunks_of(keys, TP_KEYS, cut, a.splits);
   w.begin = w.chunks == 1 ? 0 : chunk_begin(keys, TP_KEYS, w.chunks, it.chunk);
   w.end = w.chunks == 1 ? keys : min(keys, chunk_begin(keys, TP_KEYS, w.chunks, it.chunk + 1));
   auto tiles = [&](int g) {
@@ -534,10 +550,12 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       uint32_t loads = 0, tiles = 0;
       const uint32_t q_bytes = static_cast<uint32_t>(per * a.group) * HD * 2;
       ItemWalk walk(a, lane);
+      const float cut = walk.cut(a, TP_KEYS);
+      if (a.splits > 1 && blockIdx.x == 0 && lane == 0) a.partial[HD + 2] = cut;
       bool ok = true;
       auto publish = [&](uint32_t i, Work& w) {
-        const Item it = walk.find(a, lane, TP_KEYS, item_of(i));
-        if (it.some) w = work_of(a, it);
+        const Item it = walk.find(a, lane, TP_KEYS, cut, item_of(i));
+        if (it.some) w = work_of(a, it, cut);
         else w.toks = -1;
         if (!wait(w_empty + 8u * (i % TP_WORK), i / TP_WORK + 1)) return false;
         if (lane == 0) {
@@ -999,6 +1017,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptArgs a) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int64_t row = at / a.heads;
   if (row >= a.q_rows) return;
+  const float cut = a.partial[HD + 2];
   int chunks = 0;
   for (int b0 = 0; b0 < a.bs; b0 += 32) {
     const int b = b0 + lane;
@@ -1007,7 +1026,7 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptArgs a) {
     const unsigned who = __ballot_sync(0xffffffffu, here);
     if (who == 0) continue;
     const int m = here ? span_of(a.cu_k != nullptr ? a.cu_k : a.cu_q, b, a.k_rows, nullptr).len : 0;
-    const int own = here ? ItemWalk::chunks(a, qs.len, m, static_cast<int>(row - qs.begin) / a.tokens, TP_KEYS) : 0;
+    const int own = here ? ItemWalk::chunks(a, qs.len, m, static_cast<int>(row - qs.begin) / a.tokens, TP_KEYS, cut) : 0;
     chunks = __shfl_sync(0xffffffffu, own, __ffs(who) - 1);
     break;
   }
@@ -1062,18 +1081,20 @@ int launch_prompt_tc_hd(const PromptArgs& a, int hd, cudaStream_t st) {
 // The shape of a call's items on the tensor cores.  Where there are fewer items than SMs (few
 // rows, long keys) the keys of each are split: into as many parts as make the last SM finish
 // first, in units of a tile of keys (1.5 us), with two for an item's start and end and two for
-// the merge.  The lengths are on the device: all sequences are taken to be as long as the mean.
+// the merge.  The lengths are on the device: here all sequences are taken to be as long as the mean.
+// Of up to 32 sequences the kernel then cuts longer ones into more parts, up to three times as many,
+// and no more in all than the rule's rounds of the SMs.
 // 4 x 60 tokens behind 12000, 32 heads (32 items): 4 parts 63 us, 5 95, 6 90, 9 74, 13 87; 16 tokens
 // behind 30000 (8 items): 16 parts 40 us, 13 44, 9 54, 4 99; unsplit 208 for 4 x 60 behind up to 16000.
-struct PromptPlan { int group, parts, tokens, splits; };
+struct PromptPlan { int group, parts, tokens, splits, units; float cut; };
 constexpr int TP_MAX_SPLITS = 16;
 PromptPlan plan_prompt(int64_t q_rows, int64_t k_rows, int bs, int heads, int kv_heads) {
-  PromptPlan p;
+  PromptPlan p{};
   const int G = heads / kv_heads;
   p.group = G < TP_ROWS ? G : TP_ROWS;
   p.parts = (G + p.group - 1) / p.group;
   p.tokens = 2 * (TP_ROWS / p.group);
-  p.splits = 1;
+  p.splits = p.units = 1;
   const int64_t n = bs > 0 ? (q_rows + bs - 1) / bs : 0, m = bs > 0 ? (k_rows + bs - 1) / bs : 0;
   const int64_t items = bs * ((n + p.tokens - 1) / p.tokens) * kv_heads * p.parts, tiles = (m + TP_KEYS - 1) / TP_KEYS;
   if (items >= sm_count()) return p;
@@ -1085,6 +1106,9 @@ PromptPlan plan_prompt(int64_t q_rows, int64_t k_rows, int bs, int heads, int kv
       p.splits = s;
     }
   }
+  p.cut = static_cast<float>(p.splits) / static_cast<float>(std::max<int64_t>(tiles, 1));
+  p.units = static_cast<int>((items * p.splits + sm_count() - 1) / sm_count() * sm_count() / (kv_heads * p.parts));
+  if (p.splits > 1 && bs > 1 && bs <= 32) p.splits = std::min(TP_MAX_SPLITS, 3 * p.splits);
   return p;
 }
 
@@ -1147,6 +1171,7 @@ int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype
   }
   const PromptPlan p = plan_prompt(q_rows, k_rows, bs, heads, kv_heads);
   a.group = p.group; a.inv_group = (65536 + p.group - 1) / p.group; a.parts = p.parts; a.tokens = p.tokens; a.splits = p.splits;
+  a.cut = p.cut; a.units = p.units;
   return dtype == B200MOE_DT_F16 ? launch_prompt_tc_hd<__half>(a, head_dim, st) : launch_prompt_tc_hd<__nv_bfloat16>(a, head_dim, st);
 }
 
