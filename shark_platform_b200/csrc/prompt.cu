@@ -30,6 +30,7 @@ struct PromptArgs {
   int tokens;             // of a tile
   int splits;             // parts that the keys of a tile are cut into, at most
   unsigned units;         // parts of one kv head that should come out
+  bool uneven;            // or two or three times as many, whichever ends first
   float cut;              // parts for each tile of keys, where the sequences are not looked at
   float* partial;         // [row of q][head][splits][HD + 4]: numerator, maximum, denominator; the first: cut
   float scale, softcap;
@@ -92,9 +93,22 @@ struct ItemWalk {
     const unsigned count = (n + a.tokens - 1) / a.tokens, most = (m + step - 1) / step;
     const unsigned items = __reduce_add_sync(0xffffffffu, count), tiles = __reduce_add_sync(0xffffffffu, count * most);
     const unsigned longest = __reduce_max_sync(0xffffffffu, count > 0 ? most : 0);
-    if (items >= a.units || tiles == 0) return 0.f;
-    return fminf(__fdividef(static_cast<float>(a.units - items), static_cast<float>(tiles)),
-                 __fdividef(static_cast<float>(a.splits), static_cast<float>(longest)));
+    const float most_parts = __fdividef(static_cast<float>(a.splits), static_cast<float>(longest));
+    auto within = [&](float units) {
+      return fminf(most_parts, __fdividef(fmaxf(units - static_cast<float>(items), 0.f), static_cast<float>(tiles)));
+    };
+    if (tiles == 0) return 0.f;
+    const float units = static_cast<float>(a.units);
+    if (!a.uneven) return within(units);
+    float best = 0.f, least = 3e38f;
+#pragma unroll 1
+    for (float r = 1.f; r <= 3.f; r += 1.f) {
+      const float x = within(r * units);
+      const int mine = chunks_of(m, step, x, a.splits);
+      const float time = r * static_cast<float>(__reduce_max_sync(0xffffffffu, count > 0 ? (most + mine - 1) / mine : 0) + 2);
+      if (time < least) least = time, best = x;
+    }
+    return best;
   }
   __device__ __forceinline__ Item find(const PromptArgs& a, int lane, int step, float cut, long long i) {
     const int each = a.kv_heads * a.parts;
@@ -1082,11 +1096,16 @@ int launch_prompt_tc_hd(const PromptArgs& a, int hd, cudaStream_t st) {
 // rows, long keys) the keys of each are split: into as many parts as make the last SM finish
 // first, in units of a tile of keys (1.5 us), with two for an item's start and end and two for
 // the merge.  The lengths are on the device: here all sequences are taken to be as long as the mean.
-// Of up to 32 sequences the kernel then cuts longer ones into more parts, up to three times as many,
-// and no more in all than the rule's rounds of the SMs.
+// Of 2 to 32 sequences the kernel then cuts longer ones into more parts, up to three times as many,
+// and no more in all than the rule's rounds of the SMs.  Where the mean asks for no parts, long keys
+// (a quarter of the rows new at most, 8 tiles) get up to four, in the best of one to three rounds.
 // 4 x 60 tokens behind 12000, 32 heads (32 items): 4 parts 63 us, 5 95, 6 90, 9 74, 13 87; 16 tokens
 // behind 30000 (8 items): 16 parts 40 us, 13 44, 9 54, 4 99; unsplit 208 for 4 x 60 behind up to 16000.
-struct PromptPlan { int group, parts, tokens, splits, units; float cut; };
+// As many parts for each sequence, or by its length: 30 tokens behind 30000 and three times 1000
+// 103 and 50 us; 8 x 16 behind 100 to 8000 60 and 34; 12 x 30 behind 500 to 11500 103 and 91; 4 x 60
+// behind 10000 to 16000 73 and 68, all behind 12000 63 and 65.  One part, or up to four: 16 x 3 behind 1000 to 7000
+// 89 and 75, one of them behind 16000, 4000 else, 192 and 88, all behind 4000 56 and 60.
+struct PromptPlan { int group, parts, tokens, splits, units; bool uneven; float cut; };
 constexpr int TP_MAX_SPLITS = 16;
 PromptPlan plan_prompt(int64_t q_rows, int64_t k_rows, int bs, int heads, int kv_heads) {
   PromptPlan p{};
@@ -1108,7 +1127,10 @@ PromptPlan plan_prompt(int64_t q_rows, int64_t k_rows, int bs, int heads, int kv
   }
   p.cut = static_cast<float>(p.splits) / static_cast<float>(std::max<int64_t>(tiles, 1));
   p.units = static_cast<int>((items * p.splits + sm_count() - 1) / sm_count() * sm_count() / (kv_heads * p.parts));
-  if (p.splits > 1 && bs > 1 && bs <= 32) p.splits = std::min(TP_MAX_SPLITS, 3 * p.splits);
+  if (bs > 1 && bs <= 32) {
+    p.uneven = p.splits == 1 && tiles >= 8 && k_rows >= 4 * q_rows;
+    p.splits = p.uneven ? 4 : p.splits > 1 ? std::min(TP_MAX_SPLITS, 3 * p.splits) : 1;
+  }
   return p;
 }
 
@@ -1171,7 +1193,7 @@ int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype
   }
   const PromptPlan p = plan_prompt(q_rows, k_rows, bs, heads, kv_heads);
   a.group = p.group; a.inv_group = (65536 + p.group - 1) / p.group; a.parts = p.parts; a.tokens = p.tokens; a.splits = p.splits;
-  a.cut = p.cut; a.units = p.units;
+  a.cut = p.cut; a.units = p.units; a.uneven = p.uneven;
   return dtype == B200MOE_DT_F16 ? launch_prompt_tc_hd<__half>(a, head_dim, st) : launch_prompt_tc_hd<__nv_bfloat16>(a, head_dim, st);
 }
 

@@ -247,6 +247,21 @@ def test_split_keys(lens, lens_k, heads, kvh, hd, dtype):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("lens,before,heads,kvh", [
+    ([3] * 16, [300] * 15 + [5000], 8, 8), ([3] * 16, [1100] * 16, 8, 8),          # one part each by the mean
+    ([16] * 8, [8000, 500, 200, 4000, 0, 900, 300, 2000], 4, 2), ([1] * 32, list(range(0, 3200, 100)), 4, 1),
+    ([1] * 40, [2000] + [700] * 39, 4, 1),                                          # more sequences than lanes
+    ([70, 0, 5], [3000, 3000, 9000], 4, 2), ([1, 0, 0, 0], [9000, 0, 100, 0], 2, 2)], ids=str)
+def test_split_keys_of_uneven_sequences(lens, before, heads, kvh):
+    lens_k = [n + m for n, m in zip(lens, before)]
+    for dtype, softcap in ((BF, None), (HF, 20.0)):
+        q, k, v, cu, cu_k = _inputs(lens, lens_k, heads, kvh, 64, dtype, seed=19)
+        got = _call(q, k, v, cu, cu_k, softcap=softcap)
+        _check(got, q, k, v, cu, cu_k, softcap=softcap)
+        assert torch.equal(got, _call(q, k, v, cu, cu_k, softcap=softcap))
+    assert _status() == 0
+
+
 def test_split_keys_with_bad_values():
     """An infinity in one part and a NaN in another: the rows that attend them."""
     q, k, v, cu, cu_k = _inputs([60], [5000], 8, 2, 128, BF, seed=13)
