@@ -10,8 +10,9 @@
 // (of a group of more heads than a tile has rows, a part of them); row r of a tile is token
 // r / heads, head r % heads, so that one read of k and v serves all of them.  A CTA takes items
 // i, i + CTAs, ...; the list is ordered by the tile's place in its sequence, last tiles first:
-// they have the most keys, and the short ones fill the end.  It is made by every warp on its
-// own from the sequences' bounds on the device: the host does not know them.
+// they have the most keys, and the short ones fill the end.  It is made on the device from the
+// sequences' bounds, which the host does not know: by the loading warp for the others, or (32-bit
+// rows) by every warp on its own.
 #include "kv_attend.cuh"
 #include "tcgen05.cuh"
 
