@@ -27,6 +27,9 @@ struct AttendArgs {
 // activations, and softcaps above CAP_FAST: there what the fast form of the softcap is off by,
 // CAP_FAST * 2^-22 = 2^-14 of a probability, would begin to show).
 constexpr float CAP_FAST = 256.f;
+// Caps above 2^100 are taken as that, so that c log2(e) and scale / c stay numbers of 32 bits: up to
+// scores of 2^88 either cap changes a score by less than 2^-24 of it.  0: no cap.
+inline float usable_softcap(float c) { return c > 0.f ? fminf(c, 1.2676506e30f) : 0.f; }
 enum { BITS_ONE = 0, BITS_P = 1, BITS_BOTH = 2 };
 constexpr int AT_THREADS = 128, AT_WARPS = 4;
 constexpr int AT_UNIT = 32;   // positions of a warp's step

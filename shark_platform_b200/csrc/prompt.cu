@@ -772,9 +772,13 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, s_at = tmem + lanes + g * TP_KEYS, o_at = tmem + lanes + 2 * TP_KEYS + g * HD;
     // (never zero: an unseen score is -infinity times it)
     const float by = fmaxf(CAP ? fabsf(a.scale) / a.softcap : fabsf(a.scale) * LOG2E, 1e-37f), cap2 = a.softcap * LOG2E;
-    // c log2(e) tanh(S by) as a polynomial in S, where its coefficients are within 32 bits
+    // c log2(e) tanh(S by) as a polynomial in S, where its coefficients are within 32 bits: with the
+    // scale of a head of 64 or 128 for caps from 1e-3 to 7e4.  It is off by a part of the score, so that
+    // the cap's size does not matter.
     const float by3 = by * by * by, poly[4] = {TANH[0] * cap2 * by, TANH[1] * cap2 * by3, TANH[2] * cap2 * by3 * (by * by), TANH[3] * cap2 * by3 * (by3 * by)};
-    const bool usual = by > 1e-4f && by < 1e4f && cap2 > 1e-3f && cap2 < 1e4f;
+    const bool usual = by > 1e-6f && by < 1e4f && cap2 > 1e-3f && poly[3] < -1e-38f;
+    // Else c - 2 c / (exp(2 z) + 1), which is off by 2^-22 of the cap: for caps above CAP_FAST tanhf instead.
+    const bool fast = a.softcap <= CAP_FAST;
     auto token_of = [&](int r) { return static_cast<int>((static_cast<uint32_t>(r) * a.inv_group) >> 16); };  // r / group
     const int mine = g * per + token_of(row);
     uint32_t loads = 0, tiles = 0;  // items with keys; S tiles taken
@@ -840,7 +844,7 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * by;
             unseen(__float_as_uint(100.f / by));
           }
-          up = up == -INFINITY ? up : fmaf(-2.f * cap2, rcp(ex2(up * (2.f * LOG2E)) + 1.f), cap2);
+          up = up == -INFINITY ? up : cap2 * tanhf(up);
         } else {
           if (masked) {
 #pragma unroll
@@ -916,7 +920,7 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             }
             give(c, p);
           }
-        } else if constexpr (CAP) {  // by the exponential; S once more from tensor memory (P takes the part that is read)
+        } else if constexpr (CAP) {  // S once more from tensor memory (P takes the part that is read)
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t z[32], p[16];
@@ -927,7 +931,8 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
               float x[2];
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                const float f = fmaf(-2.f * cap2, rcp(ex2(__uint_as_float(z[2 * e + k]) * (by * (2.f * LOG2E))) + 1.f), cap2 - from);
+                const float t = __uint_as_float(z[2 * e + k]) * by;
+                const float f = fast ? fmaf(-2.f * cap2, rcp(ex2(t * (2.f * LOG2E)) + 1.f), cap2 - from) : fmaf(cap2, tanhf(t), -from);
                 x[k] = 32 * c + 2 * e + k < some ? ex2(f) : 0.f;
               }
               sum[e % 2] = add2(sum[e % 2], pair(x[0], x[1]));
@@ -1183,7 +1188,7 @@ int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype
   a.partial = static_cast<float*>(scratch);
   a.q = q; a.k = k; a.v = v; a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
   a.cu_q = cu_q; a.cu_k = cu_k; a.out = out; a.q_rows = q_rows; a.k_rows = k_rows; a.out_dtype = out_dtype;
-  a.bs = bs; a.heads = heads; a.kv_heads = kv_heads; a.scale = scale; a.softcap = softcap > 0.f ? softcap : 0.f;
+  a.bs = bs; a.heads = heads; a.kv_heads = kv_heads; a.scale = scale; a.softcap = usable_softcap(softcap);
   a.status = device_status_ptr();
   if (a.status == nullptr) return B200MOE_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -1,0 +1,57 @@
+"""Attention of whole prompts at the ends of its range, against its definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import test_gpu_prompt as base
+from oracle import prompt_oracle as po
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32, EPS = base.BF, base.HF, base.F32, base.EPS
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("softcap", [300.0, 884.0, 1250.0, 1e4, 1e5, 1e6, 1e7, 1e8, 1e12, 3.4e38])
+def test_large_softcaps(softcap, hd, dtype):
+    """Ordinary scores far below the cap: as without one, in the largest error and in the 2-norm.
+    The cap's own error is 2^-20.8 of a score at most, of scores up to 16 and twice in a weight:
+    within 2^-15."""
+    for lens, lens_k in (([190, 33], None), ([40], [3000])):
+        q, k, v, cu, cu_k = base._inputs(lens, lens_k, 4, 2, hd, dtype, seed=int(math.log(softcap)))
+        got = base._call(q, k, v, cu, cu_k, softcap=softcap)
+        p_eps = 0.0 if dtype == F32 else EPS[dtype]
+        want, room = po.packed(q, k, v, cu, cu_k, hd ** -0.5, softcap, p_eps, EPS[dtype])
+        off = (got.cpu().double() - want).abs()
+        assert (off - room).max() <= 0, float(off.max())
+        assert float(off.norm() / want.norm()) <= math.sqrt(p_eps ** 2 + EPS[dtype] ** 2) / math.sqrt(3) + 2.0 ** -15
+    assert base._status() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("softcap", [200.0, 400.0, 3000.0, 1e5])
+def test_scores_near_large_softcaps(softcap, dtype):
+    """Scores of a part of the cap up to several caps, which only the keys' last tiles have; q and k
+    along one direction, so that a score's terms are of one sign.  A score S of 32 bits is off by
+    (hd + 8) 2^-23 S, its capped value by as much of its slope, sech^2, and by 2^-20 of the cap's
+    magnitude where it is computed apart from its neighbours': the weights of two scores near each
+    other differ by that at most.  The values are of one sign and of one size, so that the output
+    is off by half a step and by what the weights are."""
+    hd, n = 64, 400
+    g = torch.Generator().manual_seed(3)
+    sign = torch.randint(0, 2, (hd,), generator=g) * 2.0 - 1
+    q = (sign * 4).repeat(n, 2, 1).to(dtype)
+    top = 3 * softcap / (hd * 4 / 8)
+    size = torch.cat([torch.zeros(200), torch.linspace(0, top, 200)])
+    k = (sign * size[:, None, None]).repeat(1, 1, 1).to(dtype)
+    v = (1 + torch.rand(n, 1, hd, generator=g)).to(dtype)
+    cu = torch.tensor([0, n])
+    got = base._call(q, k, v, cu, softcap=softcap)
+    want = po.attend(q, k, v, hd ** -0.5, softcap)
+    off = (got.cpu().double() - want).abs()
+    # the largest slope times S is c z sech^2(z) <= 0.45 c
+    weight = 2 * softcap * (0.45 * (hd + 8) * 2.0 ** -23 + 2.0 ** -20)
+    p_eps = 0.0 if dtype == F32 else EPS[dtype]
+    assert (off - want.abs() * (p_eps + EPS[dtype] + min(weight, 1.0) + 2.0 ** -18)).max() <= 0
