@@ -1073,7 +1073,7 @@ int b200moe_kv4_attend(const void* q, int q_dtype, int64_t q_stride, const void*
                        (2.0 + START_STEPS + pages_per_seq * static_cast<double>(a.stride) / AT_STEP) < 2147483647.0,
                "%s: too many positions for one call", who);
   B200_REQUIRE(static_cast<int64_t>(bs) * heads * new_tokens <= 0x7fffffff, "%s: too many rows for one call", who);
-  a.scale = scale; a.softcap = softcap;
+  a.scale = scale; a.softcap = usable_softcap(softcap);
   a.status = device_status_ptr();
   if (a.status == nullptr) return B200MOE_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
