@@ -354,7 +354,7 @@ int launch_prompt(PromptArgs& a, cudaStream_t st) {
 //   warps 0-3, 4-7  the softmax of tile 0, 1: a thread has a row.  S out of tensor memory, its
 //                   maximum, P = 2^(S - m) in the type of V back over it as the A operand of
 //                   the second product.  O is rescaled when the maximum has grown by more
-//                   than 2^8 (P stays below that), by the same threads.  The output at the end.
+//                   than 2^P_SLACK, by the same threads.  The output at the end.
 //   warps 8, 9      issue the MMAs of tile 0, 1: S(0), then PV(j), S(j + 1) ...; while one tile's
 //                   products run the other's softmax does.
 //   warp 10         makes the list of items and loads: Q of an item, K and V tiles of 128 keys
@@ -365,7 +365,8 @@ int launch_prompt(PromptArgs& a, cudaStream_t st) {
 //                   added at the end to the rows that see them.
 // Sums and statistics are fp32.  P is rounded to the type of V, as the output is after it: the
 // error against 64 bits is at most sqrt(2) of what rounding the output alone costs (2.1e-3 of 1.6e-3
-// for bf16; P in two parts would cost half again as many MMAs).
+// for bf16; P in two parts would cost half again as many MMAs), and for fp16 weights below 2^-24 of
+// the largest what P_TOP says.
 // An MMA reads P where a later one writes S: the tensor core executes a thread's MMAs in order.
 //
 // A step (128 keys of both tiles) needs 2048 clocks of the tensor core (4096 products a clock) and
@@ -393,6 +394,13 @@ struct TpCfg {
   static constexpr int SMEM = 1024 + OFF_BAR + 320;
   static_assert(SMEM <= 232448, "shared memory budget");
 };
+// P is 2^P_TOP for the maximum that was taken last, and at most 2^(P_TOP + P_SLACK).  fp16 ends at 2^16
+// and has subnormal numbers below 2^-14: weights down to 2^-24 of the largest have all their bits, of
+// smaller ones 2^-35 of it is lost at most.  (With P = 1 for the largest, 2^-25 of it: all of an output
+// whose largest weights have values of zero.)  bf16 has the exponents of 32 bits.  Rescaling from 2^4 on
+// instead, for one more bit: 16 x 1500 of 48 heads with a softcap 542 for 535 us.
+template <typename T> constexpr float P_TOP_OF = std::is_same<T, __half>::value ? 10.f : 0.f;
+template <typename T> constexpr float P_SLACK_OF = std::is_same<T, __half>::value ? 5.9f : 8.f;
 
 // V as the B operand: 64 elements a row of 128 bytes, eight keys 1024 bytes apart, the next 64
 // elements TP_SUB further.
@@ -506,6 +514,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1)
 prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const PromptArgs a) {
   using C = TpCfg<HD>;
+  constexpr float P_TOP = P_TOP_OF<T>, P_SLACK = P_SLACK_OF<T>;
   extern __shared__ uint8_t tp_smem[];
   __shared__ int s_abort, s_any_bad[TP_BAD];
   __shared__ uint32_t s_tmem;
@@ -864,11 +873,11 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           up = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * by;
         }
         up = live ? up : 0.f;
-        // The maximum is taken where it has grown by more than 2^8: what the weights are relative
+        // The maximum is taken where it has grown by more than P_SLACK: what the weights are relative
         // to from here on.  An infinite score or none makes it NaN: for the whole row.
         if (j == 0) {
           m = up < INFINITY ? up : __int_as_float(0x7fffffff);
-        } else if (__any_sync(0xffffffffu, !(up <= m + 8.f))) {
+        } else if (__any_sync(0xffffffffu, !(up <= m + P_SLACK))) {
           const float m_new = up < INFINITY ? fmaxf(m, up) : __int_as_float(0x7fffffff);
           const float alpha = m_new == -INFINITY ? 1.f : ex2(m - m_new);
           m = m_new;
@@ -885,7 +894,7 @@ prompt_attend_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             tmem_st16(o_at + 16 * c, o);
           }
         }
-        const float from = m == -INFINITY ? 0.f : m;
+        const float from = (m == -INFINITY ? 0.f : m) - P_TOP;
         const uint64_t by2 = pair(by, by), less = pair(-from, -from);
         uint64_t sum[2] = {0ull, 0ull};
         // P of 32 keys at a time; after 64 the first half of the product can start

@@ -55,3 +55,26 @@ def test_scores_near_large_softcaps(softcap, dtype):
     weight = 2 * softcap * (0.45 * (hd + 8) * 2.0 ** -23 + 2.0 ** -20)
     p_eps = 0.0 if dtype == F32 else EPS[dtype]
     assert (off - want.abs() * (p_eps + EPS[dtype] + min(weight, 1.0) + 2.0 ** -18)).max() <= 0
+
+
+@pytest.mark.parametrize("where", [0, 130, 500])
+@pytest.mark.parametrize("lens,lens_k", [([700], [700]), ([60], [4000]), ([3, 200], [1000, 900])], ids=str)
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_an_output_of_small_weights(dtype, lens, lens_k, where):
+    """One key has nearly all of the weight and a value of zero: the output is that of weights of
+    2^-18 to 2^-24 of it, each to half a step of the type of v.  All terms of a score have one
+    sign, scores are up to 15, and a weight is off by twice a score's error at most."""
+    hd = 64
+    g = torch.Generator().manual_seed(where + sum(lens))
+    cu, cu_k = base._cu(lens), base._cu(lens_k)
+    q = torch.ones(int(cu[-1]), 4, hd, dtype=dtype)
+    k = ((torch.rand(int(cu_k[-1]), 2, 1, generator=g) * 4 - 2) / 8).expand(-1, -1, hd).to(dtype).contiguous()
+    v = (0.5 + torch.rand(int(cu_k[-1]), 2, hd, generator=g)).to(dtype)
+    for b in range(len(lens)):
+        k[int(cu_k[b]) + where], v[int(cu_k[b]) + where] = 14.5 / 8, 0.0
+    got = base._call(q, k, v, cu, cu_k, out_dtype=F32)
+    want, _ = po.packed(q, k, v, cu, cu_k, hd ** -0.5)
+    p_eps = 0.0 if dtype == F32 else EPS[dtype]
+    room = want.abs() * (p_eps + 2.0 ** -24 + 2 * 16 * (hd + 8) * 2.0 ** -23 + 2.0 ** -18)
+    off = (got.cpu().double() - want).abs()
+    assert (off - room).max() <= 0, float((off / want.clamp(min=1e-30)).max())
