@@ -314,7 +314,9 @@ int launch_read4(const Read4Args& a, int hd, dim3 grid, cudaStream_t st) {
 // P is in one fp16 part for bf16 outputs and in two, 2^-22, for others; q too in two for 32-bit
 // activations (BITS_*), where the codes are taken less 8 and the offsets 8 s more, in two parts:
 // the two sums no longer cancel each other, and what the MMAs round off is 2^-23 of the output
-// instead of many times that (1e-5 of 300 positions' output, 1e-4 of 20000's).
+// instead of many times that (1e-5 of 300 positions' output, 1e-4 of 20000's).  Those offsets are
+// brought to 2^14 by a power of two of each position: m + 8 s passes fp16's range where m and s do
+// not, and below 2^-14 two parts of it would have few bits.
 //
 // A warp owns units of 32 positions with its own softmax state and two places for a unit's K
 // and V, filled by cp.async while the other is worked on.  The list of steps, its stretches
@@ -378,6 +380,17 @@ __device__ __forceinline__ void copy_small(uint32_t dst, const void* src, bool v
   if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+
+// e, -10 .. 21, with 16 |s| and |m| of a position's groups below 2^e: from the exponents of the
+// largest ones, 4 more for s (numbers below 2^-14 count as that).
+template <int CH>
+__device__ __forceinline__ int magnitude(const uint32_t (&w)[CH]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) top = __vmaxu2(top, w[c] & 0x7fff7fffu);
+  return static_cast<int>(max((top & 0xffffu) + 0x1000u, top >> 16) >> 10) - 14;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 
 template <int HD, int NT, int BITS>
 __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())) kv4_attend_kernel(const AttendArgs a) {
@@ -671,25 +684,27 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
           const uint32_t u0 = upper ? w0[CH - 2] : w0[0], v0 = upper ? w0[CH - 1] : w0[1];
           const uint32_t u1 = upper ? w1[CH - 2] : w1[0], v1 = upper ? w1[CH - 1] : w1[1];
           uint32_t a0 = __byte_perm(u0, v0, 0x7632), a1 = __byte_perm(u1, v1, 0x7632), b0 = 0u, b1 = 0u;
-          if constexpr (SPLIT) {  // 8 s more, in two parts
-            auto both = [](uint32_t u, uint32_t v, uint32_t& hi, uint32_t& lo) {
+          float unit[2] = {UNIT24, UNIT24};  // of the two positions' sums
+          if constexpr (SPLIT) {  // 8 s more, in two parts of numbers below 2^15
+            auto both = [](uint32_t u, uint32_t v, float by, uint32_t& hi, uint32_t& lo) {
               const float2 x = __half22float2(u32_as_h2(u)), y = __half22float2(u32_as_h2(v));
-              const float f = fmaf(8.f, x.x, x.y), g = fmaf(8.f, y.x, y.y);
+              const float f = fmaf(8.f, x.x, x.y) * by, g = fmaf(8.f, y.x, y.y) * by;
               const __half2 top = __floats2half2_rn(f, g);
               hi = h2_as_u32(top);
               lo = h2_as_u32(__floats2half2_rn(f - __low2float(top), g - __high2float(top)));
             };
-            both(u0, v0, a0, b0);
-            both(u1, v1, a1, b1);
+            const int e0 = magnitude<CH>(w0), e1 = magnitude<CH>(w1);
+            unit[0] = power_of_two(e0 - 14);
+            unit[1] = power_of_two(e1 - 14);
+            both(u0, v0, power_of_two(14 - e0), a0, b0);
+            both(u1, v1, power_of_two(14 - e1), a1, b1);
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             if constexpr (SPLIT) mma_first(s[h][n], a0, a1, b0, b1, qs[n], qs[n]);
             else mma_first_k8(s[h][n], a0, a1, qs[n]);
-            if constexpr (!SPLIT) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) s[h][n][k] *= UNIT24;
-            }
+            for (int k = 0; k < 4; ++k) s[h][n][k] *= unit[k >> 1];
           }
         }
 #pragma unroll
