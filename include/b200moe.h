@@ -524,7 +524,8 @@ int b200moe_attn_norm_rope_kv4_write(const void* q, const void* k, const void* v
 int b200moe_kv4_read(const void* slab, const void* scales, const b200moe_kv_cache_t* cache, int32_t block_index,
                      const int32_t* page_ids, const int32_t* seq_lens, int32_t bs, int32_t pages_per_seq,
                      int32_t max_seq_len, void* k_out, void* v_out, int out_dtype, void* stream);
-/* b200moe_kv8_attend over a cache of 4-bit codes. */
+/* b200moe_kv8_attend over a cache of 4-bit codes.  Of the rows that see it, a group of K without
+ * finite scales makes all elements NaN, one of V its own 32. */
 size_t b200moe_kv4_attend_scratch_bytes(const b200moe_kv_cache_t* cache, int32_t bs, int32_t new_tokens, int32_t heads,
                                         int32_t max_seq_len);
 int b200moe_kv4_attend(const void* q, int q_dtype, int64_t q_stride, const void* slab, const void* scales,

@@ -162,7 +162,8 @@ def norm_rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache:
     4-bit codes: every 32 values of a row have the scale (max - min) / 15 and the offset min,
     rounded to fp16, and the codes nearest to them.  Rows are independent: any position may be
     written again at any time.  A group with an infinity or a NaN, or whose scale or offset
-    is beyond fp16's range, reads as NaN."""
+    is beyond fp16's range, reads as NaN: in `kv_attend` a group of K makes the whole output of
+    the rows that see it NaN, one of V its own 32 elements."""
     return C.attention_ops.write(q, k, v, cache_state, _geometry(cache), block_index, seq_block_ids, start_positions, new_lens,
                                  freqs, q_norm, k_norm, eps, use_hf)
 

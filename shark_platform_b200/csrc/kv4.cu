@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
   constexpr float P_TOP = P_PARTS == 2 ? 11.f : 7.f, P_SLACK = 15.f - P_TOP;
   extern __shared__ __align__(128) uint8_t smem[];  // [warp][2][K | V codes, K | V scales], then [warp][row][OPITCH] fp32
   float* s_o = reinterpret_cast<float*>(smem + AT_WARPS * 2 * PLACE);
-  __shared__ float2 s_pos[AT_WARPS][AT_UNIT];       // of each position: e (-inf: dead, NaN: bad), 2^-e
+  __shared__ float2 s_pos[AT_WARPS][AT_UNIT];       // of each position: e (-inf: dead), 2^-e
   __shared__ __align__(16) uint32_t s_sv[AT_WARPS][AT_UNIT / 2][CH], s_mv[PARTS][AT_WARPS][AT_UNIT / 2][CH];  // of two positions, times 2^(4 - e) and 2^-e
   __shared__ float2 s_ml[AT_WARPS][ROWS];
   grid_dep_wait();
@@ -629,20 +629,41 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
         uint32_t w[CH];
         if constexpr (CH == 4) lds128(vs + lane * 16, w);
         else lds64(vs + lane * 8, w);
-        uint32_t top = 0;  // largest |s| in the lower, |m| in the upper half
+        auto largest = [&] {  // |s| in the lower, |m| in the upper half
+          uint32_t top = 0;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) top = __vmaxu2(top, w[c] & 0x7fff7fffu);
-        const bool bad = (top & 0xffffu) >= 0x7c00u || top >= 0x7c000000u, dead = !(live_now >> lane & 1);
+          for (int c = 0; c < CH; ++c) top = __vmaxu2(top, w[c] & 0x7fff7fffu);
+          return top;
+        };
+        uint32_t top = largest();
+        const bool dead = !(live_now >> lane & 1);
+        if (__any_sync(0xffffffffu, (top & 0xffffu) >= 0x7c00u || top >= 0x7c000000u)) {
+          // a group without finite scales is NaN in the sums of the columns that see it, zeros in the products
+          const int behind = cur.p_begin + u * AT_STEP;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            const bool bad = (w[c] & 0x7c00u) == 0x7c00u || (w[c] & 0x7c000000u) == 0x7c000000u;
+            const uint32_t where = __ballot_sync(0xffffffffu, bad);
+            if (bad) w[c] = 0u;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int count = seen(n, j) - behind;
+                if (gid == c && count > 0 && (where << (32 - min(count, 32))) != 0u) om[n][j] = __int_as_float(0x7fffffff);
+              }
+          }
+          top = largest();
+        }
         const float2 f = __half22float2(u32_as_h2(top));
         const float most = fmaxf(fmaxf(f.x * 16.f, f.y), 2.f * UNIT24);
-        const int e = bad ? 0 : static_cast<int>(__float_as_uint(most) >> 23) - 126;  // -22 .. 21
-        const float shrink = bad ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        s_pos[warp][lane] = make_float2(dead ? -INFINITY : bad ? __int_as_float(0x7fffffff) : static_cast<float>(e),
-                                        dead ? 0.f : bad ? 1.f : shrink);
-        // Times 2^(4 - e) and 2^-e in two steps, each within fp16's range; a bad position's are zeros.
+        const int e = static_cast<int>(__float_as_uint(most) >> 23) - 126;  // -22 .. 21
+        const float shrink = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        s_pos[warp][lane] = make_float2(dead ? -INFINITY : static_cast<float>(e), dead ? 0.f : shrink);
+        // Times 2^(4 - e) and 2^-e in two steps, each within fp16's range.
         // Even lanes put down the scales of two positions, odd ones their offsets.
         const int e1 = e >> 1, e2 = e - e1;
-        const uint32_t by1 = static_cast<uint32_t>((4 - e1 + 15) << 10 | (15 - e1) << 26), by_2 = bad ? 0u : static_cast<uint32_t>((15 - e2) << 10 | (15 - e2) << 26);
+        const uint32_t by1 = static_cast<uint32_t>((4 - e1 + 15) << 10 | (15 - e1) << 26), by_2 = static_cast<uint32_t>((15 - e2) << 10 | (15 - e2) << 26);
         const uint32_t choose = lane & 1 ? 0x3276u : 0x5410u;
         uint32_t both[CH], lower[CH];
 #pragma unroll
@@ -650,13 +671,13 @@ __global__ void __launch_bounds__(AT_THREADS, (attend4_resident<HD, NT, BITS>())
           uint32_t own;
           if constexpr (SPLIT) {
             float2 y = __half22float2(u32_as_h2(w[c]));
-            y = bad ? make_float2(0.f, 0.f) : make_float2(y.x * shrink, fmaf(8.f, y.x, y.y) * shrink);
+            y = make_float2(y.x * shrink, fmaf(8.f, y.x, y.y) * shrink);
             const __half2 h = __floats2half2_rn(y.x * 16.f, y.y);
             own = h2_as_u32(h);
             const uint32_t low = h2_as_u32(__float2half2_rn(y.y - __high2float(h)));
             lower[c] = __byte_perm(low, __shfl_xor_sync(0xffffffffu, low, 1), choose);
           } else {
-            own = bad ? 0u : h2_as_u32(__hmul2(__hmul2(u32_as_h2(w[c]), u32_as_h2(by1)), u32_as_h2(by_2)));
+            own = h2_as_u32(__hmul2(__hmul2(u32_as_h2(w[c]), u32_as_h2(by1)), u32_as_h2(by_2)));
           }
           both[c] = __byte_perm(own, __shfl_xor_sync(0xffffffffu, own, 1), choose);
         }

@@ -61,3 +61,44 @@ def test_keys_of_all_sizes(size, io, out_dtype, softcap, hd):
         _check(_attend(cache, state, ids, n, q, out_dtype=out_dtype, softcap=softcap)[0], q[0], k, v, top, out_dtype, p_eps, softcap,
                norm=size < 2.0 ** 13)
     assert base._status() == 0
+
+
+@pytest.mark.parametrize("io", [BF, HF, F32])
+@pytest.mark.parametrize("hd,new", [(64, 1), (64, 4), (128, 1), (128, 4)])
+@pytest.mark.parametrize("n", [100, 700])
+def test_a_bad_group_of_values_shows_in_its_elements(io, hd, new, n):
+    """NaN in the scales of some groups of V: NaN in their 32 elements of the rows that see the position,
+    the other elements as if the group were zero."""
+    gen = torch.Generator().manual_seed(n + hd)
+    cache = base._cache(2, hd, 16, layers=1)
+    per = -(-n // 16)
+    ids = base._ids(1, per, gen)
+    state = k4.fill(cache, per + 2, gen)
+    half = state[1].view(per + 2, 2, 2, 16, hd // 32, 2)
+    q = torch.randn(1, new, 8, hd, generator=gen).to(io)
+    places = [(n - 2, 0, 1), (17, 1, 0), (n // 2, 1, hd // 32 - 1), (n - 1, 1, 0)]  # position, kv head, group
+    for p, h, g in places:
+        half[int(ids[0, p // 16]), h, 1, p % 16, g] = 0.0
+    # a group whose scales would not matter beside it
+    codes, held = k4.page_views(state, cache)
+    k, v = k4.gather(codes, held, cache, 0, ids[0], n)
+    for p, h, g in places:
+        half[int(ids[0, p // 16]), h, 1, p % 16, g] = math.nan
+    got = _attend(cache, state, ids, n, q)
+    hit = torch.zeros(new, 8, hd, dtype=torch.bool)
+    for p, h, g in places:
+        hit[torch.arange(new) + n - new >= p, 4 * h:4 * h + 4, 32 * g:32 * g + 32] = True
+    assert torch.equal(torch.isnan(got[0]), hit)
+    want = po.attend(q[0], k, v, hd ** -0.5)
+    p_eps = 2.0 ** -11 if io == BF else 2.0 ** -20
+    top = float(q.double().abs().sum(-1).amax() * held.abs().max() * 16) * hd ** -0.5
+    e = p_eps + 2 * (top * (hd + 16) * 2.0 ** -23 + 2.0 ** -21) + (math.sqrt(n) + 8) * 2.0 ** -23
+    off = (got[0].double() - want).abs()[~hit]
+    assert (off - want.abs()[~hit] * EPS[io] - 3 * 16 * held.abs().max() * e).max() <= 0
+    # the read-back agrees on which
+    kk, vv = base._attention().kv_read(cache, state, block_index=0, seq_block_ids=ids.cuda(), seq_lens=torch.tensor([n]).cuda(), max_seq_len=n)
+    bad = torch.zeros(n, 2, hd, dtype=torch.bool)
+    for p, h, g in places:
+        bad[p, h, 32 * g:32 * g + 32] = True
+    assert torch.equal(torch.isnan(vv[0].cpu()), bad)
+    assert base._status() == 0
