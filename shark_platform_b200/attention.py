@@ -409,6 +409,10 @@ class B200PagedAttentionBlock(torch.nn.Module):
             v = self._linear(x, self._wv, self._bias["attn_v"]).contiguous()
         if self._wqkv is not None and any(self._bias[n] is not None for n in ("attn_q", "attn_k", "attn_v")):
             raise C.B200MoeError("projection biases are supported with unfused (quantized) weights only")
+        own = not decode and (self.attention_kernel == "b200" or
+                              (getattr(self.cache, "dtype", None) == torch.uint8 and attention_mask is None))
+        if own and torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+            raise C.B200MoeError("the packed prompt attention has no gradient: call the block under torch.no_grad()")
         tokens = bs * sl
         page_ids = seq_block_ids.to(torch.int32).contiguous()
         self._desc.page_count = slab.shape[0]
@@ -462,7 +466,6 @@ class B200PagedAttentionBlock(torch.nn.Module):
             kh = k.view(bs, sl, Hkv, hd)
             vh = v.view(bs, sl, Hkv, hd)
             before = int(start_index) if self._quantized else 0
-            own = self.attention_kernel == "b200" or (getattr(self.cache, "dtype", None) == torch.uint8 and attention_mask is None)
             if before:  # a continued prompt: the cached positions, then the new ones as they are
                 kc, vc = kv_read(self.cache, cache_state, block_index=self.block_index, seq_block_ids=page_ids,
                                  seq_lens=torch.full((bs,), before, device=dev, dtype=torch.int32), max_seq_len=before,
@@ -470,7 +473,7 @@ class B200PagedAttentionBlock(torch.nn.Module):
                 kh, vh = torch.cat([kc, kh], dim=1), torch.cat([vc, vh], dim=1)
             if own:
                 cu = torch.arange(bs + 1, device=dev, dtype=torch.int32)
-                rows = lambda x, heads: x.detach().reshape(-1, heads, hd)
+                rows = lambda x, heads: x.reshape(-1, heads, hd)
                 attn = prompt_attend(rows(q, H), rows(kh, Hkv), rows(vh, Hkv), cu_seqlens=cu * sl,
                                      cu_seqlens_k=cu * (before + sl) if before else None, scale=float(scale),
                                      softcap=self.softcap, out_dtype=torch.float16 if direct else q.dtype)
