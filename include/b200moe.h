@@ -554,6 +554,18 @@ int b200moe_prompt_attend(const void* q, const void* k, const void* v, int dtype
                           int64_t k_rows, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, float softcap,
                           void* out, int out_dtype, void* scratch, size_t scratch_bytes, void* stream);
 
+/* Whether masks are causal, for callers of b200moe_prompt_attend that were given some: sets the
+ * bounds bit of the status word where one is not.  mask: `masks` of `rows` rows of `columns` numbers,
+ * batch_stride and row_stride elements apart, columns >= rows, the last of them the rows' own
+ * positions.  Zero: seen; -5000 and below: not seen; anything else is no mask.  Rows of tokens see all
+ * columns up to their own position and none behind it.  A mask has as many tokens as rows that see
+ * their own position, or as new_lens says (at most `rows`; [bs]; NULL: nothing): masks b * per_seq ... are
+ * sequence b's (bs * per_seq of them), or with per_seq 0 every sequence's.  Rows behind the tokens see none of
+ * the columns of such rows. */
+int b200moe_causal_mask_check(const void* mask, int dtype, int64_t batch_stride, int64_t row_stride, int32_t masks,
+                              int32_t rows, int32_t columns, const int32_t* new_lens, int32_t bs, int32_t per_seq,
+                              void* stream);
+
 /* A stream of batches from host memory (no reference counterpart: the
  * reference's eager layer takes whatever device its tensors are on).  The
  * pipeline keeps `depth` steps in flight: the host->device copy of a step's

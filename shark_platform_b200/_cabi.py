@@ -181,6 +181,7 @@ _PROTOS = {
     "b200moe_prompt_attend": (c_int, [_P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, c_int32, c_int64, c_int64,
                                       c_int32, c_int32, c_int32, c_float, c_float, _P, c_int, _P, c_size_t, _P]),
     "b200moe_prompt_attend_scratch_bytes": (c_size_t, [c_int, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32]),
+    "b200moe_causal_mask_check": (c_int, [_P, c_int, c_int64, c_int64, c_int32, c_int32, c_int32, _P, c_int32, c_int32, _P]),
     "b200moe_pipeline_bytes": (c_size_t, [_L, c_int, c_int32, c_int32]),
     "b200moe_pipeline_create": (c_int, [_L, c_int, c_int32, c_int, c_int32, _P, c_size_t, POINTER(c_void_p)]),
     "b200moe_pipeline_submit": (c_int, [_P, _P, _P, c_int32, _P]),

@@ -229,14 +229,37 @@ def _is_quantized(t) -> bool:
     return _moe._layout_name(t) in _moe._SUPPORTED
 
 
+def _check_causal(mask: torch.Tensor, bs: int, new_lens: Optional[torch.Tensor], device) -> None:
+    """Sets the status word's bounds bit where a row of tokens of `mask` [..., sl, sl or more] sees
+    other positions than the causal ones.  A position is seen where the mask is zero (True, for truth
+    values) and not where it is -5000 or less; anything else is no mask.  The tokens of a sequence are
+    the rows that see their own position, and those that new_lens says."""
+    if mask.dtype == torch.bool:
+        mask = torch.zeros(mask.shape, device=mask.device).masked_fill_(~mask, float("-inf"))
+    mask = mask.to(device, mask.dtype if mask.dtype in _DT else torch.float32)
+    for d in range(mask.dim() - 2):  # expanded dimensions once
+        if mask.stride(d) == 0:
+            mask = mask.narrow(d, 0, 1)
+    own = mask.dim() == 4 and mask.shape[0] == bs  # each sequence has its own
+    per = mask.shape[1] if own else 0
+    mask = mask.reshape(-1, *mask.shape[-2:])
+    if mask.stride(2) != 1:
+        mask = mask.contiguous()
+    lens = None if new_lens is None else new_lens.to(device, torch.int32).contiguous()
+    with torch.cuda.device(device):
+        C.check(C.lib.b200moe_causal_mask_check(_p(mask), _DT[mask.dtype], mask.stride(0), mask.stride(1), *mask.shape, _p(lens), bs, per,
+                                                _moe._stream()), "causal_mask_check")
+
+
 class B200PagedAttentionBlock(torch.nn.Module):
     """Drop-in for PagedLlamaAttentionBlock (same constructor keywords, same
     `forward` keywords).
 
-    `attention_kernel="b200"` takes `prompt_attend` for prompts.  It is causal by itself: of
-    an `attention_mask` it takes for granted that it is the causal one, with any padding
-    behind a sequence's tokens (the rows of padding are attended too and mean nothing); one
-    whose last two dimensions cannot be that is refused."""
+    `attention_kernel="b200"` takes `prompt_attend` for prompts.  It is causal by itself: an
+    `attention_mask` has to be the causal one, with any padding behind a sequence's tokens (the
+    rows of padding are attended too and mean nothing).  One whose shape cannot be that is
+    refused; its values are looked at on the device: where a row of tokens sees other
+    positions the status word's bounds bit is set (`moe.device_status` raises)."""
 
     def __init__(self, theta, *, block_index: int, cache, head_count: int, head_dim: int, head_count_kv: int,
                  rms_epsilon: float, attention_kernel: str = "decomposed", attention_scale: Optional[float] = None,
@@ -376,7 +399,9 @@ class B200PagedAttentionBlock(torch.nn.Module):
             raise C.B200MoeError("new_lens is for prefill; a negative start position marks a padding sequence of a step")
         if not decode and self.attention_kernel == "b200" and attention_mask is not None:
             seen = {sl, int(start_index) + sl} if self._quantized else {sl}
-            if attention_mask.dim() < 2 or attention_mask.shape[-2] != sl or attention_mask.shape[-1] not in seen:
+            lead = attention_mask.shape[:-2]
+            if (not 2 <= attention_mask.dim() <= 4 or attention_mask.shape[-2] != sl or attention_mask.shape[-1] not in seen or
+                    any(n not in (1, most) for n, most in zip(reversed(lead), (H, bs)))):
                 raise C.B200MoeError('attention_kernel="b200" is causal by itself: an attention_mask of '
                                      f"{list(attention_mask.shape)} is not the causal one of {sl} tokens")
         use_hf = bool(getattr(embedding, "use_hf", False))
@@ -473,6 +498,8 @@ class B200PagedAttentionBlock(torch.nn.Module):
                 kh, vh = torch.cat([kc, kh], dim=1), torch.cat([vc, vh], dim=1)
             if own:
                 cu = torch.arange(bs + 1, device=dev, dtype=torch.int32)
+                if attention_mask is not None:
+                    _check_causal(attention_mask, bs, new_lens, dev)
                 rows = lambda x, heads: x.reshape(-1, heads, hd)
                 attn = prompt_attend(rows(q, H), rows(kh, Hkv), rows(vh, Hkv), cu_seqlens=cu * sl,
                                      cu_seqlens_k=cu * (before + sl) if before else None, scale=float(scale),
