@@ -545,7 +545,8 @@ int b200moe_kv4_attend(const void* q, int q_dtype, int64_t q_stride, const void*
  * behind cu_q[bs]) give zeros.  Bounds that decrease or leave the rows set the bounds bit of the
  * status word; such a sequence is cut to the rows there are.  Any heads / kv_heads; head_dim 64
  * or 128; softcap (finite) <= 0 means none.  Infinities and NaN in k and v show in the rows that
- * attend them only.  scratch: b200moe_prompt_attend_scratch_bytes(...) bytes, 16-byte aligned, not
+ * attend them, and only there: an infinity in v as an infinity, or as NaN where its weight is zero in
+ * the products' type.  scratch: b200moe_prompt_attend_scratch_bytes(...) bytes, 16-byte aligned, not
  * shared with a call that may run at the same time (NULL where that is 0). */
 size_t b200moe_prompt_attend_scratch_bytes(int dtype, int32_t bs, int64_t q_rows, int64_t k_rows, int32_t heads,
                                            int32_t kv_heads, int32_t head_dim);

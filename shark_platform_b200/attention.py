@@ -208,8 +208,9 @@ def prompt_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqle
     (in front of the first and behind the last).  scale: 1 / sqrt(head_dim) by default; softcap:
     c * tanh(score / c).  Returns [rows, heads, head_dim] of `out_dtype`, by default q's.
 
-    Sums and softmax statistics are 32-bit.  There is no gradient: inputs that want one are
-    refused."""
+    An infinity or NaN in v shows in the rows that attend it, and only there: as an infinity, or as
+    NaN where its weight is zero in the products' type.  Sums and softmax statistics are 32-bit.
+    There is no gradient: inputs that want one are refused."""
     return C.attention_ops.prompt(q, k, v, cu_seqlens, cu_seqlens_k, scale, softcap, out_dtype)
 
 

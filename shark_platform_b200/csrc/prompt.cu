@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(SpCfg<HD>::THREADS, SpCfg<HD>::RESIDENT) promp
       }
       __syncthreads();  // K is read: the next one takes its place
       if (k0 + SP_KEYS < keys) fetch(sk, k, a.k_stride, k0 + SP_KEYS);
-      // where not all rows see all keys, a weight of zero leaves infinities and NaN out
+      // where not all rows see all keys, a weight of -0 leaves infinities and NaN out (a seen key's
+      // weight may be 0, and an infinity times that is NaN)
       const bool masked = k0 + SP_KEYS > tok0 + shift + 1;
 #pragma unroll
       for (int i = 0; i < SP_R; ++i) {
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(SpCfg<HD>::THREADS, SpCfg<HD>::RESIDENT) promp
         for (int j = 0; j < 4; ++j) {
           const float p = exp2f(s[i][j] - from);
           sum += p;
-          sp[(SP_R * ty + i) * PP + tx + 16 * j] = p;
+          sp[(SP_R * ty + i) * PP + tx + 16 * j] = s[i][j] == -INFINITY ? -0.f : p;
         }
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
@@ -288,9 +289,9 @@ __global__ void __launch_bounds__(SpCfg<HD>::THREADS, SpCfg<HD>::RESIDENT) promp
       if (k0 + SP_KEYS < keys) copy_wait<1>();
       else copy_wait<0>();
       __syncthreads();  // V is there, and the weights
-      auto products = [&](auto some) {
+      auto products = [&](auto some, int from, int to) {
 #pragma unroll 1
-        for (int j = 0; j < SP_KEYS; j += 4) {
+        for (int j = from; j < to; j += 4) {
           float4 p[SP_R];
 #pragma unroll
           for (int i = 0; i < SP_R; ++i) p[i] = *reinterpret_cast<const float4*>(sp + (SP_R * ty + i) * PP + j);
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(SpCfg<HD>::THREADS, SpCfg<HD>::RESIDENT) promp
 #pragma unroll
               for (int i = 0; i < SP_R; ++i) {
                 const float w = jj == 0 ? p[i].x : jj == 1 ? p[i].y : jj == 2 ? p[i].z : p[i].w;
-                if (decltype(some)::value && w == 0.f) continue;
+                if (decltype(some)::value && __float_as_uint(w) == 0x80000000u) continue;
                 o[i][n][0] = fmaf(w, y.x, o[i][n][0]);
                 o[i][n][1] = fmaf(w, y.y, o[i][n][1]);
                 o[i][n][2] = fmaf(w, y.z, o[i][n][2]);
@@ -311,8 +312,10 @@ __global__ void __launch_bounds__(SpCfg<HD>::THREADS, SpCfg<HD>::RESIDENT) promp
             }
         }
       };
-      if (masked) products(std::true_type());
-      else products(std::false_type());
+      // keys that all rows see; those that some do
+      const int all_see = masked ? max(0, tok0 + shift + 1 - k0) & ~3 : SP_KEYS;
+      products(std::false_type(), 0, all_see);
+      if (masked) products(std::true_type(), all_see, min(SP_KEYS, keys - k0));
     }
 #pragma unroll
     for (int i = 0; i < SP_R; ++i) {

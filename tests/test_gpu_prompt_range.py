@@ -78,3 +78,46 @@ def test_an_output_of_small_weights(dtype, lens, lens_k, where):
     room = want.abs() * (p_eps + 2.0 ** -24 + 2 * 16 * (hd + 8) * 2.0 ** -23 + 2.0 ** -18)
     off = (got.cpu().double() - want).abs()
     assert (off - room).max() <= 0, float((off / want.clamp(min=1e-30)).max())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("at", [3, 150, 290])
+def test_bad_values_of_weights_below_32_bits(dtype, bad, at):
+    """An infinity or NaN in the values of a key whose weight is 2^-400 shows in every row that sees it (as
+    an infinity or as NaN), wherever it lies among the tiles and parts, and in no other."""
+    hd = 64
+    g = torch.Generator().manual_seed(at)
+    for lens, lens_k in (([300], [300]), ([40], [2000])):
+        cu, cu_k = base._cu(lens), base._cu(lens_k)
+        n, m = lens[0], lens_k[0]
+        q = torch.ones(n, 2, hd, dtype=dtype)
+        k = ((torch.rand(m, 1, 1, generator=g) * 2 - 1) / 8).expand(-1, -1, hd).to(dtype).contiguous()
+        v = torch.randn(m, 1, hd, generator=g).to(dtype)
+        k[at] = -280.0 / 8
+        clean = base._call(q, k, v, cu, cu_k).cpu()
+        v[at, 0, 7] = bad
+        got = base._call(q, k, v, cu, cu_k).cpu()
+        sees = torch.arange(n) + m - n >= at
+        hit = torch.zeros_like(clean, dtype=torch.bool)
+        hit[sees, :, 7] = True
+        assert torch.equal(got[~hit], clean[~hit])
+        assert not torch.isfinite(got[hit]).any()
+        if math.isnan(bad):
+            assert torch.isnan(got[hit]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_an_infinite_value_before_scores_that_outgrow_it(dtype):
+    """The running sums have an infinity when a maximum 2^400 above comes."""
+    hd = 64
+    g = torch.Generator().manual_seed(1)
+    q = torch.ones(600, 2, hd, dtype=dtype)
+    k = ((torch.rand(600, 1, 1, generator=g) * 2 - 1) / 8).expand(-1, -1, hd).to(dtype).contiguous()
+    v = torch.randn(600, 1, hd, generator=g).to(dtype)
+    k[420] = 280.0 / 8
+    v[5, 0, 9] = math.inf
+    cu = torch.tensor([0, 600])
+    got = base._call(q, k, v, cu).cpu()
+    assert torch.isfinite(got[:5]).all() and not torch.isfinite(got[5:, :, 9]).any()
+    assert torch.isfinite(got[..., torch.arange(hd) != 9]).all()
