@@ -209,7 +209,8 @@ def prompt_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqle
     c * tanh(score / c).  Returns [rows, heads, head_dim] of `out_dtype`, by default q's.
 
     An infinity or NaN in v shows in the rows that attend it, and only there: as an infinity, or as
-    NaN where its weight is zero in the products' type.  Sums and softmax statistics are 32-bit.
+    NaN where its weight is zero in the products' type.  Sums and softmax statistics are 32-bit;
+    the weights of 16-bit rows are rounded to their type, also where the output is of 32 bits.
     There is no gradient: inputs that want one are refused."""
     return C.attention_ops.prompt(q, k, v, cu_seqlens, cu_seqlens_k, scale, softcap, out_dtype)
 

@@ -229,7 +229,7 @@ __device__ __forceinline__ void values_of(uint32_t codes, __half2 held, float (&
 
 // One CTA per (sequence, kv head, 16 positions); a thread takes the codes of 16 bytes of
 // output, K and V of several rows at once.  Bound by HBM: 32 sequences of up to 4000 positions, 8
-// heads of 128, to bf16 (648 MB) 115 us, 5.6 TB/s.
+// heads of 128, to bf16 (648 MB) 115 us, 5.6 TB/s; to fp32 (1.17 GB) 205, 5.7.
 constexpr int RD4_THREADS = 128, RD4_TILE = 16;
 template <typename T, int HD>
 __global__ void __launch_bounds__(RD4_THREADS) kv4_read_kernel(const Read4Args a) {
@@ -323,8 +323,8 @@ int launch_read4(const Read4Args& a, int hd, dim3 grid, cudaStream_t st) {
 // and the merge are those of the 8-bit cache.
 //
 // 32 sequences of 2000 to 4000 positions, 8 kv heads of 128, 32 heads (125 MB): bf16 36 us (int8
-// codes, 200 MB: 40), fp16 41, fp32 57; one of 32768 20 us; 8 x 8190, 48 heads, five new tokens, in two
-// tiles of 16 rows: bf16 50 us, fp16 61.  What bounds it: before the first rows 6 us, the merge 4 us, in
+// codes, 200 MB: 40), fp16 42, fp32 60; one of 32768 20 us; 8 x 8190, 48 heads, five new tokens, in two
+// tiles of 16 rows: bf16 54 us, fp16 64.  What bounds it: before the first rows 6 us, the merge 4 us, in
 // between the chain of dependent instructions of a unit (700 of a warp, issued every second clock;
 // 8 and 12 warps an SM take the same time within a tenth).
 // CTAs per SM at 32 x 4000: two 38.8 us, three 36.1, four (128 registers, the warps' states joined

@@ -166,7 +166,8 @@ __device__ __forceinline__ void zero_rest(const PromptArgs& a, int hd, int threa
 // 16 by 16 has rows 8 ty .. + 7, keys tx + 16 j of the scores and elements 4 tx + 64 n .. + 3 of the output, so
 // that 16 bytes from shared memory serve eight or four products.  K of the next tile is on its
 // way while the softmax and V's products of this one run, V during the scores.  Everything is
-// fp32.  6 x 777 tokens of 16 heads over 4 of 64 191 us, 25 TFLOP/s; 2048 of 32 over 8 of 128 968 us, 36:
+// fp32.  6 x 777 tokens of 16 heads over 4 of 64 192 us, 25 TFLOP/s; 2048 of 32 over 8 of 128 963 us, 36 (torch's
+// fused attention 2816):
 // bound by shared memory (12 loads of 16 bytes for 128 products a thread) and by the few warps that
 // fit.  (Four rows a thread 205, with K and V loaded in between 258 us; heads of 64 by 8 lanes a row and
 // 64 threads, with a third fewer loads for a product, 276.)
@@ -375,11 +376,12 @@ int launch_prompt(PromptArgs& a, cudaStream_t st) {
 // A step (128 keys of both tiles) needs 2048 clocks of the tensor core (4096 products a clock) and
 // as many of the special-function unit (16 exponentials a clock), side by side; it takes about 3100:
 // S out of tensor memory, the maximum and the way from the last P to the next S are in no other
-// unit's shadow when both tiles wait.  One B200, 32 heads over 8 of 128, bf16: 8192 tokens 420 us,
-// 1.31 PFLOP/s, 4096 118 us, 1.16; 16 x 1024 of 48 heads 257 us, with a softcap 408 (a polynomial of
-// five products a pair of scores, and a minimum beside the maximum).  An item costs about two steps
-// beside its own (start, last product, output).
-// On the way there, 8192 tokens: every role walking the list itself 545 us; descriptions of items
+// unit's shadow when both tiles wait.  One B200, 32 heads over 8 of 128, bf16, other inputs each time: 8192
+// tokens 460 to 505 us by the clock that the power limit leaves (1.1 to 1.2 PFLOP/s; 420 at best on the
+// same inputs again), 4096 123 us, 1.12; 16 x 1024 of 48 heads 272, with a softcap 475 (a polynomial of five
+// products a pair of scores, and a minimum beside the maximum).  torch's fused attention: 394, 111 and 230.
+// An item costs about two steps beside its own (start, last product, output).
+// On the way there, 8192 tokens, the same inputs again: every role walking the list itself 545 us; descriptions of items
 // with a run-time index, which puts them into local memory, 474; rows stored through shared memory
 // 434.  Not kept: two threads a row, 16 warps (both tiles then wait and compute at the same time)
 // 572 for 545; 3 to 8 of 16 pairs of exponentials as polynomials of degree 4 by the fp32 units 474 for
